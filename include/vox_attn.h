@@ -360,6 +360,123 @@ int    vox_attn_decode(vox_engine * e, const vox_decode_args * a, void * workspa
  *     partials: keep calls on one stream, or order them yourself. */
 int    vox_attn_decode_static(vox_engine * e, const vox_decode_args * a, void * stream);
 
+/* ---------------------------------------------------------------- shared prefixes ------ */
+
+/* Streams that start with the same rows (a voice prompt) keep them once, as the streams of a second cache, and every
+ * decode step computes the attention to them once for all streams that share them: the queries of those streams are
+ * the rows of one matrix product, so the prefix is read once per step and layer instead of once per stream.
+ * The reference has no counterpart: it holds one cache per request (src/minicpm.cpp:144-193).
+ *
+ * A plan says which stream starts with which prefix (arranged on the host, kept on the device).
+ *   prefix_of  host array [n_streams]: a stream of the prefix cache in [0, n_prefixes), or -1 for none
+ * vox_prefix_plan_set changes the assignment in stream order (not during a capture: it copies from the host); calls
+ * captured with the plan follow it.  A plan belongs to its engine's device and must outlive the calls that use it. */
+typedef struct vox_prefix_plan vox_prefix_plan;
+int  vox_prefix_plan_create(vox_engine * e, int n_streams, int n_prefixes, int n_heads, int n_kv_heads, const int32_t * prefix_of,
+                            vox_prefix_plan ** out);
+int  vox_prefix_plan_set(vox_prefix_plan * p, const int32_t * prefix_of, void * stream);
+void vox_prefix_plan_destroy(vox_prefix_plan * p);
+
+/* One-token attention over (prefix rows, own rows): out = softmax over both of scale * q.k, times v.
+ *   own          as for vox_attn_decode (kv_len counts own rows only; k_new / v_new, rope_table and flags mean the same;
+ *                the table is built for positions that count the prefix).  stream_order must be NULL.
+ *   prefix       the cache that holds the prefixes: same type and kv heads as own.cache, own.layer is taken of both; it may
+ *                be own.cache itself (streams of it that the call does not decode)
+ *   prefix_len   device array [streams of the prefix cache]: rows of each prefix
+ *   prefix_bound host-known upper bound of every prefix_len in use (sizes the grid and the workspace; 0: no prefix is read)
+ *   lse          optional, [H, n_streams] f32: the natural log-sum-exp of every row's scores (-inf: nothing visible),
+ *                which vox_kv_observe takes
+ * prefix, plan and prefix_len all NULL: own rows only (vox_attn_decode with lse).  Results agree with vox_attn_decode over a
+ * cache that holds both parts to rounding; q8_0 weights are not rounded to f16 here (error under 1e-5 of the output's RMS).
+ * A stream whose rows are all masked (no prefix row, no own row) gives zeros.
+ * workspace: vox_attn_decode_shared_workspace_bytes, 16-byte aligned.  The engine's device must be the current one. */
+typedef struct {
+    vox_decode_args         own;
+    const vox_kv_cache *    prefix;
+    const vox_prefix_plan * plan;
+    const int32_t *         prefix_len;
+    int32_t                 prefix_bound;
+    float *                 lse;
+} vox_decode_shared_args;
+
+size_t vox_attn_decode_shared_workspace_bytes(const vox_decode_shared_args * a);
+int    vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, void * workspace, size_t workspace_bytes,
+                              void * stream);
+
+/* ---------------------------------------------------------------- bounded caches ------- */
+
+/* The attention weight that every cache row has received, the measure by which vox_kv_evict chooses.  For the rows j < kv_len
+ * of every (stream, kv head) of one layer:
+ *   score[j] = (j new ? 0 : decay * score[j]) + sum over the n_q queries i and the heads of the group of
+ *              softmax_j(scale * q_i . k_j),     query i seeing rows j <= kv_len - n_q + i
+ *   q          [D, H, n_q, n_streams] f32, strides in bytes: the queries of the last n_q rows (one in a decode step; the
+ *              last ones of a prompt, up to 64); a query that would lie before row 0 sees nothing and adds nothing
+ *   rope_table as for vox_attn_decode (only with n_q == 1), or NULL: q is rotated already
+ *   lse        optional, [H, n_streams] f32, only with n_q == 1: the log-sum-exp the weights are taken against
+ *              (vox_attn_decode_shared returns it), when rows outside this cache have a share in the softmax
+ *   n_new      the last n_new rows of every stream are new: their score starts here, and row_pos[j] becomes
+ *              n_seen - kv_len + j, the token's position in its stream
+ *   score, row_pos  [max_len, HK, n_streams] f32 / int32 on the device, rows contiguous, strides nb_head, nb_stream in bytes
+ *              (the same for both); row_pos may be NULL.  Rows at kv_len and beyond are left as they are.
+ *   n_seen     device array [n_streams]: tokens every stream has seen, the new ones included (NULL: kv_len)
+ *   kv_bound   host-known upper bound of every kv_len; a longer stream raises VOX_ATTN_DEVICE_STATE and is left alone
+ * No atomics: the same call gives the same bits.  workspace: vox_kv_observe_workspace_bytes, 16-byte aligned. */
+typedef struct {
+    const vox_kv_cache * cache;
+    int32_t         layer;
+    int32_t         n_streams;
+    int32_t         n_heads;
+    int32_t         n_q;
+    const int32_t * kv_len;
+    const int32_t * n_seen;
+    int32_t         kv_bound;
+    const float *   q;
+    size_t          q_nb_head, q_nb_tok, q_nb_stream;
+    const float *   rope_table;
+    const float *   lse;
+    float           scale;
+    float           decay;
+    int32_t         n_new;
+    float *         score;
+    int32_t *       row_pos;
+    size_t          nb_head, nb_stream;
+} vox_kv_observe_args;
+
+size_t vox_kv_observe_workspace_bytes(const vox_kv_observe_args * a);
+int    vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspace, size_t workspace_bytes, void * stream);
+
+/* Cuts every stream with more than `budget` rows to `budget`, for layers layer0 .. layer0 + n_layers - 1 in one launch.
+ * In every (layer, stream, kv head) the rows with the largest score stay, of equal ones those of lower index (a NaN counts
+ * as less than any number); the first n_sink tokens (row_pos < n_sink) and the last n_recent (row_pos >= n_seen - n_recent)
+ * stay whatever their score.  Kept rows at index `budget` and above move, in order, into the places of rows that go, in
+ * order: K, V, score and row_pos together.  The order of cache rows does not matter to attention (every row carries its
+ * rotary embedding), so nothing else moves, and a step that gives up one row costs one row.  A stream's next row goes
+ * to index new_len; its rotary position is its count of tokens, which kv_len no longer is.
+ *   kv_len     device array [n_streams]; kv_bound its host-known upper bound (a longer stream raises
+ *              VOX_ATTN_DEVICE_STATE and is left alone, its new_len its kv_len)
+ *   n_sink + n_recent <= budget;  budget >= 1
+ *   score, row_pos  as vox_kv_observe leaves them, layers nb_layer bytes apart
+ *   new_len    device out [n_streams]: min(kv_len, budget); not kv_len itself
+ *   kept       optional out [budget, HK, n_streams, n_layers] int32 contiguous: for every row below new_len the index it had
+ *              (rows beyond are left as they are)
+ * Rows at new_len and beyond are left as they are. */
+typedef struct {
+    vox_kv_cache *  cache;
+    int32_t         layer0, n_layers;
+    int32_t         n_streams;
+    const int32_t * kv_len;
+    const int32_t * n_seen; /* NULL: kv_len */
+    int32_t         kv_bound;
+    int32_t         budget, n_sink, n_recent;
+    float *         score;
+    int32_t *       row_pos;
+    size_t          nb_head, nb_stream, nb_layer;
+    int32_t *       new_len;
+    int32_t *       kept;
+} vox_kv_evict_args;
+
+int vox_kv_evict(vox_engine * e, const vox_kv_evict_args * a, void * stream);
+
 /* ---------------------------------------------------------------- LocDiT --------------- */
 
 /* All attention of ONE CFM timestep in ONE launch: every layer, both CFG branches, every head,

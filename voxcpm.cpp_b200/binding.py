@@ -78,6 +78,26 @@ class DecodeArgs(C.Structure):
                 ("rope_table", C.c_void_p), ("stream_order", C.c_void_p)]
 
 
+class DecodeSharedArgs(C.Structure):
+    _fields_ = [("own", DecodeArgs), ("prefix", C.c_void_p), ("plan", C.c_void_p), ("prefix_len", C.c_void_p), ("prefix_bound", C.c_int32),
+                ("lse", C.c_void_p)]
+
+
+class ObserveArgs(C.Structure):
+    _fields_ = [("cache", C.c_void_p), ("layer", C.c_int32), ("n_streams", C.c_int32), ("n_heads", C.c_int32), ("n_q", C.c_int32),
+                ("kv_len", C.c_void_p), ("n_seen", C.c_void_p), ("kv_bound", C.c_int32), ("q", C.c_void_p), ("q_nb_head", C.c_size_t),
+                ("q_nb_tok", C.c_size_t), ("q_nb_stream", C.c_size_t), ("rope_table", C.c_void_p), ("lse", C.c_void_p), ("scale", C.c_float),
+                ("decay", C.c_float), ("n_new", C.c_int32), ("score", C.c_void_p), ("row_pos", C.c_void_p), ("nb_head", C.c_size_t),
+                ("nb_stream", C.c_size_t)]
+
+
+class EvictArgs(C.Structure):
+    _fields_ = [("cache", C.c_void_p), ("layer0", C.c_int32), ("n_layers", C.c_int32), ("n_streams", C.c_int32), ("kv_len", C.c_void_p),
+                ("n_seen", C.c_void_p), ("kv_bound", C.c_int32), ("budget", C.c_int32), ("n_sink", C.c_int32), ("n_recent", C.c_int32),
+                ("score", C.c_void_p), ("row_pos", C.c_void_p), ("nb_head", C.c_size_t), ("nb_stream", C.c_size_t), ("nb_layer", C.c_size_t),
+                ("new_len", C.c_void_p), ("kept", C.c_void_p)]
+
+
 class QkvArgs(C.Structure):
     _fields_ = [("n_streams", C.c_int32), ("hidden", C.c_int32), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32),
                 ("head_dim", C.c_int32), ("x", C.c_void_p), ("x_nb_stream", C.c_size_t), ("w_qkv", C.c_void_p),
@@ -178,6 +198,14 @@ def lib() -> C.CDLL:
         "vox_attn_decode_workspace_bytes": (sz, [i32, i32, i32, i32]),
         "vox_attn_decode": (i32, [vp, C.POINTER(DecodeArgs), vp, sz, vp]),
         "vox_attn_decode_static": (i32, [vp, C.POINTER(DecodeArgs), vp]),
+        "vox_prefix_plan_create": (i32, [vp, i32, i32, i32, i32, vp, C.POINTER(vp)]),
+        "vox_prefix_plan_set": (i32, [vp, vp, vp]),
+        "vox_prefix_plan_destroy": (None, [vp]),
+        "vox_attn_decode_shared_workspace_bytes": (sz, [C.POINTER(DecodeSharedArgs)]),
+        "vox_attn_decode_shared": (i32, [vp, C.POINTER(DecodeSharedArgs), vp, sz, vp]),
+        "vox_kv_observe_workspace_bytes": (sz, [C.POINTER(ObserveArgs)]),
+        "vox_kv_observe": (i32, [vp, C.POINTER(ObserveArgs), vp, sz, vp]),
+        "vox_kv_evict": (i32, [vp, C.POINTER(EvictArgs), vp]),
         "vox_attn_locdit_step": (i32, [vp, C.POINTER(LocditArgs), vp]),
         "vox_group_create": (i32, [vp, C.POINTER(GroupConfig), C.POINTER(vp)]),
         "vox_group_destroy": (None, [vp]),
@@ -410,6 +438,20 @@ class KVCache:
         _check(lib().vox_kv_view(self.h, layer, stream_id, seq_len, C.byref(k), C.byref(v)))
         return k, v
 
+    def planes(self):
+        """The K and V rows of an f16 cache as torch tensors [layers, streams, kv heads, max_len, 64]: views of the cache's own
+        memory (``vox_kv_view`` gives its address).  They keep the cache alive; ``close`` ends them."""
+        import torch
+        c = self.cfg
+        shape = (c.n_layers, c.n_streams, c.n_kv_heads, c.max_len, 64)
+
+        class Memory:  # what torch.as_tensor takes as device memory that it does not own; the tensor holds on to it
+            def __init__(self, owner, address):
+                self.owner = owner
+                self.__cuda_array_interface__ = {"shape": shape, "typestr": "<f2", "data": (address, False), "version": 3}
+
+        return tuple(torch.as_tensor(Memory(self, x.data), device=f"cuda:{self.engine.device}") for x in self.view(0, 0, c.max_len))
+
     def row_bytes(self):
         return 128 if self.cfg.type == F16 else 68
 
@@ -469,6 +511,88 @@ class KVCache:
         a = self._decode_args(layer, q, kv_len, kv_bound, dst, scale, k_new, v_new, False, rope_table, None)
         _check(lib().vox_attn_decode_static(self.engine.h, C.byref(a), _stream_ptr(stream)))
         return dst
+
+
+    def decode_shared(self, layer, q, kv_len, kv_bound, prefix=None, plan=None, prefix_len=None, prefix_bound=0, scale=0.125, stream=None,
+                      dst=None, k_new=None, v_new=None, cache_stable=False, rope_table=None, lse=None, workspace=None):
+        """``vox_attn_decode_shared``: as ``decode``, over the rows of a prefix that several streams share and the streams' own.
+        ``prefix``: the KVCache that holds the prefixes; ``plan``: a PrefixPlan; ``prefix_len`` int32 device [prefixes];
+        ``lse`` [n_streams, H] f32 receives the log-sum-exp.  Returns [n_streams, H, 64]."""
+        import torch
+        S, H, D = q.shape
+        if dst is None:
+            dst = torch.empty((S, H, D), dtype=torch.float32, device=q.device)
+        a = DecodeSharedArgs()
+        a.own = self._decode_args(layer, q, kv_len, kv_bound, dst, scale, k_new, v_new, cache_stable, rope_table, None)
+        a.prefix = prefix.h if prefix is not None else None
+        a.plan = plan.h if plan is not None else None
+        a.prefix_len = prefix_len.data_ptr() if prefix_len is not None else None
+        a.prefix_bound = prefix_bound
+        a.lse = lse.data_ptr() if lse is not None else None
+        ws = workspace if workspace is not None else self.engine.workspace(lib().vox_attn_decode_shared_workspace_bytes(C.byref(a)))
+        _check(lib().vox_attn_decode_shared(self.engine.h, C.byref(a), C.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(stream)))
+        return dst
+
+    def observe(self, layer, q, kv_len, kv_bound, score, row_pos=None, n_seen=None, n_new=1, lse=None, decay=1.0, scale=0.125,
+                rope_table=None, stream=None, workspace=None):
+        """``vox_kv_observe``: adds the attention weight that the queries q [n_streams, n_q, H, 64] (the last n_q rows') give to
+        every row to ``score`` [n_streams, HK, rows] f32, and notes the positions of the ``n_new`` new rows in ``row_pos``
+        (int32, the same shape and strides)."""
+        S, n_q, H, D = q.shape
+        a = ObserveArgs(self.h, layer, S, H, n_q, kv_len.data_ptr(), n_seen.data_ptr() if n_seen is not None else None, kv_bound, q.data_ptr(),
+                        q.stride(2) * 4, q.stride(1) * 4, q.stride(0) * 4)
+        a.rope_table = rope_table.data_ptr() if rope_table is not None else None
+        a.lse = lse.data_ptr() if lse is not None else None
+        a.scale, a.decay, a.n_new = scale, decay, n_new
+        a.score = score.data_ptr()
+        a.row_pos = row_pos.data_ptr() if row_pos is not None else None
+        assert score.stride(-1) == 1 and (row_pos is None or row_pos.stride() == score.stride())
+        a.nb_head, a.nb_stream = score.stride(-2) * 4, score.stride(-3) * 4
+        ws = workspace if workspace is not None else self.engine.workspace(lib().vox_kv_observe_workspace_bytes(C.byref(a)))
+        _check(lib().vox_kv_observe(self.engine.h, C.byref(a), C.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(stream)))
+
+    def evict(self, kv_len, kv_bound, budget, score, row_pos, n_seen, new_len, n_sink=4, n_recent=32, kept=None, layer0=0, stream=None):
+        """``vox_kv_evict``: cuts the streams' rows to ``budget`` by ``score`` in the layers that ``score`` and ``row_pos``
+        [n_layers, n_streams, HK, rows] span; ``new_len`` int32 [n_streams] receives the lengths, ``kept`` (int32
+        [n_layers, n_streams, HK, budget], optional) the rows' former indices."""
+        assert score.stride(-1) == 1 and row_pos.stride() == score.stride() and (kept is None or kept.is_contiguous())
+        a = EvictArgs(self.h, layer0, score.shape[0], score.shape[1], kv_len.data_ptr(), n_seen.data_ptr() if n_seen is not None else None,
+                      kv_bound, budget, n_sink, n_recent, score.data_ptr(), row_pos.data_ptr(), score.stride(2) * 4, score.stride(1) * 4,
+                      score.stride(0) * 4, new_len.data_ptr(), kept.data_ptr() if kept is not None else None)
+        _check(lib().vox_kv_evict(self.engine.h, C.byref(a), _stream_ptr(stream)))
+
+
+class PrefixPlan:
+    """``vox_prefix_plan``: which stream starts with which prefix (a stream of the prefix cache; -1: none)."""
+
+    def __init__(self, engine: Engine, prefix_of, n_prefixes, n_heads=16, n_kv_heads=2):
+        a = self._ints(prefix_of)
+        h = C.c_void_p()
+        _check(lib().vox_prefix_plan_create(engine.h, len(a), n_prefixes, n_heads, n_kv_heads, a.ctypes.data_as(C.c_void_p), C.byref(h)))
+        self.engine, self.h, self.n_streams = engine, h, len(a)
+        engine._children.add(self)
+
+    @staticmethod
+    def _ints(prefix_of):
+        import numpy as np
+        return np.ascontiguousarray(prefix_of, np.int32)
+
+    def set(self, prefix_of, stream=None):
+        """Another assignment, in stream order."""
+        a = self._ints(prefix_of)
+        assert a.shape == (self.n_streams,)
+        _check(lib().vox_prefix_plan_set(self.h, a.ctypes.data_as(C.c_void_p), _stream_ptr(stream)))
+
+    def close(self):
+        if self.h and self.engine.h:
+            lib().vox_prefix_plan_destroy(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Group:

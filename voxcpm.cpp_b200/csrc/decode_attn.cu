@@ -36,6 +36,7 @@
 // applied in f32 to the per-block score accumulators (K) and folded into the softmax weights (V),
 // so Q is never quantised.
 #include "kv_cache.cuh"
+#include "shared_prefix.cuh"
 
 #include <algorithm>
 #include <cstdlib>
@@ -47,6 +48,7 @@ namespace {
 constexpr int kConsumerWarps = 4;
 constexpr int kThreads       = (kConsumerWarps + 1) * 32;
 constexpr int kPartialStride = 66;  // max, sum, acc[64]
+constexpr float kWeightShift = 10.0f;
 constexpr int kMaxGqa        = 8;   // query heads per kv head (rows 0-7 of the A operand)
 
 // Developer build (-DVOX_ATTN_DEVELOPER): every CTA notes the time (globaltimer, ns) at which it passes a few points
@@ -110,6 +112,10 @@ struct DecodeParams {
     const uint8_t * mask;
     size_t          mask_nb_head, mask_nb_stream;
     int             mask_ne2, mask_ne3;
+    // kShared kernels: the partial results of the rows that streams share (shared_prefix.cuh), folded into every result
+    // before it is written; the natural log-sum-exp of every row's softmax (NULL: not wanted)
+    PrefixFold      shared;
+    float *         lse;
 };
 
 __device__ __forceinline__ int clamp_len(const DecodeParams & p, int len) { return max(0, min(len, p.max_len)); }
@@ -303,6 +309,8 @@ template <bool Q8> struct Ring {
     // launch (one tile per pass): 4 CTAs x 96 registers x 5 stages 45.6 us; 5 x 72 x 4: 48.1 us; 3 x 105 x 6: 48.2 us.
     // Stages are held while their tile is worked on, so depth pays: 4 CTAs x 6 stages (the most that fits) 43.8 -> 42.5 us.
     static constexpr int kCtasPerSm  = Q8 ? 4 : 3;
+    // (the kShared form of q8_0 needs more than the 96 registers that four CTAs leave a thread)
+    static constexpr int ctas_per_sm(bool shared) { return Q8 && !shared ? 4 : 3; }
     static constexpr int kDataBytes  = Q8 ? kKvTile * 64 : kKvTile * 128;
     static constexpr int kStageBytes = Q8 ? 9 * 1024 : 2 * kDataBytes;
     static constexpr int kTxBytes    = Q8 ? kQ8TileBytes : 2 * kDataBytes;
@@ -311,22 +319,6 @@ template <bool Q8> struct Ring {
     static_assert(kStageBytes >= kConsumerWarps * kMaxGqa * kPartialStride * 4, "a stage must hold the warps' partials");
 };
 
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ float half_lo(uint32_t x) { return __half2float(__ushort_as_half((unsigned short) (x & 0xffffu))); }
-__device__ __forceinline__ float half_hi(uint32_t x) { return __half2float(__ushort_as_half((unsigned short) (x >> 16))); }
-
-// Bytes of a q8_0 tile -> f16 tensor-core operands without arithmetic.  The tiles hold u = q + 128 (1..255); a byte
-// in the low half of a 16-bit word whose high half is zero is the (subnormal) f16 number u * 2^-24, which mma.sync
-// takes as it is.  `selector` picks which two bytes of the word go to the two halves (PRMT, 4 = a zero byte).  The
-// products then carry (q + 128) * 2^-24: the factor goes into the step that consumes the accumulator anyway, and the
-// 128 comes out of the accumulator as 128 times the sum of the other operand, taken once (K: the row sums of Q per
-// 32-value block, known when Q is loaded; V: the running sums of the weights).
-constexpr float kTwo24 = 16777216.0f, kTwoM24 = 1.0f / 16777216.0f;
-__device__ __forceinline__ uint32_t u8_pair_to_half2(uint32_t bytes, uint32_t selector) { return __byte_perm(bytes, 0u, selector); }
 // product of two packed pairs of halves, as bits
 __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
@@ -393,11 +385,44 @@ __device__ __forceinline__ bool mbar_wait_cluster_bounded(uint32_t bar, uint32_t
 
 __device__ __forceinline__ void fence_acq_rel_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
 
+// One head's result leaves: (max, sum, acc) of the stream's own rows for output columns d0 .. d0+3, 16 threads per head.
+// With kShared the partials of the rows that the stream shares are folded in first, in key order (their kernel runs just
+// before this one and may still be running: the dependency wait comes here, as late as it can).
+template <bool kShared>
+__device__ __forceinline__ void write_result(const DecodeParams & p, int stream, int kvh, int hh, int d0, float M, float L, float (&acc)[4]) {
+    const int head = kvh * p.gqa + hh;
+    if constexpr (kShared) {
+        if (p.shared.ml != nullptr) {
+            pdl_wait();
+            pdl_launch_dependents();
+            prefix_fold(p.shared, stream, kvh, hh, p.n_kv_heads, p.gqa, d0, M, L, acc);
+        }
+        if (p.lse != nullptr && d0 == 0) p.lse[(size_t) stream * p.n_heads + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    }
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;  // nothing visible -> zeros, as the reference
+    *reinterpret_cast<float4 *>(p.dst + ((size_t) stream * p.n_heads + head) * kHeadDim + d0) =
+        make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+}
+// a stream without a row of its own: zeros, or what its shared rows give; by the consumer warps of a CTA
+template <bool kShared>
+__device__ __forceinline__ void write_empty(const DecodeParams & p, int stream, int head0, int n_heads, int tid) {
+    if constexpr (kShared) {
+        for (int j = tid; j < n_heads * 16; j += kConsumerWarps * 32) {
+            const int head = head0 + (j >> 4);
+            float     acc[4] = {0.f, 0.f, 0.f, 0.f};
+            write_result<true>(p, stream, head / p.gqa, head % p.gqa, (j & 15) * 4, -INFINITY, 0.0f, acc);
+        }
+    } else {
+        float4 * out = reinterpret_cast<float4 *>(p.dst + ((size_t) stream * p.n_heads + head0) * kHeadDim);
+        for (int j = tid; j < n_heads * kHeadDim / 4; j += kConsumerWarps * 32) out[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+}
+
 // The fold of NP pairs at once by one thread (head hh of each pair, output columns d0 .. d0+3): the partials of a pair
 // (runs b0 .. b1 of the launch; the run that holds the pair's first tile wrote its slot 1, the others their slot 0) are
 // read W at a time, the loads of a batch issued together (each is a round trip to L2, and a pair may have been cut 17
 // ways).  pend[k] = stream, kv head, b0, b1.
-template <int NP, int W>
+template <bool kShared, int NP, int W>
 __device__ __forceinline__ void fold_pairs(const DecodeParams & p, const int (*pend)[4], int k0, int hh, int d0) {
     int   b0[NP], b1[NP];
     float M[NP], L[NP], acc[NP][4];
@@ -420,7 +445,7 @@ __device__ __forceinline__ void fold_pairs(const DecodeParams & p, const int (*p
                 const int     cc = min(b0[k] + c + u, b1[k]);
                 const float * pc = p.partial + ((size_t) cc * 2 + (cc == b0[k] ? 1 : 0)) * p.gqa * kPartialStride + hh * kPartialStride;
                 mc[k][u] = b0[k] + c + u <= b1[k] ? __ldcg(pc) : -INFINITY;
-                lc[k][u] = __ldcg(pc + 1);
+                lc[k][u] = kShared && b0[k] + c + u > b1[k] ? 0.0f : __ldcg(pc + 1);
                 lo[k][u] = __ldcg(reinterpret_cast<const float2 *>(pc + 2 + d0));
                 hi[k][u] = __ldcg(reinterpret_cast<const float2 *>(pc + 4 + d0));
             }
@@ -430,7 +455,8 @@ __device__ __forceinline__ void fold_pairs(const DecodeParams & p, const int (*p
         for (int k = 0; k < NP; ++k)
 #pragma unroll
             for (int u = 0; u < W; ++u) {
-                if (mc[k][u] == -INFINITY) continue;  // past the pair's last partial, or a partial that saw nothing
+                // past the pair's last partial, or a partial that saw nothing (kShared: the sum of a row of NaN stays in)
+                if (mc[k][u] == -INFINITY && !(kShared && lc[k][u] != 0.0f)) continue;
                 const float Mn = fmaxf(M[k], mc[k][u]);
                 const float fo = exp2f(M[k] - Mn);  // M == -inf: 0
                 const float fw = exp2f(mc[k][u] - Mn);
@@ -443,16 +469,13 @@ __device__ __forceinline__ void fold_pairs(const DecodeParams & p, const int (*p
             }
     }
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-        const int   stream = pend[k0 + k][0], head = pend[k0 + k][1] * p.gqa + hh;
-        const float inv    = L[k] > 0.0f ? 1.0f / L[k] : 0.0f;
-        *reinterpret_cast<float4 *>(p.dst + ((size_t) stream * p.n_heads + head) * kHeadDim + d0) =
-            make_float4(acc[k][0] * inv, acc[k][1] * inv, acc[k][2] * inv, acc[k][3] * inv);
-    }
+    for (int k = 0; k < NP; ++k) write_result<kShared>(p, pend[k0 + k][0], pend[k0 + k][1], hh, d0, M[k], L[k], acc[k]);
 }
 
-template <bool Q8>
-__global__ void __launch_bounds__(kThreads, Ring<Q8>::kCtasPerSm)
+// kShared: the form behind vox_attn_decode_shared.  Results take in the partials of shared rows, the log-sum-exp can
+// be returned, and q8_0 weights keep 22 bits (value and remainder, as the f16 form's do) instead of 11.
+template <bool Q8, bool kShared>
+__global__ void __launch_bounds__(kThreads, Ring<Q8>::ctas_per_sm(kShared))
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeParams p) {
     using R = Ring<Q8>;
     constexpr int kStages = R::kStages;
@@ -531,10 +554,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                 pdl_wait();
                 pdl_launch_dependents();
             }
-            if (warp < kConsumerWarps) {
-                float4 * out = reinterpret_cast<float4 *>(p.dst + ((size_t) w.stream * p.n_heads + (size_t) w.kvh * p.gqa) * kHeadDim);
-                for (int j = tid; j < p.gqa * kHeadDim / 4; j += kConsumerWarps * 32) out[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+            if (warp < kConsumerWarps) write_empty<kShared>(p, w.stream, w.kvh * p.gqa, p.gqa, tid);
             return;
         }
     } else {
@@ -553,17 +573,21 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         cut_note[0] = cut.aligned; cut_note[1] = cut.f0; cut_note[2] = cut.run; cut_note[3] = cut.b0; cut_note[4] = cut.b1;
         DECODE_TRACE(1);
     }
-    if (n_tiles == 0 && blockIdx.x != 0) return;  // more CTAs than runs: nothing to do
+    // more CTAs than runs: nothing to do (with shared rows every CTA takes a part of the streams that have no rows)
+    if (n_tiles == 0 && blockIdx.x != 0 && !(kShared && any_empty)) return;
     }
 
     if (warp == kConsumerWarps) {
         // ------------------------------------------------------------------ producer
         // All lanes walk the run (the arriving row is converted by the whole warp); lane 0 issues the copies.
         bool waited = !p.early;
+        // Behind the kernel of the shared rows: that kernel has passed its own dependency wait before this one could
+        // start, so all that this warp reads is complete; only its partials are not, and write_result waits for them.
+        const bool behind_prefix = kShared && p.early == kBehindPrefix;
         int  issued = 0;
         for (int it = 0; it < n_tiles; ++it) {
             const bool append_here = p.k_new != nullptr && w.t == w.tiles - 1;  // the arriving row lies in the pair's last tile
-            if (!waited && (append_here || it >= p.early_tiles)) {  // the first tiles were requested while the previous kernel drained
+            if (!waited && !behind_prefix && (append_here || it >= p.early_tiles)) {  // the first tiles were requested while the previous kernel drained
                 pdl_wait();
                 pdl_launch_dependents();
                 waited = true;
@@ -646,18 +670,17 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 
     // ---------------------------------------------------------------------- consumers
     const int g = lane >> 2, t = lane & 3;
-    if (p.early) {  // Q is written by the kernel before this one
+    if (p.early && !(kShared && p.early == kBehindPrefix)) {  // Q is written by the kernel before this one
         pdl_wait();
         pdl_launch_dependents();
     }
     if (tid == 0) DECODE_TRACE(2);
-    if (blockIdx.x == 0 && any_empty) {
+    if ((kShared || blockIdx.x == 0) && any_empty) {
         // a stream with no visible rows has no tile in the list: its result is zeros (ops.cpp:8333)
-        for (int i = 0; i < p.n_streams; ++i) {
+        for (int i = kShared ? (int) blockIdx.x : 0; i < p.n_streams; i += kShared ? (int) gridDim.x : 1) {
             const int len = clamp_len(p, p.kv_len ? p.kv_len[i] : p.kv_len_const);
             if (len > 0) continue;
-            float4 * out = reinterpret_cast<float4 *>(p.dst + (size_t) i * p.n_heads * kHeadDim);
-            for (int j = tid; j < p.n_heads * kHeadDim / 4; j += kConsumerWarps * 32) out[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            write_empty<kShared>(p, i, 0, p.n_heads, tid);
         }
     }
 
@@ -752,6 +775,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         // q8_0: sums of the V-scaled weights (accumulator tile of the product with ones: [0] = [1] = head g with the
         // scales of block 0, [2] = [3] = with those of block 1)
         float v_bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float v_unit = 1.0f, v_limit = -1.0f;  // kShared q8_0: see the products below
 
         // Tiles per pass of a consumer warp: one.  Two (both cache types were tried: two independent tiles in one pass
         // give the scheduler something to overlap the dependency chains with) measured the same or slower: f16 50.6
@@ -870,14 +894,17 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                 const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
                 const float m_use = m_new == -INFINITY ? 0.0f : m_new;
                 m                 = m_new;
+                // kShared, f16: weights up to 2^10 instead of 1, so that the remainders of small ones are still normal f16
+                // numbers (their spacing below 2^-14 is 2^-24: seen from a weight of 1 that loses the last two bits)
+                const float m_exp = kShared && !Q8 ? m_use - kWeightShift : m_use;
                 float pr[U][2][2];
                 float psum_q8 = 0.0f;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        pr[u][j][0] = ex2_approx(sv[u][j][0] - m_use);
-                        pr[u][j][1] = ex2_approx(sv[u][j][1] - m_use);
+                        pr[u][j][0] = ex2_approx(sv[u][j][0] - m_exp);
+                        pr[u][j][1] = ex2_approx(sv[u][j][1] - m_exp);
                         psum_q8 += pr[u][j][0] + pr[u][j][1];
                     }
                 if (__any_sync(0xffffffffu, alpha != 1.0f)) {  // after the first tiles the running maxima rarely move
@@ -907,6 +934,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                         for (int n2 = 0; n2 < 4; ++n2) {
                             uint32_t b0, b1, b2, b3;
                             ldmatrix_x4_trans(vb + v_row * 128 + (((2 * n2 + v_chk) ^ (v_row & 7)) << 4), b0, b1, b2, b3);
+                            if (kShared && edge) {  // rows past the length may hold anything: zero times a NaN is none
+                                const uint32_t k0 = keep_rows(p0[u] + 2 * t, c1), k1 = keep_rows(p0[u] + 8 + 2 * t, c1);
+                                b0 &= k0; b1 &= k1; b2 &= k0; b3 &= k1;
+                            }
                             mma_16816(o[2 * n2], pa, b0, b1);
                             mma_16816(o[2 * n2 + 1], pa, b2, b3);
                         }
@@ -924,6 +955,67 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                         // serves both chunk pairs; of each accumulator tile the half that belongs to its block is kept.
                         const uint32_t vsc = kb + 2 * R::kDataBytes + kKvTile * 4;
                         uint32_t       pa[4];
+                        if constexpr (kShared) {
+                            // As the f16 form carries its weights: one operand per 32-column block, rows 0-7 the weights
+                            // times the scales of the block rounded to f16, rows 8-15 what the rounding left.  As many
+                            // products as below (there one operand serves both blocks and half of every tile is dropped),
+                            // and both halves of a tile belong to its columns.
+                            // The products are taken in units of v_unit, a power of two that follows the largest scale seen (as the
+                            // running maximum does, but it moves only when a scale outgrows it by 2^8): the f16 parts of
+                            // weights of any magnitude of V neither overflow nor lose bits below 2^-14.
+                            uint2 d0 = lds64(vsc + s_off), d1 = lds64(vsc + s_off + 32);
+                            if (edge) {  // rows past the length may hold anything: zero times a NaN is none
+                                const int pos = p0[u] + 2 * t;
+                                if (pos >= c1) d0.x = 0u;
+                                if (pos + 1 >= c1) d0.y = 0u;
+                                if (pos + 8 >= c1) d1.x = 0u;
+                                if (pos + 9 >= c1) d1.y = 0u;
+                            }
+                            const __half2 big = __hmax2(__hmax2(__habs2(as_half2(d0.x)), __habs2(as_half2(d0.y))),
+                                                        __hmax2(__habs2(as_half2(d1.x)), __habs2(as_half2(d1.y))));
+                            float dm = fmaxf(__low2float(big), __high2float(big));
+                            if (__any_sync(0xffffffffu, dm > v_limit)) {
+                                dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 1));
+                                dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 2));
+                                const float unit = dm > 0.0f ? __uint_as_float(__float_as_uint(dm) & 0x7f800000u) : kTwoM24;
+                                const float f    = v_unit / unit;
+#pragma unroll
+                                for (int n = 0; n < 8; ++n) {
+                                    o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f;
+                                }
+                                v_bias[0] *= f; v_bias[2] *= f;
+                                v_unit  = unit;
+                                v_limit = dm > 0.0f ? unit * 256.0f : 0.0f;
+                            }
+                            const float to_units = 32.0f / v_unit;
+                            uint32_t    pb[2][4];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const uint2 ds = j ? d1 : d0;
+                                const float p0s = pr[u][j][0] * to_units, p1s = pr[u][j][1] * to_units;
+#pragma unroll
+                                for (int b = 0; b < 2; ++b) {
+                                    float h0, l0, h1, l1;
+                                    split_hi_lo(p0s * (b ? half_hi(ds.x) : half_lo(ds.x)), h0, l0);
+                                    split_hi_lo(p1s * (b ? half_hi(ds.y) : half_lo(ds.y)), h1, l1);
+                                    pb[b][2 * j]     = pack_half2(h0, h1);
+                                    pb[b][2 * j + 1] = pack_half2(l0, l1);
+                                }
+                            }
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                // the weights' sums, which the +128 of the V bytes multiplies, from a tile of ones
+                                float sums[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_16816(sums, pb[b], 0x3c003c00u, 0x3c003c00u);
+                                v_bias[2 * b] += sums[0] + sums[2];
+                                uint32_t r0, r1, r2, r3;
+                                ldmatrix_x4_trans(vb + (v_off ^ (b << 5)), r0, r1, r2, r3);
+                                mma_16816(o[4 * b + 0], pb[b], u8_pair_to_half2(r0, 0x4240), u8_pair_to_half2(r1, 0x4240));
+                                mma_16816(o[4 * b + 1], pb[b], u8_pair_to_half2(r0, 0x4341), u8_pair_to_half2(r1, 0x4341));
+                                mma_16816(o[4 * b + 2], pb[b], u8_pair_to_half2(r2, 0x4240), u8_pair_to_half2(r3, 0x4240));
+                                mma_16816(o[4 * b + 3], pb[b], u8_pair_to_half2(r2, 0x4341), u8_pair_to_half2(r3, 0x4341));
+                            }
+                        } else {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const uint2    ds  = lds64(vsc + s_off + 32 * j);  // halves: (pos: b0, b1), (pos + 1: b0, b1)
@@ -950,6 +1042,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                             mma_16816(o[4 * cp + 2], pa, u8_pair_to_half2(r2, 0x4240), u8_pair_to_half2(r3, 0x4240));
                             mma_16816(o[4 * cp + 3], pa, u8_pair_to_half2(r2, 0x4341), u8_pair_to_half2(r3, 0x4341));
                         }
+                        }
                     }
                 }
             }
@@ -974,8 +1067,13 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const float b = -128.0f * v_bias[n < 4 ? 0 : 2];
-                o[n][0] = fmaf(n < 4 ? o[n][0] : o[n][2], kTwo24, b);
-                o[n][1] = fmaf(n < 4 ? o[n][1] : o[n][3], kTwo24, b);
+                if constexpr (kShared) {
+                    o[n][0] = fmaf(o[n][0] + o[n][2], kTwo24, b) * (v_unit / 32.0f);
+                    o[n][1] = fmaf(o[n][1] + o[n][3], kTwo24, b) * (v_unit / 32.0f);
+                } else {
+                    o[n][0] = fmaf(n < 4 ? o[n][0] : o[n][2], kTwo24, b);
+                    o[n][1] = fmaf(n < 4 ? o[n][1] : o[n][3], kTwo24, b);
+                }
                 o[n][2] = o[n][3] = 0.0f;
             }
         }
@@ -988,7 +1086,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         float *   scratch    = reinterpret_cast<float *>(smem_gen + last_stage * R::kStageBytes);
         {
             float * mine = scratch + (warp * 8 + g) * kPartialStride;
-            if (t == 0) { mine[0] = m; mine[1] = l; }
+            if (t == 0) { mine[0] = kShared && !Q8 ? m - kWeightShift : m; mine[1] = l; }
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 // output column of accumulator registers 0/2 and 1/3 of tile n
@@ -1020,10 +1118,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                     for (int d = 0; d < 4; ++d) acc[d] += src[2 + d0 + d] * fw;
                 }
                 if (whole) {
-                    const int   head = kvh * p.gqa + hh;
-                    const float inv  = L > 0.0f ? 1.0f / L : 0.0f;  // nothing visible -> zeros, as the reference
-                    *reinterpret_cast<float4 *>(p.dst + ((size_t) stream * p.n_heads + head) * kHeadDim + d0) =
-                        make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+                    write_result<kShared>(p, stream, kvh, hh, d0, M, L, acc);
                 } else if (kClusterMode && p.cluster > 0) {
                     // into the first CTA of the cluster: slot `rank`, behind its ring
                     const uint32_t dstp = dsmem_addr(smem_base + n_stages * R::kStageBytes + (uint32_t) ((rank * kMaxGqa + hh) * kPartialStride) * 4, 0);
@@ -1073,16 +1168,14 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                     for (int r = 0; r < parts; ++r) {  // in list order, the running maximum raised part by part
                         const float * src = slots + (r * kMaxGqa + hh) * kPartialStride;
                         const float   mc  = src[0];
-                        if (mc == -INFINITY) continue;
+                        if (mc == -INFINITY && !(kShared && src[1] != 0.0f)) continue;
                         const float Mn = fmaxf(M, mc), fo = exp2f(M - Mn), fw = exp2f(mc - Mn);
                         M = Mn;
                         L = L * fo + src[1] * fw;
 #pragma unroll
                         for (int d = 0; d < 4; ++d) acc[d] = acc[d] * fo + src[2 + d0 + d] * fw;
                     }
-                    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-                    *reinterpret_cast<float4 *>(p.dst + ((size_t) w.stream * p.n_heads + (size_t) w.kvh * p.gqa + hh) * kHeadDim + d0) =
-                        make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+                    write_result<kShared>(p, w.stream, w.kvh, hh, d0, M, L, acc);
                 }
             }
         }
@@ -1118,8 +1211,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             if (hh < p.gqa) {
                 // a CTA that drew the last ticket of both its cut pairs folds them side by side: the loads of both are
                 // in flight together, instead of one fold waiting for its round trips to L2 after the other
-                if (flags == 3) fold_pairs<2, kFoldWidth / 2>(p, pending, 0, hh, d0);
-                else            fold_pairs<1, kFoldWidth>(p, pending, flags == 2 ? 1 : 0, hh, d0);
+                if (flags == 3) fold_pairs<kShared, 2, kFoldWidth / 2>(p, pending, 0, hh, d0);
+                else            fold_pairs<kShared, 1, kFoldWidth>(p, pending, flags == 2 ? 1 : 0, hh, d0);
             }
         }
     }
@@ -1141,10 +1234,10 @@ namespace vox {
 //     per pair at 17 or fewer;
 //   - a launch with fewer tiles than that gets fewer CTAs.
 // The cut itself happens on the device from the lengths of the moment; kv_bound only sizes the grid.
-void decode_plan(const vox_engine * e, bool q8, int n_streams, int n_kv_heads, int kv_bound, int * grid, int * run_min) {
+void decode_plan(const vox_engine * e, bool q8, int n_streams, int n_kv_heads, int kv_bound, int * grid, int * run_min, bool shared = false) {
     const long long tiles_bound = std::max(1, (std::max(kv_bound, 1) + kKvTile - 1) / kKvTile);
     const long long pairs       = std::max(1LL, (long long) n_streams * n_kv_heads);
-    const int       fit         = q8 ? Ring<true>::kCtasPerSm : Ring<false>::kCtasPerSm;
+    const int       fit         = q8 ? Ring<true>::ctas_per_sm(shared) : Ring<false>::ctas_per_sm(shared);
     int             wave        = fit;
     int             sms         = kDecodeMaxSms;
     if (e != nullptr) {
@@ -1178,11 +1271,14 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
                   size_t q_nb_stream, float * dst, float scale, void * workspace, size_t workspace_bytes, int * counters,
                   cudaStream_t stream, const vox_kv_cache * append_to, const float * k_new, const float * v_new,
                   size_t new_nb_head, size_t new_nb_stream, bool early, const float * rope_table, const int32_t * order,
-                  const vox_tensor * mask) {
-    const uint32_t bit = q8 ? (1u << 9) : (1u << 8);
+                  const vox_tensor * mask, const SharedRows * rows) {
+    const bool     shared = rows != nullptr;
+    const auto     kernel = q8 ? (shared ? decode_kernel<true, true> : decode_kernel<true, false>)
+                               : (shared ? decode_kernel<false, true> : decode_kernel<false, false>);
+    const int      smem = q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
+    const uint32_t bit  = 1u << ((q8 ? 9 : 8) + (shared ? 16 : 0));
     if (!(e->attr_mask & bit)) {
-        if (q8) VOX_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<true>::kSmemBytes));
-        else    VOX_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<false>::kSmemBytes));
+        VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         e->attr_mask |= bit;
     }
     VOX_REQUIRE(n_streams > 0 && n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= kMaxGqa,
@@ -1200,6 +1296,13 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
     p.status = e->status_dev;
     p.counters = counters;
     p.early = early ? 1 : 0;
+    p.shared = PrefixFold{};
+    p.lse    = nullptr;
+    if (shared) {
+        p.shared = rows->fold;
+        p.lse    = rows->lse;
+        if (rows->fold.ml != nullptr && pdl_enabled()) p.early = kBehindPrefix;
+    }
     {
         const int depth = q8 ? Ring<true>::kStages : Ring<false>::kStages;
         const int tuned = e->decode_early_tiles;
@@ -1240,7 +1343,7 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
         p.mask_ne2 = (int) mask->ne[2]; p.mask_ne3 = (int) mask->ne[3];
     }
     int grid = 1;
-    decode_plan(e, q8, n_streams, n_kv_heads, kv_bound, &grid, &p.run_min);
+    decode_plan(e, q8, n_streams, n_kv_heads, kv_bound, &grid, &p.run_min, shared);
     const size_t need = (size_t) 2 * grid * p.gqa * kPartialStride * sizeof(float);
     VOX_REQUIRE(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0,
                 VOX_ATTN_WORKSPACE_TOO_SMALL, "decode needs %zu workspace bytes (8-byte aligned), got %zu", need, workspace_bytes);
@@ -1266,7 +1369,7 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
 
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) grid); cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int n_attr = 0;
@@ -1282,8 +1385,7 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
     }
     cfg.attrs = attr;
     cfg.numAttrs = n_attr;
-    if (q8) cudaLaunchKernelEx(&cfg, decode_kernel<true>, map_k, map_v, p);
-    else    cudaLaunchKernelEx(&cfg, decode_kernel<false>, map_k, map_v, p);
+    cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p);
     return check_launch(e, q8 ? "decode_kernel<q8_0>" : "decode_kernel<f16>");
 }
 
@@ -1293,7 +1395,7 @@ int launch_decode_f16(vox_engine * e, const CUtensorMap & map_k, const CUtensorM
                       float scale, const vox_tensor * mask, void * workspace, size_t workspace_bytes, cudaStream_t stream) {
     return launch_decode(e, false, map_k, map_v, nullptr, 0, 0, 0, n_kv, n_streams, n_heads, n_kv_heads, nullptr, n_kv, n_kv, q,
                          q_nb_head, q_nb_stream, dst, scale, workspace, workspace_bytes, e->counters_dev, stream, nullptr, nullptr,
-                         nullptr, 0, 0, false, nullptr, nullptr, mask);
+                         nullptr, 0, 0, false, nullptr, nullptr, mask, nullptr);
 }
 
 // ---- single-token calls over q8_0 K/V in ggml's block layout (the operator called on a caller's own quantised
@@ -1395,7 +1497,7 @@ int launch_decode_q8_blocks(vox_engine * e, const vox_attn_args * a, void * work
     return launch_decode(e, true, none, none, base, pair_bytes, pair_bytes * HK, 0, n_pad, B, (int) a->q.ne[2], HK, nullptr, n_kv, n_kv,
                          static_cast<const float *>(a->q.data), a->q.nb[2], a->q.nb[3], static_cast<float *>(a->dst.data), a->scale,
                          workspace, partials, e->counters_dev, st, nullptr, nullptr, nullptr, 0, 0, false, nullptr, nullptr,
-                         a->mask.data ? &a->mask : nullptr);
+                         a->mask.data ? &a->mask : nullptr, nullptr);
 }
 
 }  // namespace vox
@@ -1430,7 +1532,8 @@ int check_decode_args(const vox_engine * e, const vox_decode_args * a, const cha
     return VOX_ATTN_OK;
 }
 
-int decode_checked(vox_engine * e, const vox_decode_args * a, void * workspace, size_t workspace_bytes, void * stream) {
+int decode_checked(vox_engine * e, const vox_decode_args * a, void * workspace, size_t workspace_bytes, void * stream,
+                   const SharedRows * rows = nullptr) {
     const vox_kv_cache * c       = a->cache;
     const bool           appends = a->k_new != nullptr;
     int * counters = c->counters + (size_t) a->layer * c->cfg.n_streams * c->cfg.n_kv_heads;
@@ -1440,10 +1543,18 @@ int decode_checked(vox_engine * e, const vox_decode_args * a, void * workspace, 
                          a->n_streams, a->n_heads, c->cfg.n_kv_heads, a->kv_len, 0, a->kv_bound, a->q, a->q_nb_head, a->q_nb_stream,
                          a->dst, a->scale, workspace, workspace_bytes, counters, static_cast<cudaStream_t>(stream),
                          appends ? c : nullptr, a->k_new, a->v_new, a->new_nb_head, a->new_nb_stream,
-                         (a->flags & VOX_DECODE_CACHE_STABLE) != 0, a->rope_table, a->stream_order, nullptr);
+                         (a->flags & VOX_DECODE_CACHE_STABLE) != 0, a->rope_table, a->stream_order, nullptr, rows);
 }
 
 }  // namespace
+
+namespace vox {
+int check_decode(const vox_engine * e, const vox_decode_args * a, const char * who) { return check_decode_args(e, a, who); }
+int launch_decode_shared(vox_engine * e, const vox_decode_args * a, const SharedRows & rows, void * workspace, size_t workspace_bytes,
+                         cudaStream_t stream) {
+    return decode_checked(e, a, workspace, workspace_bytes, stream, &rows);
+}
+}  // namespace vox
 
 #ifdef VOX_ATTN_DEVELOPER
 // out: kTraceCtas x kTracePoints times in ns (0 entry, 1 work list cut, 2 consumers past the dependency wait, 3 first tile

@@ -81,6 +81,26 @@ __device__ __forceinline__ void q8_0_quantize_pair(float x0, float x1, char2 & q
 __device__ __forceinline__ uchar2 q8_0_biased(char2 q) {
     return make_uchar2((unsigned char) ((int) q.x + 128), (unsigned char) ((int) q.y + 128));
 }
+
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float half_lo(uint32_t x) { return __half2float(__ushort_as_half((unsigned short) (x & 0xffffu))); }
+__device__ __forceinline__ float half_hi(uint32_t x) { return __half2float(__ushort_as_half((unsigned short) (x >> 16))); }
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2 *>(&x); }
+// the halves of a register that holds rows pos, pos + 1, as bits: those below `len` are kept
+__device__ __forceinline__ uint32_t keep_rows(int pos, int len) { return (pos < len ? 0x0000ffffu : 0u) | (pos + 1 < len ? 0xffff0000u : 0u); }
+
+// Bytes of a q8_0 tile -> f16 tensor-core operands without arithmetic.  The tiles hold u = q + 128 (1..255); a byte
+// in the low half of a 16-bit word whose high half is zero is the (subnormal) f16 number u * 2^-24, which mma.sync
+// takes as it is.  `selector` picks which two bytes of the word go to the two halves (PRMT, 4 = a zero byte).  The
+// products then carry (q + 128) * 2^-24: the factor goes into the step that consumes the accumulator anyway, and the
+// 128 comes out of the accumulator as 128 times the sum of the other operand, taken once (K: the row sums of Q per
+// 32-value block, known when Q is loaded; V: the running sums of the weights).
+constexpr float kTwo24 = 16777216.0f, kTwoM24 = 1.0f / 16777216.0f;
+__device__ __forceinline__ uint32_t u8_pair_to_half2(uint32_t bytes, uint32_t selector) { return __byte_perm(bytes, 0u, selector); }
 #endif
 
 }  // namespace vox
