@@ -96,6 +96,9 @@ SHARED = {
     "six heads": ("f16", [i % 2 for i in range(50)], [257, 1000], [1 + 7 * i for i in range(50)], 6, 1),
     "one stream, long prefix": ("f16", [0], [9000], [3], 16, 2),
     "few rows per tile, long": ("f16", [0, 0, 0, 1, 1], [4100, 2050], [1, 40, 500, 2, 3], 16, 2),
+    "full row tiles, edges": ("f16", [i % 8 for i in range(128)], [1, 63, 64, 65, 127, 128, 129, 193], [i % 5 for i in range(128)], 16, 2),
+    "full row tiles, long": ("f16", [i % 2 for i in range(40)], [5000, 1601], [1 + i for i in range(40)], 16, 2),
+    "full row tiles, six heads": ("f16", [0] * 45, [777], [3] * 45, 6, 1),
     "q8_0 one row of each": ("q8_0", [0], [1], [1], 16, 2),
     "q8_0 tile edges": ("q8_0", [0, 1, 2, 3, 4, 5], [63, 64, 65, 127, 128, 129], [129, 128, 127, 65, 64, 63], 16, 2),
     "q8_0 mixed": ("q8_0", [2, -1, 0, 2, -1, 1, 2, 0, 0, 2, 1], [700, 33, 1025], [5, 0, 300, 1, 66, 0, 8, 640, 17, 2, 90], 16, 2),

@@ -7,6 +7,7 @@
 // (decode_attn.cu), bound by HBM.  The prefix rows are this kernel's: the queries of all streams that share a prefix are
 // the rows of one matrix product against it, so the prefix leaves HBM once for all of them instead of once per stream.
 #include "shared_prefix.cuh"
+#include "tcgen05.cuh"
 
 #include <algorithm>
 #include <exception>
@@ -21,6 +22,7 @@ using namespace vox;
 struct vox_prefix_plan {
     vox_engine *         e = nullptr;
     int                  n_streams = 0, n_prefixes = 0, gqa = 0, max_tiles = 0;
+    bool                 full = false;  // the row tiles are more than half full on average
     std::vector<int32_t> host;
     int32_t *            dev = nullptr;
     size_t tiles_at() const { return 4; }
@@ -56,7 +58,7 @@ struct SharedParams {
     const int32_t * order;
     const int32_t * len;       // [prefix]
     float2 *        ml;
-    float *         acc;
+    float4 *        acc;
     int             n_prefixes, n_kv_heads, gqa, layer, max_len;
     int             chunk, max_chunks;
     float           scale_log2;
@@ -458,19 +460,331 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 if (row >= w.rows) continue;
                 const size_t at = (size_t) w.slot * kPrefixRows + row;
                 if (t == 0) p.ml[at] = make_float2(m[h], l[h]);
-                float * out = p.acc + at * kHeadDim;
+                float * out = reinterpret_cast<float *>(p.acc + (size_t) w.slot * 16 * kPrefixRows + row);
+                auto    col = [](int d) { return (size_t) (d >> 2) * kPrefixRows * 4 + (d & 3); };  // place of output column d
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
                     if constexpr (Q8) {  // tile n: chunk n / 2, this lane 16 (n / 2) + 4t + (n % 2) and two further
                         const int d = 16 * (n >> 1) + 4 * t + (n & 1);
-                        out[d] = o[n][2 * h];
-                        out[d + 2] = o[n][2 * h + 1];
+                        out[col(d)]     = o[n][2 * h];
+                        out[col(d + 2)] = o[n][2 * h + 1];
                     } else {
-                        *reinterpret_cast<float2 *>(out + 8 * n + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                        *reinterpret_cast<float2 *>(out + col(8 * n + 2 * t)) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
                     }
                 }
             }
         }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Full row tiles on the 5th-generation tensor cores (f16 caches).
+//
+// One CTA takes one (row tile, kv head, chunk of keys).  Q (scaled by scale * log2 e) lies in shared memory as two f16 tiles,
+// value and remainder; scores S = Q_lo.K + Q_hi.K (the small part first: the accumulator truncates) come 64 keys at a time
+// into one of six score buffers in TMEM.  Two groups of four softmax warps take them in turn, a thread per row: 64 scores
+// out of TMEM, weights 2^(S - ref) back over them as two packed f16 tiles (value and remainder, 22 bits), from where the
+// tensor core takes them as the A operand of P.V.  Every group has an output accumulator and a reference maximum of its
+// own, so the groups never wait for one another; they are joined once, at the end.  The reference of a row is raised only
+// when a maximum exceeds it by 2^8 (its accumulator is then rescaled in TMEM).
+//   warps 0-3, 4-7  softmax groups    warp 8  K/V copies    warp 9  issues S = Q.K    warp 10  issues O += P.V
+constexpr int kTcThreads = 11 * 32;
+constexpr int kTcStages  = 4;
+constexpr int kSub       = 64;                    // keys of a score tile
+constexpr int kSBufs     = 6;
+constexpr int kTcOCol    = kSBufs * kSub;         // two accumulators of 64 columns behind the score buffers
+constexpr int kQTile     = kPrefixRows * 128;
+constexpr int kTcStage   = 2 * kKeys * 128;       // 128 rows of K, 128 rows of V
+constexpr int kTcSmem    = 2 * kQTile + kTcStages * kTcStage + 1024;
+constexpr float kTcShift = 6.0f;                  // weights up to 2^(8 + 6): their remainders stay normal f16 numbers
+
+// multiply this thread's accumulator row by f; rare, kept out of line so that its registers do not weigh on the loop
+__device__ __noinline__ void rescale_row(uint32_t t_o, float f) {
+    tc_fence_after();
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        float o[32];
+        tmem_ld32(t_o + 32 * h, o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] *= f;
+        tmem_st32(t_o + 32 * h, o);
+    }
+    tc_fence_before();
+}
+
+__global__ void __launch_bounds__(kTcThreads, 1)
+shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int      abort_flag;
+    __shared__ float2   other_ml[kPrefixRows];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t sQ = smem_base, sKV = sQ + 2 * kQTile;
+    const int      tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = full0 + 8 * kTcStages, bS0 = empty0 + 8 * kTcStages, bP0 = bS0 + 8 * kSBufs,
+                   bF0 = bP0 + 8 * kSBufs, bO = bF0 + 8 * kSBufs;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < kTcStages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < kSBufs; ++s) {
+            mbar_init(bS0 + 8 * s, 1);
+            mbar_init(bP0 + 8 * s, 4);  // one arrival per warp of the group that took the tile
+            mbar_init(bF0 + 8 * s, 1);
+        }
+        mbar_init(bO, 1);
+        fence_mbar_init();
+    }
+    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // The decode kernel behind this one relies on this order: its CTAs start once every CTA here has passed the wait.
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&tmem_slot);
+    Item           w;
+    const bool     work = (int) blockIdx.x < p.plan[0] * p.n_kv_heads * p.max_chunks && load_item(p, blockIdx.x, w);
+    if (!work) w.key0 = w.key1 = 0;
+    const int n_keys = w.key1 - w.key0, n_tiles = (n_keys + kKeys - 1) / kKeys, n_sub = (n_keys + kSub - 1) / kSub;
+
+    auto give_up = [&]() {
+        atomicOr(p.status, kStatusTimeout);
+        atomicExch(&abort_flag, 1);
+    };
+    auto aborted   = [&]() { return *reinterpret_cast<volatile int *>(&abort_flag) != 0; };
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0; };
+    auto load_tile = [&](int T) {  // one lane
+        const int      st = T % kTcStages, boxes = n_keys - T * kKeys > kSub ? 2 : 1;
+        const uint32_t bar = full0 + 8 * st, dst = sKV + st * kTcStage;
+        mbar_expect_tx(bar, boxes * 2 * kSub * 128);
+        for (int b = 0; b < boxes; ++b) {
+            tma_load_5d(dst + b * kSub * 128, &map_k, bar, 0, w.key0 + T * kKeys + b * kSub, w.kvh, w.prefix, p.layer);
+            tma_load_5d(dst + kKeys * 128 + b * kSub * 128, &map_v, bar, 0, w.key0 + T * kKeys + b * kSub, w.kvh, w.prefix, p.layer);
+        }
+    };
+    if (warp == 8) {
+        if (lane == 0)
+            for (int T = 0; T < min(n_tiles, kTcStages); ++T) load_tile(T);
+    } else if (warp < 8 && work) {
+        // Q: two threads per row, 32 head dimensions each
+        const int  row = tid >> 1, half = tid & 1;
+        const bool live = row < w.rows;
+        const int  at = live ? row : 0, stream = p.order[w.first + at / p.gqa], head = w.kvh * p.gqa + at % p.gqa;
+        const float * src = reinterpret_cast<const float *>(p.q + (size_t) stream * p.q_nb_stream + (size_t) head * p.q_nb_head);
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 v = *reinterpret_cast<const float2 *>(src + 32 * half + 2 * i);
+            x[2 * i] = v.x; x[2 * i + 1] = v.y;
+        }
+        if (p.rope != nullptr) {  // the other half of the row is the neighbouring thread's
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float2 r = p.rope[(size_t) stream * (kHeadDim / 2) + i];
+                const float  y = __shfl_xor_sync(0xffffffffu, x[i], 1);
+                x[i] = half ? __fadd_rn(__fmul_rn(y, r.y), __fmul_rn(x[i], r.x)) : __fsub_rn(__fmul_rn(x[i], r.x), __fmul_rn(y, r.y));
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float h0, l0, h1, l1;
+                split_hi_lo(live ? x[8 * c + 2 * i] * p.scale_log2 : 0.0f, h0, l0);
+                split_hi_lo(live ? x[8 * c + 2 * i + 1] * p.scale_log2 : 0.0f, h1, l1);
+                hi[i] = pack_half2(h0, h1);
+                lo[i] = pack_half2(l0, l1);
+            }
+            uint8_t * dst = smem_gen + row * 128 + (((4 * half + c) ^ (row & 7)) << 4);
+            *reinterpret_cast<uint4 *>(dst)          = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4 *>(dst + kQTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+
+    if (warp == 8) {
+        // ------------------------------------------------------------------ copies
+        if (lane == 0) {
+            bool ok = true;
+            int  T  = min(n_tiles, kTcStages);
+            for (; T < n_tiles && ok; ++T) {
+                if (!mbar_wait_bounded(empty0 + 8 * (T % kTcStages), ((T / kTcStages) - 1) & 1) || aborted()) { ok = false; break; }
+                load_tile(T);
+            }
+            if (!ok) {
+                give_up();
+                for (int i = max(0, T - kTcStages); i < T; ++i) mbar_wait_bounded(full0 + 8 * (i % kTcStages), (i / kTcStages) & 1);
+            }
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------------ scores (all lanes in the loop, one issues)
+        constexpr uint32_t idesc = idesc_f16(kSub, false);
+        const uint64_t     dQ = smem_desc_sw128(sQ), dQlo = smem_desc_sw128(sQ + kQTile), dK = smem_desc_sw128(sKV);
+        const bool         leader = elect_one();
+        bool               ok = true;
+        for (int U = 0; U < n_sub && ok; ++U) {
+            const int T = U >> 1, st = T % kTcStages, sb = U % kSBufs;
+            if (!warp_wait(full0 + 8 * st, (T / kTcStages) & 1) || (U >= kSBufs && !warp_wait(bF0 + 8 * sb, ((U / kSBufs) - 1) & 1))) { ok = false; break; }
+            tc_fence_after();
+            if (leader) {
+                const uint32_t dS = tmem + kSub * sb;
+                const uint64_t k0 = dK + (uint64_t) (st * (kTcStage >> 4) + (U & 1) * ((kSub * 128) >> 4));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma_f16(dS, dQlo + k * 2, k0 + k * 2, idesc, k > 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma_f16(dS, dQ + k * 2, k0 + k * 2, idesc, 1);
+                tc_commit(bS0 + 8 * sb);
+            }
+            __syncwarp();
+        }
+        if (!ok && lane == 0) give_up();
+    } else if (warp == 10) {
+        // ------------------------------------------------------------------ output
+        constexpr uint32_t idesc = idesc_f16(kHeadDim, true);
+        const uint64_t     dV = smem_desc_sw128_mn(sKV + kKeys * 128, 16);
+        const bool         leader = elect_one();
+        bool               ok = true;
+        for (int U = 0; U < n_sub && ok; ++U) {
+            const int T = U >> 1, st = T % kTcStages, sb = U % kSBufs;
+            if (!warp_wait(full0 + 8 * st, (T / kTcStages) & 1) || !warp_wait(bP0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
+            tc_fence_after();
+            if (leader) {
+                const uint32_t tP = tmem + kSub * sb, tO = tmem + kTcOCol + kHeadDim * (U & 1);
+                const uint64_t v0 = dV + (uint64_t) (st * (kTcStage >> 4) + (U & 1) * ((kSub * 128) >> 4));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + 8 * k, v0 + k * (2048 >> 4), idesc, U > 1 || k > 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + kSub / 2 + 8 * k, v0 + k * (2048 >> 4), idesc, 1);
+                tc_commit(bF0 + 8 * sb);
+                if ((U & 1) || U == n_sub - 1) tc_commit(empty0 + 8 * st);
+                if (U == n_sub - 1) tc_commit(bO);
+            }
+            __syncwarp();
+        }
+        if (!ok && lane == 0) give_up();
+    } else {
+        // ------------------------------------------------------------------ softmax: a thread per row
+        const int      group = warp >> 2, row = tid & 127;
+        const uint32_t t_row = tmem + ((uint32_t) (32 * (warp & 3)) << 16), t_o = t_row + kTcOCol + kHeadDim * group;
+        float          m = -INFINITY, l = 0.0f;
+        bool           ok = true;
+        for (int U = group; U < n_sub; U += 2) {
+            const int sb = U % kSBufs, left = n_keys - U * kSub;  // keys of this tile and after
+            if (!mbar_wait_bounded(bS0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t t_s = t_row + kSub * sb;
+            uint32_t       r[kSub];
+            tmem_ld64_sync(t_s, r);
+            if (left < kSub) {
+#pragma unroll
+                for (int i = 0; i < kSub; ++i)
+                    if (i >= left) r[i] = 0xff800000u;
+                // rows past the prefix may hold anything, and zero times a NaN is none: V's are cleared
+                const int T = U >> 1, st = T % kTcStages;
+                if (!mbar_wait_bounded(full0 + 8 * st, (T / kTcStages) & 1)) { ok = false; break; }
+                if (row >= left && row < kSub) {
+                    uint4 * v = reinterpret_cast<uint4 *>(smem_gen + (sKV - smem_base) + st * kTcStage + kKeys * 128 + ((U & 1) * kSub + row) * 128);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+            }
+            float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kSub; i += 4) {
+                t0 = max3(t0, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+                t1 = max3(t1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+            }
+            const float top = fmaxf(t0, t1);
+            if (U < 2) {
+                m = top;
+            } else {
+                const bool raise = top > m + 8.0f;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float f = raise ? ex2_approx(m - top) : 1.0f;
+                    if (raise) m = top;
+                    l *= f;
+                    // the accumulator is at rest once P.V of the group's last tile has retired
+                    if (!mbar_wait_bounded(bF0 + 8 * ((U - 2) % kSBufs), ((U - 2) / kSBufs) & 1)) { ok = false; break; }
+                    rescale_row(t_o, f);
+                }
+            }
+            const float ref = m - kTcShift;
+#pragma unroll
+            for (int g = 0; g < kSub / 16; ++g) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float p0 = ex2_approx(__uint_as_float(r[16 * g + 2 * i]) - ref);
+                    const float p1 = ex2_approx(__uint_as_float(r[16 * g + 2 * i + 1]) - ref);
+                    const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
+                    const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                    hi[i] = pack_half2(h0, h1);
+                    lo[i] = pack_half2(p0 - h0, p1 - h1);
+                    l += p0 + p1;
+                }
+                tmem_st8_nowait(t_s + 8 * g, hi);
+                tmem_st8_nowait(t_s + kSub / 2 + 8 * g, lo);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bP0 + 8 * sb);
+        }
+        if (ok && n_sub > 0 && !mbar_wait_bounded(bO, 0)) ok = false;
+        if (!ok) give_up();
+        ok = named_bar_all(1, 256, ok && !aborted());
+        if (ok && work) {
+            tc_fence_after();
+            // the second group's part goes through the ring's memory (every copy has been consumed)
+            float4 * const other = reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base));
+            const bool     both  = n_sub > 1;
+            uint32_t       r[64];
+            if (group == 0 || both) tmem_ld64_sync(t_o, r);
+            if (group == 1 && both) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c)
+                    other[c * kPrefixRows + row] = make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3]));
+                other_ml[row] = make_float2(m, l);
+            }
+            named_bar_sync(1, 256);
+            if (group == 0 && row < w.rows) {
+                float fa = 1.0f, fb = 0.0f;
+                if (both) {
+                    const float2 b  = other_ml[row];
+                    const float  mn = fmaxf(m, b.x);
+                    fa = m == -INFINITY ? 0.0f : exp2f(m - mn);
+                    fb = b.x == -INFINITY ? 0.0f : exp2f(b.x - mn);
+                    l  = l * fa + b.y * fb;
+                    m  = mn;
+                }
+                p.ml[(size_t) w.slot * kPrefixRows + row] = make_float2(m - kTcShift, l);
+                float4 * out = p.acc + (size_t) w.slot * 16 * kPrefixRows + row;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    float4 x = make_float4(__uint_as_float(r[4 * c]) * fa, __uint_as_float(r[4 * c + 1]) * fa, __uint_as_float(r[4 * c + 2]) * fa, __uint_as_float(r[4 * c + 3]) * fa);
+                    if (both) {
+                        const float4 y = other[c * kPrefixRows + row];
+                        x = make_float4(fmaf(y.x, fb, x.x), fmaf(y.y, fb, x.y), fmaf(y.z, fb, x.z), fmaf(y.w, fb, x.w));
+                    }
+                    out[c * kPrefixRows] = x;
+                }
+            }
+        }
+    }
+    // common exit: every role has left its loop; release TMEM
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
     }
 }
 
@@ -531,6 +845,7 @@ int arrange(vox_prefix_plan * pl, const int32_t * prefix_of) {
             }
         }
     h[0] = n_tiles;
+    pl->full = 2 * start[pl->n_prefixes - 1] > n_tiles * per_tile;
     return VOX_ATTN_OK;
 }
 
@@ -647,7 +962,7 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
         VOX_REQUIRE(slots < (1u << 30), VOX_ATTN_UNSUPPORTED, "vox_attn_decode_shared: more than 2^30 partial results");
         uint8_t * ws = static_cast<uint8_t *>(workspace) + own;
         rows.fold.ml  = reinterpret_cast<float2 *>(ws);
-        rows.fold.acc = reinterpret_cast<float *>(ws + aligned(slots * kPrefixRows * sizeof(float2)));
+        rows.fold.acc = reinterpret_cast<float4 *>(ws + aligned(slots * kPrefixRows * sizeof(float2)));
         rows.fold.place = pl->dev + pl->place_at();
         rows.fold.of    = pl->dev + pl->of_at();
         rows.fold.len   = a->prefix_len;
@@ -659,23 +974,24 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
         p.rope  = reinterpret_cast<const float2 *>(a->own.rope_table);
         p.plan  = pl->dev; p.tiles = pl->dev + pl->tiles_at(); p.order = pl->dev + pl->order_at();
         p.len   = a->prefix_len;
-        p.ml = const_cast<float2 *>(rows.fold.ml); p.acc = const_cast<float *>(rows.fold.acc);
+        p.ml = const_cast<float2 *>(rows.fold.ml); p.acc = const_cast<float4 *>(rows.fold.acc);
         p.n_prefixes = pl->n_prefixes; p.n_kv_heads = HK; p.gqa = pl->gqa; p.layer = a->own.layer; p.max_len = pc->cfg.max_len;
         p.chunk = ch.chunk; p.max_chunks = ch.max_chunks;
         p.scale_log2 = a->own.scale * 1.4426950408889634f;
         p.q8_tiles = pc->k_data + (size_t) a->own.layer * pc->nb_layer;
         p.q8_nb_head = pc->nb_head; p.q8_nb_stream = pc->nb_stream;
         p.status = e->status_dev;
-        const auto     kernel = q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
-        const int      smem   = q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
-        const uint32_t bit    = 1u << (q8 ? 19 : 18);
+        const bool     tc     = !q8 && pl->full;
+        const auto     kernel = tc ? shared_rows_tc_kernel : q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
+        const int      smem   = tc ? kTcSmem : q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
+        const uint32_t bit    = 1u << (tc ? 21 : q8 ? 19 : 18);
         if (!(e->attr_mask & bit)) {
             VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             e->attr_mask |= bit;
         }
-        const unsigned grid = (unsigned) std::min<size_t>(slots, (size_t) e->sm_count);
-        launch_pdl(kernel, dim3(grid), dim3(kThreads), (size_t) smem, st, pc->map_k, pc->map_v, p);
-        rc = check_launch(e, q8 ? "shared_rows_kernel<q8_0>" : "shared_rows_kernel<f16>");
+        const unsigned grid = (unsigned) (tc ? slots : std::min<size_t>(slots, (size_t) e->sm_count));
+        launch_pdl(kernel, dim3(grid), dim3(tc ? kTcThreads : kThreads), (size_t) smem, st, pc->map_k, pc->map_v, p);
+        rc = check_launch(e, tc ? "shared_rows_tc_kernel" : q8 ? "shared_rows_kernel<q8_0>" : "shared_rows_kernel<f16>");
         if (rc != VOX_ATTN_OK) return rc;
     }
     return launch_decode_shared(e, &a->own, rows, workspace, own, st);

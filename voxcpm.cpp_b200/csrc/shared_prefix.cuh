@@ -16,7 +16,7 @@ constexpr int kBehindPrefix = 2;
 
 struct PrefixFold {
     const float2 *  ml;       // [slot][kPrefixRows] (max, sum); NULL: no shared rows in this call
-    const float *   acc;      // [slot][kPrefixRows][64]
+    const float4 *  acc;      // [slot][16][kPrefixRows]: output columns 4c .. 4c+3 of a row at [c][row]
     const int32_t * place;    // [stream] row tile * kPrefixRows + place in the tile, -1: the stream shares nothing
     const int32_t * of;       // [stream] its prefix
     const int32_t * len;      // [prefix] rows
@@ -48,16 +48,17 @@ __device__ __forceinline__ void prefix_fold(const PrefixFold & f, int stream, in
     if (place < 0) return;
     const int n    = prefix_chunks(max(0, min(f.len[f.of[stream]], f.max_len)), f.chunk, f.max_chunks);
     const int tile = place / kPrefixRows;
-    size_t    row  = ((size_t) (tile * n_kv_heads + kvh) * f.max_chunks) * kPrefixRows + (place - tile * kPrefixRows) * gqa + hh;
+    const int    row  = (place - tile * kPrefixRows) * gqa + hh;
+    const size_t slot = (size_t) (tile * n_kv_heads + kvh) * f.max_chunks;
     constexpr int W = 4;  // partials in flight: each is a round trip to L2
     for (int c = 0; c < n; c += W) {
         float2 ml[W];
         float4 o[W];
 #pragma unroll
         for (int u = 0; u < W; ++u) {
-            const size_t at = row + (size_t) min(c + u, n - 1) * kPrefixRows;
-            ml[u] = __ldcg(f.ml + at);
-            o[u]  = __ldcg(reinterpret_cast<const float4 *>(f.acc + at * kHeadDim + d0));
+            const size_t at = slot + min(c + u, n - 1);
+            ml[u] = __ldcg(f.ml + at * kPrefixRows + row);
+            o[u]  = __ldcg(f.acc + (at * 16 + (d0 >> 2)) * kPrefixRows + row);
         }
 #pragma unroll
         for (int u = 0; u < W; ++u) {
