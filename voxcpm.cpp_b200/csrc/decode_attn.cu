@@ -112,10 +112,9 @@ struct DecodeParams {
     const uint8_t * mask;
     size_t          mask_nb_head, mask_nb_stream;
     int             mask_ne2, mask_ne3;
-    // kShared kernels: the partial results of the rows that streams share (shared_prefix.cuh), folded into every result
-    // before it is written; the natural log-sum-exp of every row's softmax (NULL: not wanted)
-    PrefixFold      shared;
+    // kShared kernels: where the natural log-sum-exp of every row goes, and its (max, sum) in units of log2 (NULL: not wanted)
     float *         lse;
+    float2 *        ml;
 };
 
 __device__ __forceinline__ int clamp_len(const DecodeParams & p, int len) { return max(0, min(len, p.max_len)); }
@@ -319,6 +318,10 @@ template <bool Q8> struct Ring {
     static_assert(kStageBytes >= kConsumerWarps * kMaxGqa * kPartialStride * 4, "a stage must hold the warps' partials");
 };
 
+template <bool kSigned>
+__device__ __forceinline__ uint32_t byte_pair(uint32_t bytes, uint32_t selector) {
+    return kSigned ? s8_pair_to_half2(bytes, selector) : u8_pair_to_half2(bytes, selector);
+}
 // product of two packed pairs of halves, as bits
 __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
@@ -385,36 +388,29 @@ __device__ __forceinline__ bool mbar_wait_cluster_bounded(uint32_t bar, uint32_t
 
 __device__ __forceinline__ void fence_acq_rel_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
 
-// One head's result leaves: (max, sum, acc) of the stream's own rows for output columns d0 .. d0+3, 16 threads per head.
-// With kShared the partials of the rows that the stream shares are folded in first, in key order (their kernel runs just
-// before this one and may still be running: the dependency wait comes here, as late as it can).
+// One head's result leaves: (max, sum, acc) for output columns d0 .. d0+3, 16 threads per head.
 template <bool kShared>
-__device__ __forceinline__ void write_result(const DecodeParams & p, int stream, int kvh, int hh, int d0, float M, float L, float (&acc)[4]) {
-    const int head = kvh * p.gqa + hh;
+__device__ __forceinline__ void write_result(const DecodeParams & p, int stream, int kvh, int hh, int d0, float M, float L, const float (&acc)[4]) {
+    const size_t row = (size_t) stream * p.n_heads + kvh * p.gqa + hh;
     if constexpr (kShared) {
-        if (p.shared.ml != nullptr) {
-            pdl_wait();
-            pdl_launch_dependents();
-            prefix_fold(p.shared, stream, kvh, hh, p.n_kv_heads, p.gqa, d0, M, L, acc);
+        if (d0 == 0) {
+            if (p.lse != nullptr) p.lse[row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+            if (p.ml != nullptr) p.ml[row] = make_float2(M, L);
         }
-        if (p.lse != nullptr && d0 == 0) p.lse[(size_t) stream * p.n_heads + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
     }
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;  // nothing visible -> zeros, as the reference
-    *reinterpret_cast<float4 *>(p.dst + ((size_t) stream * p.n_heads + head) * kHeadDim + d0) =
-        make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<float4 *>(p.dst + row * kHeadDim + d0) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
 }
-// a stream without a row of its own: zeros, or what its shared rows give; by the consumer warps of a CTA
+// a stream without a row of its own: zeros; by the consumer warps of a CTA
 template <bool kShared>
 __device__ __forceinline__ void write_empty(const DecodeParams & p, int stream, int head0, int n_heads, int tid) {
+    float4 * out = reinterpret_cast<float4 *>(p.dst + ((size_t) stream * p.n_heads + head0) * kHeadDim);
+    for (int j = tid; j < n_heads * kHeadDim / 4; j += kConsumerWarps * 32) out[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (kShared) {
-        for (int j = tid; j < n_heads * 16; j += kConsumerWarps * 32) {
-            const int head = head0 + (j >> 4);
-            float     acc[4] = {0.f, 0.f, 0.f, 0.f};
-            write_result<true>(p, stream, head / p.gqa, head % p.gqa, (j & 15) * 4, -INFINITY, 0.0f, acc);
+        for (int j = tid; j < n_heads; j += kConsumerWarps * 32) {
+            if (p.lse != nullptr) p.lse[(size_t) stream * p.n_heads + head0 + j] = -INFINITY;
+            if (p.ml != nullptr) p.ml[(size_t) stream * p.n_heads + head0 + j] = make_float2(-INFINITY, 0.0f);
         }
-    } else {
-        float4 * out = reinterpret_cast<float4 *>(p.dst + ((size_t) stream * p.n_heads + head0) * kHeadDim);
-        for (int j = tid; j < n_heads * kHeadDim / 4; j += kConsumerWarps * 32) out[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
 }
 
@@ -472,8 +468,9 @@ __device__ __forceinline__ void fold_pairs(const DecodeParams & p, const int (*p
     for (int k = 0; k < NP; ++k) write_result<kShared>(p, pend[k0 + k][0], pend[k0 + k][1], hh, d0, M[k], L[k], acc[k]);
 }
 
-// kShared: the form behind vox_attn_decode_shared.  Results take in the partials of shared rows, the log-sum-exp can
-// be returned, and q8_0 weights keep 22 bits (value and remainder, as the f16 form's do) instead of 11.
+// kShared: the form behind vox_attn_decode_shared, whose results another kernel joins with those of the shared rows: the
+// (max, sum) of every row and its log-sum-exp can be returned, rows past a stream's length may hold anything, and q8_0
+// weights keep 22 bits (value and remainder, as the f16 form's do) instead of 11.
 template <bool Q8, bool kShared>
 __global__ void __launch_bounds__(kThreads, Ring<Q8>::ctas_per_sm(kShared))
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeParams p) {
@@ -573,7 +570,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         cut_note[0] = cut.aligned; cut_note[1] = cut.f0; cut_note[2] = cut.run; cut_note[3] = cut.b0; cut_note[4] = cut.b1;
         DECODE_TRACE(1);
     }
-    // more CTAs than runs: nothing to do (with shared rows every CTA takes a part of the streams that have no rows)
+    // more CTAs than runs: nothing to do (kShared: every CTA takes a part of the streams that have no rows)
     if (n_tiles == 0 && blockIdx.x != 0 && !(kShared && any_empty)) return;
     }
 
@@ -581,13 +578,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         // ------------------------------------------------------------------ producer
         // All lanes walk the run (the arriving row is converted by the whole warp); lane 0 issues the copies.
         bool waited = !p.early;
-        // Behind the kernel of the shared rows: that kernel has passed its own dependency wait before this one could
-        // start, so all that this warp reads is complete; only its partials are not, and write_result waits for them.
-        const bool behind_prefix = kShared && p.early == kBehindPrefix;
         int  issued = 0;
         for (int it = 0; it < n_tiles; ++it) {
             const bool append_here = p.k_new != nullptr && w.t == w.tiles - 1;  // the arriving row lies in the pair's last tile
-            if (!waited && !behind_prefix && (append_here || it >= p.early_tiles)) {  // the first tiles were requested while the previous kernel drained
+            if (!waited && (append_here || it >= p.early_tiles)) {  // the first tiles were requested while the previous kernel drained
                 pdl_wait();
                 pdl_launch_dependents();
                 waited = true;
@@ -670,7 +664,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 
     // ---------------------------------------------------------------------- consumers
     const int g = lane >> 2, t = lane & 3;
-    if (p.early && !(kShared && p.early == kBehindPrefix)) {  // Q is written by the kernel before this one
+    if (p.early) {  // Q is written by the kernel before this one
         pdl_wait();
         pdl_launch_dependents();
     }
@@ -764,7 +758,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                 for (int b = 0; b < 2; ++b) {
                     q_bias[b] += __shfl_xor_sync(0xffffffffu, q_bias[b], 1);
                     q_bias[b] += __shfl_xor_sync(0xffffffffu, q_bias[b], 2);
-                    q_bias[b] *= 128.0f * kTwoM24;
+                    q_bias[b] *= kShared ? 0.0f : 128.0f * kTwoM24;
                 }
             }
         }
@@ -832,10 +826,12 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                             sv[u][j][1] = sc[j][1] + sc[j][3];
                         }
                     } else {
+                        constexpr float kBytes = kShared ? 1.0f : kTwo24;
                         const uint32_t ksc = kb + 2 * R::kDataBytes;
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             // one accumulator per 32-value block; the hi rows start at minus the bias of the block
+                            // (kShared: the operands are the signed numbers themselves, see s8_pair_to_half2)
                             float     sc[2][4] = {{-q_bias[0], -q_bias[0], 0.f, 0.f}, {-q_bias[1], -q_bias[1], 0.f, 0.f}};
 #if defined(VOX_ATTN_DEVELOPER) && defined(VOX_ABL_NOK)
                             if (false)
@@ -843,13 +839,13 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 #pragma unroll
                             for (int b = 0; b < 2; ++b) {
                                 const uint2 raw = lds64(kb + ((k_off ^ (b << 5)) + 512 * j));
-                                mma_16816(sc[b], qa[2 * b], u8_pair_to_half2(raw.x, 0x4140), u8_pair_to_half2(raw.x, 0x4342));
-                                mma_16816(sc[b], qa[2 * b + 1], u8_pair_to_half2(raw.y, 0x4140), u8_pair_to_half2(raw.y, 0x4342));
+                                mma_16816(sc[b], qa[2 * b], byte_pair<kShared>(raw.x, 0x4140), byte_pair<kShared>(raw.x, 0x4342));
+                                mma_16816(sc[b], qa[2 * b + 1], byte_pair<kShared>(raw.y, 0x4140), byte_pair<kShared>(raw.y, 0x4342));
                             }
                             // scales of positions 8j+2t and 8j+2t+1, both blocks: four consecutive halves
                             const uint2 ds = lds64(ksc + s_off + 32 * j);
-                            sv[u][j][0] = ((sc[0][0] + sc[0][2]) * half_lo(ds.x) + (sc[1][0] + sc[1][2]) * half_hi(ds.x)) * kTwo24;
-                            sv[u][j][1] = ((sc[0][1] + sc[0][3]) * half_lo(ds.y) + (sc[1][1] + sc[1][3]) * half_hi(ds.y)) * kTwo24;
+                            sv[u][j][0] = ((sc[0][0] + sc[0][2]) * half_lo(ds.x) + (sc[1][0] + sc[1][2]) * half_hi(ds.x)) * kBytes;
+                            sv[u][j][1] = ((sc[0][1] + sc[0][3]) * half_lo(ds.y) + (sc[1][1] + sc[1][3]) * half_hi(ds.y)) * kBytes;
                         }
                     }
                 }
@@ -983,7 +979,6 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                                 for (int n = 0; n < 8; ++n) {
                                     o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f;
                                 }
-                                v_bias[0] *= f; v_bias[2] *= f;
                                 v_unit  = unit;
                                 v_limit = dm > 0.0f ? unit * 256.0f : 0.0f;
                             }
@@ -1004,16 +999,12 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                             }
 #pragma unroll
                             for (int b = 0; b < 2; ++b) {
-                                // the weights' sums, which the +128 of the V bytes multiplies, from a tile of ones
-                                float sums[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma_16816(sums, pb[b], 0x3c003c00u, 0x3c003c00u);
-                                v_bias[2 * b] += sums[0] + sums[2];
                                 uint32_t r0, r1, r2, r3;
                                 ldmatrix_x4_trans(vb + (v_off ^ (b << 5)), r0, r1, r2, r3);
-                                mma_16816(o[4 * b + 0], pb[b], u8_pair_to_half2(r0, 0x4240), u8_pair_to_half2(r1, 0x4240));
-                                mma_16816(o[4 * b + 1], pb[b], u8_pair_to_half2(r0, 0x4341), u8_pair_to_half2(r1, 0x4341));
-                                mma_16816(o[4 * b + 2], pb[b], u8_pair_to_half2(r2, 0x4240), u8_pair_to_half2(r3, 0x4240));
-                                mma_16816(o[4 * b + 3], pb[b], u8_pair_to_half2(r2, 0x4341), u8_pair_to_half2(r3, 0x4341));
+                                mma_16816(o[4 * b + 0], pb[b], s8_pair_to_half2(r0, 0x4240), s8_pair_to_half2(r1, 0x4240));
+                                mma_16816(o[4 * b + 1], pb[b], s8_pair_to_half2(r0, 0x4341), s8_pair_to_half2(r1, 0x4341));
+                                mma_16816(o[4 * b + 2], pb[b], s8_pair_to_half2(r2, 0x4240), s8_pair_to_half2(r3, 0x4240));
+                                mma_16816(o[4 * b + 3], pb[b], s8_pair_to_half2(r2, 0x4341), s8_pair_to_half2(r3, 0x4341));
                             }
                         } else {
 #pragma unroll
@@ -1068,8 +1059,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             for (int n = 0; n < 8; ++n) {
                 const float b = -128.0f * v_bias[n < 4 ? 0 : 2];
                 if constexpr (kShared) {
-                    o[n][0] = fmaf(o[n][0] + o[n][2], kTwo24, b) * (v_unit / 32.0f);
-                    o[n][1] = fmaf(o[n][1] + o[n][3], kTwo24, b) * (v_unit / 32.0f);
+                    o[n][0] = (o[n][0] + o[n][2]) * (v_unit / 32.0f);
+                    o[n][1] = (o[n][1] + o[n][3]) * (v_unit / 32.0f);
                 } else {
                     o[n][0] = fmaf(n < 4 ? o[n][0] : o[n][2], kTwo24, b);
                     o[n][1] = fmaf(n < 4 ? o[n][1] : o[n][3], kTwo24, b);
@@ -1245,7 +1236,8 @@ void decode_plan(const vox_engine * e, bool q8, int n_streams, int n_kv_heads, i
         if (tuned > 0) wave = std::min(tuned, fit);
         sms = std::min(sms, e->sm_count);
     }
-    const long long rmin = std::max(4LL, (tiles_bound + 15) / 16);
+    // beside shared rows streams of a few own rows are common: a CTA per pair rather than several pairs in a row
+    const long long rmin = std::max(shared ? std::min(4LL, tiles_bound) : 4LL, (tiles_bound + 15) / 16);
     const long long want = (pairs * tiles_bound + rmin - 1) / rmin;
     *run_min = (int) rmin;
     *grid    = (int) std::max(1LL, std::min<long long>(want, (long long) sms * wave));
@@ -1253,12 +1245,18 @@ void decode_plan(const vox_engine * e, bool q8, int n_streams, int n_kv_heads, i
 
 // Two partial slots per CTA of the largest grid either cache type would get (the caller of the size query
 // does not say which type, nor which device: the bound assumes kDecodeMaxSms SMs, and launches never use more).
-size_t decode_workspace_bytes(int n_streams, int n_heads, int n_kv_heads, int kv_bound) {
+static size_t partials_bytes(int n_streams, int n_heads, int n_kv_heads, int kv_bound, bool shared) {
     if (n_streams <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0) return 0;
     int g_f16, g_q8, rmin;
-    decode_plan(nullptr, false, n_streams, n_kv_heads, kv_bound, &g_f16, &rmin);
-    decode_plan(nullptr, true, n_streams, n_kv_heads, kv_bound, &g_q8, &rmin);
+    decode_plan(nullptr, false, n_streams, n_kv_heads, kv_bound, &g_f16, &rmin, shared);
+    decode_plan(nullptr, true, n_streams, n_kv_heads, kv_bound, &g_q8, &rmin, shared);
     return (size_t) 2 * std::max(g_f16, g_q8) * (n_heads / n_kv_heads) * kPartialStride * sizeof(float);
+}
+size_t decode_workspace_bytes(int n_streams, int n_heads, int n_kv_heads, int kv_bound) {
+    return partials_bytes(n_streams, n_heads, n_kv_heads, kv_bound, false);
+}
+size_t decode_shared_workspace_bytes(int n_streams, int n_heads, int n_kv_heads, int kv_bound) {
+    return partials_bytes(n_streams, n_heads, n_kv_heads, kv_bound, true);
 }
 
 // K/V described by tensor maps (f16: a cache layer, or caller tensors) or, for q8_0, by the start of the layer's tiles
@@ -1271,7 +1269,7 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
                   size_t q_nb_stream, float * dst, float scale, void * workspace, size_t workspace_bytes, int * counters,
                   cudaStream_t stream, const vox_kv_cache * append_to, const float * k_new, const float * v_new,
                   size_t new_nb_head, size_t new_nb_stream, bool early, const float * rope_table, const int32_t * order,
-                  const vox_tensor * mask, const SharedRows * rows) {
+                  const vox_tensor * mask, const OwnRows * rows) {
     const bool     shared = rows != nullptr;
     const auto     kernel = q8 ? (shared ? decode_kernel<true, true> : decode_kernel<true, false>)
                                : (shared ? decode_kernel<false, true> : decode_kernel<false, false>);
@@ -1279,6 +1277,7 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
     const uint32_t bit  = 1u << ((q8 ? 9 : 8) + (shared ? 16 : 0));
     if (!(e->attr_mask & bit)) {
         VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (shared) VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
         e->attr_mask |= bit;
     }
     VOX_REQUIRE(n_streams > 0 && n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= kMaxGqa,
@@ -1296,13 +1295,8 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
     p.status = e->status_dev;
     p.counters = counters;
     p.early = early ? 1 : 0;
-    p.shared = PrefixFold{};
-    p.lse    = nullptr;
-    if (shared) {
-        p.shared = rows->fold;
-        p.lse    = rows->lse;
-        if (rows->fold.ml != nullptr && pdl_enabled()) p.early = kBehindPrefix;
-    }
+    p.lse = shared ? rows->lse : nullptr;
+    p.ml  = shared ? rows->ml : nullptr;
     {
         const int depth = q8 ? Ring<true>::kStages : Ring<false>::kStages;
         const int tuned = e->decode_early_tiles;
@@ -1533,7 +1527,7 @@ int check_decode_args(const vox_engine * e, const vox_decode_args * a, const cha
 }
 
 int decode_checked(vox_engine * e, const vox_decode_args * a, void * workspace, size_t workspace_bytes, void * stream,
-                   const SharedRows * rows = nullptr) {
+                   const OwnRows * rows = nullptr) {
     const vox_kv_cache * c       = a->cache;
     const bool           appends = a->k_new != nullptr;
     int * counters = c->counters + (size_t) a->layer * c->cfg.n_streams * c->cfg.n_kv_heads;
@@ -1550,7 +1544,7 @@ int decode_checked(vox_engine * e, const vox_decode_args * a, void * workspace, 
 
 namespace vox {
 int check_decode(const vox_engine * e, const vox_decode_args * a, const char * who) { return check_decode_args(e, a, who); }
-int launch_decode_shared(vox_engine * e, const vox_decode_args * a, const SharedRows & rows, void * workspace, size_t workspace_bytes,
+int launch_decode_shared(vox_engine * e, const vox_decode_args * a, const OwnRows & rows, void * workspace, size_t workspace_bytes,
                          cudaStream_t stream) {
     return decode_checked(e, a, workspace, workspace_bytes, stream, &rows);
 }

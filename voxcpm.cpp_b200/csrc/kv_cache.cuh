@@ -101,6 +101,13 @@ __device__ __forceinline__ uint32_t keep_rows(int pos, int len) { return (pos < 
 // 32-value block, known when Q is loaded; V: the running sums of the weights).
 constexpr float kTwo24 = 16777216.0f, kTwoM24 = 1.0f / 16777216.0f;
 __device__ __forceinline__ uint32_t u8_pair_to_half2(uint32_t bytes, uint32_t selector) { return __byte_perm(bytes, 0u, selector); }
+// The same pairs as signed numbers q, for one instruction more: u under a byte 0x64 is the f16 number 1024 + u, and 1024 + 128
+// comes off exactly.  Where the +128 would be summed over many rows and taken out at the end, it costs the sum its last bits
+// (5e-6 of the output's RMS at 2000 rows against 5e-7).
+__device__ __forceinline__ uint32_t s8_pair_to_half2(uint32_t bytes, uint32_t selector) {
+    const __half2 r = __hsub2(as_half2(__byte_perm(bytes, 0x64646464u, selector)), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
 #endif
 
 }  // namespace vox

@@ -2,10 +2,21 @@
 //
 //   out[s] = softmax over (prefix rows of s, own rows of s) of scale * q[s].k, times v
 //
-// A stream's softmax splits into the part over its prefix and the part over its own rows; each part is a (max, sum,
-// unnormalised output) and two parts join as two chunks of split-KV decode do.  The own rows are the decode kernel's work
-// (decode_attn.cu), bound by HBM.  The prefix rows are this kernel's: the queries of all streams that share a prefix are
-// the rows of one matrix product against it, so the prefix leaves HBM once for all of them instead of once per stream.
+// A stream's softmax splits into the part over its own rows and the part over its prefix; each part is a (max, sum,
+// unnormalised output), and two parts join as two chunks of split-KV decode do.  The own rows are the decode kernel's work
+// (decode_attn.cu, bound by HBM): it runs first and leaves its result in dst with the (max, sum) of every row beside it.
+// The prefix rows are this file's: the queries of all streams that share a prefix are the rows of one matrix product
+// against it, so the prefix leaves HBM once for all of them instead of once per stream.  Its kernel starts as soon as the
+// decode kernel's CTAs have started, runs beside them (on small calls) or in the room they leave as they finish (on large
+// ones; decode CTAs end up to 20 us apart on 256 ragged streams), and waits for the decode kernel only to join the results.
+//
+// Streams are packed into row tiles of up to 128 rows (128 / gqa streams of one prefix, gqa rows each).  A (row tile, kv
+// head) is the work of one thread-block cluster of up to eight CTAs, which share out the prefix's 128-key tiles; their
+// partial results meet through distributed shared memory, every CTA joining a share of the rows.  Nothing goes through
+// global memory but the inputs and the result.
+// (Measured against it: the prefix kernel first, partials in global memory, folded by the decode kernel as it wrote every
+// result: 61.7 us for 256 streams under two prompts of 4096 rows and up to 2048 rows of their own, 16.9 us for 32 streams
+// under four of 700; the folds' round trips to L2 and the decode kernel's late start were a third of it.)
 #include "shared_prefix.cuh"
 #include "tcgen05.cuh"
 
@@ -16,28 +27,194 @@
 
 using namespace vox;
 
+namespace {
+constexpr int kRows = 128;       // rows of a row tile
+constexpr int kKeys = 128;       // keys of a tile
+constexpr int kMaxCluster = 8;
+}
+
 // The streams of a call, arranged by prefix.  Host copy of the arrangement and its device arrays (one allocation):
-//   [0] number of row tiles, then  tiles [max_tiles][4] = prefix, first entry of order, streams, 0;  order [n_streams];
-//   place [n_streams];  of [n_streams]
+//   tiles [max_tiles][2] = prefix, streams (0: not in use);  members [max_tiles][128 / gqa]: their streams
 struct vox_prefix_plan {
     vox_engine *         e = nullptr;
-    int                  n_streams = 0, n_prefixes = 0, gqa = 0, max_tiles = 0;
+    int                  n_streams = 0, n_prefixes = 0, gqa = 0, max_tiles = 0, n_tiles = 0;
     bool                 full = false;  // the row tiles are more than half full on average
-    std::vector<int32_t> host;
+    std::vector<int32_t> host, next;    // next: scratch of the arrangement
     int32_t *            dev = nullptr;
-    size_t tiles_at() const { return 4; }
-    size_t order_at() const { return 4 + (size_t) max_tiles * 4; }
-    size_t place_at() const { return order_at() + n_streams; }
-    size_t of_at() const { return place_at() + n_streams; }
-    size_t words() const { return of_at() + n_streams; }
+    int    per_tile() const { return kRows / gqa; }
+    size_t members_at() const { return (size_t) max_tiles * 2; }
+    size_t words() const { return members_at() + (size_t) max_tiles * per_tile(); }
 };
 
 namespace {
 
-constexpr int kWarps    = 8;                    // consumer warps
-constexpr int kThreads  = (kWarps + 1) * 32;
-constexpr int kKeys     = 128;                  // keys per ring stage
-constexpr int kMergeStride = 66;
+struct SharedParams {
+    const uint8_t * q;
+    size_t          q_nb_head, q_nb_stream;
+    const float2 *  rope;
+    const int2 *    tiles;
+    const int32_t * members;   // [tile][per_tile]
+    const int32_t * len;       // [prefix]
+    int             per_tile, n_kv_heads, n_heads, gqa, layer, max_len, cluster;
+    float           scale_log2;
+    const uint8_t * q8_tiles;
+    size_t          q8_nb_head, q8_nb_stream;
+    float *         dst;       // the own rows' results, and then the joined ones
+    const float2 *  ml;        // (max, sum) of the own rows
+    float *         lse;
+    int *           status;
+};
+
+// The work of a CTA.  What the plan says of it is read before any wait (the plan changes only in stream order and never by a
+// kernel); the length of the prefix is as old as the other inputs of the call, which were complete before the decode
+// kernel in front let this one start.
+struct Item {
+    int             prefix, rows, kvh, rank, key0, key1;
+    const int32_t * streams;
+};
+__device__ __forceinline__ Item load_item(const SharedParams & p) {
+    Item      w;
+    const int pair = (int) blockIdx.x / p.cluster, tile = pair / p.n_kv_heads;
+    const int2 t = p.tiles[tile];
+    w.kvh     = pair - tile * p.n_kv_heads;
+    w.rank    = (int) blockIdx.x - pair * p.cluster;
+    w.prefix  = t.x;
+    w.rows    = t.y * p.gqa;
+    w.streams = p.members + (size_t) tile * p.per_tile;
+    const int len = t.y > 0 ? max(0, min(p.len[t.x], p.max_len)) : 0, n = (len + kKeys - 1) / kKeys;
+    if (len == 0) w.rows = 0;
+    w.key0 = (w.rank * n / p.cluster) * kKeys;
+    w.key1 = min(len, ((w.rank + 1) * n / p.cluster) * kKeys);
+    return w;
+}
+
+// ---- the join.  A CTA's partial results lie in its shared memory: part[v][17] float4 (a row's 64 columns, padded by 16
+// bytes against bank conflicts) and ml[v], where v = group * stride + row and a row has a result from every one of
+// `groups` groups of warps.  256 threads take part; the others only arrive at the cluster barriers.
+constexpr int kPartPitch = 17;
+
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 peer_ld2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_ld4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// The weight of a part with maximum m against the maximum M over all parts; a part that saw nothing (-inf) has none.  (A row of
+// NaN has the maximum -inf and the sum NaN, which stays NaN.)
+__device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2_approx(m - M); }
+
+// Called by all threads of the CTA; `tid` < 256 do the work.  joined: one more ml array of kRows entries; rows_at: where the rows
+// of the tile lie in dst (stream * n_heads + head).
+__device__ __forceinline__ void join_and_write(const SharedParams & p, const Item & w, float4 * part, float2 * ml, float2 * joined, const int * rows_at,
+                                               int groups, int stride, bool ok, int tid) {
+    const bool mine = tid < 256;
+    const int  n = w.rows * 16, first = w.rank * 256 + tid, pace = p.cluster * 256;
+    constexpr int W = 2;  // a thread's rows in flight: a row at a time would wait for L2 once per row
+    float2 own_ml[W];
+    float4 own[W];
+    auto fetch_own = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+            const int i = min(i0 + u * pace, n - 1), at = rows_at[i >> 4];
+            own_ml[u] = __ldcg(p.ml + at);
+            own[u]    = __ldcg(reinterpret_cast<const float4 *>(p.dst + (size_t) at * kHeadDim) + (i & 15));
+        }
+    };
+    __syncwarp();
+    if (mine) {
+        named_bar_sync(1, 256);
+        if (!ok || w.key0 >= w.key1) {
+            for (int row = tid; row < kRows; row += 256) joined[row] = make_float2(-INFINITY, 0.0f);
+        } else if (groups == 1) {
+            if (tid < w.rows) joined[tid] = ml[tid];
+        } else {
+            if (tid < w.rows) {
+                float M = -INFINITY, L = 0.0f;
+                for (int g = 0; g < groups; ++g) M = fmaxf(M, ml[g * stride + tid].x);
+                for (int g = 0; g < groups; ++g) {
+                    const float2 x = ml[g * stride + tid];
+                    const float  f = part_weight(x.x, M);
+                    L = fmaf(x.y, f, L);
+                    ml[g * stride + tid].x = f;
+                }
+                joined[tid] = make_float2(M, L);
+            }
+            named_bar_sync(1, 256);
+            for (int i = tid; i < n; i += 256) {
+                const int row = i >> 4, c = i & 15;
+                float4    a = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int g = 0; g < groups; ++g) {
+                    const float4 x = part[(g * stride + row) * kPartPitch + c];
+                    const float  f = ml[g * stride + row].x;
+                    a = make_float4(fmaf(x.x, f, a.x), fmaf(x.y, f, a.y), fmaf(x.z, f, a.z), fmaf(x.w, f, a.w));
+                }
+                part[row * kPartPitch + c] = a;  // only this thread looks at column group c of this row
+            }
+        }
+    }
+    pdl_wait();  // the decode kernel's results
+    pdl_launch_dependents();
+    if (mine && first < n) fetch_own(first);
+    cluster_sync_all();
+    if (mine) {
+        const uint32_t part0 = smem_u32(part), joined0 = smem_u32(joined);
+        for (int i0 = first; i0 < n; i0 += W * pace) {
+            if (i0 != first) fetch_own(i0);
+#pragma unroll
+            for (int u = 0; u < W; ++u) {
+                const int i = i0 + u * pace, row = i >> 4, c = i & 15;
+                if (i >= n) break;
+                float2 m[kMaxCluster];
+                float4 x[kMaxCluster];
+                float  M = own_ml[u].x;
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r)
+                    if (r < p.cluster) {
+                        m[r] = peer_ld2(peer_addr(joined0 + row * 8, r));
+                        x[r] = peer_ld4(peer_addr(part0 + (row * kPartPitch + c) * 16, r));
+                    }
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r)
+                    if (r < p.cluster) M = fmaxf(M, m[r].x);
+                // the own rows' result is normalised: its sum is taken back in
+                const float f0 = part_weight(own_ml[u].x, M), s0 = f0 * own_ml[u].y;
+                float       L = s0;
+                float4      a = make_float4(own[u].x * s0, own[u].y * s0, own[u].z * s0, own[u].w * s0);
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r)
+                    if (r < p.cluster && !(m[r].x == -INFINITY && m[r].y == 0.0f)) {  // nothing was written for a part without keys
+                        const float f = part_weight(m[r].x, M);
+                        L = fmaf(m[r].y, f, L);
+                        a = make_float4(fmaf(x[r].x, f, a.x), fmaf(x[r].y, f, a.y), fmaf(x[r].z, f, a.z), fmaf(x[r].w, f, a.w));
+                    }
+                const int   at  = rows_at[row];
+                const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;  // NaN stays NaN
+                reinterpret_cast<float4 *>(p.dst + (size_t) at * kHeadDim)[c] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+                if (c == 0 && p.lse != nullptr) p.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+            }
+        }
+    }
+    cluster_sync_all();  // nobody leaves while its shared memory is read
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Row tiles of any fill and either cache type, on mma.sync: eight warps, arranged as row groups of 16 x key groups (a tile
+// of few rows has the 128 keys of a ring stage spread over the warps), and a warp that copies.
+constexpr int kWarps   = 8;
+constexpr int kThreads = (kWarps + 1) * 32;
 
 template <bool Q8> struct Ring {
     static constexpr int kStages     = Q8 ? 4 : 3;
@@ -45,43 +222,197 @@ template <bool Q8> struct Ring {
     static constexpr int kBoxTx      = Q8 ? kQ8TileBytes : kBoxBytes;
     static constexpr int kVOff       = Q8 ? kQ8VBytesOff : kKvTile * 128;
     static constexpr int kStageBytes = 2 * kBoxBytes;
-    static constexpr int kMergeBytes = (kWarps / 2) * 16 * kMergeStride * 4;
-    static constexpr int kSmemBytes  = kStages * kStageBytes + kMergeBytes + 1024;
+    static constexpr int kSmemBytes  = kStages * kStageBytes + 1024;
+    static_assert(kStages * kStageBytes >= kRows * kPartPitch * 16, "the partial results take the ring's memory");
+};
+constexpr float kShift = 10.0f;  // f16 caches: weights up to 2^10, so that the remainders of small ones are normal f16 numbers
+
+// what a warp holds of its 16 rows: row g of a lane is [0], row g + 8 is [1]
+struct Rows {
+    uint32_t qh[4][4], ql[4][4];
+    float    o[8][4], m[2], l[2];
+    float    v_unit, v_limit;  // q8_0: the unit of the weights that take V's scales in, and the scale at which it moves
 };
 
-struct SharedParams {
-    const uint8_t * q;
-    size_t          q_nb_head, q_nb_stream;
-    const float2 *  rope;
-    const int32_t * plan;      // [0] row tiles
-    const int32_t * tiles;     // [tile][4]
-    const int32_t * order;
-    const int32_t * len;       // [prefix]
-    float2 *        ml;
-    float4 *        acc;
-    int             n_prefixes, n_kv_heads, gqa, layer, max_len;
-    int             chunk, max_chunks;
-    float           scale_log2;
-    const uint8_t * q8_tiles;
-    size_t          q8_nb_head, q8_nb_stream;
-    int *           status;
-};
-
-struct Item {
-    int prefix, first, rows, kvh, key0, key1, slot;
-};
-// item i of the launch: chunk fastest, then kv head, then row tile; false where there is nothing to do
-__device__ __forceinline__ bool load_item(const SharedParams & p, int i, Item & w) {
-    const int chunk = i % p.max_chunks, pair = i / p.max_chunks;
-    w.kvh = pair % p.n_kv_heads;
-    const int4 t = *reinterpret_cast<const int4 *>(p.tiles + 4 * (size_t) (pair / p.n_kv_heads));
-    w.prefix = t.x; w.first = t.y; w.rows = t.z * p.gqa;
-    const int len = max(0, min(p.len[w.prefix], p.max_len));
-    if (chunk >= prefix_chunks(len, p.chunk, p.max_chunks)) return false;
-    w.key0 = chunk * p.chunk;
-    w.key1 = chunk == p.max_chunks - 1 ? len : min(len, w.key0 + p.chunk);
-    w.slot = i;
-    return true;
+// One step of the online softmax: NK * 16 keys from row r0 of the 64-row box at `box`; `pos` is the first one's place, `end`
+// where the keys end.
+template <bool Q8, int NK>
+__device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, int end, int lane) {
+    using R = Ring<Q8>;
+    const int g = lane >> 2, t = lane & 3;
+    float     sc[2 * NK][4];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        if constexpr (!Q8) {
+            const int k_row = r0 + 16 * k + ((lane >> 4) << 3) + (lane & 7), k_chk = (lane >> 3) & 1;
+            float     small[2][4];  // the remainders' products apart: the accumulator truncates at the size of what it holds
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[2 * k + j][e] = small[j][e] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4(box + k_row * 128 + (((2 * c + k_chk) ^ (k_row & 7)) << 4), b0, b1, b2, b3);
+                mma_16816(sc[2 * k], x.qh[c], b0, b1);
+                mma_16816(sc[2 * k + 1], x.qh[c], b2, b3);
+                mma_16816(small[0], x.ql[c], b0, b1);
+                mma_16816(small[1], x.ql[c], b2, b3);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[2 * k + j][e] += small[j][e];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float     part[2][4];  // one accumulator per 32-value block
+                const int row = r0 + 16 * k + 8 * j + g;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    part[b][0] = part[b][1] = part[b][2] = part[b][3] = 0.0f;
+                    const uint2 raw = lds64(box + row * 64 + (((2 * b + (t >> 1)) ^ ((row >> 1) & 3)) << 4) + ((t & 1) << 3));
+                    const uint32_t x0 = s8_pair_to_half2(raw.x, 0x4140), x1 = s8_pair_to_half2(raw.x, 0x4342);
+                    const uint32_t y0 = s8_pair_to_half2(raw.y, 0x4140), y1 = s8_pair_to_half2(raw.y, 0x4342);
+                    mma_16816(part[b], x.ql[2 * b], x0, x1);
+                    mma_16816(part[b], x.ql[2 * b + 1], y0, y1);
+                    mma_16816(part[b], x.qh[2 * b], x0, x1);
+                    mma_16816(part[b], x.qh[2 * b + 1], y0, y1);
+                }
+                const uint2 ds = lds64(box + kQ8KScaleOff + (r0 + 16 * k + 8 * j + 2 * t) * 4);
+                sc[2 * k + j][0] = part[0][0] * half_lo(ds.x) + part[1][0] * half_hi(ds.x);
+                sc[2 * k + j][1] = part[0][1] * half_lo(ds.y) + part[1][1] * half_hi(ds.y);
+                sc[2 * k + j][2] = part[0][2] * half_lo(ds.x) + part[1][2] * half_hi(ds.x);
+                sc[2 * k + j][3] = part[0][3] * half_lo(ds.y) + part[1][3] * half_hi(ds.y);
+            }
+        }
+    }
+    const bool edge = pos + 16 * NK > end;
+    if (edge) {
+#pragma unroll
+        for (int j = 0; j < 2 * NK; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (pos + 8 * j + 2 * t + (e & 1) >= end) sc[j][e] = -INFINITY;
+    }
+    float alpha[2], m_exp[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2 * NK; ++j) top = max3(top, sc[j][2 * h], sc[j][2 * h + 1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = fmaxf(x.m[h], top);
+        alpha[h] = m_new == -INFINITY ? 1.0f : ex2_approx(x.m[h] - m_new);
+        m_exp[h] = (m_new == -INFINITY ? 0.0f : m_new) - (Q8 ? 0.0f : kShift);
+        x.m[h]   = m_new;
+    }
+    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            x.o[n][0] *= alpha[0]; x.o[n][1] *= alpha[0]; x.o[n][2] *= alpha[1]; x.o[n][3] *= alpha[1];
+        }
+        x.l[0] *= alpha[0];
+        x.l[1] *= alpha[1];
+    }
+    if constexpr (Q8) {
+        // V's scales go into the weights; rows past the end count as zeros.  The products are taken in units of v_unit, a
+        // power of two that follows the largest scale seen: f16 parts of weights for values of any size neither overflow
+        // nor lose bits below 2^-14.
+        float dm = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2 * NK; ++j) {
+            const uint2   ds  = lds64(box + kQ8VScaleOff + (r0 + 8 * j + 2 * t) * 4);
+            const __half2 lo = __habs2(as_half2(ds.x)), hi = __habs2(as_half2(ds.y));
+            if (pos + 8 * j + 2 * t < end) dm = fmaxf(dm, fmaxf(__low2float(lo), __high2float(lo)));
+            if (pos + 8 * j + 2 * t + 1 < end) dm = fmaxf(dm, fmaxf(__low2float(hi), __high2float(hi)));
+        }
+        if (__any_sync(0xffffffffu, dm > x.v_limit)) {
+            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 1));
+            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 2));
+            const float unit = dm > 0.0f ? __uint_as_float(__float_as_uint(dm) & 0x7f800000u) : kTwoM24;
+            const float f    = x.v_unit / unit;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                x.o[n][0] *= f; x.o[n][1] *= f; x.o[n][2] *= f; x.o[n][3] *= f;
+            }
+            x.v_unit  = unit;
+            x.v_limit = dm > 0.0f ? unit * 256.0f : 0.0f;
+        }
+    }
+    const float to_units = Q8 ? 32.0f / x.v_unit : 1.0f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        float pr[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pr[j][e] = ex2_approx(sc[2 * k + j][e] - m_exp[e >> 1]);
+        const int      v_row = r0 + 16 * k + (((lane >> 3) & 1) << 3) + (lane & 7), v_chk = lane >> 4, pos_k = pos + 16 * k + 2 * t;
+        const uint32_t vb = box + R::kVOff;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x.l[h] += (pr[0][2 * h] + pr[0][2 * h + 1]) + (pr[1][2 * h] + pr[1][2 * h + 1]);
+        if constexpr (!Q8) {
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float h0, l0, h1, l1;
+                    split_hi_lo(pr[j][2 * h], h0, l0);
+                    split_hi_lo(pr[j][2 * h + 1], h1, l1);
+                    ph[2 * j + h] = pack_half2(h0, h1);
+                    pl[2 * j + h] = pack_half2(l0, l1);
+                }
+#pragma unroll
+            for (int n2 = 0; n2 < 4; ++n2) {
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4_trans(vb + v_row * 128 + (((2 * n2 + v_chk) ^ (v_row & 7)) << 4), b0, b1, b2, b3);
+                if (edge) {  // rows past the end may hold anything: zero times a NaN is none
+                    const uint32_t keep0 = keep_rows(pos_k, end), keep1 = keep_rows(pos_k + 8, end);
+                    b0 &= keep0; b1 &= keep1; b2 &= keep0; b3 &= keep1;
+                }
+                mma_16816(x.o[2 * n2], ph, b0, b1);
+                mma_16816(x.o[2 * n2 + 1], ph, b2, b3);
+                mma_16816(x.o[2 * n2], pl, b0, b1);
+                mma_16816(x.o[2 * n2 + 1], pl, b2, b3);
+            }
+        } else {
+            uint2 ds[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                ds[j] = lds64(box + kQ8VScaleOff + (r0 + 16 * k + 8 * j + 2 * t) * 4);
+                if (pos_k + 8 * j >= end) ds[j].x = 0u;
+                if (pos_k + 8 * j + 1 >= end) ds[j].y = 0u;
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float s0 = to_units * (b ? half_hi(ds[j].x) : half_lo(ds[j].x)), s1 = to_units * (b ? half_hi(ds[j].y) : half_lo(ds[j].y));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float h0, l0, h1, l1;
+                        split_hi_lo(pr[j][2 * h] * s0, h0, l0);
+                        split_hi_lo(pr[j][2 * h + 1] * s1, h1, l1);
+                        ph[2 * j + h] = pack_half2(h0, h1);
+                        pl[2 * j + h] = pack_half2(l0, l1);
+                    }
+                }
+                uint32_t r[4];
+                ldmatrix_x4_trans(vb + v_row * 64 + (((v_chk + 2 * b) ^ ((v_row >> 1) & 3)) << 4), r[0], r[1], r[2], r[3]);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {  // chunk n / 2 of 16 columns, even or odd ones
+                    const uint32_t sel = n & 1 ? 0x4341 : 0x4240;
+                    const uint32_t b0 = s8_pair_to_half2(r[2 * (n >> 1)], sel), b1 = s8_pair_to_half2(r[2 * (n >> 1) + 1], sel);
+                    mma_16816(x.o[4 * b + n], ph, b0, b1);
+                    mma_16816(x.o[4 * b + n], pl, b0, b1);
+                }
+            }
+        }
+    }
 }
 
 template <bool Q8>
@@ -91,10 +422,17 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * R::kStages];
     __shared__ int      abort_flag;
+    __shared__ float2   ml[kRows], joined[kRows];
+    __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    float *        merge     = reinterpret_cast<float *>(smem_raw + (smem_base - smem_u32(smem_raw)) + R::kStages * R::kStageBytes);
+    float4 * const part      = reinterpret_cast<float4 *>(smem_raw + (smem_base - smem_u32(smem_raw)));
     const int      tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[R::kStages]);
+    const Item     w = load_item(p);
+    if (w.rows == 0) {  // the same for the whole cluster
+        pdl_wait();
+        return;
+    }
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < R::kStages; ++s) {
@@ -103,29 +441,26 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         fence_mbar_init();
     }
+    if (tid < w.rows) rows_at[tid] = w.streams[tid / p.gqa] * p.n_heads + w.kvh * p.gqa + tid % p.gqa;
     __syncthreads();
-    // The decode kernel behind this one relies on this order: its CTAs start once every CTA here has passed the wait.
-    pdl_wait();
-    pdl_launch_dependents();
-    const int n_items = p.plan[0] * p.n_kv_heads * p.max_chunks;
+    const int n_tiles = (w.key1 - w.key0 + kKeys - 1) / kKeys;
+    bool      ok = true;
+    // Warps of a row tile: groups of 16 rows, and as many key groups as that leaves
+    const int groups = (w.rows + 15) >> 4;
+    const int rg     = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
+    const int kg = kWarps / rg;
 
     if (warp == kWarps) {
-        // ------------------------------------------------------------------ producer: one lane
-        if (lane != 0) return;
-        int  it = 0;
-        bool good = true;
-        for (int i = blockIdx.x; i < n_items && good; i += gridDim.x) {
-            Item w;
-            if (!load_item(p, i, w)) continue;
-            for (int key = w.key0; key < w.key1 && good; key += kKeys, ++it) {
-                const int s = it % R::kStages;
+        // ------------------------------------------------------------------ copies: one lane
+        if (lane == 0) {
+            int it = 0;
+            for (; it < n_tiles; ++it) {
+                const int s = it % R::kStages, key = w.key0 + it * kKeys;
                 if (it >= R::kStages && !mbar_wait_bounded(empty0 + 8 * s, ((it / R::kStages) - 1) & 1)) {
                     atomicOr(p.status, kStatusTimeout);
                     atomicExch(&abort_flag, 1);
-                    good = false;
                 }
-                if (good && *reinterpret_cast<volatile int *>(&abort_flag)) good = false;
-                if (!good) break;
+                if (*reinterpret_cast<volatile int *>(&abort_flag)) break;
                 const int      boxes = w.key1 - key > kKvTile ? 2 : 1;
                 const uint32_t bar   = full0 + 8 * s;
                 mbar_expect_tx(bar, boxes * R::kBoxTx);
@@ -143,42 +478,32 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                     }
                 }
             }
+            if (*reinterpret_cast<volatile int *>(&abort_flag))  // copies already issued land before the CTA retires
+                for (int i = max(0, it - R::kStages); i < it; ++i) mbar_wait_bounded(full0 + 8 * (i % R::kStages), (i / R::kStages) & 1);
         }
-        if (*reinterpret_cast<volatile int *>(&abort_flag))  // copies already issued land before the CTA retires
-            for (int i = max(0, it - R::kStages); i < it; ++i) mbar_wait_bounded(full0 + 8 * (i % R::kStages), (i / R::kStages) & 1);
-        return;
-    }
-
-    // ---------------------------------------------------------------------- consumers
-    const int g = lane >> 2, t = lane & 3;
-    int       it = 0;
-    for (int i = blockIdx.x; i < n_items; i += gridDim.x) {
-        Item w;
-        if (!load_item(p, i, w)) continue;
-        // Warps are arranged as row groups of 16 x key groups: a tile of few rows has its keys spread over the warps.
-        const int groups = (w.rows + 15) >> 4;
-        const int rg     = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
-        const int kg = kWarps / rg, wr = warp % rg, wk = warp / rg, span = kKeys / kg;
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------------ consumers
+        const int  g = lane >> 2, t = lane & 3;
+        const int  wr = warp % rg, wk = warp / rg, span = kKeys / kg;
         const bool busy = wr < groups;
-
-        // Q: rows g and g + 8 of this warp's 16, as hi + lo (the order of the head dimensions as in the decode kernel)
-        uint32_t qh[4][4], ql[4][4];
-        float    q_bias[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        Rows       x;
+        // Q: rows g and g + 8 of this warp's 16, as value + remainder (the order of the head dimensions as in the decode kernel)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int  row  = 16 * wr + g + 8 * h;
             const bool live = row < w.rows;
             const int  at   = live ? row : 0;
-            const int  stream = p.order[w.first + at / p.gqa], head = w.kvh * p.gqa + at % p.gqa;
+            const int  stream = rows_at[at] / p.n_heads, head = rows_at[at] % p.n_heads;
             const float * qrow = reinterpret_cast<const float *>(p.q + (size_t) stream * p.q_nb_stream + (size_t) head * p.q_nb_head);
             float xs[4][4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int d0 = Q8 ? 32 * (c >> 1) + 8 * t + 4 * (c & 1) : 16 * c + 2 * t;
                 const int d1 = Q8 ? d0 + 2 : d0 + 8;
-                const float2 x = *reinterpret_cast<const float2 *>(qrow + d0);
-                const float2 y = *reinterpret_cast<const float2 *>(qrow + d1);
-                xs[c][0] = x.x; xs[c][1] = x.y; xs[c][2] = y.x; xs[c][3] = y.y;
+                const float2 a = *reinterpret_cast<const float2 *>(qrow + d0);
+                const float2 b = *reinterpret_cast<const float2 *>(qrow + d1);
+                xs[c][0] = a.x; xs[c][1] = a.y; xs[c][2] = b.x; xs[c][3] = b.y;
             }
             if (p.rope != nullptr) {
                 const float2 * tb = p.rope + (size_t) stream * (kHeadDim / 2);
@@ -200,302 +525,88 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 float hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) split_hi_lo(live ? xs[c][e] * p.scale_log2 : 0.0f, hi[e], lo[e]);
-                qh[c][h]     = pack_half2(hi[0], hi[1]);
-                qh[c][h + 2] = pack_half2(hi[2], hi[3]);
-                ql[c][h]     = pack_half2(lo[0], lo[1]);
-                ql[c][h + 2] = pack_half2(lo[2], lo[3]);
-                if constexpr (Q8) q_bias[h][c >> 1] += ((hi[0] + lo[0]) + (hi[1] + lo[1])) + ((hi[2] + lo[2]) + (hi[3] + lo[3]));
-            }
-            if constexpr (Q8) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    q_bias[h][b] += __shfl_xor_sync(0xffffffffu, q_bias[h][b], 1);
-                    q_bias[h][b] += __shfl_xor_sync(0xffffffffu, q_bias[h][b], 2);
-                    q_bias[h][b] *= 128.0f * kTwoM24;
-                }
+                x.qh[c][h]     = pack_half2(hi[0], hi[1]);
+                x.qh[c][h + 2] = pack_half2(hi[2], hi[3]);
+                x.ql[c][h]     = pack_half2(lo[0], lo[1]);
+                x.ql[c][h + 2] = pack_half2(lo[2], lo[3]);
             }
         }
-
-        float o[8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        float v_bias[2][2] = {{0.f, 0.f}, {0.f, 0.f}}, v_unit = 1.0f, v_limit = -1.0f;
 #pragma unroll
-        for (int n = 0; n < 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-        bool ok = true;
-        for (int key = w.key0; key < w.key1; key += kKeys, ++it) {
-            const int s = it % R::kStages;
+        for (int n = 0; n < 8; ++n) x.o[n][0] = x.o[n][1] = x.o[n][2] = x.o[n][3] = 0.0f;
+        x.m[0] = x.m[1] = -INFINITY;
+        x.l[0] = x.l[1] = 0.0f;
+        x.v_unit = 1.0f;
+        x.v_limit = -1.0f;
+        for (int it = 0; it < n_tiles; ++it) {
+            const int s = it % R::kStages, key = w.key0 + it * kKeys;
             if (!mbar_wait_bounded(full0 + 8 * s, (it / R::kStages) & 1)) {
                 *reinterpret_cast<volatile int *>(&abort_flag) = 1;
                 ok = false;
                 break;
             }
             if (busy) {
-                for (int k0 = wk * span; k0 < (wk + 1) * span && key + k0 < w.key1; k0 += 16) {
-                    const uint32_t box = smem_base + s * R::kStageBytes + (k0 >> 6) * R::kBoxBytes;
-                    const int      r0  = k0 & 63, pos0 = key + k0;
-                    const bool     edge = pos0 + 16 > w.key1;
-                    float          sc[2][4];
-                    if constexpr (!Q8) {
-                        const int k_row = r0 + ((lane >> 4) << 3) + (lane & 7), k_chk = (lane >> 3) & 1;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t b0, b1, b2, b3;
-                            ldmatrix_x4(box + k_row * 128 + (((2 * c + k_chk) ^ (k_row & 7)) << 4), b0, b1, b2, b3);
-                            mma_16816(sc[0], qh[c], b0, b1);
-                            mma_16816(sc[1], qh[c], b2, b3);
-                            mma_16816(sc[0], ql[c], b0, b1);
-                            mma_16816(sc[1], ql[c], b2, b3);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            float part[2][4];
-                            const int row = r0 + 8 * j + g;
-#pragma unroll
-                            for (int b = 0; b < 2; ++b) {
-                                part[b][0] = part[b][1] = -q_bias[0][b];
-                                part[b][2] = part[b][3] = -q_bias[1][b];
-                                const uint2 raw = lds64(box + row * 64 + (((2 * b + (t >> 1)) ^ ((row >> 1) & 3)) << 4) + ((t & 1) << 3));
-                                const uint32_t x0 = u8_pair_to_half2(raw.x, 0x4140), x1 = u8_pair_to_half2(raw.x, 0x4342);
-                                const uint32_t y0 = u8_pair_to_half2(raw.y, 0x4140), y1 = u8_pair_to_half2(raw.y, 0x4342);
-                                mma_16816(part[b], qh[2 * b], x0, x1);
-                                mma_16816(part[b], qh[2 * b + 1], y0, y1);
-                                mma_16816(part[b], ql[2 * b], x0, x1);
-                                mma_16816(part[b], ql[2 * b + 1], y0, y1);
-                            }
-                            const uint2 ds = lds64(box + kQ8KScaleOff + (r0 + 8 * j + 2 * t) * 4);
-                            sc[j][0] = (part[0][0] * half_lo(ds.x) + part[1][0] * half_hi(ds.x)) * kTwo24;
-                            sc[j][1] = (part[0][1] * half_lo(ds.y) + part[1][1] * half_hi(ds.y)) * kTwo24;
-                            sc[j][2] = (part[0][2] * half_lo(ds.x) + part[1][2] * half_hi(ds.x)) * kTwo24;
-                            sc[j][3] = (part[0][3] * half_lo(ds.y) + part[1][3] * half_hi(ds.y)) * kTwo24;
-                        }
-                    }
-                    if (edge) {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (pos0 + 8 * j + 2 * t + (e & 1) >= w.key1) sc[j][e] = -INFINITY;
-                    }
-                    float alpha[2], m_exp[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float top = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        const float m_new = fmaxf(m[h], top);
-                        alpha[h] = m_new == -INFINITY ? 1.0f : ex2_approx(m[h] - m_new);
-                        m_exp[h] = (m_new == -INFINITY ? 0.0f : m_new) - (Q8 ? 0.0f : 10.0f);
-                        m[h]     = m_new;
-                    }
-                    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            o[n][0] *= alpha[0]; o[n][1] *= alpha[0]; o[n][2] *= alpha[1]; o[n][3] *= alpha[1];
-                        }
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            l[h] *= alpha[h];
-                            v_bias[h][0] *= alpha[h]; v_bias[h][1] *= alpha[h];
-                        }
-                    }
-                    float pr[2][4];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) pr[j][e] = ex2_approx(sc[j][e] - m_exp[e >> 1]);
-                    const int v_row = r0 + (((lane >> 3) & 1) << 3) + (lane & 7), v_chk = lane >> 4;
-                    const uint32_t vb = box + R::kVOff;
-                    if constexpr (!Q8) {
-                        uint32_t ph[4], pl[4];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                float h0, l0, h1, l1;
-                                split_hi_lo(pr[j][2 * h], h0, l0);
-                                split_hi_lo(pr[j][2 * h + 1], h1, l1);
-                                ph[2 * j + h] = pack_half2(h0, h1);
-                                pl[2 * j + h] = pack_half2(l0, l1);
-                                l[h] += (h0 + l0) + (h1 + l1);
-                            }
-#pragma unroll
-                        for (int n2 = 0; n2 < 4; ++n2) {
-                            uint32_t b0, b1, b2, b3;
-                            ldmatrix_x4_trans(vb + v_row * 128 + (((2 * n2 + v_chk) ^ (v_row & 7)) << 4), b0, b1, b2, b3);
-                            if (edge) {  // rows past the length may hold anything: zero times a NaN is none
-                                const uint32_t keep0 = keep_rows(pos0 + 2 * t, w.key1), keep1 = keep_rows(pos0 + 8 + 2 * t, w.key1);
-                                b0 &= keep0; b1 &= keep1; b2 &= keep0; b3 &= keep1;
-                            }
-                            mma_16816(o[2 * n2], ph, b0, b1);
-                            mma_16816(o[2 * n2 + 1], ph, b2, b3);
-                            mma_16816(o[2 * n2], pl, b0, b1);
-                            mma_16816(o[2 * n2 + 1], pl, b2, b3);
-                        }
-                    } else {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            l[h] += (pr[0][2 * h] + pr[0][2 * h + 1]) + (pr[1][2 * h] + pr[1][2 * h + 1]);
-                        uint2 ds[2];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            ds[j] = lds64(box + kQ8VScaleOff + (r0 + 8 * j + 2 * t) * 4);
-                            if (pos0 + 8 * j + 2 * t >= w.key1) ds[j].x = 0u;
-                            if (pos0 + 8 * j + 2 * t + 1 >= w.key1) ds[j].y = 0u;
-                        }
-                        // products in units of v_unit, as in the decode kernel
-                        const __half2 big = __hmax2(__hmax2(__habs2(as_half2(ds[0].x)), __habs2(as_half2(ds[0].y))),
-                                                    __hmax2(__habs2(as_half2(ds[1].x)), __habs2(as_half2(ds[1].y))));
-                        float dm = fmaxf(__low2float(big), __high2float(big));
-                        if (__any_sync(0xffffffffu, dm > v_limit)) {
-                            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 1));
-                            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 2));
-                            const float unit = dm > 0.0f ? __uint_as_float(__float_as_uint(dm) & 0x7f800000u) : kTwoM24;
-                            const float f    = v_unit / unit;
-#pragma unroll
-                            for (int n = 0; n < 8; ++n) {
-                                o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f;
-                            }
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) { v_bias[h][0] *= f; v_bias[h][1] *= f; }
-                            v_unit  = unit;
-                            v_limit = dm > 0.0f ? unit * 256.0f : 0.0f;
-                        }
-                        const float to_units = 32.0f / v_unit;
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            uint32_t ph[4], pl[4];
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const float s0 = to_units * (b ? half_hi(ds[j].x) : half_lo(ds[j].x)), s1 = to_units * (b ? half_hi(ds[j].y) : half_lo(ds[j].y));
-#pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    float h0, l0, h1, l1;
-                                    split_hi_lo(pr[j][2 * h] * s0, h0, l0);
-                                    split_hi_lo(pr[j][2 * h + 1] * s1, h1, l1);
-                                    ph[2 * j + h] = pack_half2(h0, h1);
-                                    pl[2 * j + h] = pack_half2(l0, l1);
-                                }
-                            }
-                            float sums[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_16816(sums, ph, 0x3c003c00u, 0x3c003c00u);
-                            mma_16816(sums, pl, 0x3c003c00u, 0x3c003c00u);
-                            v_bias[0][b] += sums[0];
-                            v_bias[1][b] += sums[2];
-                            uint32_t r[4];
-                            ldmatrix_x4_trans(vb + v_row * 64 + (((v_chk + 2 * b) ^ ((v_row >> 1) & 3)) << 4), r[0], r[1], r[2], r[3]);
-#pragma unroll
-                            for (int n = 0; n < 4; ++n) {  // chunk n / 2 of 16 columns, even or odd ones
-                                const uint32_t sel = n & 1 ? 0x4341 : 0x4240;
-                                const uint32_t b0 = u8_pair_to_half2(r[2 * (n >> 1)], sel), b1 = u8_pair_to_half2(r[2 * (n >> 1) + 1], sel);
-                                mma_16816(o[4 * b + n], ph, b0, b1);
-                                mma_16816(o[4 * b + n], pl, b0, b1);
-                            }
-                        }
-                    }
+                const int k0 = wk * span;
+                const uint32_t box = smem_base + s * R::kStageBytes + (k0 >> 6) * R::kBoxBytes;
+                if (kg == 8) {
+                    if (key + k0 < w.key1) step<Q8, 1>(x, box, k0 & 63, key + k0, w.key1, lane);
+                } else {
+#pragma unroll 1
+                    for (int b = 0; b < span && key + k0 + b < w.key1; b += 32)
+                        step<Q8, 2>(x, box + (((k0 & 63) + b) >> 6) * R::kBoxBytes, (k0 + b) & 63, key + k0 + b, w.key1, lane);
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty0 + 8 * s);
         }
         if (*reinterpret_cast<volatile int *>(&abort_flag)) ok = false;
-        if (!named_bar_all(1, kWarps * 32, ok)) {
-            if (tid == 0) {
-                *reinterpret_cast<volatile int *>(&abort_flag) = 1;
-                atomicOr(p.status, kStatusTimeout);
-            }
-            return;
-        }
-
-        // ---- the item's result: warps of one row group and several key groups are merged, half of them at a time
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if (!Q8) m[h] -= 10.0f;
-        }
-        if constexpr (Q8) {
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[n][e] = fmaf(o[n][e], kTwo24, -128.0f * v_bias[e >> 1][n >> 2]) * (v_unit / 32.0f);
-        }
-        for (int half = kg >> 1; half >= 1; half >>= 1) {
-            float * mine = merge + ((size_t) ((wk - half) * rg + wr) * 16) * kMergeStride;
-            if (wk >= half && wk < 2 * half) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float * row = mine + (g + 8 * h) * kMergeStride;
-                    if (t == 0) *reinterpret_cast<float2 *>(row) = make_float2(m[h], l[h]);
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) *reinterpret_cast<float2 *>(row + 2 + 8 * n + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-                }
-            }
-            named_bar_sync(1, kWarps * 32);
-            if (wk < half) {
-                const float * theirs = merge + ((size_t) (wk * rg + wr) * 16) * kMergeStride;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float * row = theirs + (g + 8 * h) * kMergeStride;
-                    const float2  ml  = *reinterpret_cast<const float2 *>(row);
-                    const float   mn  = fmaxf(m[h], ml.x);
-                    const float   fa = m[h] == -INFINITY ? 0.0f : exp2f(m[h] - mn), fb = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - mn);
-                    m[h] = mn;
-                    l[h] = l[h] * fa + ml.y * fb;
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        const float2 x = *reinterpret_cast<const float2 *>(row + 2 + 8 * n + 2 * t);
-                        o[n][2 * h]     = o[n][2 * h] * fa + x.x * fb;
-                        o[n][2 * h + 1] = o[n][2 * h + 1] * fa + x.y * fb;
-                    }
-                }
-            }
-            named_bar_sync(1, kWarps * 32);
-        }
-        if (wk == 0 && busy) {
+        if (!ok && lane == 0) atomicOr(p.status, kStatusTimeout);
+        ok = named_bar_all(1, kWarps * 32, ok);  // and the ring is no longer read
+        if (ok) {
+            const int v0 = (wk * rg + wr) * 16;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = 16 * wr + g + 8 * h;
-                if (row >= w.rows) continue;
-                const size_t at = (size_t) w.slot * kPrefixRows + row;
-                if (t == 0) p.ml[at] = make_float2(m[h], l[h]);
-                float * out = reinterpret_cast<float *>(p.acc + (size_t) w.slot * 16 * kPrefixRows + row);
-                auto    col = [](int d) { return (size_t) (d >> 2) * kPrefixRows * 4 + (d & 3); };  // place of output column d
+                float l = x.l[h];
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                const int row = v0 + g + 8 * h;
+                if (t == 0) ml[row] = make_float2(x.m[h] - (Q8 ? 0.0f : kShift), l);
+                float * out = reinterpret_cast<float *>(part + row * kPartPitch);
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
                     if constexpr (Q8) {  // tile n: chunk n / 2, this lane 16 (n / 2) + 4t + (n % 2) and two further
                         const int d = 16 * (n >> 1) + 4 * t + (n & 1);
-                        out[col(d)]     = o[n][2 * h];
-                        out[col(d + 2)] = o[n][2 * h + 1];
+                        out[d]     = x.o[n][2 * h] * (x.v_unit / 32.0f);
+                        out[d + 2] = x.o[n][2 * h + 1] * (x.v_unit / 32.0f);
                     } else {
-                        *reinterpret_cast<float2 *>(out + col(8 * n + 2 * t)) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                        *reinterpret_cast<float2 *>(out + 8 * n + 2 * t) = make_float2(x.o[n][2 * h], x.o[n][2 * h + 1]);
                     }
                 }
             }
         }
     }
+    join_and_write(p, w, part, ml, joined, rows_at, kg, 16 * rg, ok, tid);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Full row tiles on the 5th-generation tensor cores (f16 caches).
 //
-// One CTA takes one (row tile, kv head, chunk of keys).  Q (scaled by scale * log2 e) lies in shared memory as two f16 tiles,
+// Q (scaled by scale * log2 e) lies in shared memory as two f16 tiles,
 // value and remainder; scores S = Q_lo.K + Q_hi.K (the small part first: the accumulator truncates) come 64 keys at a time
 // into one of six score buffers in TMEM.  Two groups of four softmax warps take them in turn, a thread per row: 64 scores
 // out of TMEM, weights 2^(S - ref) back over them as two packed f16 tiles (value and remainder, 22 bits), from where the
 // tensor core takes them as the A operand of P.V.  Every group has an output accumulator and a reference maximum of its
-// own, so the groups never wait for one another; they are joined once, at the end.  The reference of a row is raised only
+// own, so the groups never wait for one another; they are joined at the end, as the CTAs are.  The reference of a row is raised only
 // when a maximum exceeds it by 2^8 (its accumulator is then rescaled in TMEM).
 //   warps 0-3, 4-7  softmax groups    warp 8  K/V copies    warp 9  issues S = Q.K    warp 10  issues O += P.V
 constexpr int kTcThreads = 11 * 32;
-constexpr int kTcStages  = 4;
+constexpr int kTcStages  = 3;                     // leaves room on the SM for a CTA of the decode kernel
 constexpr int kSub       = 64;                    // keys of a score tile
 constexpr int kSBufs     = 6;
 constexpr int kTcOCol    = kSBufs * kSub;         // two accumulators of 64 columns behind the score buffers
-constexpr int kQTile     = kPrefixRows * 128;
+constexpr int kQTile     = kRows * 128;
 constexpr int kTcStage   = 2 * kKeys * 128;       // 128 rows of K, 128 rows of V
 constexpr int kTcSmem    = 2 * kQTile + kTcStages * kTcStage + 1024;
+static_assert(kTcStages * kTcStage >= 2 * kRows * kPartPitch * 16, "the groups' partial results take the ring's memory");
 constexpr float kTcShift = 6.0f;                  // weights up to 2^(8 + 6): their remainders stay normal f16 numbers
 
 // multiply this thread's accumulator row by f; rare, kept out of line so that its registers do not weigh on the loop
@@ -518,13 +629,19 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int      abort_flag;
-    __shared__ float2   other_ml[kPrefixRows];
+    __shared__ float2   ml[2 * kRows], joined[kRows];
+    __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t sQ = smem_base, sKV = sQ + 2 * kQTile;
     const int      tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = full0 + 8 * kTcStages, bS0 = empty0 + 8 * kTcStages, bP0 = bS0 + 8 * kSBufs,
                    bF0 = bP0 + 8 * kSBufs, bO = bF0 + 8 * kSBufs;
+    const Item     w = load_item(p);
+    if (w.rows == 0) {  // the same for the whole cluster
+        pdl_wait();
+        return;
+    }
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < kTcStages; ++s) {
@@ -540,16 +657,11 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         fence_mbar_init();
     }
     if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (tid < w.rows) rows_at[tid] = w.streams[tid / p.gqa] * p.n_heads + w.kvh * p.gqa + tid % p.gqa;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    // The decode kernel behind this one relies on this order: its CTAs start once every CTA here has passed the wait.
-    pdl_wait();
-    pdl_launch_dependents();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&tmem_slot);
-    Item           w;
-    const bool     work = (int) blockIdx.x < p.plan[0] * p.n_kv_heads * p.max_chunks && load_item(p, blockIdx.x, w);
-    if (!work) w.key0 = w.key1 = 0;
     const int n_keys = w.key1 - w.key0, n_tiles = (n_keys + kKeys - 1) / kKeys, n_sub = (n_keys + kSub - 1) / kSub;
 
     auto give_up = [&]() {
@@ -570,45 +682,52 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     if (warp == 8) {
         if (lane == 0)
             for (int T = 0; T < min(n_tiles, kTcStages); ++T) load_tile(T);
-    } else if (warp < 8 && work) {
-        // Q: two threads per row, 32 head dimensions each
-        const int  row = tid >> 1, half = tid & 1;
-        const bool live = row < w.rows;
-        const int  at = live ? row : 0, stream = p.order[w.first + at / p.gqa], head = w.kvh * p.gqa + at % p.gqa;
-        const float * src = reinterpret_cast<const float *>(p.q + (size_t) stream * p.q_nb_stream + (size_t) head * p.q_nb_head);
-        float x[32];
+    } else if (warp < 8) {
+        // Q: 16 threads per row, four head dimensions each; a warp's eight loads are all in flight.  (Two threads per row, a
+        // float2 at a time, took 4 us: every load of a warp touched 16 rows.)
+        const int c = lane & 15;
+        float4    x[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float2 v = *reinterpret_cast<const float2 *>(src + 32 * half + 2 * i);
-            x[2 * i] = v.x; x[2 * i + 1] = v.y;
+        for (int i = 0; i < 8; ++i) {
+            const int row = warp * 16 + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
+            const float * src = reinterpret_cast<const float *>(p.q + (size_t) (at / p.n_heads) * p.q_nb_stream + (size_t) (at % p.n_heads) * p.q_nb_head) + 4 * c;
+            const float2  a = *reinterpret_cast<const float2 *>(src), b = *reinterpret_cast<const float2 *>(src + 2);
+            x[i] = make_float4(a.x, a.y, b.x, b.y);
         }
-        if (p.rope != nullptr) {  // the other half of the row is the neighbouring thread's
+        if (p.rope != nullptr) {  // elements d and d + 32 are partners: lanes c and c ^ 8
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float2 r = p.rope[(size_t) stream * (kHeadDim / 2) + i];
-                const float  y = __shfl_xor_sync(0xffffffffu, x[i], 1);
-                x[i] = half ? __fadd_rn(__fmul_rn(y, r.y), __fmul_rn(x[i], r.x)) : __fsub_rn(__fmul_rn(x[i], r.x), __fmul_rn(y, r.y));
+            for (int i = 0; i < 8; ++i) {
+                const int row = warp * 16 + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
+                const float2 * tb = p.rope + (size_t) (at / p.n_heads) * (kHeadDim / 2) + 4 * (c & 7);
+                const float *  xi = &x[i].x;
+                float          y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 r = tb[e];
+                    const float  other = __shfl_xor_sync(0xffffffffu, xi[e], 8);
+                    y[e] = c & 8 ? __fadd_rn(__fmul_rn(other, r.y), __fmul_rn(xi[e], r.x)) : __fsub_rn(__fmul_rn(xi[e], r.x), __fmul_rn(other, r.y));
+                }
+                x[i] = make_float4(y[0], y[1], y[2], y[3]);
             }
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float h0, l0, h1, l1;
-                split_hi_lo(live ? x[8 * c + 2 * i] * p.scale_log2 : 0.0f, h0, l0);
-                split_hi_lo(live ? x[8 * c + 2 * i + 1] * p.scale_log2 : 0.0f, h1, l1);
-                hi[i] = pack_half2(h0, h1);
-                lo[i] = pack_half2(l0, l1);
-            }
-            uint8_t * dst = smem_gen + row * 128 + (((4 * half + c) ^ (row & 7)) << 4);
-            *reinterpret_cast<uint4 *>(dst)          = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4 *>(dst + kQTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int i = 0; i < 8; ++i) {
+            const int    row = warp * 16 + 2 * i + (lane >> 4);
+            const bool   live = row < w.rows;
+            float        h[4], l[4];
+            split_hi_lo(live ? x[i].x * p.scale_log2 : 0.0f, h[0], l[0]);
+            split_hi_lo(live ? x[i].y * p.scale_log2 : 0.0f, h[1], l[1]);
+            split_hi_lo(live ? x[i].z * p.scale_log2 : 0.0f, h[2], l[2]);
+            split_hi_lo(live ? x[i].w * p.scale_log2 : 0.0f, h[3], l[3]);
+            uint8_t * dst = smem_gen + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8;
+            *reinterpret_cast<uint2 *>(dst)          = make_uint2(pack_half2(h[0], h[1]), pack_half2(h[2], h[3]));
+            *reinterpret_cast<uint2 *>(dst + kQTile) = make_uint2(pack_half2(l[0], l[1]), pack_half2(l[2], l[3]));
         }
         fence_proxy_async_smem();
     }
     __syncthreads();
 
+    bool all_ok = true;  // of the softmax warps
     if (warp == 8) {
         // ------------------------------------------------------------------ copies
         if (lane == 0) {
@@ -740,45 +859,24 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
         if (ok && n_sub > 0 && !mbar_wait_bounded(bO, 0)) ok = false;
         if (!ok) give_up();
-        ok = named_bar_all(1, 256, ok && !aborted());
-        if (ok && work) {
+        all_ok = named_bar_all(1, 256, ok && !aborted());  // every copy has been consumed: the ring's memory is free
+        if (all_ok) {
             tc_fence_after();
-            // the second group's part goes through the ring's memory (every copy has been consumed)
-            float4 * const other = reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base));
-            const bool     both  = n_sub > 1;
-            uint32_t       r[64];
-            if (group == 0 || both) tmem_ld64_sync(t_o, r);
-            if (group == 1 && both) {
+            float4 * const part = reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)) + (group * kRows + row) * kPartPitch;
+            if (group >= n_sub) {  // a group without keys
+#pragma unroll
+                for (int c = 0; c < 16; ++c) part[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            } else {
+                uint32_t r[64];
+                tmem_ld64_sync(t_o, r);
 #pragma unroll
                 for (int c = 0; c < 16; ++c)
-                    other[c * kPrefixRows + row] = make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3]));
-                other_ml[row] = make_float2(m, l);
+                    part[c] = make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3]));
             }
-            named_bar_sync(1, 256);
-            if (group == 0 && row < w.rows) {
-                float fa = 1.0f, fb = 0.0f;
-                if (both) {
-                    const float2 b  = other_ml[row];
-                    const float  mn = fmaxf(m, b.x);
-                    fa = m == -INFINITY ? 0.0f : exp2f(m - mn);
-                    fb = b.x == -INFINITY ? 0.0f : exp2f(b.x - mn);
-                    l  = l * fa + b.y * fb;
-                    m  = mn;
-                }
-                p.ml[(size_t) w.slot * kPrefixRows + row] = make_float2(m - kTcShift, l);
-                float4 * out = p.acc + (size_t) w.slot * 16 * kPrefixRows + row;
-#pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    float4 x = make_float4(__uint_as_float(r[4 * c]) * fa, __uint_as_float(r[4 * c + 1]) * fa, __uint_as_float(r[4 * c + 2]) * fa, __uint_as_float(r[4 * c + 3]) * fa);
-                    if (both) {
-                        const float4 y = other[c * kPrefixRows + row];
-                        x = make_float4(fmaf(y.x, fb, x.x), fmaf(y.y, fb, x.y), fmaf(y.z, fb, x.z), fmaf(y.w, fb, x.w));
-                    }
-                    out[c * kPrefixRows] = x;
-                }
-            }
+            ml[group * kRows + row] = make_float2(m - kTcShift, l);
         }
     }
+    join_and_write(p, w, reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)), ml, joined, rows_at, 2, kRows, all_ok, tid);
     // common exit: every role has left its loop; release TMEM
     tc_fence_before();
     __syncthreads();
@@ -788,26 +886,14 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
 }
 
-// Keys per chunk and chunks per prefix.  Enough items for every SM where the prefixes are long enough (a chunk holds at
-// least one stage), and no more than kPrefixMaxChunks partials per row.
-struct Chunks { int chunk, max_chunks; };
-Chunks plan_chunks(int sms, int max_tiles, int n_kv_heads, int prefix_bound) {
-    const int pairs  = std::max(1, max_tiles * n_kv_heads);
-    const int wanted = std::min(kPrefixMaxChunks, std::max(1, (sms + pairs - 1) / pairs));
-    const int bound  = std::max(1, prefix_bound);
-    Chunks    c;
-    c.chunk      = std::max(kKeys, ((bound + wanted - 1) / wanted + kKeys - 1) / kKeys * kKeys);
-    c.max_chunks = (bound + c.chunk - 1) / c.chunk;
-    return c;
+// CTAs per (row tile, kv head): as many as fill the SMs once, eight at most.  A second, thinner wave costs more than SMs left
+// idle.  No more than the prefix has tiles, but four where row tiles are full: the CTAs also share out the rows to be joined.
+int cluster_size(int sms, int n_tiles, int n_kv_heads, int prefix_bound, bool full) {
+    const int useful = std::max((prefix_bound + kKeys - 1) / kKeys, full ? 4 : 1);
+    return std::max(1, std::min(std::min(kMaxCluster, sms / std::max(1, n_tiles * n_kv_heads)), useful));
 }
 
 size_t aligned(size_t n) { return (n + 255) & ~(size_t) 255; }
-
-size_t shared_rows_bytes(const vox_prefix_plan * pl, int n_kv_heads, int prefix_bound) {
-    const Chunks c     = plan_chunks(kDecodeMaxSms, pl->max_tiles, n_kv_heads, prefix_bound);
-    const size_t slots = (size_t) pl->max_tiles * n_kv_heads * c.max_chunks;
-    return aligned(slots * kPrefixRows * sizeof(float2)) + aligned(slots * kPrefixRows * kHeadDim * sizeof(float));
-}
 
 // Arranges the streams by prefix: a counting sort, then row tiles of one prefix each.  An entry out of range is refused
 // before anything of the plan changes.
@@ -818,34 +904,36 @@ int arrange(vox_prefix_plan * pl, const int32_t * prefix_of) {
     std::vector<int32_t> start;
     try {
         start.assign((size_t) pl->n_prefixes + 1, 0);
+        pl->next.assign((size_t) pl->n_prefixes, 0);
         pl->host.assign(pl->words(), 0);
     } catch (const std::exception &) {
         set_error("out of host memory");
         return VOX_ATTN_OUT_OF_MEMORY;
     }
-    int32_t * h = pl->host.data(), * order = h + pl->order_at(), * place = h + pl->place_at(), * of = h + pl->of_at();
+    int32_t * h = pl->host.data();
+    // start[g]: streams of the prefixes before g; then, as they are placed, how far prefix g has come
     for (int s = 0; s < pl->n_streams; ++s)
         if (prefix_of[s] >= 0) start[prefix_of[s] + 1] += 1;
-    for (int g = 0; g < pl->n_prefixes; ++g) start[g + 1] += start[g];
-    // start[g] moves to the end of prefix g's streams while they are placed: afterwards it is the first of prefix g + 1
-    for (int s = 0; s < pl->n_streams; ++s) {
-        place[s] = -1;
-        if (prefix_of[s] >= 0) order[start[prefix_of[s]]++] = s;
-    }
-    const int per_tile = kPrefixRows / pl->gqa;
-    int       n_tiles  = 0;
-    for (int g = 0, first = 0; g < pl->n_prefixes; first = start[g++])
-        for (int m0 = first; m0 < start[g]; m0 += per_tile, ++n_tiles) {
-            const int n = std::min(per_tile, start[g] - m0);
-            int32_t * t = h + pl->tiles_at() + 4 * (size_t) n_tiles;
-            t[0] = g; t[1] = m0; t[2] = n;
-            for (int j = 0; j < n; ++j) {
-                place[order[m0 + j]] = n_tiles * kPrefixRows + j;
-                of[order[m0 + j]]    = g;
-            }
+    const int per_tile = pl->per_tile();
+    int       placed   = 0, n_tiles = 0;
+    for (int g = 0; g < pl->n_prefixes; ++g) {  // from counts to first tiles
+        const int n = start[g + 1];
+        start[g]    = n_tiles;
+        for (int left = n; left > 0; left -= per_tile, ++n_tiles) {
+            h[2 * (size_t) n_tiles]     = g;
+            h[2 * (size_t) n_tiles + 1] = std::min(left, per_tile);
         }
-    h[0] = n_tiles;
-    pl->full = 2 * start[pl->n_prefixes - 1] > n_tiles * per_tile;
+        placed += n;
+    }
+    std::vector<int32_t> & next = pl->next;
+    for (int s = 0; s < pl->n_streams; ++s) {
+        const int g = prefix_of[s];
+        if (g < 0) continue;
+        const int j = next[g]++, tile = start[g] + j / per_tile;
+        h[pl->members_at() + (size_t) tile * per_tile + j % per_tile] = s;
+    }
+    pl->n_tiles = n_tiles;
+    pl->full    = 2 * placed > n_tiles * per_tile;
     return VOX_ATTN_OK;
 }
 
@@ -892,7 +980,7 @@ int vox_prefix_plan_create(vox_engine * e, int n_streams, int n_prefixes, int n_
     VOX_REQUIRE(pl != nullptr, VOX_ATTN_OUT_OF_MEMORY, "out of host memory");
     pl->e = e; pl->n_streams = n_streams; pl->n_prefixes = n_prefixes; pl->gqa = n_heads / n_kv_heads;
     // full tiles, and one that is not full for every prefix in use
-    pl->max_tiles = n_streams / (kPrefixRows / pl->gqa) + std::min(n_streams, n_prefixes);
+    pl->max_tiles = n_streams / (kRows / pl->gqa) + std::min(n_streams, n_prefixes);
     int rc = arrange(pl, prefix_of);
     if (rc == VOX_ATTN_OK) {
         cudaError_t err = cudaMalloc(reinterpret_cast<void **>(&pl->dev), pl->words() * sizeof(int32_t));
@@ -932,10 +1020,9 @@ int vox_prefix_plan_set(vox_prefix_plan * pl, const int32_t * prefix_of, void * 
 }
 
 size_t vox_attn_decode_shared_workspace_bytes(const vox_decode_shared_args * a) {
-    if (a == nullptr || a->own.cache == nullptr) return 0;
-    const int    HK  = a->own.cache->cfg.n_kv_heads;
-    const size_t own = decode_workspace_bytes(a->own.n_streams, a->own.n_heads, HK, a->own.kv_bound);
-    return aligned(own) + (a->plan != nullptr ? shared_rows_bytes(a->plan, HK, a->prefix_bound) : 0);
+    if (a == nullptr || a->own.cache == nullptr || a->own.n_streams <= 0 || a->own.n_heads <= 0) return 0;
+    const size_t own = decode_shared_workspace_bytes(a->own.n_streams, a->own.n_heads, a->own.cache->cfg.n_kv_heads, a->own.kv_bound);
+    return aligned(own) + (a->plan != nullptr ? (size_t) a->own.n_streams * a->own.n_heads * sizeof(float2) : 0);
 }
 
 int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, void * workspace, size_t workspace_bytes, void * stream) {
@@ -947,54 +1034,51 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     const size_t need = vox_attn_decode_shared_workspace_bytes(a);
     VOX_REQUIRE(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                 VOX_ATTN_WORKSPACE_TOO_SMALL, "vox_attn_decode_shared needs %zu workspace bytes (16-byte aligned), got %zu", need, workspace_bytes);
-    cudaStream_t         st  = static_cast<cudaStream_t>(stream);
-    const vox_kv_cache * c   = a->own.cache;
-    const int            HK  = c->cfg.n_kv_heads;
-    const size_t         own = aligned(decode_workspace_bytes(a->own.n_streams, a->own.n_heads, HK, a->own.kv_bound));
-    SharedRows           rows{};
-    rows.lse = a->lse;
-    if (a->plan != nullptr && a->prefix_bound > 0) {
-        const vox_prefix_plan * pl = a->plan;
-        const vox_kv_cache *    pc = a->prefix;
-        const bool              q8 = pc->cfg.type == VOX_TYPE_Q8_0;
-        const Chunks            ch = plan_chunks(kDecodeMaxSms, pl->max_tiles, HK, a->prefix_bound);
-        const size_t            slots = (size_t) pl->max_tiles * HK * ch.max_chunks;
-        VOX_REQUIRE(slots < (1u << 30), VOX_ATTN_UNSUPPORTED, "vox_attn_decode_shared: more than 2^30 partial results");
-        uint8_t * ws = static_cast<uint8_t *>(workspace) + own;
-        rows.fold.ml  = reinterpret_cast<float2 *>(ws);
-        rows.fold.acc = reinterpret_cast<float4 *>(ws + aligned(slots * kPrefixRows * sizeof(float2)));
-        rows.fold.place = pl->dev + pl->place_at();
-        rows.fold.of    = pl->dev + pl->of_at();
-        rows.fold.len   = a->prefix_len;
-        rows.fold.max_len = pc->cfg.max_len;
-        rows.fold.chunk = ch.chunk; rows.fold.max_chunks = ch.max_chunks;
-        SharedParams p;
-        p.q = reinterpret_cast<const uint8_t *>(a->own.q);
-        p.q_nb_head = a->own.q_nb_head; p.q_nb_stream = a->own.q_nb_stream;
-        p.rope  = reinterpret_cast<const float2 *>(a->own.rope_table);
-        p.plan  = pl->dev; p.tiles = pl->dev + pl->tiles_at(); p.order = pl->dev + pl->order_at();
-        p.len   = a->prefix_len;
-        p.ml = const_cast<float2 *>(rows.fold.ml); p.acc = const_cast<float4 *>(rows.fold.acc);
-        p.n_prefixes = pl->n_prefixes; p.n_kv_heads = HK; p.gqa = pl->gqa; p.layer = a->own.layer; p.max_len = pc->cfg.max_len;
-        p.chunk = ch.chunk; p.max_chunks = ch.max_chunks;
-        p.scale_log2 = a->own.scale * 1.4426950408889634f;
-        p.q8_tiles = pc->k_data + (size_t) a->own.layer * pc->nb_layer;
-        p.q8_nb_head = pc->nb_head; p.q8_nb_stream = pc->nb_stream;
-        p.status = e->status_dev;
-        const bool     tc     = !q8 && pl->full;
-        const auto     kernel = tc ? shared_rows_tc_kernel : q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
-        const int      smem   = tc ? kTcSmem : q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
-        const uint32_t bit    = 1u << (tc ? 21 : q8 ? 19 : 18);
-        if (!(e->attr_mask & bit)) {
-            VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-            e->attr_mask |= bit;
-        }
-        const unsigned grid = (unsigned) (tc ? slots : std::min<size_t>(slots, (size_t) e->sm_count));
-        launch_pdl(kernel, dim3(grid), dim3(tc ? kTcThreads : kThreads), (size_t) smem, st, pc->map_k, pc->map_v, p);
-        rc = check_launch(e, tc ? "shared_rows_tc_kernel" : q8 ? "shared_rows_kernel<q8_0>" : "shared_rows_kernel<f16>");
-        if (rc != VOX_ATTN_OK) return rc;
+    cudaStream_t            st  = static_cast<cudaStream_t>(stream);
+    const vox_prefix_plan * pl  = a->plan;
+    const int               HK  = a->own.cache->cfg.n_kv_heads;
+    const size_t            own = aligned(decode_shared_workspace_bytes(a->own.n_streams, a->own.n_heads, HK, a->own.kv_bound));
+    const bool              shares = pl != nullptr && a->prefix_bound > 0;
+    float2 * const          ml  = shares ? reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + own) : nullptr;
+    rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml}, workspace, own, st);
+    if (rc != VOX_ATTN_OK || !shares) return rc;
+    const vox_kv_cache * pc = a->prefix;
+    const bool           q8 = pc->cfg.type == VOX_TYPE_Q8_0, tc = !q8 && pl->full;
+    SharedParams         p;
+    p.q = reinterpret_cast<const uint8_t *>(a->own.q);
+    p.q_nb_head = a->own.q_nb_head; p.q_nb_stream = a->own.q_nb_stream;
+    p.rope    = reinterpret_cast<const float2 *>(a->own.rope_table);
+    p.tiles   = reinterpret_cast<const int2 *>(pl->dev);
+    p.members = pl->dev + pl->members_at();
+    p.len     = a->prefix_len;
+    p.per_tile = pl->per_tile(); p.n_kv_heads = HK; p.n_heads = a->own.n_heads; p.gqa = pl->gqa; p.layer = a->own.layer; p.max_len = pc->cfg.max_len;
+    p.cluster    = cluster_size(std::min(kDecodeMaxSms, e->sm_count), pl->n_tiles, HK, a->prefix_bound, pl->full);
+    p.scale_log2 = a->own.scale * 1.4426950408889634f;
+    p.q8_tiles   = pc->k_data + (size_t) a->own.layer * pc->nb_layer;
+    p.q8_nb_head = pc->nb_head; p.q8_nb_stream = pc->nb_stream;
+    p.dst = a->own.dst; p.ml = ml; p.lse = a->lse;
+    p.status = e->status_dev;
+    const auto     kernel = tc ? shared_rows_tc_kernel : q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
+    const int      smem   = tc ? kTcSmem : q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
+    const uint32_t bit    = 1u << (tc ? 21 : q8 ? 19 : 18);
+    if (!(e->attr_mask & bit)) {
+        VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        // all of the SM's memory as shared memory, so that a CTA fits beside one of the decode kernel's
+        VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+        e->attr_mask |= bit;
     }
-    return launch_decode_shared(e, &a->own, rows, workspace, own, st);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) (pl->max_tiles * HK * p.cluster)); cfg.blockDim = dim3(tc ? kTcThreads : kThreads);
+    cfg.dynamicSmemBytes = (size_t) smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned) p.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, pc->map_k, pc->map_v, p);
+    return check_launch(e, tc ? "shared_rows_tc_kernel" : q8 ? "shared_rows_kernel<q8_0>" : "shared_rows_kernel<f16>");
 }
 
 }  // extern "C"
