@@ -28,22 +28,26 @@
 using namespace vox;
 
 namespace {
-constexpr int kRows = 128;       // rows of a row tile
+constexpr int kRows = 128;       // rows of a full row tile
+constexpr int kHalfRows = 64;    // of a row tile for the mma.sync kernel
+constexpr int kJoin = 128;       // threads that join results
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kMaxCluster = 8;
 }
 
-// The streams of a call, arranged by prefix.  Host copy of the arrangement and its device arrays (one allocation):
-//   tiles [max_tiles][2] = prefix, streams (0: not in use);  members [max_tiles][128 / gqa]: their streams
+// The streams of a call, arranged by prefix, twice: into row tiles of 128 rows ([0]) and of 64 ([1]).  Host copy and device
+// arrays (one allocation) of either:
+//   tiles [max_tiles][2] = prefix, streams (0: not in use);  members [max_tiles][rows / gqa]: their streams
 struct vox_prefix_plan {
     vox_engine *         e = nullptr;
-    int                  n_streams = 0, n_prefixes = 0, gqa = 0, max_tiles = 0, n_tiles = 0;
-    bool                 full = false;  // the row tiles are more than half full on average
+    int                  n_streams = 0, n_prefixes = 0, gqa = 0, max_tiles[2] = {0, 0}, n_tiles[2] = {0, 0};
+    bool                 full = false;  // the tiles of 128 rows are more than half full on average
     std::vector<int32_t> host, next;    // next: scratch of the arrangement
     int32_t *            dev = nullptr;
-    int    per_tile() const { return kRows / gqa; }
-    size_t members_at() const { return (size_t) max_tiles * 2; }
-    size_t words() const { return members_at() + (size_t) max_tiles * per_tile(); }
+    int    per_tile(int k) const { return (k ? kHalfRows : kRows) / gqa; }
+    size_t tiles_at(int k) const { return k ? (members_at(0) + (size_t) max_tiles[0] * per_tile(0) + 1) & ~(size_t) 1 : 0; }
+    size_t members_at(int k) const { return tiles_at(k) + (size_t) max_tiles[k] * 2; }
+    size_t words() const { return members_at(1) + (size_t) max_tiles[1] * per_tile(1); }
 };
 
 namespace {
@@ -90,8 +94,10 @@ __device__ __forceinline__ Item load_item(const SharedParams & p) {
 
 // ---- the join.  A CTA's partial results lie in its shared memory: part[v][17] float4 (a row's 64 columns, padded by 16
 // bytes against bank conflicts) and ml[v], where v = group * stride + row and a row has a result from every one of
-// `groups` groups of warps.  256 threads take part; the others only arrive at the cluster barriers.
+// `groups` groups of warps.  kJoin threads take part; the others only arrive at the cluster barriers.
 constexpr int kPartPitch = 17;
+constexpr int kMlWords   = kRows / 2 + kMaxCluster * kRows / 4;  // ml: a row's (max, sum) each, later those of a share and its weights
+static_assert(kMlWords >= kRows, "ml");
 
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -116,28 +122,20 @@ __device__ __forceinline__ float4 peer_ld4(uint32_t addr) {
 // NaN has the maximum -inf and the sum NaN, which stays NaN.)
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2_approx(m - M); }
 
-// Called by all threads of the CTA; `tid` < 256 do the work.  joined: one more ml array of kRows entries; rows_at: where the rows
-// of the tile lie in dst (stream * n_heads + head).
+// Called by all threads of the CTA; `tid` < kJoin do the work.  joined: one more ml array of kRows entries; rows_at: where the rows
+// of the tile lie in dst (stream * n_heads + head); share: memory for this CTA's share of the rows, apart from `part`.
+// All that can be done before the decode kernel has ended is done before it: the parts of the CTA's warps and then of the
+// cluster's CTAs are joined, every CTA taking a share of the rows, so that only one part is left to join with the own rows'.
+// The loops are kept short: this code runs once per CTA, and what it costs cold is fetching its instructions (8 us of a
+// call when the joins of four rows and eight CTAs were written out).
 __device__ __forceinline__ void join_and_write(const SharedParams & p, const Item & w, float4 * part, float2 * ml, float2 * joined, const int * rows_at,
-                                               int groups, int stride, bool ok, int tid) {
-    const bool mine = tid < 256;
-    const int  n = w.rows * 16, first = w.rank * 256 + tid, pace = p.cluster * 256;
-    constexpr int W = 2;  // a thread's rows in flight: a row at a time would wait for L2 once per row
-    float2 own_ml[W];
-    float4 own[W];
-    auto fetch_own = [&](int i0) {
-#pragma unroll
-        for (int u = 0; u < W; ++u) {
-            const int i = min(i0 + u * pace, n - 1), at = rows_at[i >> 4];
-            own_ml[u] = __ldcg(p.ml + at);
-            own[u]    = __ldcg(reinterpret_cast<const float4 *>(p.dst + (size_t) at * kHeadDim) + (i & 15));
-        }
-    };
+                                               float4 * share, int groups, int stride, bool ok, int tid) {
+    const bool mine = tid < kJoin;
     __syncwarp();
     if (mine) {
-        named_bar_sync(1, 256);
+        named_bar_sync(1, kJoin);
         if (!ok || w.key0 >= w.key1) {
-            for (int row = tid; row < kRows; row += 256) joined[row] = make_float2(-INFINITY, 0.0f);
+            if (tid < w.rows) joined[tid] = make_float2(-INFINITY, 0.0f);
         } else if (groups == 1) {
             if (tid < w.rows) joined[tid] = ml[tid];
         } else {
@@ -152,8 +150,8 @@ __device__ __forceinline__ void join_and_write(const SharedParams & p, const Ite
                 }
                 joined[tid] = make_float2(M, L);
             }
-            named_bar_sync(1, 256);
-            for (int i = tid; i < n; i += 256) {
+            named_bar_sync(1, kJoin);
+            for (int i = tid; i < w.rows * 16; i += kJoin) {
                 const int row = i >> 4, c = i & 15;
                 float4    a = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int g = 0; g < groups; ++g) {
@@ -165,65 +163,93 @@ __device__ __forceinline__ void join_and_write(const SharedParams & p, const Ite
             }
         }
     }
-    pdl_wait();  // the decode kernel's results
-    pdl_launch_dependents();
-    if (mine && first < n) fetch_own(first);
-    cluster_sync_all();
-    if (mine) {
-        const uint32_t part0 = smem_u32(part), joined0 = smem_u32(joined);
-        for (int i0 = first; i0 < n; i0 += W * pace) {
-            if (i0 != first) fetch_own(i0);
-#pragma unroll
-            for (int u = 0; u < W; ++u) {
-                const int i = i0 + u * pace, row = i >> 4, c = i & 15;
-                if (i >= n) break;
-                float2 m[kMaxCluster];
-                float4 x[kMaxCluster];
-                float  M = own_ml[u].x;
-#pragma unroll
-                for (int r = 0; r < kMaxCluster; ++r)
-                    if (r < p.cluster) {
-                        m[r] = peer_ld2(peer_addr(joined0 + row * 8, r));
-                        x[r] = peer_ld4(peer_addr(part0 + (row * kPartPitch + c) * 16, r));
-                    }
-#pragma unroll
-                for (int r = 0; r < kMaxCluster; ++r)
-                    if (r < p.cluster) M = fmaxf(M, m[r].x);
-                // the own rows' result is normalised: its sum is taken back in
-                const float f0 = part_weight(own_ml[u].x, M), s0 = f0 * own_ml[u].y;
-                float       L = s0;
-                float4      a = make_float4(own[u].x * s0, own[u].y * s0, own[u].z * s0, own[u].w * s0);
-#pragma unroll
-                for (int r = 0; r < kMaxCluster; ++r)
-                    if (r < p.cluster && !(m[r].x == -INFINITY && m[r].y == 0.0f)) {  // nothing was written for a part without keys
-                        const float f = part_weight(m[r].x, M);
-                        L = fmaf(m[r].y, f, L);
-                        a = make_float4(fmaf(x[r].x, f, a.x), fmaf(x[r].y, f, a.y), fmaf(x[r].z, f, a.z), fmaf(x[r].w, f, a.w));
-                    }
-                const int   at  = rows_at[row];
-                const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;  // NaN stays NaN
-                reinterpret_cast<float4 *>(p.dst + (size_t) at * kHeadDim)[c] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-                if (c == 0 && p.lse != nullptr) p.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    // this CTA's share of the rows: row0 .. row0 + n_rows - 1, in share[] and ml[] (row 0 first)
+    const int row0 = w.rank * w.rows / p.cluster, n_rows = (w.rank + 1) * w.rows / p.cluster - row0;
+    if (p.cluster > 1) {
+        cluster_sync_all();
+        if (mine) {
+            const uint32_t joined0 = smem_u32(joined), part0 = smem_u32(part);
+            float * const  f = reinterpret_cast<float *>(ml + kRows / 2);  // [rank][64]: a share is at most 64 rows, whose ml lies below
+            if (tid < n_rows) {
+                float M = -INFINITY, L = 0.0f;
+#pragma unroll 4
+                for (int r = 0; r < p.cluster; ++r) M = fmaxf(M, peer_ld2(peer_addr(joined0 + (row0 + tid) * 8, r)).x);
+#pragma unroll 4
+                for (int r = 0; r < p.cluster; ++r) {
+                    const float2 x = peer_ld2(peer_addr(joined0 + (row0 + tid) * 8, r));
+                    const float  wt = part_weight(x.x, M);
+                    L = fmaf(x.y, wt, L);
+                    // a part without keys was never written (and a row of NaN has a part, of weight NaN)
+                    f[r * (kRows / 2) + tid] = x.x == -INFINITY && x.y == 0.0f ? -1.0f : x.y != x.y ? x.y : wt;
+                }
+                ml[tid] = make_float2(M, L);
+            }
+            named_bar_sync(1, kJoin);
+            for (int i = tid; i < n_rows * 16; i += kJoin) {
+                const int row = i >> 4, c = i & 15;
+                float4    a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (int r = 0; r < p.cluster; ++r) {
+                    const float wt = f[r * (kRows / 2) + row];
+                    if (wt == -1.0f) continue;
+                    const float4 x = peer_ld4(peer_addr(part0 + ((row0 + row) * kPartPitch + c) * 16, r));
+                    a = make_float4(fmaf(x.x, wt, a.x), fmaf(x.y, wt, a.y), fmaf(x.z, wt, a.z), fmaf(x.w, wt, a.w));
+                }
+                share[row * kPartPitch + c] = a;
             }
         }
+        cluster_sync_all();  // nobody's shared memory is read any longer by another CTA
+    } else {
+        share = part;
+        ml    = joined;
+        if (mine) named_bar_sync(1, kJoin);
     }
-    cluster_sync_all();  // nobody leaves while its shared memory is read
+    pdl_wait();  // the decode kernel's results
+    pdl_launch_dependents();
+    if (!mine) return;
+    constexpr int W = 4;  // a thread's rows in flight: a row at a time would wait for L2 once per row
+#pragma unroll 1
+    for (int i0 = tid; i0 < n_rows * 16; i0 += W * kJoin) {
+        float2 own_ml[W];
+        float4 own[W];
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+            const int i = min(i0 + u * kJoin, n_rows * 16 - 1), at = rows_at[row0 + (i >> 4)];
+            own_ml[u] = __ldcg(p.ml + at);
+            own[u]    = __ldcg(reinterpret_cast<const float4 *>(p.dst + (size_t) at * kHeadDim) + (i & 15));
+        }
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+            const int i = i0 + u * kJoin, row = i >> 4, c = i & 15;
+            if (i >= n_rows * 16) break;
+            const float2 b = ml[row];
+            const float4 x = share[row * kPartPitch + c];
+            const float  M = fmaxf(own_ml[u].x, b.x), fa = part_weight(own_ml[u].x, M) * own_ml[u].y, fb = part_weight(b.x, M);
+            const float  L = fmaf(b.y, fb, fa), inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;  // NaN stays NaN
+            const int    at = rows_at[row0 + row];
+            // the own rows' result is normalised: its sum is taken back in
+            reinterpret_cast<float4 *>(p.dst + (size_t) at * kHeadDim)[c] =
+                make_float4(fmaf(own[u].x, fa, x.x * fb) * inv, fmaf(own[u].y, fa, x.y * fb) * inv, fmaf(own[u].z, fa, x.z * fb) * inv, fmaf(own[u].w, fa, x.w * fb) * inv);
+            if (c == 0 && p.lse != nullptr) p.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Row tiles of any fill and either cache type, on mma.sync: eight warps, arranged as row groups of 16 x key groups (a tile
-// of few rows has the 128 keys of a ring stage spread over the warps), and a warp that copies.
-constexpr int kWarps   = 8;
+// Row tiles of 64 rows, of any fill and either cache type, on mma.sync: four warps, arranged as row groups of 16 x key groups
+// (a tile of few rows has the 128 keys of a ring stage spread over the warps), and a warp that copies.
+constexpr int kWarps   = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
 
 template <bool Q8> struct Ring {
-    static constexpr int kStages     = Q8 ? 4 : 3;
+    static constexpr int kStages     = Q8 ? 4 : 2;  // room for two CTAs of the decode kernel on the SM
     static constexpr int kBoxBytes   = Q8 ? 9 * 1024 : 2 * kKvTile * 128;  // 64 rows of K and V
     static constexpr int kBoxTx      = Q8 ? kQ8TileBytes : kBoxBytes;
     static constexpr int kVOff       = Q8 ? kQ8VBytesOff : kKvTile * 128;
     static constexpr int kStageBytes = 2 * kBoxBytes;
     static constexpr int kSmemBytes  = kStages * kStageBytes + 1024;
-    static_assert(kStages * kStageBytes >= kRows * kPartPitch * 16, "the partial results take the ring's memory");
+    static_assert(kStages * kStageBytes >= kHalfRows * kPartPitch * 16, "the partial results take the ring's memory");
+    static_assert(kStages * kStageBytes >= (kHalfRows + kHalfRows / 2) * kPartPitch * 16, "and a share of them with it");
 };
 constexpr float kShift = 10.0f;  // f16 caches: weights up to 2^10, so that the remainders of small ones are normal f16 numbers
 
@@ -416,13 +442,13 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
 }
 
 template <bool Q8>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __maxnreg__(152)  // room for two CTAs of the decode kernel (2 x 160 x 128 registers) on the SM
 shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedParams p) {
     using R = Ring<Q8>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * R::kStages];
     __shared__ int      abort_flag;
-    __shared__ float2   ml[kRows], joined[kRows];
+    __shared__ float2   ml[kMlWords], joined[kRows];
     __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     float4 * const part      = reinterpret_cast<float4 *>(smem_raw + (smem_base - smem_u32(smem_raw)));
@@ -447,7 +473,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     bool      ok = true;
     // Warps of a row tile: groups of 16 rows, and as many key groups as that leaves
     const int groups = (w.rows + 15) >> 4;
-    const int rg     = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : 8;
+    const int rg     = groups <= 1 ? 1 : groups <= 2 ? 2 : 4;
     const int kg = kWarps / rg;
 
     if (warp == kWarps) {
@@ -547,13 +573,9 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             if (busy) {
                 const int k0 = wk * span;
                 const uint32_t box = smem_base + s * R::kStageBytes + (k0 >> 6) * R::kBoxBytes;
-                if (kg == 8) {
-                    if (key + k0 < w.key1) step<Q8, 1>(x, box, k0 & 63, key + k0, w.key1, lane);
-                } else {
 #pragma unroll 1
-                    for (int b = 0; b < span && key + k0 + b < w.key1; b += 32)
-                        step<Q8, 2>(x, box + (((k0 & 63) + b) >> 6) * R::kBoxBytes, (k0 + b) & 63, key + k0 + b, w.key1, lane);
-                }
+                for (int b = 0; b < span && key + k0 + b < w.key1; b += 32)
+                    step<Q8, 2>(x, box + (((k0 & 63) + b) >> 6) * R::kBoxBytes, (k0 + b) & 63, key + k0 + b, w.key1, lane);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty0 + 8 * s);
@@ -584,29 +606,30 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             }
         }
     }
-    join_and_write(p, w, part, ml, joined, rows_at, kg, 16 * rg, ok, tid);
+    join_and_write(p, w, part, ml, joined, rows_at, part + kHalfRows * kPartPitch, kg, 16 * rg, ok, tid);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Full row tiles on the 5th-generation tensor cores (f16 caches).
 //
-// Q (scaled by scale * log2 e) lies in shared memory as two f16 tiles,
-// value and remainder; scores S = Q_lo.K + Q_hi.K (the small part first: the accumulator truncates) come 64 keys at a time
-// into one of six score buffers in TMEM.  Two groups of four softmax warps take them in turn, a thread per row: 64 scores
-// out of TMEM, weights 2^(S - ref) back over them as two packed f16 tiles (value and remainder, 22 bits), from where the
-// tensor core takes them as the A operand of P.V.  Every group has an output accumulator and a reference maximum of its
-// own, so the groups never wait for one another; they are joined at the end, as the CTAs are.  The reference of a row is raised only
-// when a maximum exceeds it by 2^8 (its accumulator is then rescaled in TMEM).
-//   warps 0-3, 4-7  softmax groups    warp 8  K/V copies    warp 9  issues S = Q.K    warp 10  issues O += P.V
-constexpr int kTcThreads = 11 * 32;
-constexpr int kTcStages  = 3;                     // leaves room on the SM for a CTA of the decode kernel
-constexpr int kSub       = 64;                    // keys of a score tile
+// Q (scaled by scale * log2 e) lies in shared memory as two f16 tiles, value and remainder; scores S = Q_lo.K + Q_hi.K (the
+// small part first: the accumulator truncates) come 64 keys at a time into one of six score buffers in TMEM.  Four softmax
+// warps, a thread per row: 64 scores out of TMEM, weights 2^(S - ref) back over them as two packed f16 tiles (value and
+// remainder, 22 bits), from where the tensor core takes them as the A operand of P.V.  The reference of a row is raised
+// only when a maximum exceeds it by 2^8 (its accumulator is then rescaled in TMEM).
+//   warps 0-3  softmax      warp 4  issues S = Q.K      warp 5  issues O += P.V, and the copies of K and V (64 rows a stage)
+// 192 threads of 128 registers and 83 KB of shared memory: the CTA runs beside two CTAs of the decode kernel, whose time is
+// HBM's.  (With two softmax groups, 352 threads and 128-key stages it was no faster on its own and had to wait for the
+// decode kernel's CTAs to leave: 57.4 us for 256 streams under two prompts of 4096 rows.)
+constexpr int kTcThreads = 6 * 32;
+constexpr int kTcStages  = 3;
+constexpr int kSub       = 64;                    // keys of a score tile and of a stage
 constexpr int kSBufs     = 6;
-constexpr int kTcOCol    = kSBufs * kSub;         // two accumulators of 64 columns behind the score buffers
+constexpr int kTcOCol    = kSBufs * kSub;         // the accumulator: 64 columns behind the score buffers
 constexpr int kQTile     = kRows * 128;
-constexpr int kTcStage   = 2 * kKeys * 128;       // 128 rows of K, 128 rows of V
+constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V
 constexpr int kTcSmem    = 2 * kQTile + kTcStages * kTcStage + 1024;
-static_assert(kTcStages * kTcStage >= 2 * kRows * kPartPitch * 16, "the groups' partial results take the ring's memory");
+static_assert(kTcStages * kTcStage >= kRows * kPartPitch * 16, "the partial results take the ring's memory");
 constexpr float kTcShift = 6.0f;                  // weights up to 2^(8 + 6): their remainders stay normal f16 numbers
 
 // multiply this thread's accumulator row by f; rare, kept out of line so that its registers do not weigh on the loop
@@ -623,13 +646,13 @@ __device__ __noinline__ void rescale_row(uint32_t t_o, float f) {
     tc_fence_before();
 }
 
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __maxnreg__(128)
 shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int      abort_flag;
-    __shared__ float2   ml[2 * kRows], joined[kRows];
+    __shared__ float2   ml[kMlWords], joined[kRows];
     __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -650,19 +673,19 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
         for (int s = 0; s < kSBufs; ++s) {
             mbar_init(bS0 + 8 * s, 1);
-            mbar_init(bP0 + 8 * s, 4);  // one arrival per warp of the group that took the tile
+            mbar_init(bP0 + 8 * s, 4);  // one arrival per softmax warp
             mbar_init(bF0 + 8 * s, 1);
         }
         mbar_init(bO, 1);
         fence_mbar_init();
     }
-    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (warp == 4) tmem_alloc(smem_u32(&tmem_slot), 512);
     if (tid < w.rows) rows_at[tid] = w.streams[tid / p.gqa] * p.n_heads + w.kvh * p.gqa + tid % p.gqa;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&tmem_slot);
-    const int n_keys = w.key1 - w.key0, n_tiles = (n_keys + kKeys - 1) / kKeys, n_sub = (n_keys + kSub - 1) / kSub;
+    const int n_keys = w.key1 - w.key0, n_sub = (n_keys + kSub - 1) / kSub;
 
     auto give_up = [&]() {
         atomicOr(p.status, kStatusTimeout);
@@ -670,26 +693,25 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     };
     auto aborted   = [&]() { return *reinterpret_cast<volatile int *>(&abort_flag) != 0; };
     auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0; };
-    auto load_tile = [&](int T) {  // one lane
-        const int      st = T % kTcStages, boxes = n_keys - T * kKeys > kSub ? 2 : 1;
-        const uint32_t bar = full0 + 8 * st, dst = sKV + st * kTcStage;
-        mbar_expect_tx(bar, boxes * 2 * kSub * 128);
-        for (int b = 0; b < boxes; ++b) {
-            tma_load_5d(dst + b * kSub * 128, &map_k, bar, 0, w.key0 + T * kKeys + b * kSub, w.kvh, w.prefix, p.layer);
-            tma_load_5d(dst + kKeys * 128 + b * kSub * 128, &map_v, bar, 0, w.key0 + T * kKeys + b * kSub, w.kvh, w.prefix, p.layer);
-        }
+    auto load_tile = [&](int U) {  // one lane
+        const uint32_t bar = full0 + 8 * (U % kTcStages), dst = sKV + (U % kTcStages) * kTcStage;
+        mbar_expect_tx(bar, kTcStage);
+        tma_load_5d(dst, &map_k, bar, 0, w.key0 + U * kSub, w.kvh, w.prefix, p.layer);
+        tma_load_5d(dst + kSub * 128, &map_v, bar, 0, w.key0 + U * kSub, w.kvh, w.prefix, p.layer);
     };
-    if (warp == 8) {
+    if (warp == 5) {
         if (lane == 0)
-            for (int T = 0; T < min(n_tiles, kTcStages); ++T) load_tile(T);
-    } else if (warp < 8) {
-        // Q: 16 threads per row, four head dimensions each; a warp's eight loads are all in flight.  (Two threads per row, a
+            for (int U = 0; U < min(n_sub, kTcStages); ++U) load_tile(U);
+    } else if (warp < 4) {
+        // Q: 16 threads per row, four head dimensions each; eight loads of a warp in flight.  (Two threads per row, a
         // float2 at a time, took 4 us: every load of a warp touched 16 rows.)
         const int c = lane & 15;
-        float4    x[8];
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+        float4 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int row = warp * 16 + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
+            const int row = 32 * warp + 16 * half + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
             const float * src = reinterpret_cast<const float *>(p.q + (size_t) (at / p.n_heads) * p.q_nb_stream + (size_t) (at % p.n_heads) * p.q_nb_head) + 4 * c;
             const float2  a = *reinterpret_cast<const float2 *>(src), b = *reinterpret_cast<const float2 *>(src + 2);
             x[i] = make_float4(a.x, a.y, b.x, b.y);
@@ -697,7 +719,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (p.rope != nullptr) {  // elements d and d + 32 are partners: lanes c and c ^ 8
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int row = warp * 16 + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
+                const int row = 32 * warp + 16 * half + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
                 const float2 * tb = p.rope + (size_t) (at / p.n_heads) * (kHeadDim / 2) + 4 * (c & 7);
                 const float *  xi = &x[i].x;
                 float          y[4];
@@ -712,7 +734,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int    row = warp * 16 + 2 * i + (lane >> 4);
+            const int    row = 32 * warp + 16 * half + 2 * i + (lane >> 4);
             const bool   live = row < w.rows;
             float        h[4], l[4];
             split_hi_lo(live ? x[i].x * p.scale_log2 : 0.0f, h[0], l[0]);
@@ -723,38 +745,25 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             *reinterpret_cast<uint2 *>(dst)          = make_uint2(pack_half2(h[0], h[1]), pack_half2(h[2], h[3]));
             *reinterpret_cast<uint2 *>(dst + kQTile) = make_uint2(pack_half2(l[0], l[1]), pack_half2(l[2], l[3]));
         }
+        }
         fence_proxy_async_smem();
     }
     __syncthreads();
 
     bool all_ok = true;  // of the softmax warps
-    if (warp == 8) {
-        // ------------------------------------------------------------------ copies
-        if (lane == 0) {
-            bool ok = true;
-            int  T  = min(n_tiles, kTcStages);
-            for (; T < n_tiles && ok; ++T) {
-                if (!mbar_wait_bounded(empty0 + 8 * (T % kTcStages), ((T / kTcStages) - 1) & 1) || aborted()) { ok = false; break; }
-                load_tile(T);
-            }
-            if (!ok) {
-                give_up();
-                for (int i = max(0, T - kTcStages); i < T; ++i) mbar_wait_bounded(full0 + 8 * (i % kTcStages), (i / kTcStages) & 1);
-            }
-        }
-    } else if (warp == 9) {
+    if (warp == 4) {
         // ------------------------------------------------------------------ scores (all lanes in the loop, one issues)
         constexpr uint32_t idesc = idesc_f16(kSub, false);
         const uint64_t     dQ = smem_desc_sw128(sQ), dQlo = smem_desc_sw128(sQ + kQTile), dK = smem_desc_sw128(sKV);
         const bool         leader = elect_one();
         bool               ok = true;
         for (int U = 0; U < n_sub && ok; ++U) {
-            const int T = U >> 1, st = T % kTcStages, sb = U % kSBufs;
-            if (!warp_wait(full0 + 8 * st, (T / kTcStages) & 1) || (U >= kSBufs && !warp_wait(bF0 + 8 * sb, ((U / kSBufs) - 1) & 1))) { ok = false; break; }
+            const int st = U % kTcStages, sb = U % kSBufs;
+            if (!warp_wait(full0 + 8 * st, (U / kTcStages) & 1) || (U >= kSBufs && !warp_wait(bF0 + 8 * sb, ((U / kSBufs) - 1) & 1))) { ok = false; break; }
             tc_fence_after();
             if (leader) {
                 const uint32_t dS = tmem + kSub * sb;
-                const uint64_t k0 = dK + (uint64_t) (st * (kTcStage >> 4) + (U & 1) * ((kSub * 128) >> 4));
+                const uint64_t k0 = dK + (uint64_t) (st * (kTcStage >> 4));
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc_mma_f16(dS, dQlo + k * 2, k0 + k * 2, idesc, k > 0);
 #pragma unroll
@@ -764,37 +773,46 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             __syncwarp();
         }
         if (!ok && lane == 0) give_up();
-    } else if (warp == 10) {
-        // ------------------------------------------------------------------ output
+    } else if (warp == 5) {
+        // ------------------------------------------------------------------ output, and the copies behind it
         constexpr uint32_t idesc = idesc_f16(kHeadDim, true);
-        const uint64_t     dV = smem_desc_sw128_mn(sKV + kKeys * 128, 16);
+        const uint64_t     dV = smem_desc_sw128_mn(sKV + kSub * 128, 16);
         const bool         leader = elect_one();
         bool               ok = true;
+        int                loaded = min(n_sub, kTcStages);
         for (int U = 0; U < n_sub && ok; ++U) {
-            const int T = U >> 1, st = T % kTcStages, sb = U % kSBufs;
-            if (!warp_wait(full0 + 8 * st, (T / kTcStages) & 1) || !warp_wait(bP0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
+            const int st = U % kTcStages, sb = U % kSBufs;
+            if (!warp_wait(full0 + 8 * st, (U / kTcStages) & 1) || !warp_wait(bP0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
             tc_fence_after();
             if (leader) {
-                const uint32_t tP = tmem + kSub * sb, tO = tmem + kTcOCol + kHeadDim * (U & 1);
-                const uint64_t v0 = dV + (uint64_t) (st * (kTcStage >> 4) + (U & 1) * ((kSub * 128) >> 4));
+                const uint32_t tP = tmem + kSub * sb, tO = tmem + kTcOCol;
+                const uint64_t v0 = dV + (uint64_t) (st * (kTcStage >> 4));
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + 8 * k, v0 + k * (2048 >> 4), idesc, U > 1 || k > 0);
+                for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + 8 * k, v0 + k * (2048 >> 4), idesc, U > 0 || k > 0);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + kSub / 2 + 8 * k, v0 + k * (2048 >> 4), idesc, 1);
                 tc_commit(bF0 + 8 * sb);
-                if ((U & 1) || U == n_sub - 1) tc_commit(empty0 + 8 * st);
+                tc_commit(empty0 + 8 * st);
                 if (U == n_sub - 1) tc_commit(bO);
             }
             __syncwarp();
+            // the stage of the tile before this one is free as soon as its P.V has retired, which was issued a tile ago
+            if (U > 0 && loaded < n_sub) {
+                if (!warp_wait(empty0 + 8 * ((U - 1) % kTcStages), ((U - 1) / kTcStages) & 1) || __any_sync(0xffffffffu, aborted())) { ok = false; break; }
+                if (lane == 0) load_tile(loaded);
+                ++loaded;
+            }
         }
-        if (!ok && lane == 0) give_up();
+        if (!ok) {
+            if (lane == 0) give_up();
+            for (int i = max(0, loaded - kTcStages); i < loaded; ++i) warp_wait(full0 + 8 * (i % kTcStages), (i / kTcStages) & 1);  // copies in flight land
+        }
     } else {
         // ------------------------------------------------------------------ softmax: a thread per row
-        const int      group = warp >> 2, row = tid & 127;
-        const uint32_t t_row = tmem + ((uint32_t) (32 * (warp & 3)) << 16), t_o = t_row + kTcOCol + kHeadDim * group;
+        const uint32_t t_row = tmem + ((uint32_t) (32 * warp) << 16), t_o = t_row + kTcOCol;
         float          m = -INFINITY, l = 0.0f;
         bool           ok = true;
-        for (int U = group; U < n_sub; U += 2) {
+        for (int U = 0; U < n_sub; ++U) {
             const int sb = U % kSBufs, left = n_keys - U * kSub;  // keys of this tile and after
             if (!mbar_wait_bounded(bS0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
             tc_fence_after();
@@ -806,10 +824,10 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 for (int i = 0; i < kSub; ++i)
                     if (i >= left) r[i] = 0xff800000u;
                 // rows past the prefix may hold anything, and zero times a NaN is none: V's are cleared
-                const int T = U >> 1, st = T % kTcStages;
-                if (!mbar_wait_bounded(full0 + 8 * st, (T / kTcStages) & 1)) { ok = false; break; }
-                if (row >= left && row < kSub) {
-                    uint4 * v = reinterpret_cast<uint4 *>(smem_gen + (sKV - smem_base) + st * kTcStage + kKeys * 128 + ((U & 1) * kSub + row) * 128);
+                const int st = U % kTcStages;
+                if (!mbar_wait_bounded(full0 + 8 * st, (U / kTcStages) & 1)) { ok = false; break; }
+                if (tid >= left && tid < kSub) {
+                    uint4 * v = reinterpret_cast<uint4 *>(smem_gen + (sKV - smem_base) + st * kTcStage + (kSub + tid) * 128);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
@@ -822,7 +840,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 t1 = max3(t1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
             }
             const float top = fmaxf(t0, t1);
-            if (U < 2) {
+            if (U == 0) {
                 m = top;
             } else {
                 const bool raise = top > m + 8.0f;
@@ -830,8 +848,8 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     const float f = raise ? ex2_approx(m - top) : 1.0f;
                     if (raise) m = top;
                     l *= f;
-                    // the accumulator is at rest once P.V of the group's last tile has retired
-                    if (!mbar_wait_bounded(bF0 + 8 * ((U - 2) % kSBufs), ((U - 2) / kSBufs) & 1)) { ok = false; break; }
+                    // the accumulator is at rest once P.V of the tile before has retired
+                    if (!mbar_wait_bounded(bF0 + 8 * ((U - 1) % kSBufs), ((U - 1) / kSBufs) & 1)) { ok = false; break; }
                     rescale_row(t_o, f);
                 }
             }
@@ -859,28 +877,27 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
         if (ok && n_sub > 0 && !mbar_wait_bounded(bO, 0)) ok = false;
         if (!ok) give_up();
-        all_ok = named_bar_all(1, 256, ok && !aborted());  // every copy has been consumed: the ring's memory is free
-        if (all_ok) {
+        all_ok = named_bar_all(1, kJoin, ok && !aborted());  // every copy has been consumed: the ring's memory is free
+        if (all_ok && n_sub > 0) {
             tc_fence_after();
-            float4 * const part = reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)) + (group * kRows + row) * kPartPitch;
-            if (group >= n_sub) {  // a group without keys
+            float4 * const part = reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)) + tid * kPartPitch;
 #pragma unroll
-                for (int c = 0; c < 16; ++c) part[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-            } else {
-                uint32_t r[64];
-                tmem_ld64_sync(t_o, r);
+            for (int h = 0; h < 2; ++h) {
+                uint32_t r[32];
+                tmem_ld32_sync(t_o + 32 * h, r);
 #pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    part[c] = make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3]));
+                for (int c = 0; c < 8; ++c)
+                    part[8 * h + c] = make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3]));
             }
-            ml[group * kRows + row] = make_float2(m - kTcShift, l);
+            ml[tid] = make_float2(m - kTcShift, l);
         }
     }
-    join_and_write(p, w, reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)), ml, joined, rows_at, 2, kRows, all_ok, tid);
+    // (the queries' tiles are done with: every score has been used)
+    join_and_write(p, w, reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)), ml, joined, rows_at, reinterpret_cast<float4 *>(smem_gen), 1, kRows, all_ok, tid);
     // common exit: every role has left its loop; release TMEM
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 4) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -901,39 +918,40 @@ int arrange(vox_prefix_plan * pl, const int32_t * prefix_of) {
     for (int s = 0; s < pl->n_streams; ++s)
         VOX_REQUIRE(prefix_of[s] >= -1 && prefix_of[s] < pl->n_prefixes, VOX_ATTN_INVALID_ARGUMENT,
                     "prefix_of[%d] = %d: not a prefix in [0, %d), nor -1", s, prefix_of[s], pl->n_prefixes);
-    std::vector<int32_t> start;
+    std::vector<int32_t> start, count;
     try {
-        start.assign((size_t) pl->n_prefixes + 1, 0);
+        start.assign((size_t) pl->n_prefixes, 0);
+        count.assign((size_t) pl->n_prefixes, 0);
         pl->next.assign((size_t) pl->n_prefixes, 0);
         pl->host.assign(pl->words(), 0);
     } catch (const std::exception &) {
         set_error("out of host memory");
         return VOX_ATTN_OUT_OF_MEMORY;
     }
-    int32_t * h = pl->host.data();
-    // start[g]: streams of the prefixes before g; then, as they are placed, how far prefix g has come
     for (int s = 0; s < pl->n_streams; ++s)
-        if (prefix_of[s] >= 0) start[prefix_of[s] + 1] += 1;
-    const int per_tile = pl->per_tile();
-    int       placed   = 0, n_tiles = 0;
-    for (int g = 0; g < pl->n_prefixes; ++g) {  // from counts to first tiles
-        const int n = start[g + 1];
-        start[g]    = n_tiles;
-        for (int left = n; left > 0; left -= per_tile, ++n_tiles) {
-            h[2 * (size_t) n_tiles]     = g;
-            h[2 * (size_t) n_tiles + 1] = std::min(left, per_tile);
+        if (prefix_of[s] >= 0) count[prefix_of[s]] += 1;
+    for (int k = 0; k < 2; ++k) {
+        const int per_tile = pl->per_tile(k);
+        int32_t * tiles = pl->host.data() + pl->tiles_at(k), * members = pl->host.data() + pl->members_at(k);
+        int       placed = 0, n_tiles = 0;
+        for (int g = 0; g < pl->n_prefixes; ++g) {
+            start[g]    = n_tiles;
+            pl->next[g] = 0;
+            for (int left = count[g]; left > 0; left -= per_tile, ++n_tiles) {
+                tiles[2 * (size_t) n_tiles]     = g;
+                tiles[2 * (size_t) n_tiles + 1] = std::min(left, per_tile);
+            }
+            placed += count[g];
         }
-        placed += n;
+        for (int s = 0; s < pl->n_streams; ++s) {
+            const int g = prefix_of[s];
+            if (g < 0) continue;
+            const int j = pl->next[g]++;
+            members[(size_t) (start[g] + j / per_tile) * per_tile + j % per_tile] = s;
+        }
+        pl->n_tiles[k] = n_tiles;
+        if (k == 0) pl->full = 2 * placed > n_tiles * per_tile;
     }
-    std::vector<int32_t> & next = pl->next;
-    for (int s = 0; s < pl->n_streams; ++s) {
-        const int g = prefix_of[s];
-        if (g < 0) continue;
-        const int j = next[g]++, tile = start[g] + j / per_tile;
-        h[pl->members_at() + (size_t) tile * per_tile + j % per_tile] = s;
-    }
-    pl->n_tiles = n_tiles;
-    pl->full    = 2 * placed > n_tiles * per_tile;
     return VOX_ATTN_OK;
 }
 
@@ -980,7 +998,7 @@ int vox_prefix_plan_create(vox_engine * e, int n_streams, int n_prefixes, int n_
     VOX_REQUIRE(pl != nullptr, VOX_ATTN_OUT_OF_MEMORY, "out of host memory");
     pl->e = e; pl->n_streams = n_streams; pl->n_prefixes = n_prefixes; pl->gqa = n_heads / n_kv_heads;
     // full tiles, and one that is not full for every prefix in use
-    pl->max_tiles = n_streams / (kRows / pl->gqa) + std::min(n_streams, n_prefixes);
+    for (int k = 0; k < 2; ++k) pl->max_tiles[k] = n_streams / pl->per_tile(k) + std::min(n_streams, n_prefixes);
     int rc = arrange(pl, prefix_of);
     if (rc == VOX_ATTN_OK) {
         cudaError_t err = cudaMalloc(reinterpret_cast<void **>(&pl->dev), pl->words() * sizeof(int32_t));
@@ -1040,7 +1058,7 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     const size_t            own = aligned(decode_shared_workspace_bytes(a->own.n_streams, a->own.n_heads, HK, a->own.kv_bound));
     const bool              shares = pl != nullptr && a->prefix_bound > 0;
     float2 * const          ml  = shares ? reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + own) : nullptr;
-    rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml}, workspace, own, st);
+    rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml, shares}, workspace, own, st);
     if (rc != VOX_ATTN_OK || !shares) return rc;
     const vox_kv_cache * pc = a->prefix;
     const bool           q8 = pc->cfg.type == VOX_TYPE_Q8_0, tc = !q8 && pl->full;
@@ -1048,11 +1066,12 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     p.q = reinterpret_cast<const uint8_t *>(a->own.q);
     p.q_nb_head = a->own.q_nb_head; p.q_nb_stream = a->own.q_nb_stream;
     p.rope    = reinterpret_cast<const float2 *>(a->own.rope_table);
-    p.tiles   = reinterpret_cast<const int2 *>(pl->dev);
-    p.members = pl->dev + pl->members_at();
+    const int k = tc ? 0 : 1;
+    p.tiles   = reinterpret_cast<const int2 *>(pl->dev + pl->tiles_at(k));
+    p.members = pl->dev + pl->members_at(k);
     p.len     = a->prefix_len;
-    p.per_tile = pl->per_tile(); p.n_kv_heads = HK; p.n_heads = a->own.n_heads; p.gqa = pl->gqa; p.layer = a->own.layer; p.max_len = pc->cfg.max_len;
-    p.cluster    = cluster_size(std::min(kDecodeMaxSms, e->sm_count), pl->n_tiles, HK, a->prefix_bound, pl->full);
+    p.per_tile = pl->per_tile(k); p.n_kv_heads = HK; p.n_heads = a->own.n_heads; p.gqa = pl->gqa; p.layer = a->own.layer; p.max_len = pc->cfg.max_len;
+    p.cluster    = cluster_size(std::min(kDecodeMaxSms, e->sm_count), pl->n_tiles[k], HK, a->prefix_bound, tc);
     p.scale_log2 = a->own.scale * 1.4426950408889634f;
     p.q8_tiles   = pc->k_data + (size_t) a->own.layer * pc->nb_layer;
     p.q8_nb_head = pc->nb_head; p.q8_nb_stream = pc->nb_stream;
@@ -1068,7 +1087,7 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
         e->attr_mask |= bit;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) (pl->max_tiles * HK * p.cluster)); cfg.blockDim = dim3(tc ? kTcThreads : kThreads);
+    cfg.gridDim = dim3((unsigned) (pl->max_tiles[k] * HK * p.cluster)); cfg.blockDim = dim3(tc ? kTcThreads : kThreads);
     cfg.dynamicSmemBytes = (size_t) smem; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
