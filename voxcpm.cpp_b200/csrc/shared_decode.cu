@@ -29,25 +29,27 @@ using namespace vox;
 
 namespace {
 constexpr int kRows = 128;       // rows of a full row tile
-constexpr int kHalfRows = 64;    // of a row tile for the mma.sync kernel
+constexpr int kHalfRows = 64;    // of the largest one for the mma.sync kernel
+constexpr int kArrangements = 4; // row tiles of 128, 64, 32 and 16 rows
 constexpr int kJoin = 128;       // threads that join results
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kMaxCluster = 8;
 }
 
-// The streams of a call, arranged by prefix, twice: into row tiles of 128 rows ([0]) and of 64 ([1]).  Host copy and device
-// arrays (one allocation) of either:
+// The streams of a call, arranged by prefix into row tiles of 128 >> k rows, k = 0 .. 3: few streams are cut into small tiles,
+// whose products take less time.  Host copy and device arrays (one allocation), per k:
 //   tiles [max_tiles][2] = prefix, streams (0: not in use);  members [max_tiles][rows / gqa]: their streams
 struct vox_prefix_plan {
     vox_engine *         e = nullptr;
-    int                  n_streams = 0, n_prefixes = 0, gqa = 0, max_tiles[2] = {0, 0}, n_tiles[2] = {0, 0};
+    int                  n_streams = 0, n_prefixes = 0, gqa = 0;
+    int                  max_tiles[kArrangements] = {}, n_tiles[kArrangements] = {};
+    size_t               at[kArrangements + 1] = {};  // where an arrangement starts
     bool                 full = false;  // the tiles of 128 rows are more than half full on average
     std::vector<int32_t> host, next;    // next: scratch of the arrangement
     int32_t *            dev = nullptr;
-    int    per_tile(int k) const { return (k ? kHalfRows : kRows) / gqa; }
-    size_t tiles_at(int k) const { return k ? (members_at(0) + (size_t) max_tiles[0] * per_tile(0) + 1) & ~(size_t) 1 : 0; }
-    size_t members_at(int k) const { return tiles_at(k) + (size_t) max_tiles[k] * 2; }
-    size_t words() const { return members_at(1) + (size_t) max_tiles[1] * per_tile(1); }
+    int    per_tile(int k) const { return (kRows >> k) / gqa; }
+    size_t members_at(int k) const { return at[k] + (size_t) max_tiles[k] * 2; }
+    size_t words() const { return at[kArrangements]; }
 };
 
 namespace {
@@ -96,8 +98,6 @@ __device__ __forceinline__ Item load_item(const SharedParams & p) {
 // bytes against bank conflicts) and ml[v], where v = group * stride + row and a row has a result from every one of
 // `groups` groups of warps.  kJoin threads take part; the others only arrive at the cluster barriers.
 constexpr int kPartPitch = 17;
-constexpr int kMlWords   = kRows / 2 + kMaxCluster * kRows / 4;  // ml: a row's (max, sum) each, later those of a share and its weights
-static_assert(kMlWords >= kRows, "ml");
 
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -169,36 +169,37 @@ __device__ __forceinline__ void join_and_write(const SharedParams & p, const Ite
         cluster_sync_all();
         if (mine) {
             const uint32_t joined0 = smem_u32(joined), part0 = smem_u32(part);
-            float * const  f = reinterpret_cast<float *>(ml + kRows / 2);  // [rank][64]: a share is at most 64 rows, whose ml lies below
-            if (tid < n_rows) {
-                float M = -INFINITY, L = 0.0f;
-#pragma unroll 4
-                for (int r = 0; r < p.cluster; ++r) M = fmaxf(M, peer_ld2(peer_addr(joined0 + (row0 + tid) * 8, r)).x);
-#pragma unroll 4
-                for (int r = 0; r < p.cluster; ++r) {
-                    const float2 x = peer_ld2(peer_addr(joined0 + (row0 + tid) * 8, r));
-                    const float  wt = part_weight(x.x, M);
-                    L = fmaf(x.y, wt, L);
-                    // a part without keys was never written (and a row of NaN has a part, of weight NaN)
-                    f[r * (kRows / 2) + tid] = x.x == -INFINITY && x.y == 0.0f ? -1.0f : x.y != x.y ? x.y : wt;
-                }
-                ml[tid] = make_float2(M, L);
-            }
-            named_bar_sync(1, kJoin);
+#pragma unroll 1
             for (int i = tid; i < n_rows * 16; i += kJoin) {
                 const int row = i >> 4, c = i & 15;
-                float4    a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                for (int r = 0; r < p.cluster; ++r) {
-                    const float wt = f[r * (kRows / 2) + row];
-                    if (wt == -1.0f) continue;
-                    const float4 x = peer_ld4(peer_addr(part0 + ((row0 + row) * kPartPitch + c) * 16, r));
-                    a = make_float4(fmaf(x.x, wt, a.x), fmaf(x.y, wt, a.y), fmaf(x.z, wt, a.z), fmaf(x.w, wt, a.w));
+                float2    m[kMaxCluster];
+                float4    x[kMaxCluster];
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) {  // all on their way together
+                    m[r] = make_float2(-INFINITY, 0.0f);
+                    x[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r < p.cluster) {
+                        m[r] = peer_ld2(peer_addr(joined0 + (row0 + row) * 8, r));
+                        x[r] = peer_ld4(peer_addr(part0 + ((row0 + row) * kPartPitch + c) * 16, r));
+                    }
+                }
+                float  M = -INFINITY, L = 0.0f;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) M = fmaxf(M, m[r].x);
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) {
+                    if (m[r].x == -INFINITY && m[r].y == 0.0f) continue;  // a part without keys was never written
+                    const float f = part_weight(m[r].x, M);
+                    L = fmaf(m[r].y, f, L);
+                    a = make_float4(fmaf(x[r].x, f, a.x), fmaf(x[r].y, f, a.y), fmaf(x[r].z, f, a.z), fmaf(x[r].w, f, a.w));
                 }
                 share[row * kPartPitch + c] = a;
+                if (c == 0) ml[row] = make_float2(M, L);
             }
+            named_bar_sync(1, kJoin);
         }
-        cluster_sync_all();  // nobody's shared memory is read any longer by another CTA
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for at the end: nobody leaves while its memory is read
     } else {
         share = part;
         ml    = joined;
@@ -206,10 +207,9 @@ __device__ __forceinline__ void join_and_write(const SharedParams & p, const Ite
     }
     pdl_wait();  // the decode kernel's results
     pdl_launch_dependents();
-    if (!mine) return;
     constexpr int W = 4;  // a thread's rows in flight: a row at a time would wait for L2 once per row
 #pragma unroll 1
-    for (int i0 = tid; i0 < n_rows * 16; i0 += W * kJoin) {
+    for (int i0 = tid; mine && i0 < n_rows * 16; i0 += W * kJoin) {
         float2 own_ml[W];
         float4 own[W];
 #pragma unroll
@@ -233,6 +233,8 @@ __device__ __forceinline__ void join_and_write(const SharedParams & p, const Ite
             if (c == 0 && p.lse != nullptr) p.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
         }
     }
+    __syncwarp();
+    if (p.cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -448,7 +450,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * R::kStages];
     __shared__ int      abort_flag;
-    __shared__ float2   ml[kMlWords], joined[kRows];
+    __shared__ float2   ml[kRows], joined[kRows];
     __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     float4 * const part      = reinterpret_cast<float4 *>(smem_raw + (smem_base - smem_u32(smem_raw)));
@@ -652,7 +654,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int      abort_flag;
-    __shared__ float2   ml[kMlWords], joined[kRows];
+    __shared__ float2   ml[kRows], joined[kRows];
     __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -904,10 +906,19 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 }
 
 // CTAs per (row tile, kv head): as many as fill the SMs once, eight at most.  A second, thinner wave costs more than SMs left
-// idle.  No more than the prefix has tiles, but four where row tiles are full: the CTAs also share out the rows to be joined.
-int cluster_size(int sms, int n_tiles, int n_kv_heads, int prefix_bound, bool full) {
-    const int useful = std::max((prefix_bound + kKeys - 1) / kKeys, full ? 4 : 1);
+// idle.  No more than the prefix has tiles of keys, but four where row tiles are full: the CTAs also share out the rows.
+int cluster_size(int sms, int n_tiles, int n_kv_heads, int n_keys, bool full) {
+    const int useful = std::max((n_keys + kKeys - 1) / kKeys, full ? 4 : 1);
     return std::max(1, std::min(std::min(kMaxCluster, sms / std::max(1, n_tiles * n_kv_heads)), useful));
+}
+
+// The arrangement for the mma.sync kernel: the smallest row tiles whose CTAs still fit the SMs once with the keys cut as
+// finely as can be.  A warp works on 16 rows, so smaller tiles leave every warp fewer keys.
+int small_arrangement(const vox_prefix_plan * pl, int sms, int n_kv_heads, int n_keys) {
+    const int finest = std::min(kMaxCluster, (n_keys + kKeys - 1) / kKeys);
+    for (int k = kArrangements - 1; k > 1; --k)
+        if (pl->n_tiles[k] * n_kv_heads * finest <= sms) return k;
+    return 1;
 }
 
 size_t aligned(size_t n) { return (n + 255) & ~(size_t) 255; }
@@ -930,9 +941,9 @@ int arrange(vox_prefix_plan * pl, const int32_t * prefix_of) {
     }
     for (int s = 0; s < pl->n_streams; ++s)
         if (prefix_of[s] >= 0) count[prefix_of[s]] += 1;
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kArrangements; ++k) {
         const int per_tile = pl->per_tile(k);
-        int32_t * tiles = pl->host.data() + pl->tiles_at(k), * members = pl->host.data() + pl->members_at(k);
+        int32_t * tiles = pl->host.data() + pl->at[k], * members = pl->host.data() + pl->members_at(k);
         int       placed = 0, n_tiles = 0;
         for (int g = 0; g < pl->n_prefixes; ++g) {
             start[g]    = n_tiles;
@@ -998,7 +1009,10 @@ int vox_prefix_plan_create(vox_engine * e, int n_streams, int n_prefixes, int n_
     VOX_REQUIRE(pl != nullptr, VOX_ATTN_OUT_OF_MEMORY, "out of host memory");
     pl->e = e; pl->n_streams = n_streams; pl->n_prefixes = n_prefixes; pl->gqa = n_heads / n_kv_heads;
     // full tiles, and one that is not full for every prefix in use
-    for (int k = 0; k < 2; ++k) pl->max_tiles[k] = n_streams / pl->per_tile(k) + std::min(n_streams, n_prefixes);
+    for (int k = 0; k < kArrangements; ++k) {
+        pl->max_tiles[k] = n_streams / pl->per_tile(k) + std::min(n_streams, n_prefixes);
+        pl->at[k + 1] = (pl->members_at(k) + (size_t) pl->max_tiles[k] * pl->per_tile(k) + 1) & ~(size_t) 1;  // 8-byte pairs
+    }
     int rc = arrange(pl, prefix_of);
     if (rc == VOX_ATTN_OK) {
         cudaError_t err = cudaMalloc(reinterpret_cast<void **>(&pl->dev), pl->words() * sizeof(int32_t));
@@ -1066,12 +1080,12 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     p.q = reinterpret_cast<const uint8_t *>(a->own.q);
     p.q_nb_head = a->own.q_nb_head; p.q_nb_stream = a->own.q_nb_stream;
     p.rope    = reinterpret_cast<const float2 *>(a->own.rope_table);
-    const int k = tc ? 0 : 1;
-    p.tiles   = reinterpret_cast<const int2 *>(pl->dev + pl->tiles_at(k));
+    const int sms = std::min(kDecodeMaxSms, e->sm_count), k = tc ? 0 : small_arrangement(pl, sms, HK, a->prefix_bound);
+    p.tiles   = reinterpret_cast<const int2 *>(pl->dev + pl->at[k]);
     p.members = pl->dev + pl->members_at(k);
     p.len     = a->prefix_len;
     p.per_tile = pl->per_tile(k); p.n_kv_heads = HK; p.n_heads = a->own.n_heads; p.gqa = pl->gqa; p.layer = a->own.layer; p.max_len = pc->cfg.max_len;
-    p.cluster    = cluster_size(std::min(kDecodeMaxSms, e->sm_count), pl->n_tiles[k], HK, a->prefix_bound, tc);
+    p.cluster    = cluster_size(sms, pl->n_tiles[k], HK, a->prefix_bound, tc);
     p.scale_log2 = a->own.scale * 1.4426950408889634f;
     p.q8_tiles   = pc->k_data + (size_t) a->own.layer * pc->nb_layer;
     p.q8_nb_head = pc->nb_head; p.q8_nb_stream = pc->nb_stream;
