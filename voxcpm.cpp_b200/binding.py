@@ -238,6 +238,19 @@ def _stream_ptr(stream):
     return C.c_void_p(stream if isinstance(stream, int) else stream.cuda_stream)
 
 
+def _raw_stream(device: int) -> int:
+    """The current stream of a device as an address (torch.cuda.current_stream builds an object: 3 us)."""
+    global _raw_stream
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _raw_stream = get if get is not None else lambda d: torch.cuda.current_stream(d).cuda_stream
+    return _raw_stream(device)
+
+
+def _addr(x):
+    return None if x is None else x.data_ptr()
+
+
 def attn_args(q, k, v, dst, mask=None, scale=0.125, k_type=None, v_type=None) -> AttnArgs:
     a = AttnArgs()
     a.q = Tensor.from_torch(q)
@@ -298,6 +311,18 @@ class Engine:
         if self._ws is None or self._ws.numel() < nbytes:
             self._ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=f"cuda:{self.device}")
         return self._ws
+
+    def _run(self, call, args, size, workspace, stream):
+        """One call with a workspace: the caller's, or the engine's, which grows when the call says that it is too small (asking
+        for the size every time costs a third of what the launch does)."""
+        ptr = C.byref(args)
+        st = _raw_stream(self.device) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+        ws = workspace if workspace is not None else self._ws if self._ws is not None else self.workspace(1 << 16)
+        rc = call(self.h, ptr, ws.data_ptr(), ws.numel(), st)
+        if rc == 3 and workspace is None:
+            ws = self.workspace(size(ptr))
+            rc = call(self.h, ptr, ws.data_ptr(), ws.numel(), st)
+        _check(rc)
 
     def forward(self, q, k, v, mask=None, scale=0.125, stream=None, dst=None):
         """``ggml_flash_attn_ext`` on device tensors: q [B,H,n_q,64] f32, k/v [B,HK,n_kv,*],
@@ -518,19 +543,17 @@ class KVCache:
         """``vox_attn_decode_shared``: as ``decode``, over the rows of a prefix that several streams share and the streams' own.
         ``prefix``: the KVCache that holds the prefixes; ``plan``: a PrefixPlan; ``prefix_len`` int32 device [prefixes];
         ``lse`` [n_streams, H] f32 receives the log-sum-exp.  Returns [n_streams, H, 64]."""
-        import torch
         S, H, D = q.shape
         if dst is None:
-            dst = torch.empty((S, H, D), dtype=torch.float32, device=q.device)
-        a = DecodeSharedArgs()
-        a.own = self._decode_args(layer, q, kv_len, kv_bound, dst, scale, k_new, v_new, cache_stable, rope_table, None)
-        a.prefix = prefix.h if prefix is not None else None
-        a.plan = plan.h if plan is not None else None
-        a.prefix_len = prefix_len.data_ptr() if prefix_len is not None else None
-        a.prefix_bound = prefix_bound
-        a.lse = lse.data_ptr() if lse is not None else None
-        ws = workspace if workspace is not None else self.engine.workspace(lib().vox_attn_decode_shared_workspace_bytes(C.byref(a)))
-        _check(lib().vox_attn_decode_shared(self.engine.h, C.byref(a), C.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(stream)))
+            dst = q.new_empty((S, H, D))
+        q_s = q.stride()
+        n_s = k_new.stride() if k_new is not None else (0, 0)
+        own = DecodeArgs(self.h, layer, S, H, kv_len.data_ptr(), kv_bound, q.data_ptr(), q_s[1] * 4, q_s[0] * 4, dst.data_ptr(), scale,
+                         _addr(k_new), _addr(v_new), n_s[1] * 4, n_s[0] * 4, 1 if cache_stable else 0, _addr(rope_table), None)
+        a = DecodeSharedArgs(own, prefix.h if prefix is not None else None, plan.h if plan is not None else None, _addr(prefix_len),
+                             prefix_bound, _addr(lse))
+        L = lib()
+        self.engine._run(L.vox_attn_decode_shared, a, L.vox_attn_decode_shared_workspace_bytes, workspace, stream)
         return dst
 
     def observe(self, layer, q, kv_len, kv_bound, score, row_pos=None, n_seen=None, n_new=1, lse=None, decay=1.0, scale=0.125,
@@ -539,27 +562,23 @@ class KVCache:
         every row to ``score`` [n_streams, HK, rows] f32, and notes the positions of the ``n_new`` new rows in ``row_pos``
         (int32, the same shape and strides)."""
         S, n_q, H, D = q.shape
-        a = ObserveArgs(self.h, layer, S, H, n_q, kv_len.data_ptr(), n_seen.data_ptr() if n_seen is not None else None, kv_bound, q.data_ptr(),
-                        q.stride(2) * 4, q.stride(1) * 4, q.stride(0) * 4)
-        a.rope_table = rope_table.data_ptr() if rope_table is not None else None
-        a.lse = lse.data_ptr() if lse is not None else None
-        a.scale, a.decay, a.n_new = scale, decay, n_new
-        a.score = score.data_ptr()
-        a.row_pos = row_pos.data_ptr() if row_pos is not None else None
-        assert score.stride(-1) == 1 and (row_pos is None or row_pos.stride() == score.stride())
-        a.nb_head, a.nb_stream = score.stride(-2) * 4, score.stride(-3) * 4
-        ws = workspace if workspace is not None else self.engine.workspace(lib().vox_kv_observe_workspace_bytes(C.byref(a)))
-        _check(lib().vox_kv_observe(self.engine.h, C.byref(a), C.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(stream)))
+        q_s, s_s = q.stride(), score.stride()
+        assert s_s[-1] == 1 and (row_pos is None or row_pos.stride() == s_s)
+        a = ObserveArgs(self.h, layer, S, H, n_q, kv_len.data_ptr(), _addr(n_seen), kv_bound, q.data_ptr(), q_s[2] * 4, q_s[1] * 4, q_s[0] * 4,
+                        _addr(rope_table), _addr(lse), scale, decay, n_new, score.data_ptr(), _addr(row_pos), s_s[-2] * 4, s_s[-3] * 4)
+        L = lib()
+        self.engine._run(L.vox_kv_observe, a, L.vox_kv_observe_workspace_bytes, workspace, stream)
 
     def evict(self, kv_len, kv_bound, budget, score, row_pos, n_seen, new_len, n_sink=4, n_recent=32, kept=None, layer0=0, stream=None):
         """``vox_kv_evict``: cuts the streams' rows to ``budget`` by ``score`` in the layers that ``score`` and ``row_pos``
         [n_layers, n_streams, HK, rows] span; ``new_len`` int32 [n_streams] receives the lengths, ``kept`` (int32
         [n_layers, n_streams, HK, budget], optional) the rows' former indices."""
-        assert score.stride(-1) == 1 and row_pos.stride() == score.stride() and (kept is None or kept.is_contiguous())
-        a = EvictArgs(self.h, layer0, score.shape[0], score.shape[1], kv_len.data_ptr(), n_seen.data_ptr() if n_seen is not None else None,
-                      kv_bound, budget, n_sink, n_recent, score.data_ptr(), row_pos.data_ptr(), score.stride(2) * 4, score.stride(1) * 4,
-                      score.stride(0) * 4, new_len.data_ptr(), kept.data_ptr() if kept is not None else None)
-        _check(lib().vox_kv_evict(self.engine.h, C.byref(a), _stream_ptr(stream)))
+        s_s = score.stride()
+        assert s_s[3] == 1 and row_pos.stride() == s_s and (kept is None or kept.is_contiguous())
+        a = EvictArgs(self.h, layer0, score.shape[0], score.shape[1], kv_len.data_ptr(), _addr(n_seen), kv_bound, budget, n_sink, n_recent,
+                      score.data_ptr(), row_pos.data_ptr(), s_s[2] * 4, s_s[1] * 4, s_s[0] * 4, new_len.data_ptr(), _addr(kept))
+        st = _raw_stream(self.engine.device) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+        _check(lib().vox_kv_evict(self.engine.h, C.byref(a), st))
 
 
 class PrefixPlan:
