@@ -545,9 +545,27 @@ class EvictCase:
     ([600, 512, 530], 8, 0, 0),
     ([600, 512, 530], 8, 8, 0),
     ([600, 512, 530], 40, 0, 40),
+    ([5000, 4100], 4000, 4, 32),
+    ([700, 701, 699, 3, 702], 699, 4, 690),
+    ([9, 10, 11, 12, 8, 7], 8, 1, 2),
+    ([5, 4, 3, 2, 1, 0], 1, 0, 0),
+    ([1025, 1026, 1027, 1028], 1024, 4, 32),
+    ([5000, 2100], 900, 4, 32),
 ])
 def test_eviction_matches_the_definition(kind, lens, budget, n_sink, n_recent, engine, pkg):
     EvictCase(engine, pkg, kind, lens, 2, 2, max(lens) + 9).check(budget, n_sink, n_recent)
+
+
+@pytest.mark.parametrize("budget", [24000, 49000, 50])
+@pytest.mark.parametrize("spread", ["ties", "close", "wide"])
+def test_eviction_from_the_longest_row_lists(budget, spread, engine, pkg):
+    """Lists whose keys do not fit shared memory beside the moving rows (24000 of 49152), scores that are all alike, that differ in
+    their last bits alone, and that span all magnitudes."""
+    import torch
+    c = EvictCase(engine, pkg, "f16", [49152], 1, 1, 49152)
+    w = torch.rand(c.score.shape, generator=gen(2), device="cuda")
+    c.score.copy_({"ties": torch.where(w < 0.7, 0.25, 0.5), "close": 1 + (w * 3000).floor() * 2.0 ** -23, "wide": torch.exp2(w * 250 - 125)}[spread])
+    c.check(budget, 4, 32)
 
 
 @pytest.mark.parametrize("heads", [1, 3])

@@ -1,9 +1,15 @@
 // Eviction from the cache by accumulated attention weight (vox_kv_evict).
 //
 // Per (layer, stream, kv head) with more rows than the budget: the `budget` largest keys stay (a key orders the rows as the
-// contract does: protected rows above every score, scores as numbers, NaN below), found by a radix select over the keys;
-// then the i-th kept row at or above the budget moves to the i-th place below it whose row goes.  Sources and
-// destinations never overlap, so rows move in place and in any order.
+// contract does: protected rows above every score, scores as numbers, NaN below; equal keys by index), then the i-th kept
+// row at or above the budget moves to the i-th place below it whose row goes.  Sources and destinations never overlap, so
+// rows move in place and in any order.
+//
+// One CTA per row list, keys in shared memory.  The border between what stays and what goes is found by a histogram of the
+// keys' top 11 bits (sign, exponent and two bits of the mantissa: a bin is a quarter of an octave) and, as a rule, by ranking the few
+// hundred keys of the bin it falls in against one another; only a bin with more keys than that (many equal scores) is cut
+// further, 11 and 10 bits at a time.  Lists are few when one stream is cut: then a cluster of CTAs takes each, every CTA
+// selecting for itself (the scores are in L2) and moving a share of the rows.
 #include "kv_cache.cuh"
 
 #include <algorithm>
@@ -12,14 +18,20 @@ using namespace vox;
 
 namespace {
 
-constexpr int kThreads  = 512;
-constexpr int kMaxRows  = 49152;   // the two lists of moving rows fit shared memory up to here
+constexpr int kThreads   = 256;
+constexpr int kWarps     = kThreads / 32;
+constexpr int kBits      = 11;
+constexpr int kBins      = 1 << kBits;
+constexpr int kRanked    = 96;       // keys of a bin that are ranked against one another
+constexpr int kMaxRows   = 49152;    // rows are numbered in 16 bits in the lists of moving rows
+constexpr size_t kSmemMost = 200 * 1024;  // keys that fit stay in shared memory; those of longer row lists are made again
+constexpr int kMaxCluster = 8;
 
 struct EvictParams {
     uint8_t * k_data;
     uint8_t * v_data;
     size_t    c_nb_head, c_nb_stream, c_nb_layer;
-    int       q8, layer0, n_kv_heads, n_streams, kv_bound, budget, n_sink, n_recent, n_list;
+    int       q8, layer0, n_kv_heads, n_streams, kv_bound, budget, n_sink, n_recent, n_list, keys_kept, cluster;
     const int32_t * kv_len;
     const int32_t * n_seen;
     uint8_t * score;
@@ -37,8 +49,17 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// exclusive prefix sums over the block of two counts packed in one word, and their total
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t * warp_sums, uint32_t & total) {
+// one of the eight 16-byte pieces of a q8_0 row: four of K, four of V; the first of either also takes its two scales
+__device__ __forceinline__ void move_q8_piece(uint8_t * pair, int from, int to, int piece) {
+    const uint32_t  bytes = piece & 4 ? kQ8VBytesOff : 0, scales = piece & 4 ? kQ8VScaleOff : kQ8KScaleOff;
+    const uint8_t * a = pair + q8_tile_off(from);
+    uint8_t *       b = pair + q8_tile_off(to);
+    *reinterpret_cast<uint4 *>(b + bytes + q8_byte_off(to, 16 * (piece & 3))) = *reinterpret_cast<const uint4 *>(a + bytes + q8_byte_off(from, 16 * (piece & 3)));
+    if ((piece & 3) == 0) *reinterpret_cast<uint32_t *>(b + scales + q8_scale_off(to, 0)) = *reinterpret_cast<const uint32_t *>(a + scales + q8_scale_off(from, 0));
+}
+
+// Exclusive prefix sums over the block, and their total.  Two buffers of warp sums in turn, so that one barrier is enough.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t (*warp_sums)[kWarps], int & turn, uint32_t & total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t  incl = x;
 #pragma unroll
@@ -46,12 +67,13 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t * warp_sums,
         const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += y;
     }
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = incl;
+    turn ^= 1;
+    if (lane == 31) warp_sums[turn][warp] = incl;
     __syncthreads();
     uint32_t before = 0, all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-        const uint32_t s = warp_sums[w];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const uint32_t s = warp_sums[turn][w];
         if (w < warp) before += s;
         all += s;
     }
@@ -59,12 +81,206 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t * warp_sums,
     return before + incl - x;
 }
 
-__global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
-    extern __shared__ int32_t lists[];  // sources, then destinations
-    __shared__ uint32_t hist[256], warp_sums[kThreads / 32], chosen[2];
-    int32_t * const src = lists, * const dst = lists + p.n_list;
+__global__ void __launch_bounds__(kThreads, 6) evict_kernel(const EvictParams p) {
+    extern __shared__ uint32_t smem[];  // keys (if they are kept), then sources and destinations of the rows that move
+    __shared__ uint32_t hist[kBins], warp_sums[2][kWarps], found[3];
+    uint32_t * const keys = smem;
+    uint16_t * const src  = reinterpret_cast<uint16_t *>(smem + (p.keys_kept ? (p.kv_bound + 3) / 4 * 4 : 0)), * const dst = src + p.n_list;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int kvh = blockIdx.x % p.n_kv_heads, stream = (blockIdx.x / p.n_kv_heads) % p.n_streams, layer = blockIdx.x / (p.n_kv_heads * p.n_streams);
+    int turn = 0, rank = 0, list = blockIdx.x;
+    if (p.cluster > 1) {
+        list = blockIdx.x / p.cluster;
+        rank = blockIdx.x - list * p.cluster;
+    }
+    const int kvh = list % p.n_kv_heads, stream = (list / p.n_kv_heads) % p.n_streams, layer = list / (p.n_kv_heads * p.n_streams);
+    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int len = max(0, p.kv_len[stream]);
+    const bool first = kvh == 0 && layer == 0 && rank == 0 && tid == 0;
+    if (len > p.kv_bound) {
+        if (first) { atomicOr(p.status, kStatusBadState); p.new_len[stream] = len; }
+        return;
+    }
+    if (first) p.new_len[stream] = min(len, p.budget);
+    int32_t * const kept = p.kept ? p.kept + (((size_t) layer * p.n_streams + stream) * p.n_kv_heads + kvh) * p.budget : nullptr;
+    if (len <= p.budget) {
+        if (kept && rank == 0) for (int j = tid; j < len; j += kThreads) kept[j] = j;
+        return;
+    }
+    const size_t at = (size_t) layer * p.nb_layer + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head;
+    float *   const score = reinterpret_cast<float *>(p.score + at);
+    int32_t * const pos   = reinterpret_cast<int32_t *>(p.row_pos + at);
+    const int recent = (p.n_seen ? p.n_seen[stream] : len) - p.n_recent;
+    auto make_key = [&](int j) {
+        const int q = pos[j];
+        return q < p.n_sink || q >= recent ? 0xffffffffu : ordered(score[j]);
+    };
+    auto key_of = [&](int j) { return p.keys_kept ? keys[j] : make_key(j); };
+    __syncthreads();
+#pragma unroll 4
+    for (int j = tid; j < len; j += kThreads) {
+        const uint32_t k = make_key(j);
+        if (p.keys_kept) keys[j] = k;
+        atomicAdd(&hist[k >> (32 - kBits)], 1u);
+    }
+    __syncthreads();
+
+    // The border: keys above `edge` stay, and of those equal to it the ones up to index `last`.
+    uint32_t edge = 0, mask = 0;
+    int      last = len, need = p.budget;
+    for (int shift = 32 - kBits;;) {
+        // the bin, from the top, in which the count reaches `need`
+        const int bits = min(kBits, 32 - __popc(mask)), bins = 1 << bits, per = max(1, bins / kThreads);
+        const int top  = bins - 1 - tid * per;
+        uint32_t  mine = 0, total;
+        if (top >= 0)
+            for (int i = 0; i < per; ++i) mine += hist[top - i];
+        uint32_t before = block_scan(mine, warp_sums, turn, total);
+        if (before < (uint32_t) need && before + mine >= (uint32_t) need) {
+            int bin = top;
+            while (before + hist[bin] < (uint32_t) need) before += hist[bin--];
+            found[0] = (uint32_t) bin;
+            found[1] = before;
+            found[2] = hist[bin];
+        }
+        __syncthreads();
+        edge |= found[0] << shift;
+        mask |= (uint32_t) (bins - 1) << shift;
+        need -= (int) found[1];
+        const int n_bin = (int) found[2];
+        if (shift == 0) {
+            if (n_bin > need) {  // equal keys on both sides of the border: the first `need` of them stay
+                __syncthreads();
+                for (int j0 = 0, seen = 0; j0 < len && seen < need; j0 += 4 * kThreads) {
+                    uint32_t count = 0, n;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) count += j0 + 4 * tid + e < len && key_of(j0 + 4 * tid + e) == edge ? 1u : 0u;
+                    uint32_t r = seen + block_scan(count, warp_sums, turn, n);
+                    if (r < (uint32_t) need && r + count >= (uint32_t) need) {
+                        int j = j0 + 4 * tid;
+                        for (;; ++j)
+                            if (key_of(j) == edge && ++r == (uint32_t) need) break;
+                        found[0] = (uint32_t) j;
+                    }
+                    seen += (int) n;
+                }
+                __syncthreads();
+                last = (int) found[0];
+            }
+            break;
+        }
+        __syncthreads();
+        if (n_bin <= kRanked) {  // rank the keys of the bin against one another; the histogram's memory holds them
+            uint32_t * const bin_key = hist, * const bin_row = hist + kRanked;
+            if (tid == 0) found[2] = 0;
+            __syncthreads();
+            for (int j = tid; j < len; j += kThreads) {
+                const uint32_t k = key_of(j);
+                if ((k & mask) == edge) {
+                    const uint32_t i = atomicAdd(&found[2], 1u);
+                    bin_key[i] = k;
+                    bin_row[i] = (uint32_t) j;
+                }
+            }
+            __syncthreads();
+            for (int i = tid; i < n_bin; i += kThreads) {
+                const uint32_t k = bin_key[i], j = bin_row[i];
+                int            above = 0;
+                for (int o = 0; o < n_bin; ++o) above += bin_key[o] > k || (bin_key[o] == k && bin_row[o] < j);
+                if (above == need - 1) {  // the last one that stays
+                    found[0] = k;
+                    found[1] = j;
+                }
+            }
+            __syncthreads();
+            edge = found[0];
+            last = (int) found[1];
+            break;
+        }
+        const int next = max(0, shift - kBits), width = shift - next;
+        for (int i = tid; i < (1 << width); i += kThreads) hist[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < len; j += kThreads) {
+            const uint32_t k = key_of(j);
+            if ((k & mask) == edge) atomicAdd(&hist[(k >> next) & ((1u << width) - 1u)], 1u);
+        }
+        __syncthreads();
+        shift = next;
+    }
+
+    // In index order: the places below the budget whose rows go, the rows above it that stay.  Four rows per thread.
+    uint32_t marks = 0;  // places in the low half, rows in the high half
+    for (int j0 = 0; j0 < len; j0 += 4 * kThreads) {
+        const int j = j0 + 4 * tid;
+        uint32_t  flags = 0, count = 0, n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (j + e >= len) continue;
+            const uint32_t k = key_of(j + e);
+            const bool     stays = k > edge || (k == edge && j + e <= last), low = j + e < p.budget;
+            if (stays != low) {
+                flags |= 1u << e;
+                count += low ? 1u : 0x10000u;
+            }
+            if (kept && low && stays && rank == 0) kept[j + e] = j + e;
+        }
+        uint32_t mark = marks + block_scan(count, warp_sums, turn, n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (!(flags >> e & 1u)) continue;
+            if (j + e < p.budget) {
+                dst[mark & 0xffffu] = (uint16_t) (j + e);
+                mark += 1u;
+            } else {
+                src[mark >> 16] = (uint16_t) (j + e);
+                mark += 0x10000u;
+            }
+        }
+        marks += n;
+    }
+    __syncthreads();
+    if (p.cluster > 1) {  // every CTA of the cluster has read the scores and positions that are about to change
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    const int n_move = (int) (marks & 0xffffu);
+    for (int i = rank * kThreads + tid; i < n_move; i += p.cluster * kThreads) {
+        const int a = src[i], b = dst[i];
+        score[b] = score[a];
+        pos[b]   = pos[a];
+        if (kept) kept[b] = a;
+    }
+    const size_t pair = (size_t) (p.layer0 + layer) * p.c_nb_layer + (size_t) stream * p.c_nb_stream + (size_t) kvh * p.c_nb_head;
+    if (!p.q8) {  // 16 lanes a row: 8 x 16 bytes of K, 8 of V; four rows of a lane in flight
+        uint8_t * const base = (lane & 8 ? p.v_data : p.k_data) + pair + (lane & 7) * 16;
+        const int       pace = 2 * kWarps * p.cluster;
+        constexpr int   U = 4;
+        for (int i = 2 * (rank * kWarps + warp) + (lane >> 4); i < n_move; i += U * pace) {
+            uint4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u * pace < n_move) x[u] = *reinterpret_cast<const uint4 *>(base + (size_t) src[i + u * pace] * 128);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u * pace < n_move) *reinterpret_cast<uint4 *>(base + (size_t) dst[i + u * pace] * 128) = x[u];
+        }
+    } else {      // 8 lanes a row
+#pragma unroll 2
+        for (int i = 4 * (rank * kWarps + warp) + (lane >> 3); i < n_move; i += 4 * kWarps * p.cluster) move_q8_piece(p.k_data + pair, src[i], dst[i], lane & 7);
+    }
+}
+
+// Few rows to give up (a stream that gains a row a step gives one up a step): no border is looked for, the rows that go are,
+// one after the other, by reductions over the block.  They go in the order of their keys, of equal ones the highest
+// index first, so the next is the least of those after the last.
+constexpr int kFew        = 4;
+constexpr int kFewThreads = 128;
+__global__ void __launch_bounds__(kFewThreads, 12) evict_few_kernel(const EvictParams p) {
+    __shared__ uint32_t least_key[2][kFewThreads / 32];
+    __shared__ int      least_row[2][kFewThreads / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, list = blockIdx.x;
+    const int kvh = list % p.n_kv_heads, stream = (list / p.n_kv_heads) % p.n_streams, layer = list / (p.n_kv_heads * p.n_streams);
     pdl_wait();
     pdl_launch_dependents();
     const int len = max(0, p.kv_len[stream]);
@@ -75,95 +291,87 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
     }
     if (first) p.new_len[stream] = min(len, p.budget);
     int32_t * const kept = p.kept ? p.kept + (((size_t) layer * p.n_streams + stream) * p.n_kv_heads + kvh) * p.budget : nullptr;
-    if (len <= p.budget) {
-        if (kept) for (int j = tid; j < len; j += kThreads) kept[j] = j;
-        return;
-    }
     const size_t at = (size_t) layer * p.nb_layer + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head;
     float *   const score = reinterpret_cast<float *>(p.score + at);
     int32_t * const pos   = reinterpret_cast<int32_t *>(p.row_pos + at);
-    const int recent = (p.n_seen ? p.n_seen[stream] : len) - p.n_recent;
-    auto key_of = [&](int j) {
-        const int q = pos[j];
-        return q < p.n_sink || q >= recent ? 0xffffffffu : ordered(score[j]);
+    const int recent = (p.n_seen ? p.n_seen[stream] : len) - p.n_recent, n_go = len - p.budget;
+    int       gone[kFew];
+    uint32_t  last_key = 0;
+    int       last_row = 0x7fffffff;
+#pragma unroll
+    for (int g = 0; g < kFew; ++g) {
+        gone[g] = 0x7fffffff;
+        if (g >= n_go) continue;
+        uint32_t key = 0xffffffffu;
+        int      row = -1;
+#pragma unroll 8
+        for (int j = tid; j < len; j += kFewThreads) {
+            const int      q = pos[j];
+            const float    w = score[j];
+            const uint32_t k = q < p.n_sink || q >= recent ? 0xffffffffu : ordered(w);
+            const bool     later = k > last_key || (k == last_key && j < last_row);
+            if (later && (k < key || (k == key && j > row))) { key = k; row = j; }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const uint32_t k = __shfl_xor_sync(0xffffffffu, key, o);
+            const int      r = __shfl_xor_sync(0xffffffffu, row, o);
+            if (k < key || (k == key && r > row)) { key = k; row = r; }
+        }
+        if (lane == 0) { least_key[g & 1][warp] = key; least_row[g & 1][warp] = row; }
+        __syncthreads();
+#pragma unroll
+        for (int o = 0; o < kFewThreads / 32; ++o) {
+            const uint32_t k = least_key[g & 1][o];
+            const int      r = least_row[g & 1][o];
+            if (o == 0 || k < key || (k == key && r > row)) { key = k; row = r; }
+        }
+        last_key = key;
+        last_row = row;
+        gone[g]  = row;
+    }
+    if (n_go <= 0) {
+        if (kept) for (int j = tid; j < len; j += kFewThreads) kept[j] = j;
+        return;
+    }
+#pragma unroll
+    for (int a = 0; a + 1 < kFew; ++a)  // by index
+#pragma unroll
+        for (int b = 0; b + 1 < kFew - a; ++b) {
+            const int lo = min(gone[b], gone[b + 1]), hi = max(gone[b], gone[b + 1]);
+            gone[b] = lo;
+            gone[b + 1] = hi;
+        }
+    auto goes = [&](int j) {
+        bool g = false;
+#pragma unroll
+        for (int i = 0; i < kFew; ++i) g |= gone[i] == j;
+        return g;
     };
-    // radix select: the largest keys' common byte prefix, a byte per pass; `need` of the keys that match it so far stay
-    uint32_t prefix = 0, mask = 0;
-    int      need   = p.budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < len; j += kThreads) {
-            const uint32_t k = key_of(j);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (warp == 0) {  // the bin, from the top, in which the count reaches `need`
-            uint32_t mine = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) mine += hist[255 - 8 * lane - i];
-            uint32_t incl = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
-            }
-            uint32_t before = incl - mine;
-            if (before < (uint32_t) need && incl >= (uint32_t) need) {
-                int bin = 255 - 8 * lane;
-                while (before + hist[bin] < (uint32_t) need) before += hist[bin--];
-                chosen[0] = (uint32_t) bin;
-                chosen[1] = before;
-            }
-        }
-        __syncthreads();
-        prefix |= chosen[0] << shift;
-        mask   |= 0xffu << shift;
-        need   -= (int) chosen[1];
-        __syncthreads();
-    }
-    // rows above the key `prefix` stay, and the first `need` that have it.  In index order: the places below the budget
-    // whose rows go, the rows above it that stay
-    uint32_t ties = 0, lists_n = 0;  // lists_n: holes in the low half, movers in the high half (both below 2^16)
-    for (int j0 = 0; j0 < len; j0 += kThreads) {
-        const int      j = j0 + tid;
-        const uint32_t k = j < len ? key_of(j) : 0u;
-        const bool     tie = j < len && k == prefix;
-        uint32_t       n_tie, n_list;
-        const uint32_t rank = ties + block_scan(tie ? 1u : 0u, warp_sums, n_tie);
-        const bool     keep = j < len && (k > prefix || (tie && rank < (uint32_t) need));
-        const bool     hole = j < p.budget && !keep, mover = j >= p.budget && keep;
-        const uint32_t mark = lists_n + block_scan((hole ? 1u : 0u) | (mover ? 0x10000u : 0u), warp_sums, n_list);
-        if (hole) dst[mark & 0xffffu] = j;
-        if (mover) src[mark >> 16] = j;
-        if (kept && j < p.budget && keep) kept[j] = j;
-        ties += n_tie;
-        lists_n += n_list;
-    }
-    __syncthreads();
-    const int n_move = (int) (lists_n & 0xffffu);
-    for (int i = tid; i < n_move; i += kThreads) {
-        const int a = src[i], b = dst[i];
-        score[b] = score[a];
-        pos[b]   = pos[a];
-        if (kept) kept[b] = a;
-    }
+    if (kept)
+        for (int j = tid; j < p.budget; j += kFewThreads)
+            if (!goes(j)) kept[j] = j;
+    __syncthreads();  // every thread has read the scores
     const size_t pair = (size_t) (p.layer0 + layer) * p.c_nb_layer + (size_t) stream * p.c_nb_stream + (size_t) kvh * p.c_nb_head;
-    if (!p.q8) {  // 16 lanes a row: 8 x 16 bytes of K, 8 of V
-        uint8_t * const base = (lane & 8 ? p.v_data : p.k_data) + pair + (lane & 7) * 16;
-        for (int i = 2 * warp + (lane >> 4); i < n_move; i += 2 * (kThreads / 32))
-            *reinterpret_cast<uint4 *>(base + (size_t) dst[i] * 128) = *reinterpret_cast<const uint4 *>(base + (size_t) src[i] * 128);
-    } else {      // 8 lanes a row: 4 x 16 bytes of K, 4 of V; the first of either also takes its two scales
-        const int      piece = lane & 3;
-        const uint32_t bytes = lane & 4 ? kQ8VBytesOff : 0, scales = lane & 4 ? kQ8VScaleOff : kQ8KScaleOff;
-        for (int i = 4 * warp + (lane >> 3); i < n_move; i += 4 * (kThreads / 32)) {
-            const uint8_t * a = p.k_data + pair + q8_tile_off(src[i]);
-            uint8_t *       b = p.k_data + pair + q8_tile_off(dst[i]);
-            *reinterpret_cast<uint4 *>(b + bytes + q8_byte_off(dst[i], 16 * piece)) =
-                *reinterpret_cast<const uint4 *>(a + bytes + q8_byte_off(src[i], 16 * piece));
-            if (piece == 0)
-                *reinterpret_cast<uint32_t *>(b + scales + q8_scale_off(dst[i], 0)) = *reinterpret_cast<const uint32_t *>(a + scales + q8_scale_off(src[i], 0));
+    int from = p.budget;
+#pragma unroll
+    for (int g = 0; g < kFew; ++g) {
+        const int to = gone[g];
+        if (to >= p.budget) break;  // the rows that go above the budget are left behind
+        while (goes(from)) ++from;
+        if (warp == g % (kFewThreads / 32)) {  // a warp a row
+            if (lane == 31) {
+                score[to] = score[from];
+                pos[to]   = pos[from];
+                if (kept) kept[to] = from;
+            } else if (!p.q8 && lane < 16) {
+                uint8_t * const base = (lane & 8 ? p.v_data : p.k_data) + pair + (lane & 7) * 16;
+                *reinterpret_cast<uint4 *>(base + (size_t) to * 128) = *reinterpret_cast<const uint4 *>(base + (size_t) from * 128);
+            } else if (p.q8 && lane < 8) {
+                move_q8_piece(p.k_data + pair, from, to, lane);
+            }
         }
+        ++from;
     }
 }
 
@@ -208,12 +416,31 @@ extern "C" int vox_kv_evict(vox_engine * e, const vox_kv_evict_args * a, void * 
     p.score = reinterpret_cast<uint8_t *>(a->score); p.row_pos = reinterpret_cast<uint8_t *>(a->row_pos);
     p.nb_head = a->nb_head; p.nb_stream = a->nb_stream; p.nb_layer = a->nb_layer;
     p.new_len = a->new_len; p.kept = a->kept; p.status = e->status_dev;
-    const size_t   smem = (size_t) 2 * p.n_list * sizeof(int32_t);
-    const uint32_t bit  = 1u << 20;
+    if (a->kv_bound - a->budget <= kFew) {
+        launch_pdl(evict_few_kernel, dim3((unsigned) (a->n_layers * a->n_streams * p.n_kv_heads)), dim3(kFewThreads), 0, static_cast<cudaStream_t>(stream), p);
+        return check_launch(e, "evict_few_kernel");
+    }
+    const size_t    key_bytes = (size_t) (a->kv_bound + 3) / 4 * 16, list_bytes = (size_t) 2 * p.n_list * sizeof(uint16_t);
+    p.keys_kept = key_bytes + list_bytes <= kSmemMost;
+    const size_t    smem  = (p.keys_kept ? key_bytes : 0) + list_bytes;
+    const long long lists = (long long) a->n_layers * a->n_streams * p.n_kv_heads;
+    // few lists: as many CTAs to a list as give every SM two, if the rows that may move are enough to share
+    p.cluster = (int) std::max(1LL, std::min<long long>(std::min<long long>(kMaxCluster, 2LL * e->sm_count / lists), p.n_list / 64));
+    const uint32_t bit = 1u << 20;
     if (!(e->attr_mask & bit)) {
-        VOX_CUDA_TRY(cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxRows / 2) * 2 * (int) sizeof(int32_t)));
+        VOX_CUDA_TRY(cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) kSmemMost));
         e->attr_mask |= bit;
     }
-    launch_pdl(evict_kernel, dim3((unsigned) (a->n_layers * a->n_streams * p.n_kv_heads)), dim3(kThreads), smem, static_cast<cudaStream_t>(stream), p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) (lists * p.cluster)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned) p.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, evict_kernel, p);
     return check_launch(e, "evict_kernel");
 }
