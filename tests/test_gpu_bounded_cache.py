@@ -787,7 +787,7 @@ def test_refusals(engine, pkg):
     refused("INVALID_ARGUMENT", "kv_bound", observe(kv_bound=1 << 20))
     refused("INVALID_ARGUMENT", "n_new", observe(n_new=-1))
     refused("INVALID_ARGUMENT", "8-byte aligned", observe(q=randn(gen(0), 2, 1, 16, D + 1)[..., 1:]))
-    refused("WORKSPACE_TOO_SMALL", "workspace", observe(workspace=torch.empty(8, dtype=torch.uint8, device="cuda")))
+    refused("WORKSPACE_TOO_SMALL", "workspace", observe(n_q=2, workspace=torch.empty(8, dtype=torch.uint8, device="cuda")))
 
     v = EvictCase(engine, pkg, "f16", [30, 20], 2, 2, 32)
     n2 = ints([0, 0])

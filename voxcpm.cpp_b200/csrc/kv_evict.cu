@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t (*warp_sums)
     return before + incl - x;
 }
 
-__global__ void __launch_bounds__(kThreads, 6) evict_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p) {
     extern __shared__ uint32_t smem[];  // keys (if they are kept), then sources and destinations of the rows that move
     __shared__ uint32_t hist[kBins], warp_sums[2][kWarps], found[3];
     uint32_t * const keys = smem;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 6) evict_kernel(const EvictParams p)
 // index first, so the next is the least of those after the last.
 constexpr int kFew        = 4;
 constexpr int kFewThreads = 128;
-__global__ void __launch_bounds__(kFewThreads, 12) evict_few_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kFewThreads, 16) evict_few_kernel(const EvictParams p) {
     __shared__ uint32_t least_key[2][kFewThreads / 32];
     __shared__ int      least_row[2][kFewThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, list = blockIdx.x;

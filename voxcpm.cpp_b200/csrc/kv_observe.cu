@@ -1,12 +1,15 @@
-// The attention weight that every cache row receives, summed over the queries and heads that look at it (vox_kv_observe).
+// The attention weight that every cache row receives from the query of a step (vox_kv_observe with n_q == 1).
 //
-//   score[j] = (j new ? 0 : decay * score[j]) + sum_rows 2^(s[row][j] - lse[row]),   s = scale * log2 e * q.k
+//   score[j] = (j new ? 0 : decay * score[j]) + sum over heads of 2^(s[head][j] - lse[head]),   s = scale * log2 e * q.k
 //
-// V plays no part, so a call reads K (128 or 68 bytes a row) and 8 bytes of score: bound by HBM for a decode step, by the
-// exponentials and products for a window of queries.
-#include "kv_cache.cuh"
-
-#include <algorithm>
+// V plays no part, so a call reads K (128 or 68 bytes a row) and 8 bytes of score: bound by HBM.  A CTA takes 512 keys of a
+// (stream, kv head), a warp 64 of them, from global memory straight into the operands of the products (a lane's 16-byte
+// loads; nothing is shared between warps, so nothing passes through shared memory).  The softmax's (max, sum) are
+//   given:    the log-sum-exp is an input; every CTA for itself;
+//   cluster:  up to 4096 keys: the CTAs of a pair are a cluster and exchange (max, sum) through distributed shared memory
+//             while the scores wait in registers: K is read once, in one launch;
+//   two:      longer streams: a launch that finds the (max, sum) of every CTA's keys, and one that joins them.
+#include "kv_observe.cuh"
 
 using namespace vox;
 
@@ -16,29 +19,13 @@ constexpr int kWarps     = 8;
 constexpr int kThreads   = kWarps * 32;
 constexpr int kWarpKeys  = 64;                  // keys a warp keeps as operands
 constexpr int kChunk     = kWarps * kWarpKeys;  // keys of a CTA
-constexpr int kMaxQ      = 64;
-constexpr int kMaxRows   = kMaxQ * 8;
+constexpr int kMaxGroup  = 8;                   // query heads of a kv head
+constexpr int kMaxCluster = 8;
 
-struct ObserveParams {
-    const uint8_t * k;         // f16: the layer's K rows; q8_0: the layer's tiles
-    size_t          k_nb_head, k_nb_stream;
-    const int32_t * kv_len;
-    const int32_t * n_seen;
-    const uint8_t * q;
-    size_t          q_nb_head, q_nb_tok, q_nb_stream;
-    const float2 *  rope;
-    const float *   lse;
-    float           scale_log2, decay;
-    int             n_heads, n_kv_heads, gqa, n_q, n_new, kv_bound, n_chunks;
-    uint8_t *       score;
-    uint8_t *       row_pos;
-    size_t          nb_head, nb_stream;
-    float2 *        stats;     // [pair][chunk][n_q * gqa] (max, sum)
-    int *           status;
-};
+enum { kGiven, kCluster, kFind, kJoin };        // which launch (see above); kFind and kJoin are the two
 
-// One 16-row operand of the queries: rows 16 * group + g and + 8 as value and remainder.  For one query (at most 8 rows)
-// the remainders take rows 8 .. 15 of the same operand and `lo` is unused.
+// The query rows of the group (at most 8) as value and remainder: the values are rows 0 .. 7 of the products' A operand, the
+// remainders rows 8 .. 15.
 // The 64 head dimensions go to the k-steps in the order in which a lane's 16-byte loads (q8_0: 8-byte loads) of a K row
 // deliver them: any order will do as long as both operands use the same one.
 //   f16 : k-step c, d = 32 (c / 2) + 8t + 4 (c % 2) + {0 .. 3}         (a lane's two loads start at d = 8t and 32 + 8t)
@@ -67,53 +54,35 @@ __device__ __forceinline__ KeyTile<Q8> load_keys(const uint8_t * pair, int row, 
     return k;
 }
 
-// scores of 16 rows x 8 keys.  One query: sc[0], sc[1] are row g, keys 2t and 2t + 1 (value and remainder added);
-// otherwise sc[2], sc[3] are row g + 8.
-template <bool Q8, bool kOne>
-__device__ __forceinline__ void score_tile(float (&sc)[4], const uint32_t (&hi)[4][4], const uint32_t (&lo)[4][4], const float (&bias)[2][2],
-                                           const KeyTile<Q8> & k, int lane) {
+// scores of 8 rows x 8 keys: sc[0], sc[1] are row g, keys 2t and 2t + 1
+template <bool Q8>
+__device__ __forceinline__ void score_tile(float (&sc)[2], const uint32_t (&q)[4][4], const KeyTile<Q8> & k, int lane) {
     if constexpr (!Q8) {
-        sc[0] = sc[1] = sc[2] = sc[3] = 0.0f;
+        float          x[4] = {0.f, 0.f, 0.f, 0.f};
         const uint32_t b[4][2] = {{k.x[0].x, k.x[0].y}, {k.x[0].z, k.x[0].w}, {k.x[1].x, k.x[1].y}, {k.x[1].z, k.x[1].w}};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            mma_16816(sc, hi[c], b[c][0], b[c][1]);
-            if (!kOne) mma_16816(sc, lo[c], b[c][0], b[c][1]);
-        }
-        if (kOne) { sc[0] += sc[2]; sc[1] += sc[3]; }
+        for (int c = 0; c < 4; ++c) mma_16816(x, q[c], b[c][0], b[c][1]);
+        sc[0] = x[0] + x[2];
+        sc[1] = x[1] + x[3];
     } else {
         // keys 2t and 2t + 1 of this tile: their scales are with the lanes that hold those keys' bytes (lane = 4 * key)
         const uint32_t d0 = __shfl_sync(0xffffffffu, k.d, 8 * (lane & 3)), d1 = __shfl_sync(0xffffffffu, k.d, 8 * (lane & 3) + 4);
-        float part[2][4];
+        float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // one accumulator per 32-value block
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            part[b][0] = part[b][1] = -bias[0][b];
-            part[b][2] = part[b][3] = kOne ? 0.0f : -bias[1][b];
-            const uint32_t x0 = u8_pair_to_half2(k.x[b].x, 0x4140), x1 = u8_pair_to_half2(k.x[b].x, 0x4342);
-            const uint32_t y0 = u8_pair_to_half2(k.x[b].y, 0x4140), y1 = u8_pair_to_half2(k.x[b].y, 0x4342);
-            mma_16816(part[b], hi[2 * b], x0, x1);
-            mma_16816(part[b], hi[2 * b + 1], y0, y1);
-            if (!kOne) {
-                mma_16816(part[b], lo[2 * b], x0, x1);
-                mma_16816(part[b], lo[2 * b + 1], y0, y1);
-            } else {
-                part[b][0] += part[b][2];
-                part[b][1] += part[b][3];
-            }
+            mma_16816(x[b], q[2 * b], s8_pair_to_half2(k.x[b].x, 0x4140), s8_pair_to_half2(k.x[b].x, 0x4342));
+            mma_16816(x[b], q[2 * b + 1], s8_pair_to_half2(k.x[b].y, 0x4140), s8_pair_to_half2(k.x[b].y, 0x4342));
         }
-        sc[0] = (part[0][0] * half_lo(d0) + part[1][0] * half_hi(d0)) * kTwo24;
-        sc[1] = (part[0][1] * half_lo(d1) + part[1][1] * half_hi(d1)) * kTwo24;
-        if (!kOne) {
-            sc[2] = (part[0][2] * half_lo(d0) + part[1][2] * half_hi(d0)) * kTwo24;
-            sc[3] = (part[0][3] * half_lo(d1) + part[1][3] * half_hi(d1)) * kTwo24;
-        }
+        sc[0] = (x[0][0] + x[0][2]) * half_lo(d0) + (x[1][0] + x[1][2]) * half_hi(d0);
+        sc[1] = (x[0][1] + x[0][3]) * half_lo(d1) + (x[1][1] + x[1][3]) * half_hi(d1);
     }
 }
 
-// One row's 16 values of this lane, rotated and scaled, as value and remainder.
-__device__ __forceinline__ void load_query(const ObserveParams & p, int stream, int kvh, int row, bool live, int t, float (&hi)[4][4], float (&lo)[4][4]) {
-    const int     i = live ? row / p.gqa : 0, head = kvh * p.gqa + (live ? row - i * p.gqa : 0);
-    const float * src = reinterpret_cast<const float *>(p.q + (size_t) stream * p.q_nb_stream + (size_t) i * p.q_nb_tok + (size_t) head * p.q_nb_head);
+// the operand, from the query rows rotated and scaled
+__device__ __forceinline__ void load_query(const ObserveParams & p, int stream, int kvh, int lane, uint32_t (&op)[4][4]) {
+    const int     g = lane >> 2, t = lane & 3;
+    const bool    live = g < p.gqa;
+    const float * src = reinterpret_cast<const float *>(p.q + (size_t) stream * p.q_nb_stream + (size_t) (kvh * p.gqa + (live ? g : 0)) * p.q_nb_head);
     float x[4][4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -133,176 +102,144 @@ __device__ __forceinline__ void load_query(const ObserveParams & p, int stream, 
             }
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < 4; ++c) {
+        float h[4], l[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split_hi_lo(live ? x[c][e] * p.scale_log2 : 0.0f, hi[c][e], lo[c][e]);
-}
-
-// the operands of rows 16 * group + g (and + 8), and what the +128 of the K bytes adds to their scores
-template <bool Q8, bool kOne>
-__device__ __forceinline__ void load_group(const ObserveParams & p, int stream, int kvh, int group, int rows, int lane, uint32_t (&hi)[4][4],
-                                           uint32_t (&lo)[4][4], float (&bias)[2][2]) {
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int h = 0; h < (kOne ? 1 : 2); ++h) {
-        const int row = 16 * group + g + 8 * h;
-        float     xh[4][4], xl[4][4];
-        load_query(p, stream, kvh, row, row < rows, t, xh, xl);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            hi[c][h]     = pack_half2(xh[c][0], xh[c][1]);
-            hi[c][h + 2] = pack_half2(xh[c][2], xh[c][3]);
-            if (kOne) {
-                hi[c][1] = pack_half2(xl[c][0], xl[c][1]);
-                hi[c][3] = pack_half2(xl[c][2], xl[c][3]);
-            } else {
-                lo[c][h]     = pack_half2(xl[c][0], xl[c][1]);
-                lo[c][h + 2] = pack_half2(xl[c][2], xl[c][3]);
-            }
-        }
-        if constexpr (Q8) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int c = 2 * b; c < 2 * b + 2; ++c)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum += xh[c][e] + xl[c][e];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                bias[h][b] = sum * (128.0f * kTwoM24);
-            }
-        }
+        for (int e = 0; e < 4; ++e) split_hi_lo(live ? x[c][e] * p.scale_log2 : 0.0f, h[e], l[e]);
+        op[c][0] = pack_half2(h[0], h[1]);
+        op[c][1] = pack_half2(l[0], l[1]);
+        op[c][2] = pack_half2(h[2], h[3]);
+        op[c][3] = pack_half2(l[2], l[3]);
     }
 }
 
-// kWeights = false: the (max, sum) of every row over the CTA's keys.  kWeights = true: the weights' sums over the rows.
-template <bool Q8, bool kOne, bool kWeights>
-__global__ void __launch_bounds__(kThreads, kOne ? 2 : 1) observe_kernel(const ObserveParams p) {
-    __shared__ float2 row_stat[kMaxRows];           // kWeights: (max, 1 / sum) of every row of the pair
-    __shared__ float2 warp_stat[kWarps][kMaxRows];  // otherwise: (max, sum) of every row over a warp's keys
+// two parts' (max, sum) as one; (-inf, 0) is a part that saw nothing, (-inf, NaN) one of NaN
+__device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
+    const float M = fmaxf(a.x, b.x);
+    const float fa = a.x == -INFINITY ? 1.0f : exp2f(a.x - M), fb = b.x == -INFINITY ? 1.0f : exp2f(b.x - M);  // a sum of 0 or NaN stays so
+    return make_float2(M, fmaf(a.y, fa, b.y * fb));
+}
+// as the weights take them: (max, 1 / sum); a row that saw nothing adds nothing
+__device__ __forceinline__ float2 as_weights(float2 s) { return s.y == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(s.x, 1.0f / s.y); }
+
+template <bool Q8, int kMode>
+__global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParams p) {
+    __shared__ float2 row_stat[kMaxGroup], cta_stat[kMaxGroup], warp_stat[kWarps][kMaxGroup];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int chunk = blockIdx.x, kvh = blockIdx.y % p.n_kv_heads, stream = blockIdx.y / p.n_kv_heads;
-    const int rows = p.n_q * p.gqa;
     pdl_wait();
     pdl_launch_dependents();
     const int len = p.kv_len[stream];
-    if (len > p.kv_bound) {  // longer than the call said: nothing of it is touched
-        if (tid == 0 && kvh == 0 && chunk == 0) atomicOr(p.status, kStatusBadState);
+    if (len > p.kv_bound || len <= 0) {  // longer than the call said: nothing of it is touched (the same for a whole cluster)
+        if (len > 0 && tid == 0 && kvh == 0 && chunk == 0) atomicOr(p.status, kStatusBadState);
         return;
     }
     const int first = chunk * kChunk + warp * kWarpKeys;
-    if (chunk * kChunk >= len) return;
-    const float2 * all = p.stats + (size_t) blockIdx.y * p.n_chunks * rows;
-    if (kWeights) {
-        const int n = (len + kChunk - 1) / kChunk;
-        for (int r = tid; r < rows; r += kThreads) {
-            if (p.lse != nullptr) {
-                // kept as the scores are, in units of log2, in two parts: one would lose 2^-24 of its size
-                const float x = p.lse[(size_t) stream * p.n_heads + kvh * p.gqa + r], hi = x * 1.4426950408889634f;
-                const float rest = fmaf(x, 1.4426950408889634f, -hi) + x * 1.9259629911266175e-8f;
-                row_stat[r] = make_float2(hi, ex2_approx(-rest));
-                if (isinf(hi)) row_stat[r].y = 1.0f;
-                continue;
-            }
-            float M = -INFINITY, L = 0.0f;
-            for (int c = 0; c < n; ++c) {
-                const float2 x  = __ldcg(all + (size_t) c * rows + r);
-                const float  mn = fmaxf(M, x.x);
-                if (x.x == -INFINITY && x.y == 0.0f) continue;
-                L = L * exp2f(M - mn) + x.y * exp2f(x.x - mn);
-                M = mn;
-            }
-            row_stat[r] = L == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(M, 1.0f / L);  // a row that sees nothing adds nothing
-        }
-        __syncthreads();
-    }
-    KeyTile<Q8> keys[kWarpKeys / 8];
+    if (kMode != kCluster && chunk * kChunk >= len) return;
+    // everything the CTA reads is asked for before anything is waited for
+    KeyTile<Q8>     keys[kWarpKeys / 8];
     const uint8_t * pair = p.k + (size_t) stream * p.k_nb_stream + (size_t) kvh * p.k_nb_head;
 #pragma unroll
     for (int n = 0; n < kWarpKeys / 8; ++n) keys[n] = load_keys<Q8>(pair, first + 8 * n + g, t, first + 8 * n + g < len);
-    float colsum[kWarpKeys / 8][2];
+    float * const score = reinterpret_cast<float *>(p.score + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head);
+    const int     mine = first + 8 * g + 2 * t;  // the two keys whose scores this lane writes
+    float         old[2] = {0.0f, 0.0f};
+    if (kMode != kFind) {
 #pragma unroll
-    for (int n = 0; n < kWarpKeys / 8; ++n) colsum[n][0] = colsum[n][1] = 0.0f;
-    if (first < len) {
-        for (int group = 0; 16 * group < rows; ++group) {
-            uint32_t hi[4][4], lo[4][4];
-            float    bias[2][2];
-            load_group<Q8, kOne>(p, stream, kvh, group, rows, lane, hi, lo, bias);
-            int    last[2];  // last key that rows g and g + 8 see
-            float2 st[2];
-            float  m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int e = 0; e < 2; ++e)
+            if (mine + e < len - p.n_new) old[e] = score[mine + e];
+    }
+    if (kMode == kGiven && tid < p.gqa) {
+        // kept as the scores are, in units of log2, in two parts: one would lose 2^-24 of its size
+        const float x = p.lse[(size_t) stream * p.n_heads + kvh * p.gqa + tid], hi = x * 1.4426950408889634f;
+        const float rest = fmaf(x, 1.4426950408889634f, -hi) + x * 1.9259629911266175e-8f;
+        row_stat[tid] = make_float2(hi, isinf(hi) ? 1.0f : ex2_approx(-rest));
+    }
+    if (kMode == kJoin && tid < p.gqa) {
+        const float2 * all = p.stats + (size_t) blockIdx.y * p.n_chunks * p.gqa + tid;
+        float2         s = make_float2(-INFINITY, 0.0f);
+        for (int c = 0; c * kChunk < len; ++c) s = join_stats(s, __ldcg(all + (size_t) c * p.gqa));
+        row_stat[tid] = as_weights(s);
+    }
+    uint32_t q[4][4];
+    load_query(p, stream, kvh, lane, q);
+    float sc[kWarpKeys / 8][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = 16 * group + g + 8 * h;
-                last[h] = row < rows && !(kOne && h) ? len - p.n_q + row / p.gqa : -1;
-                if (kWeights) st[h] = row < rows ? row_stat[row] : make_float2(0.0f, 0.0f);
-            }
-            float sc[kWarpKeys / 8][4];
+    for (int n = 0; n < kWarpKeys / 8; ++n) {
+        score_tile<Q8>(sc[n], q, keys[n], lane);
 #pragma unroll
-            for (int n = 0; n < kWarpKeys / 8; ++n) {
-                score_tile<Q8, kOne>(sc[n], hi, lo, bias, keys[n], lane);
-                const int key = first + 8 * n + 2 * t;
+        for (int e = 0; e < 2; ++e)
+            if (first + 8 * n + 2 * t + e >= len) sc[n][e] = -INFINITY;
+    }
+    if (kMode == kFind || kMode == kCluster) {
+        float m = -INFINITY, l = 0.0f;
 #pragma unroll
-                for (int h = 0; h < (kOne ? 1 : 2); ++h)
+        for (int n = 0; n < kWarpKeys / 8; ++n) m = fmaxf(m, fmaxf(sc[n][0], sc[n][1]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if (key + e > last[h]) sc[n][2 * h + e] = -INFINITY;
-                        if (kWeights) colsum[n][e] += ex2_approx(sc[n][2 * h + e] - st[h].x) * st[h].y;
-                        else          m[h] = fmaxf(m[h], sc[n][2 * h + e]);
-                    }
-            }
-            if (!kWeights) {
+        for (int n = 0; n < kWarpKeys / 8; ++n) l += ex2_approx(sc[n][0] - ref) + ex2_approx(sc[n][1] - ref);
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t == 0) warp_stat[warp][g] = make_float2(m, l);
+        __syncthreads();
+        if (tid < p.gqa) {
+            float2 s = warp_stat[0][tid];
 #pragma unroll
-                for (int h = 0; h < (kOne ? 1 : 2); ++h) {
-                    m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
-                    m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
-                    const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+            for (int w = 1; w < kWarps; ++w) s = join_stats(s, warp_stat[w][tid]);
+            if (kMode == kFind) p.stats[((size_t) blockIdx.y * p.n_chunks + chunk) * p.gqa + tid] = s;
+            else                cta_stat[tid] = s;
+        }
+        if (kMode == kFind) return;
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (tid < p.gqa) {
+            const uint32_t at = smem_u32(&cta_stat[tid]);
+            float2         all[kMaxCluster], s = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-                    for (int n = 0; n < kWarpKeys / 8; ++n) l[h] += ex2_approx(sc[n][2 * h] - ref) + ex2_approx(sc[n][2 * h + 1] - ref);
-                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-                    const int row = 16 * group + g + 8 * h;
-                    if (t == 0 && row < rows) warp_stat[warp][row] = make_float2(m[h], l[h]);
+            for (int r = 0; r < kMaxCluster; ++r) {  // all on their way together
+                all[r] = s;
+                if (r < p.n_chunks) {
+                    uint32_t peer;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(r));
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(all[r].x), "=f"(all[r].y) : "r"(peer) : "memory");
                 }
             }
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) s = join_stats(s, all[r]);
+            row_stat[tid] = as_weights(s);
         }
-    } else if (!kWeights) {
-        for (int r = lane; r < rows; r += 32) warp_stat[warp][r] = make_float2(-INFINITY, 0.0f);
-    }
-    if (!kWeights) {
         __syncthreads();
-        for (int r = tid; r < rows; r += kThreads) {
-            float M = -INFINITY, L = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, warp_stat[w][r].x);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float2 x = warp_stat[w][r];
-                L += x.x == -INFINITY ? x.y : x.y * exp2f(x.x - M);
-            }
-            p.stats[((size_t) blockIdx.y * p.n_chunks + chunk) * rows + r] = make_float2(M, L);
-        }
-        return;
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for at the end: nobody leaves while its memory is read
+    } else {
+        __syncthreads();
     }
-    float *   score   = reinterpret_cast<float *>(p.score + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head);
-    int32_t * row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
-    const int base = (p.n_seen ? p.n_seen[stream] : len) - len;
+    const float2 st = g < p.gqa ? row_stat[g] : make_float2(0.0f, 0.0f);
+    float        w0 = 0.0f, w1 = 0.0f;
 #pragma unroll
     for (int n = 0; n < kWarpKeys / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float w = colsum[n][e];
+            float w = ex2_approx(sc[n][e] - st.x) * st.y;  // over the rows of the group:
             w += __shfl_xor_sync(0xffffffffu, w, 4);
             w += __shfl_xor_sync(0xffffffffu, w, 8);
             w += __shfl_xor_sync(0xffffffffu, w, 16);
-            const int key = first + 8 * n + 2 * t + e;
-            if (g == n && key < len) {  // eight row groups of lanes hold the same sum: each writes one tile
-                const bool fresh = key >= len - p.n_new;
-                score[key] = fresh ? w : fmaf(p.decay, score[key], w);
-                if (fresh && row_pos != nullptr) row_pos[key] = base + key;
-            }
+            if (g == n) (e ? w1 : w0) = w;  // every row of lanes has the sums: each writes one tile
         }
+    int32_t * row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int key = mine + e;
+        if (key >= len) break;
+        const bool fresh = key >= len - p.n_new;
+        score[key] = fresh ? (e ? w1 : w0) : fmaf(p.decay, old[e], e ? w1 : w0);
+        if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
+    }
+    if (kMode == kCluster) {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
 }
 
 int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
@@ -316,7 +253,7 @@ int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
                 a->n_heads, c->cfg.n_kv_heads);
     VOX_REQUIRE(a->n_heads / c->cfg.n_kv_heads <= 8, VOX_ATTN_UNSUPPORTED, "GQA ratio above 8 is not supported");
     VOX_REQUIRE(a->n_q >= 1, VOX_ATTN_INVALID_ARGUMENT, "n_q %d must be positive", a->n_q);
-    VOX_REQUIRE(a->n_q <= kMaxQ, VOX_ATTN_UNSUPPORTED, "n_q %d: at most %d queries look back at once", a->n_q, kMaxQ);
+    VOX_REQUIRE(a->n_q <= kObserveMaxQ, VOX_ATTN_UNSUPPORTED, "n_q %d: at most %d queries look back at once", a->n_q, kObserveMaxQ);
     VOX_REQUIRE(a->n_q == 1 || (a->lse == nullptr && a->rope_table == nullptr), VOX_ATTN_UNSUPPORTED, "lse and rope_table are taken with n_q == 1 only");
     VOX_REQUIRE(a->kv_bound >= 0 && a->kv_bound <= c->cfg.max_len, VOX_ATTN_INVALID_ARGUMENT, "kv_bound %d exceeds the cache capacity %d",
                 a->kv_bound, c->cfg.max_len);
@@ -331,15 +268,33 @@ int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
     return VOX_ATTN_OK;
 }
 
-template <bool Q8, bool kOne>
-int launch_observe(vox_engine * e, const ObserveParams & p, dim3 grid, cudaStream_t st) {
-    if (p.lse == nullptr) {
-        launch_pdl(observe_kernel<Q8, kOne, false>, grid, dim3(kThreads), 0, st, p);
-        const int rc = check_launch(e, "observe_kernel<stats>");
+int chunks_of(int kv_bound) { return (std::max(kv_bound, 1) + kChunk - 1) / kChunk; }
+
+template <bool Q8>
+int launch_observe(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
+    const dim3 grid((unsigned) p.n_chunks, (unsigned) (p.n_streams * p.n_kv_heads));
+    if (p.lse == nullptr && p.n_chunks > kMaxCluster) {
+        launch_pdl(observe_kernel<Q8, kFind>, grid, dim3(kThreads), 0, st, p);
+        const int rc = check_launch(e, "observe_kernel<statistics>");
         if (rc != VOX_ATTN_OK) return rc;
+        launch_pdl(observe_kernel<Q8, kJoin>, grid, dim3(kThreads), 0, st, p);
+        return check_launch(e, "observe_kernel<weights>");
     }
-    launch_pdl(observe_kernel<Q8, kOne, true>, grid, dim3(kThreads), 0, st, p);
-    return check_launch(e, "observe_kernel<weights>");
+    if (p.lse != nullptr) {
+        launch_pdl(observe_kernel<Q8, kGiven>, grid, dim3(kThreads), 0, st, p);
+        return check_launch(e, "observe_kernel<given>");
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(kThreads); cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = grid.x; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, observe_kernel<Q8, kCluster>, p);
+    return check_launch(e, "observe_kernel<cluster>");
 }
 
 }  // namespace
@@ -348,8 +303,10 @@ extern "C" {
 
 size_t vox_kv_observe_workspace_bytes(const vox_kv_observe_args * a) {
     if (a == nullptr || a->cache == nullptr || a->n_streams <= 0 || a->n_heads <= 0 || a->n_q <= 0 || a->kv_bound < 0 || a->lse != nullptr) return 0;
-    const size_t chunks = ((size_t) a->kv_bound + kChunk - 1) / kChunk;
-    return (size_t) a->n_streams * a->n_heads * a->n_q * chunks * sizeof(float2);
+    const int HK = a->cache->cfg.n_kv_heads;
+    if (a->n_q > 1) return observe_window_bytes(a->n_streams, HK, a->n_heads / HK * a->n_q, a->kv_bound);
+    const int chunks = chunks_of(a->kv_bound);
+    return chunks <= kMaxCluster ? 0 : (size_t) a->n_streams * a->n_heads * chunks * sizeof(float2);
 }
 
 int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspace, size_t workspace_bytes, void * stream) {
@@ -372,15 +329,15 @@ int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspa
     p.rope = reinterpret_cast<const float2 *>(a->rope_table); p.lse = a->lse;
     p.scale_log2 = a->scale * 1.4426950408889634f; p.decay = a->decay;
     p.n_heads = a->n_heads; p.n_kv_heads = c->cfg.n_kv_heads; p.gqa = a->n_heads / c->cfg.n_kv_heads;
-    p.n_q = a->n_q; p.n_new = a->n_new; p.kv_bound = a->kv_bound; p.n_chunks = (std::max(a->kv_bound, 1) + kChunk - 1) / kChunk;
+    p.n_streams = a->n_streams; p.layer = a->layer;
+    p.n_q = a->n_q; p.n_new = a->n_new; p.kv_bound = a->kv_bound; p.n_chunks = chunks_of(a->kv_bound);
     p.score = reinterpret_cast<uint8_t *>(a->score); p.row_pos = reinterpret_cast<uint8_t *>(a->row_pos);
     p.nb_head = a->nb_head; p.nb_stream = a->nb_stream;
     p.stats = static_cast<float2 *>(workspace);
     p.status = e->status_dev;
-    const dim3   grid((unsigned) p.n_chunks, (unsigned) (a->n_streams * p.n_kv_heads));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->n_q == 1) return q8 ? launch_observe<true, true>(e, p, grid, st) : launch_observe<false, true>(e, p, grid, st);
-    return q8 ? launch_observe<true, false>(e, p, grid, st) : launch_observe<false, false>(e, p, grid, st);
+    if (a->n_q > 1) return launch_observe_window(e, c, p, st);
+    return q8 ? launch_observe<true>(e, p, st) : launch_observe<false>(e, p, st);
 }
 
 }  // extern "C"
