@@ -329,6 +329,7 @@ int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspa
     p.rope = reinterpret_cast<const float2 *>(a->rope_table); p.lse = a->lse;
     p.scale_log2 = a->scale * 1.4426950408889634f; p.decay = a->decay;
     p.n_heads = a->n_heads; p.n_kv_heads = c->cfg.n_kv_heads; p.gqa = a->n_heads / c->cfg.n_kv_heads;
+    p.gqa_magic = 65536u / (uint32_t) p.gqa + 1u;
     p.n_streams = a->n_streams; p.layer = a->layer;
     p.n_q = a->n_q; p.n_new = a->n_new; p.kv_bound = a->kv_bound; p.n_chunks = chunks_of(a->kv_bound);
     p.score = reinterpret_cast<uint8_t *>(a->score); p.row_pos = reinterpret_cast<uint8_t *>(a->row_pos);

@@ -23,6 +23,7 @@ struct ObserveParams {
     uint8_t *       score;
     uint8_t *       row_pos;
     size_t          nb_head, nb_stream;
+    uint32_t        gqa_magic; // row * gqa_magic >> 16 = row / gqa for rows below 512
     float2 *        stats;     // (max, sum) of every row over a part of the keys
     int *           status;
 };

@@ -160,32 +160,64 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
         if (!have_part) break;
         const Part w = part;
 
+        auto copy_tile = [&](int t) {  // one lane
+            const int n = T + t, key = (w.tile0 + t) * kKeys, boxes = w.len - key > kKvTile ? 2 : 1;
+            if constexpr (Q8) {
+                const int st = n % kRawStages;
+                issued = n;
+                if (n >= kRawStages && !mbar_wait_bounded(rempty0 + 8 * st, ((n / kRawStages) - 1) & 1)) return false;
+                const uint32_t bar = rfull0 + 8 * st, dst = sRaw + st * kRawStage;
+                mbar_expect_tx(bar, boxes * (kRawStage / 2));
+                for (int x = 0; x < boxes; ++x) {
+                    const uint8_t * src = p.k + (size_t) w.stream * p.k_nb_stream + (size_t) w.kvh * p.k_nb_head + q8_tile_off(key + x * kKvTile);
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + x * kKvTile * 64),
+                                 "l"(src), "r"(kKvTile * 64), "r"(bar)
+                                 : "memory");
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + 2 * kKvTile * 64 + x * kKvTile * 4),
+                                 "l"(src + kQ8KScaleOff), "r"(kKvTile * 4), "r"(bar)
+                                 : "memory");
+                }
+            } else {
+                const int st = n % Z::kStages;
+                issued = n;
+                if (n >= Z::kStages && !mbar_wait_bounded(empty0 + 8 * st, ((n / Z::kStages) - 1) & 1)) return false;
+                const uint32_t bar = full0 + 8 * st, dst = sK + st * kKTile;
+                mbar_expect_tx(bar, boxes * kKvTile * 128);
+                for (int x = 0; x < boxes; ++x) tma_load_5d(dst + x * kKvTile * 128, &map_k, bar, 0, key + x * kKvTile, w.kvh, w.stream, p.layer);
+            }
+            return true;
+        };
+        bool first_ok = true;
+        if (warp == 8 && lane == 0)  // the first two while the queries are made ready
+            for (int t = 0; t < min(w.tiles, 2) && first_ok; ++t) first_ok = copy_tile(t);
+
         // ---- the queries of the pair, by all but the copying and issuing warps; in the second launch their statistics too
         if (warp < 8) {
-            const int c = lane & 15, n_rows = n_m * 128;
-            constexpr int kLoads = 8;
+            const int       c = lane & 15, n_rows = n_m * 128;
+            const uint8_t * q_base = p.q + (size_t) w.stream * p.q_nb_stream + (size_t) (w.kvh * p.gqa) * p.q_nb_head + 16 * c;
+            constexpr int kLoads = 8;  // rows of a lane in flight
 #pragma unroll 1
             for (int r0 = 2 * warp * kLoads; r0 < n_rows; r0 += 16 * kLoads) {
                 float4 x[kLoads];
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int row = r0 + 2 * i + (lane >> 4), at = row < rows ? row : 0, q = at / p.gqa, head = w.kvh * p.gqa + at - q * p.gqa;
-                    const float2 * src = reinterpret_cast<const float2 *>(p.q + (size_t) w.stream * p.q_nb_stream + (size_t) q * p.q_nb_tok + (size_t) head * p.q_nb_head) + 2 * c;
-                    const float2 lo = src[0], hi = src[1];
+                    const uint32_t row = r0 + 2 * i + (lane >> 4), at = min(row, (uint32_t) rows - 1), q = at * p.gqa_magic >> 16;  // at / gqa
+                    const uint8_t * src = q_base + q * p.q_nb_tok + (at - q * p.gqa) * p.q_nb_head;
+                    const float2 lo = *reinterpret_cast<const float2 *>(src), hi = *reinterpret_cast<const float2 *>(src + 8);
                     x[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
                 }
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int  row  = r0 + 2 * i + (lane >> 4);
-                    const bool live = row < rows;
-                    float      h[4], l[4];
-                    split_hi_lo(live ? x[i].x * p.scale_log2 : 0.0f, h[0], l[0]);
-                    split_hi_lo(live ? x[i].y * p.scale_log2 : 0.0f, h[1], l[1]);
-                    split_hi_lo(live ? x[i].z * p.scale_log2 : 0.0f, h[2], l[2]);
-                    split_hi_lo(live ? x[i].w * p.scale_log2 : 0.0f, h[3], l[3]);
+                    const int     row = r0 + 2 * i + (lane >> 4);
+                    const float   mul = p.scale_log2;
+                    const __half2 h0 = __floats2half2_rn(x[i].x * mul, x[i].y * mul), h1 = __floats2half2_rn(x[i].z * mul, x[i].w * mul);
+                    const float2  f0 = __half22float2(h0), f1 = __half22float2(h1);
+                    uint2 hi = make_uint2(*reinterpret_cast<const uint32_t *>(&h0), *reinterpret_cast<const uint32_t *>(&h1));
+                    uint2 lo = make_uint2(pack_half2(x[i].x * mul - f0.x, x[i].y * mul - f0.y), pack_half2(x[i].z * mul - f1.x, x[i].w * mul - f1.y));
+                    if (row >= rows) hi = lo = make_uint2(0u, 0u);
                     uint8_t * dst = smem_gen + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8;
-                    *reinterpret_cast<uint2 *>(dst)          = make_uint2(pack_half2(h[0], h[1]), pack_half2(h[2], h[3]));
-                    *reinterpret_cast<uint2 *>(dst + kQTile) = make_uint2(pack_half2(l[0], l[1]), pack_half2(l[2], l[3]));
+                    *reinterpret_cast<uint2 *>(dst)          = hi;
+                    *reinterpret_cast<uint2 *>(dst + kQTile) = lo;
                 }
             }
             if (kWeights) {
@@ -209,33 +241,8 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
         if (warp == 8) {
             // ------------------------------------------------------------------ copies
             if (lane == 0) {
-                bool ok = true;
-                for (int t = 0; t < w.tiles && ok; ++t) {
-                    const int n = T + t, key = (w.tile0 + t) * kKeys, boxes = w.len - key > kKvTile ? 2 : 1;
-                    if constexpr (Q8) {
-                        const int st = n % kRawStages;
-                        issued = n;
-                        if (n >= kRawStages && !mbar_wait_bounded(rempty0 + 8 * st, ((n / kRawStages) - 1) & 1)) { ok = false; break; }
-                        const uint32_t bar = rfull0 + 8 * st, dst = sRaw + st * kRawStage;
-                        mbar_expect_tx(bar, boxes * (kRawStage / 2));
-                        for (int x = 0; x < boxes; ++x) {
-                            const uint8_t * src = p.k + (size_t) w.stream * p.k_nb_stream + (size_t) w.kvh * p.k_nb_head + q8_tile_off(key + x * kKvTile);
-                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + x * kKvTile * 64),
-                                         "l"(src), "r"(kKvTile * 64), "r"(bar)
-                                         : "memory");
-                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + 2 * kKvTile * 64 + x * kKvTile * 4),
-                                         "l"(src + kQ8KScaleOff), "r"(kKvTile * 4), "r"(bar)
-                                         : "memory");
-                        }
-                    } else {
-                        const int st = n % Z::kStages;
-                        issued = n;
-                        if (n >= Z::kStages && !mbar_wait_bounded(empty0 + 8 * st, ((n / Z::kStages) - 1) & 1)) { ok = false; break; }
-                        const uint32_t bar = full0 + 8 * st, dst = sK + st * kKTile;
-                        mbar_expect_tx(bar, boxes * kKvTile * 128);
-                        for (int x = 0; x < boxes; ++x) tma_load_5d(dst + x * kKvTile * 128, &map_k, bar, 0, key + x * kKvTile, w.kvh, w.stream, p.layer);
-                    }
-                }
+                bool ok = first_ok;
+                for (int t = min(w.tiles, 2); t < w.tiles && ok; ++t) ok = copy_tile(t);
                 if (ok) issued = T + w.tiles;
                 else    give_up();
             }
@@ -328,7 +335,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                         }
                         give_back(uu);
                         if (k0 + kSub > first_cut) {  // keys that this row's query does not see, and keys past the end
-                            const int last = first_cut + (128 * i + row) / p.gqa - k0;
+                            const int last = first_cut + (int) ((uint32_t) (128 * i + row) * p.gqa_magic >> 16) - k0;
 #pragma unroll
                             for (int e = 0; e < kSub; ++e)
                                 if (e > last) r[e] = 0xff800000u;
