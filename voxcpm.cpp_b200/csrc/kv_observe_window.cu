@@ -298,7 +298,8 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                 const int n = T + t, st = n % Z::kStages, key0 = (w.tile0 + t) * kKeys;
                 float     sum = 0.0f, d0 = 1.0f, d1 = 1.0f;
                 if (Q8) {  // the scales are the converting warps'
-                    if (!mbar_wait_bounded(full0 + 8 * st, (n / Z::kStages) & 1)) { ok = false; break; }
+                    // (a warp whose wait ran out stays until the barrier at the end of the tile, which the others wait at)
+                    if (!mbar_wait_bounded(full0 + 8 * st, (n / Z::kStages) & 1)) ok = false;
                     if (kWeights) { d0 = scales[st][row].x; d1 = scales[st][row].y; }
                 }
                 auto take = [&](int uu, uint32_t (&r)[kSub]) {  // a score tile out of TMEM, and its buffer back

@@ -612,7 +612,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Full row tiles on the 5th-generation tensor cores (f16 caches).
+// Full row tiles on the 5th-generation tensor cores.
 //
 // Q (scaled by scale * log2 e) lies in shared memory as two f16 tiles, value and remainder; scores S = Q_lo.K + Q_hi.K (the
 // small part first: the accumulator truncates) come 64 keys at a time into one of six score buffers in TMEM.  Four softmax
@@ -623,22 +623,34 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // 192 threads of 128 registers and 83 KB of shared memory: the CTA runs beside two CTAs of the decode kernel, whose time is
 // HBM's.  (With two softmax groups, 352 threads and 128-key stages it was no faster on its own and had to wait for the
 // decode kernel's CTAs to leave: 57.4 us for 256 streams under two prompts of 4096 rows.)
+//
+// q8_0: the softmax warps turn a tile's bytes into f16 numbers q (exact; a tile ahead of the scores they work on) and keep the
+// scales apart.  Either 32-value block has an accumulator of its own: two of S (s = d0 S0 + d1 S1) and two of O, whose
+// weights have V's scale of their block taken in; of either O the half that belongs to its block is used.  The weights are
+// taken in units of v_unit, as in the other kernel.
 constexpr int kTcThreads = 6 * 32;
-constexpr int kTcStages  = 3;
 constexpr int kSub       = 64;                    // keys of a score tile and of a stage
-constexpr int kSBufs     = 6;
-constexpr int kTcOCol    = kSBufs * kSub;         // the accumulator: 64 columns behind the score buffers
 constexpr int kQTile     = kRows * 128;
-constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V
-constexpr int kTcSmem    = 2 * kQTile + kTcStages * kTcStage + 1024;
+constexpr int kTcStages  = 3;
+constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V, in f16
+template <bool Q8> struct Tc {
+    static constexpr int kSCols  = Q8 ? 2 * kSub : kSub;   // TMEM columns of a score tile, and of the accumulators behind the buffers
+    static constexpr int kSBufs  = Q8 ? 3 : 6;
+    static constexpr int kOCol   = kSBufs * kSCols;
+    static constexpr int kRaw    = Q8 ? 3 : 0;             // q8_0: stages of tiles as the cache holds them
+    static constexpr int kRawBytes = 8704;
+    static constexpr int kSmem   = 2 * kQTile + kTcStages * kTcStage + kRaw * kRawBytes + 1024;
+};
+static_assert(Tc<true>::kRawBytes == kQ8TileBytes, "a stage is a tile of the cache");
 static_assert(kTcStages * kTcStage >= kRows * kPartPitch * 16, "the partial results take the ring's memory");
 constexpr float kTcShift = 6.0f;                  // weights up to 2^(8 + 6): their remainders stay normal f16 numbers
 
-// multiply this thread's accumulator row by f; rare, kept out of line so that its registers do not weigh on the loop
-__device__ __noinline__ void rescale_row(uint32_t t_o, float f) {
+// multiply this thread's row of the accumulators (n blocks of 32 columns) by f; rare, kept out of line so that its registers do
+// not weigh on the loop
+__device__ __noinline__ void rescale_row(uint32_t t_o, int n, float f) {
     tc_fence_after();
 #pragma unroll 1
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < n; ++h) {
         float o[32];
         tmem_ld32(t_o + 32 * h, o);
 #pragma unroll
@@ -648,20 +660,42 @@ __device__ __noinline__ void rescale_row(uint32_t t_o, float f) {
     tc_fence_before();
 }
 
+// one row of a q8_0 tile: 64 bytes to 64 f16 at their swizzled places; zeros where the row does not exist
+__device__ __forceinline__ void expand_row(const uint8_t * bytes, uint8_t * out, int row, bool here) {
+#pragma unroll 2
+    for (int c = 0; c < 4; ++c) {
+        const uint4    x    = *reinterpret_cast<const uint4 *>(bytes + q8_byte_off(row, 16 * c));
+        const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+        uint32_t       h[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            h[2 * e]     = here ? s8_pair_to_half2(v[e], 0x4140) : 0u;
+            h[2 * e + 1] = here ? s8_pair_to_half2(v[e], 0x4342) : 0u;
+        }
+        *reinterpret_cast<uint4 *>(out + row * 128 + (((2 * c) ^ (row & 7)) << 4))     = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4 *>(out + row * 128 + (((2 * c + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+    }
+}
+
+template <bool Q8>
 __global__ void __maxnreg__(128)
 shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedParams p) {
+    constexpr int kSBufs = Tc<Q8>::kSBufs, kSCols = Tc<Q8>::kSCols, kTcOCol = Tc<Q8>::kOCol, kRaw = Q8 ? Tc<Q8>::kRaw : 1;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1];
+    __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1 + 2 * kRaw];
+    __shared__ float4   scales[Q8 ? kTcStages : 1][kSub];   // q8_0: of a row's K and V blocks
+    __shared__ uint32_t largest[kTcStages];                 // q8_0: the largest of a stage's V scales, as bits
     __shared__ uint32_t tmem_slot;
     __shared__ int      abort_flag;
     __shared__ float2   ml[kRows], joined[kRows];
     __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
-    const uint32_t sQ = smem_base, sKV = sQ + 2 * kQTile;
+    const uint32_t sQ = smem_base, sKV = sQ + 2 * kQTile, sRaw = sKV + kTcStages * kTcStage;
     const int      tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // full: a stage holds its tile in f16; empty: its products have retired; rfull, rempty: a tile's bytes have landed, are expanded
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = full0 + 8 * kTcStages, bS0 = empty0 + 8 * kTcStages, bP0 = bS0 + 8 * kSBufs,
-                   bF0 = bP0 + 8 * kSBufs, bO = bF0 + 8 * kSBufs;
+                   bF0 = bP0 + 8 * kSBufs, bO = bF0 + 8 * kSBufs, rfull0 = bO + 8, rempty0 = rfull0 + 8 * kRaw;
     const Item     w = load_item(p);
     if (w.rows == 0) {  // the same for the whole cluster
         pdl_wait();
@@ -670,8 +704,13 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < kTcStages; ++s) {
-            mbar_init(full0 + 8 * s, 1);
+            mbar_init(full0 + 8 * s, Q8 ? 4 : 1);
             mbar_init(empty0 + 8 * s, 1);
+            largest[s] = 0;
+        }
+        for (int s = 0; s < kRaw; ++s) {
+            mbar_init(rfull0 + 8 * s, 1);
+            mbar_init(rempty0 + 8 * s, 4);
         }
         for (int s = 0; s < kSBufs; ++s) {
             mbar_init(bS0 + 8 * s, 1);
@@ -695,7 +734,17 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     };
     auto aborted   = [&]() { return *reinterpret_cast<volatile int *>(&abort_flag) != 0; };
     auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0; };
+    constexpr int kAhead = Q8 ? kRaw : kTcStages;  // tiles on their way
     auto load_tile = [&](int U) {  // one lane
+        if constexpr (Q8) {
+            const uint32_t  bar = rfull0 + 8 * (U % kRaw), dst = sRaw + (U % kRaw) * Tc<Q8>::kRawBytes;
+            const uint8_t * src = p.q8_tiles + (size_t) w.prefix * p.q8_nb_stream + (size_t) w.kvh * p.q8_nb_head + q8_tile_off(w.key0 + U * kSub);
+            mbar_expect_tx(bar, kQ8TileBytes);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                         "r"((uint32_t) kQ8TileBytes), "r"(bar)
+                         : "memory");
+            return;
+        }
         const uint32_t bar = full0 + 8 * (U % kTcStages), dst = sKV + (U % kTcStages) * kTcStage;
         mbar_expect_tx(bar, kTcStage);
         tma_load_5d(dst, &map_k, bar, 0, w.key0 + U * kSub, w.kvh, w.prefix, p.layer);
@@ -703,7 +752,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     };
     if (warp == 5) {
         if (lane == 0)
-            for (int U = 0; U < min(n_sub, kTcStages); ++U) load_tile(U);
+            for (int U = 0; U < min(n_sub, kAhead); ++U) load_tile(U);
     } else if (warp < 4) {
         // Q: 16 threads per row, four head dimensions each; eight loads of a warp in flight.  (Two threads per row, a
         // float2 at a time, took 4 us: every load of a warp touched 16 rows.)
@@ -764,12 +813,12 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (!warp_wait(full0 + 8 * st, (U / kTcStages) & 1) || (U >= kSBufs && !warp_wait(bF0 + 8 * sb, ((U / kSBufs) - 1) & 1))) { ok = false; break; }
             tc_fence_after();
             if (leader) {
-                const uint32_t dS = tmem + kSub * sb;
+                const uint32_t dS = tmem + kSCols * sb;
                 const uint64_t k0 = dK + (uint64_t) (st * (kTcStage >> 4));
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc_mma_f16(dS, dQlo + k * 2, k0 + k * 2, idesc, k > 0);
+                for (int k = 0; k < 4; ++k) tc_mma_f16(Q8 ? dS + (k >> 1) * kSub : dS, dQlo + k * 2, k0 + k * 2, idesc, (Q8 ? k & 1 : k) > 0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc_mma_f16(dS, dQ + k * 2, k0 + k * 2, idesc, 1);
+                for (int k = 0; k < 4; ++k) tc_mma_f16(Q8 ? dS + (k >> 1) * kSub : dS, dQ + k * 2, k0 + k * 2, idesc, 1);
                 tc_commit(bS0 + 8 * sb);
             }
             __syncwarp();
@@ -781,50 +830,101 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const uint64_t     dV = smem_desc_sw128_mn(sKV + kSub * 128, 16);
         const bool         leader = elect_one();
         bool               ok = true;
-        int                loaded = min(n_sub, kTcStages);
+        int                loaded = min(n_sub, kAhead);
         for (int U = 0; U < n_sub && ok; ++U) {
             const int st = U % kTcStages, sb = U % kSBufs;
             if (!warp_wait(full0 + 8 * st, (U / kTcStages) & 1) || !warp_wait(bP0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
             tc_fence_after();
             if (leader) {
-                const uint32_t tP = tmem + kSub * sb, tO = tmem + kTcOCol;
                 const uint64_t v0 = dV + (uint64_t) (st * (kTcStage >> 4));
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + 8 * k, v0 + k * (2048 >> 4), idesc, U > 0 || k > 0);
+                for (int b = 0; b < (Q8 ? 2 : 1); ++b) {
+                    const uint32_t tP = tmem + kSCols * sb + kSub * b, tO = tmem + kTcOCol + kHeadDim * b;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + kSub / 2 + 8 * k, v0 + k * (2048 >> 4), idesc, 1);
+                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + 8 * k, v0 + k * (2048 >> 4), idesc, U > 0 || k > 0);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + kSub / 2 + 8 * k, v0 + k * (2048 >> 4), idesc, 1);
+                }
                 tc_commit(bF0 + 8 * sb);
                 tc_commit(empty0 + 8 * st);
                 if (U == n_sub - 1) tc_commit(bO);
             }
             __syncwarp();
-            // the stage of the tile before this one is free as soon as its P.V has retired, which was issued a tile ago
-            if (U > 0 && loaded < n_sub) {
-                if (!warp_wait(empty0 + 8 * ((U - 1) % kTcStages), ((U - 1) / kTcStages) & 1) || __any_sync(0xffffffffu, aborted())) { ok = false; break; }
+            // f16: the stage of the tile before this one is free as soon as its P.V has retired, which was issued a tile ago;
+            // q8_0: the bytes of this tile were expanded before its scores were made
+            if ((Q8 || U > 0) && loaded < n_sub) {
+                const bool free = Q8 ? warp_wait(rempty0 + 8 * (U % kRaw), (U / kRaw) & 1) : warp_wait(empty0 + 8 * ((U - 1) % kTcStages), ((U - 1) / kTcStages) & 1);
+                if (!free || __any_sync(0xffffffffu, aborted())) { ok = false; break; }
                 if (lane == 0) load_tile(loaded);
                 ++loaded;
             }
         }
         if (!ok) {
             if (lane == 0) give_up();
-            for (int i = max(0, loaded - kTcStages); i < loaded; ++i) warp_wait(full0 + 8 * (i % kTcStages), (i / kTcStages) & 1);  // copies in flight land
+            for (int i = max(0, loaded - kAhead); i < loaded; ++i)  // copies in flight land
+                warp_wait(Q8 ? rfull0 + 8 * (i % kRaw) : full0 + 8 * (i % kTcStages), (i / kAhead) & 1);
         }
     } else {
         // ------------------------------------------------------------------ softmax: a thread per row
         const uint32_t t_row = tmem + ((uint32_t) (32 * warp) << 16), t_o = t_row + kTcOCol;
-        float          m = -INFINITY, l = 0.0f;
+        float          m = -INFINITY, l = 0.0f, v_unit = 1.0f, v_limit = -1.0f;
         bool           ok = true;
-        for (int U = 0; U < n_sub; ++U) {
+        // q8_0: tile U's bytes to f16, K by the first two warps, V by the others; its scales, and the largest of V's
+        auto expand = [&](int U) {
+            const int rs = U % kRaw, st = U % kTcStages, row = tid & 63, left = n_keys - U * kSub;
+            if (!mbar_wait_bounded(rfull0 + 8 * rs, (U / kRaw) & 1) ||
+                (U >= kTcStages && !mbar_wait_bounded(empty0 + 8 * st, ((U / kTcStages) - 1) & 1))) return false;
+            const uint8_t * raw = smem_gen + (sRaw - smem_base) + rs * Tc<true>::kRawBytes;
+            uint8_t *       out = smem_gen + (sKV - smem_base) + st * kTcStage;
+            const bool      v   = tid >= kSub, here = row < left;
+            expand_row(raw + (v ? kQ8VBytesOff : 0), out + (v ? kSub * 128 : 0), row, here);
+            const uint32_t d  = here ? *reinterpret_cast<const uint32_t *>(raw + (v ? kQ8VScaleOff : kQ8KScaleOff) + row * 4) : 0u;
+            reinterpret_cast<float2 *>(&scales[Q8 ? st : 0][row])[v] = make_float2(half_lo(d), half_hi(d));
+            if (v) {
+                const __half2  a   = __habs2(as_half2(d));
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(a), __high2float(a))));
+                if (lane == 0) atomicMax(&largest[st], top);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(full0 + 8 * st);
+                mbar_arrive(rempty0 + 8 * rs);
+            }
+            return true;
+        };
+        if (Q8 && n_sub > 0) ok = expand(0);
+        for (int U = 0; U < n_sub && ok; ++U) {
             const int sb = U % kSBufs, left = n_keys - U * kSub;  // keys of this tile and after
-            if (!mbar_wait_bounded(bS0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
+            // (q8_0: a warp whose wait ran out stays until the barrier at the end of the tile, which the others wait at)
+            if (Q8 && U + 1 < n_sub && !expand(U + 1)) ok = false;
+            if (!mbar_wait_bounded(bS0 + 8 * sb, (U / kSBufs) & 1) || (Q8 && !mbar_wait_bounded(full0 + 8 * (U % kTcStages), (U / kTcStages) & 1))) {
+                ok = false;
+                if (!Q8) break;
+            }
             tc_fence_after();
-            const uint32_t t_s = t_row + kSub * sb;
+            const uint32_t t_s = t_row + kSCols * sb;
+            const float4 * sc  = scales[Q8 ? U % kTcStages : 0];
             uint32_t       r[kSub];
             tmem_ld64_sync(t_s, r);
+            if constexpr (Q8) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t x[32];
+                    tmem_ld32_sync(t_s + kSub + 32 * h, x);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 d = *reinterpret_cast<const float2 *>(sc + 32 * h + i);
+                        r[32 * h + i] = __float_as_uint(fmaf(__uint_as_float(x[i]), d.y, __uint_as_float(r[32 * h + i]) * d.x));
+                    }
+                }
+            }
             if (left < kSub) {
 #pragma unroll
                 for (int i = 0; i < kSub; ++i)
                     if (i >= left) r[i] = 0xff800000u;
+            }
+            if (!Q8 && left < kSub) {
                 // rows past the prefix may hold anything, and zero times a NaN is none: V's are cleared
                 const int st = U % kTcStages;
                 if (!mbar_wait_bounded(full0 + 8 * st, (U / kTcStages) & 1)) { ok = false; break; }
@@ -842,22 +942,59 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 t1 = max3(t1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
             }
             const float top = fmaxf(t0, t1);
+            float unit = 1.0f;  // q8_0: by how much the unit of the weights grows (the same for all rows)
+            if constexpr (Q8) {
+                const float dm = __uint_as_float(*reinterpret_cast<volatile uint32_t *>(&largest[U % kTcStages]));
+                if (dm > v_limit) {
+                    const float now = dm > 0.0f ? __uint_as_float(__float_as_uint(dm) & 0x7f800000u) : kTwoM24;
+                    unit    = v_unit / now;
+                    v_unit  = now;
+                    v_limit = dm > 0.0f ? now * 8.0f : 0.0f;
+                }
+            }
             if (U == 0) {
                 m = top;
             } else {
                 const bool raise = top > m + 8.0f;
-                if (__any_sync(0xffffffffu, raise)) {
+                if (__any_sync(0xffffffffu, raise || unit != 1.0f)) {
                     const float f = raise ? ex2_approx(m - top) : 1.0f;
                     if (raise) m = top;
                     l *= f;
-                    // the accumulator is at rest once P.V of the tile before has retired
-                    if (!mbar_wait_bounded(bF0 + 8 * ((U - 1) % kSBufs), ((U - 1) / kSBufs) & 1)) { ok = false; break; }
-                    rescale_row(t_o, f);
+                    // the accumulators are at rest once P.V of the tile before has retired
+                    if (!mbar_wait_bounded(bF0 + 8 * ((U - 1) % kSBufs), ((U - 1) / kSBufs) & 1)) {
+                        ok = false;
+                        if (!Q8) break;
+                    }
+                    rescale_row(t_o, Q8 ? 4 : 2, f * unit);
                 }
             }
-            const float ref = m - kTcShift;
+            const float ref = Q8 ? m : m - kTcShift, to_units = 4.0f / v_unit;  // weights up to 2^8 * 8 * 4 = 2^13
 #pragma unroll
             for (int g = 0; g < kSub / 16; ++g) {
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float e = ex2_approx(__uint_as_float(r[16 * g + i]) - ref);
+                        l += e;
+                        r[16 * g + i] = __float_as_uint(e * to_units);
+                    }
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float p0 = __uint_as_float(r[16 * g + 2 * i]) * (&sc[16 * g + 2 * i].z)[b];
+                            const float p1 = __uint_as_float(r[16 * g + 2 * i + 1]) * (&sc[16 * g + 2 * i + 1].z)[b];
+                            const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
+                            const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                            hi[i] = pack_half2(h0, h1);
+                            lo[i] = pack_half2(p0 - h0, p1 - h1);
+                        }
+                        tmem_st8_nowait(t_s + kSub * b + 8 * g, hi);
+                        tmem_st8_nowait(t_s + kSub * b + kSub / 2 + 8 * g, lo);
+                    }
+                    continue;
+                }
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -874,6 +1011,8 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             tmem_wait_st();
             tc_fence_before();
+            if (Q8 && !named_bar_all(1, kJoin, ok)) { ok = false; break; }  // every warp is done with the tile's scales
+            if (Q8 && tid == 0) largest[U % kTcStages] = 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(bP0 + 8 * sb);
         }
@@ -886,12 +1025,14 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t r[32];
-                tmem_ld32_sync(t_o + 32 * h, r);
+                tmem_ld32_sync(t_o + (Q8 ? kHeadDim + 32 : 32) * h, r);  // q8_0: the columns of block h from accumulator h
+                const float f = Q8 ? v_unit / 4.0f : 1.0f;
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
-                    part[8 * h + c] = make_float4(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1]), __uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3]));
+                    part[8 * h + c] = make_float4(__uint_as_float(r[4 * c]) * f, __uint_as_float(r[4 * c + 1]) * f, __uint_as_float(r[4 * c + 2]) * f,
+                                                  __uint_as_float(r[4 * c + 3]) * f);
             }
-            ml[tid] = make_float2(m - kTcShift, l);
+            ml[tid] = make_float2(Q8 ? m : m - kTcShift, l);
         }
     }
     // (the queries' tiles are done with: every score has been used)
@@ -1075,7 +1216,7 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml, shares}, workspace, own, st);
     if (rc != VOX_ATTN_OK || !shares) return rc;
     const vox_kv_cache * pc = a->prefix;
-    const bool           q8 = pc->cfg.type == VOX_TYPE_Q8_0, tc = !q8 && pl->full;
+    const bool           q8 = pc->cfg.type == VOX_TYPE_Q8_0, tc = pl->full;
     SharedParams         p;
     p.q = reinterpret_cast<const uint8_t *>(a->own.q);
     p.q_nb_head = a->own.q_nb_head; p.q_nb_stream = a->own.q_nb_stream;
@@ -1091,9 +1232,9 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     p.q8_nb_head = pc->nb_head; p.q8_nb_stream = pc->nb_stream;
     p.dst = a->own.dst; p.ml = ml; p.lse = a->lse;
     p.status = e->status_dev;
-    const auto     kernel = tc ? shared_rows_tc_kernel : q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
-    const int      smem   = tc ? kTcSmem : q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
-    const uint32_t bit    = 1u << (tc ? 21 : q8 ? 19 : 18);
+    const auto     kernel = tc ? (q8 ? shared_rows_tc_kernel<true> : shared_rows_tc_kernel<false>) : q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
+    const int      smem   = tc ? (q8 ? Tc<true>::kSmem : Tc<false>::kSmem) : q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
+    const uint32_t bit    = 1u << (tc ? (q8 ? 28 : 21) : q8 ? 19 : 18);
     if (!(e->attr_mask & bit)) {
         VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         // all of the SM's memory as shared memory, so that a CTA fits beside one of the decode kernel's
@@ -1111,7 +1252,7 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, pc->map_k, pc->map_v, p);
-    return check_launch(e, tc ? "shared_rows_tc_kernel" : q8 ? "shared_rows_kernel<q8_0>" : "shared_rows_kernel<f16>");
+    return check_launch(e, tc ? (q8 ? "shared_rows_tc_kernel<q8_0>" : "shared_rows_tc_kernel<f16>") : q8 ? "shared_rows_kernel<q8_0>" : "shared_rows_kernel<f16>");
 }
 
 }  // extern "C"
