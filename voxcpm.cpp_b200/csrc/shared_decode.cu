@@ -685,6 +685,8 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1 + 2 * kRaw];
     __shared__ float4   scales[Q8 ? kTcStages : 1][kSub];   // q8_0: of a row's K and V blocks
     __shared__ uint32_t largest[kTcStages];                 // q8_0: the largest of a stage's V scales, as bits
+    __shared__ const uint8_t * row_q[kRows];
+    __shared__ const float2 *  row_rope[kRows];
     __shared__ uint32_t tmem_slot;
     __shared__ int      abort_flag;
     __shared__ float2   ml[kRows], joined[kRows];
@@ -721,7 +723,13 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         fence_mbar_init();
     }
     if (warp == 4) tmem_alloc(smem_u32(&tmem_slot), 512);
-    if (tid < w.rows) rows_at[tid] = w.streams[tid / p.gqa] * p.n_heads + w.kvh * p.gqa + tid % p.gqa;
+    if (tid < kRows) {  // once per row: the loops below would divide over and over
+        const bool live   = tid < w.rows;
+        const int  stream = live ? w.streams[tid / p.gqa] : w.streams[0], head = w.kvh * p.gqa + (live ? tid % p.gqa : 0);
+        rows_at[tid]   = stream * p.n_heads + head;
+        row_q[tid]     = p.q + (size_t) stream * p.q_nb_stream + (size_t) head * p.q_nb_head;
+        row_rope[tid]  = p.rope + (size_t) stream * (kHeadDim / 2);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -762,16 +770,14 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         float4 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int row = 32 * warp + 16 * half + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
-            const float * src = reinterpret_cast<const float *>(p.q + (size_t) (at / p.n_heads) * p.q_nb_stream + (size_t) (at % p.n_heads) * p.q_nb_head) + 4 * c;
+            const float * src = reinterpret_cast<const float *>(row_q[32 * warp + 16 * half + 2 * i + (lane >> 4)]) + 4 * c;
             const float2  a = *reinterpret_cast<const float2 *>(src), b = *reinterpret_cast<const float2 *>(src + 2);
             x[i] = make_float4(a.x, a.y, b.x, b.y);
         }
         if (p.rope != nullptr) {  // elements d and d + 32 are partners: lanes c and c ^ 8
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int row = 32 * warp + 16 * half + 2 * i + (lane >> 4), at = row < w.rows ? rows_at[row] : 0;
-                const float2 * tb = p.rope + (size_t) (at / p.n_heads) * (kHeadDim / 2) + 4 * (c & 7);
+                const float2 * tb = row_rope[32 * warp + 16 * half + 2 * i + (lane >> 4)] + 4 * (c & 7);
                 const float *  xi = &x[i].x;
                 float          y[4];
 #pragma unroll
@@ -972,26 +978,25 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
             for (int g = 0; g < kSub / 16; ++g) {
                 if constexpr (Q8) {
+                    uint32_t hi[2][8], lo[2][8];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float e = ex2_approx(__uint_as_float(r[16 * g + i]) - ref);
-                        l += e;
-                        r[16 * g + i] = __float_as_uint(e * to_units);
+                    for (int i = 0; i < 8; ++i) {
+                        const float  e0 = ex2_approx(__uint_as_float(r[16 * g + 2 * i]) - ref), e1 = ex2_approx(__uint_as_float(r[16 * g + 2 * i + 1]) - ref);
+                        const float2 d0 = *reinterpret_cast<const float2 *>(&sc[16 * g + 2 * i].z), d1 = *reinterpret_cast<const float2 *>(&sc[16 * g + 2 * i + 1].z);
+                        l += e0 + e1;
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const float p0 = e0 * to_units * (b ? d0.y : d0.x), p1 = e1 * to_units * (b ? d1.y : d1.x);
+                            const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
+                            const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                            hi[b][i] = pack_half2(h0, h1);
+                            lo[b][i] = pack_half2(p0 - h0, p1 - h1);
+                        }
                     }
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        uint32_t hi[8], lo[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float p0 = __uint_as_float(r[16 * g + 2 * i]) * (&sc[16 * g + 2 * i].z)[b];
-                            const float p1 = __uint_as_float(r[16 * g + 2 * i + 1]) * (&sc[16 * g + 2 * i + 1].z)[b];
-                            const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
-                            const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
-                            hi[i] = pack_half2(h0, h1);
-                            lo[i] = pack_half2(p0 - h0, p1 - h1);
-                        }
-                        tmem_st8_nowait(t_s + kSub * b + 8 * g, hi);
-                        tmem_st8_nowait(t_s + kSub * b + kSub / 2 + 8 * g, lo);
+                        tmem_st8_nowait(t_s + kSub * b + 8 * g, hi[b]);
+                        tmem_st8_nowait(t_s + kSub * b + kSub / 2 + 8 * g, lo[b]);
                     }
                     continue;
                 }
