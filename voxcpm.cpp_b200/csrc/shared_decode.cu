@@ -615,27 +615,28 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // Full row tiles on the 5th-generation tensor cores.
 //
 // Q (scaled by scale * log2 e) lies in shared memory as two f16 tiles, value and remainder; scores S = Q_lo.K + Q_hi.K (the
-// small part first: the accumulator truncates) come 64 keys at a time into one of six score buffers in TMEM.  Four softmax
+// small part first: the accumulator truncates) come 64 keys at a time into one of four score buffers in TMEM.  Four softmax
 // warps, a thread per row: 64 scores out of TMEM, weights 2^(S - ref) back over them as two packed f16 tiles (value and
-// remainder, 22 bits), from where the tensor core takes them as the A operand of P.V.  The reference of a row is raised
-// only when a maximum exceeds it by 2^8 (its accumulator is then rescaled in TMEM).
+// remainder, 22 bits), from where the tensor core takes them as the A operand of P.V.  The output has four accumulators,
+// values and remainders of even and of odd tiles, added up in f32 at the end: the tensor core truncates every sum it
+// makes, and one accumulator for all came out 2.2e-6 too small after 1024 keys.  The reference of a row is raised only
+// when a maximum exceeds it by 2^8 (its accumulators are then rescaled in TMEM).
 //   warps 0-3  softmax      warp 4  issues S = Q.K      warp 5  issues O += P.V, and the copies of K and V (64 rows a stage)
 // 192 threads of 128 registers and 83 KB of shared memory: the CTA runs beside two CTAs of the decode kernel, whose time is
 // HBM's.  (With two softmax groups, 352 threads and 128-key stages it was no faster on its own and had to wait for the
 // decode kernel's CTAs to leave: 57.4 us for 256 streams under two prompts of 4096 rows.)
 //
 // q8_0: the softmax warps turn a tile's bytes into f16 numbers q (exact; a tile ahead of the scores they work on) and keep the
-// scales apart.  Either 32-value block has an accumulator of its own: two of S (s = d0 S0 + d1 S1) and two of O, whose
-// weights have V's scale of their block taken in; of either O the half that belongs to its block is used.  The weights are
-// taken in units of v_unit, as in the other kernel.
+// scales apart.  Either 32-value block has a score accumulator of its own (s = d0 S0 + d1 S1), and its 32 output columns have
+// weights of their own, with V's scale of the block taken in, in units of v_unit as in the other kernel.
 constexpr int kTcThreads = 6 * 32;
 constexpr int kSub       = 64;                    // keys of a score tile and of a stage
 constexpr int kQTile     = kRows * 128;
 constexpr int kTcStages  = 3;
 constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V, in f16
 template <bool Q8> struct Tc {
-    static constexpr int kSCols  = Q8 ? 2 * kSub : kSub;   // TMEM columns of a score tile, and of the accumulators behind the buffers
-    static constexpr int kSBufs  = Q8 ? 3 : 6;
+    static constexpr int kSCols  = Q8 ? 2 * kSub : kSub;   // TMEM columns of a score tile
+    static constexpr int kSBufs  = Q8 ? 2 : 4;             // the accumulators, 4 x 64 columns, lie behind the buffers
     static constexpr int kOCol   = kSBufs * kSCols;
     static constexpr int kRaw    = Q8 ? 3 : 0;             // q8_0: stages of tiles as the cache holds them
     static constexpr int kRawBytes = 8704;
@@ -645,12 +646,11 @@ static_assert(Tc<true>::kRawBytes == kQ8TileBytes, "a stage is a tile of the cac
 static_assert(kTcStages * kTcStage >= kRows * kPartPitch * 16, "the partial results take the ring's memory");
 constexpr float kTcShift = 6.0f;                  // weights up to 2^(8 + 6): their remainders stay normal f16 numbers
 
-// multiply this thread's row of the accumulators (n blocks of 32 columns) by f; rare, kept out of line so that its registers do
-// not weigh on the loop
-__device__ __noinline__ void rescale_row(uint32_t t_o, int n, float f) {
+// multiply this thread's row of the accumulators by f; rare, kept out of line so that its registers do not weigh on the loop
+__device__ __noinline__ void rescale_row(uint32_t t_o, float f) {
     tc_fence_after();
 #pragma unroll 1
-    for (int h = 0; h < n; ++h) {
+    for (int h = 0; h < 8; ++h) {
         float o[32];
         tmem_ld32(t_o + 32 * h, o);
 #pragma unroll
@@ -832,7 +832,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (!ok && lane == 0) give_up();
     } else if (warp == 5) {
         // ------------------------------------------------------------------ output, and the copies behind it
-        constexpr uint32_t idesc = idesc_f16(kHeadDim, true);
+        constexpr uint32_t idesc = idesc_f16(Q8 ? 32 : kHeadDim, true);
         const uint64_t     dV = smem_desc_sw128_mn(sKV + kSub * 128, 16);
         const bool         leader = elect_one();
         bool               ok = true;
@@ -845,11 +845,13 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 const uint64_t v0 = dV + (uint64_t) (st * (kTcStage >> 4));
 #pragma unroll
                 for (int b = 0; b < (Q8 ? 2 : 1); ++b) {
-                    const uint32_t tP = tmem + kSCols * sb + kSub * b, tO = tmem + kTcOCol + kHeadDim * b;
+                    // q8_0: block b's 32 columns of V, 64 bytes into the swizzle atom
+                    const uint32_t tP = tmem + kSCols * sb + kSub * b, tO = tmem + kTcOCol + 2 * kHeadDim * (U & 1) + 32 * b;
+                    const uint64_t vb = v0 + b * (64 >> 4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + 8 * k, v0 + k * (2048 >> 4), idesc, U > 0 || k > 0);
+                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + 8 * k, vb + k * (2048 >> 4), idesc, U > 1 || k > 0);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO, tP + kSub / 2 + 8 * k, v0 + k * (2048 >> 4), idesc, 1);
+                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO + kHeadDim, tP + kSub / 2 + 8 * k, vb + k * (2048 >> 4), idesc, U > 1 || k > 0);
                 }
                 tc_commit(bF0 + 8 * sb);
                 tc_commit(empty0 + 8 * st);
@@ -971,7 +973,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         ok = false;
                         if (!Q8) break;
                     }
-                    rescale_row(t_o, Q8 ? 4 : 2, f * unit);
+                    rescale_row(t_o, f * unit);
                 }
             }
             const float ref = Q8 ? m : m - kTcShift, to_units = 4.0f / v_unit;  // weights up to 2^8 * 8 * 4 = 2^13
@@ -1027,11 +1029,17 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (all_ok && n_sub > 0) {
             tc_fence_after();
             float4 * const part = reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)) + tid * kPartPitch;
+            const float f = Q8 ? v_unit / 4.0f : 1.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t r[32];
-                tmem_ld32_sync(t_o + (Q8 ? kHeadDim + 32 : 32) * h, r);  // q8_0: the columns of block h from accumulator h
-                const float f = Q8 ? v_unit / 4.0f : 1.0f;
+                uint32_t r[32], x[32];
+                tmem_ld32_sync(t_o + 32 * h, r);
+#pragma unroll 1
+                for (int o = 1; o < (n_sub > 1 ? 4 : 2); ++o) {
+                    tmem_ld32_sync(t_o + kHeadDim * o + 32 * h, x);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + __uint_as_float(x[c]));
+                }
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                     part[8 * h + c] = make_float4(__uint_as_float(r[4 * c]) * f, __uint_as_float(r[4 * c + 1]) * f, __uint_as_float(r[4 * c + 2]) * f,
