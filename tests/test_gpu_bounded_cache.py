@@ -99,6 +99,8 @@ SHARED = {
     "full row tiles, edges": ("f16", [i % 8 for i in range(128)], [1, 63, 64, 65, 127, 128, 129, 193], [i % 5 for i in range(128)], 16, 2),
     "full row tiles, long": ("f16", [i % 2 for i in range(40)], [5000, 1601], [1 + i for i in range(40)], 16, 2),
     "full row tiles, six heads": ("f16", [0] * 45, [777], [3] * 45, 6, 1),
+    "full row tiles beside long streams": ("f16", [i % 8 for i in range(128)], [1, 63, 64, 65, 127, 128, 129, 400], [2500 - 19 * i for i in range(128)], 16, 2),
+    "q8_0 full row tiles beside long streams": ("q8_0", [i % 8 for i in range(128)], [1, 63, 64, 65, 127, 128, 129, 400], [2500 - 19 * i for i in range(128)], 16, 2),
     "q8_0 one row of each": ("q8_0", [0], [1], [1], 16, 2),
     "q8_0 tile edges": ("q8_0", [0, 1, 2, 3, 4, 5], [63, 64, 65, 127, 128, 129], [129, 128, 127, 65, 64, 63], 16, 2),
     "q8_0 mixed": ("q8_0", [2, -1, 0, 2, -1, 1, 2, 0, 0, 2, 1], [700, 33, 1025], [5, 0, 300, 1, 66, 0, 8, 640, 17, 2, 90], 16, 2),
@@ -169,11 +171,12 @@ def test_shared_prefix_with_small_and_large_values(kind, v_scale, engine, pkg):
     SharedCase(engine, pkg, (kind, [0] * 16, [300], [40] * 16, 16, 2), v_scale=v_scale).check()
 
 
-@pytest.mark.parametrize("streams", [2, 20])
+@pytest.mark.parametrize("streams", [2, 20, 40])
 def test_shared_prefix_scales_that_grow_along_the_rows(streams, engine, pkg):
     """q8_0 scales over a range of 2^24 inside one softmax: the unit of the weights follows the largest so far."""
     import torch
-    c = SharedCase(engine, pkg, ("q8_0", [0] * streams, [512], [200, 64] * (streams // 2), 16, 2), junk=False)
+    own = 3000 if streams == 40 else 200  # 40: the form that runs beside two decode CTAs per SM
+    c = SharedCase(engine, pkg, ("q8_0", [0] * streams, [512], [own, 64] * (streams // 2), 16, 2), junk=False)
     for cache, n in ((c.own, 200), (c.prefix, 512)):
         rows = cache.cfg.max_len
         k = randn(gen(3), cache.cfg.n_streams, rows, 2, D)

@@ -1226,7 +1226,7 @@ namespace vox {
 //   - a launch with fewer tiles than that gets fewer CTAs.
 // The cut itself happens on the device from the lengths of the moment; kv_bound only sizes the grid.
 void decode_plan(const vox_engine * e, bool q8, int n_streams, int n_kv_heads, int kv_bound, int * grid, int * run_min, bool shared = false,
-                 bool beside = false) {
+                 int most = 0) {
     const long long tiles_bound = std::max(1, (std::max(kv_bound, 1) + kKvTile - 1) / kKvTile);
     const long long pairs       = std::max(1LL, (long long) n_streams * n_kv_heads);
     const int       fit         = q8 ? Ring<true>::ctas_per_sm(shared) : Ring<false>::ctas_per_sm(shared);
@@ -1234,7 +1234,7 @@ void decode_plan(const vox_engine * e, bool q8, int n_streams, int n_kv_heads, i
     int             sms         = kDecodeMaxSms;
     if (e != nullptr) {
         const int tuned = e->decode_wave[q8 ? 1 : 0];
-        if (beside) wave = std::min(wave, 2);
+        if (most > 0) wave = std::min(wave, most);
         if (tuned > 0) wave = std::min(tuned, fit);
         sms = std::min(sms, e->sm_count);
     }
@@ -1339,7 +1339,7 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
         p.mask_ne2 = (int) mask->ne[2]; p.mask_ne3 = (int) mask->ne[3];
     }
     int grid = 1;
-    decode_plan(e, q8, n_streams, n_kv_heads, kv_bound, &grid, &p.run_min, shared, shared && rows->beside);
+    decode_plan(e, q8, n_streams, n_kv_heads, kv_bound, &grid, &p.run_min, shared, shared ? rows->wave : 0);
     const size_t need = (size_t) 2 * grid * p.gqa * kPartialStride * sizeof(float);
     VOX_REQUIRE(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0,
                 VOX_ATTN_WORKSPACE_TOO_SMALL, "decode needs %zu workspace bytes (8-byte aligned), got %zu", need, workspace_bytes);
@@ -1353,7 +1353,7 @@ int launch_decode(vox_engine * e, bool q8, const CUtensorMap & map_k, const CUte
     const int depth  = q8 ? Ring<true>::kStages : Ring<false>::kStages;
     const int spare  = q8 ? 2 : 1;  // ring stages whose memory holds the partials instead: 18 KB / 16 KB
     const int slots  = std::min(kDecodeMaxSms, e->sm_count) *
-                      (shared && rows->beside ? 2 : q8 ? Ring<true>::kCtasPerSm : Ring<false>::kCtasPerSm);
+                      (shared && rows->wave > 0 ? rows->wave : q8 ? Ring<true>::kCtasPerSm : Ring<false>::kCtasPerSm);
     const int pairs  = n_streams * n_kv_heads;
     const int c_fit  = (q8 ? 2 * Ring<true>::kStageBytes : Ring<false>::kStageBytes) / (kMaxGqa * kPartialStride * 4);  // slots of partials that fit
     const int tiles_bound = std::max(1, (std::max(kv_bound, 1) + kKvTile - 1) / kKvTile);

@@ -621,36 +621,38 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // values and remainders of even and of odd tiles, added up in f32 at the end: the tensor core truncates every sum it
 // makes, and one accumulator for all came out 2.2e-6 too small after 1024 keys.  The reference of a row is raised only
 // when a maximum exceeds it by 2^8 (its accumulators are then rescaled in TMEM).
-//   warps 0-3  softmax      warp 4  issues S = Q.K      warp 5  issues O += P.V, and the copies of K and V (64 rows a stage)
-// 192 threads of 128 registers and 83 KB of shared memory: the CTA runs beside two CTAs of the decode kernel, whose time is
-// HBM's.  (With two softmax groups, 352 threads and 128-key stages it was no faster on its own and had to wait for the
-// decode kernel's CTAs to leave: 57.4 us for 256 streams under two prompts of 4096 rows.)
+//   warps 0 .. 4 kGroups - 1  softmax      then one warp  issues S = Q.K      and one  issues O += P.V and the copies of K and V
+// One softmax group (192 threads of 128 registers, 81 KB of shared memory; q8_0 107 KB): the CTA runs beside two CTAs of the decode
+// kernel, whose time is HBM's, and takes about 1.1 us for 64 keys (q8_0 2.3 us), most of it latency that nothing hides.
+// Two groups, which take tiles in turn with a reference and accumulators of their own, need less than two thirds of that,
+// but leave room for one decode CTA per SM only: taken where the streams' own rows are few against the prefix (see
+// vox_attn_decode_shared).
 //
 // q8_0: the softmax warps turn a tile's bytes into f16 numbers q (exact; a tile ahead of the scores they work on) and keep the
 // scales apart.  Either 32-value block has a score accumulator of its own (s = d0 S0 + d1 S1), and its 32 output columns have
 // weights of their own, with V's scale of the block taken in, in units of v_unit as in the other kernel.
-constexpr int kTcThreads = 6 * 32;
 constexpr int kSub       = 64;                    // keys of a score tile and of a stage
 constexpr int kQTile     = kRows * 128;
-constexpr int kTcStages  = 3;
 constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V, in f16
-template <bool Q8> struct Tc {
+template <bool Q8, int kGroups> struct Tc {
+    static constexpr int kThreads = (4 * kGroups + 2) * 32;
+    static constexpr int kStages  = 2 + kGroups;
     static constexpr int kSCols  = Q8 ? 2 * kSub : kSub;   // TMEM columns of a score tile
     static constexpr int kSBufs  = Q8 ? 2 : 4;             // the accumulators, 4 x 64 columns, lie behind the buffers
     static constexpr int kOCol   = kSBufs * kSCols;
-    static constexpr int kRaw    = Q8 ? 3 : 0;             // q8_0: stages of tiles as the cache holds them
+    static constexpr int kRaw    = Q8 ? kStages : 0;       // q8_0: stages of tiles as the cache holds them
     static constexpr int kRawBytes = 8704;
-    static constexpr int kSmem   = 2 * kQTile + kTcStages * kTcStage + kRaw * kRawBytes + 1024;
+    static constexpr int kSmem   = 2 * kQTile + kStages * kTcStage + kRaw * kRawBytes + 1024;
+    // the partial results, and behind those of one group its CTA's share of the rows, take the queries' and the ring's memory
+    static_assert(kRawBytes == kQ8TileBytes && 2 * kQTile + kStages * kTcStage >= 2 * kRows * kPartPitch * 16, "shared memory");
 };
-static_assert(Tc<true>::kRawBytes == kQ8TileBytes, "a stage is a tile of the cache");
-static_assert(kTcStages * kTcStage >= kRows * kPartPitch * 16, "the partial results take the ring's memory");
 constexpr float kTcShift = 6.0f;                  // weights up to 2^(8 + 6): their remainders stay normal f16 numbers
 
 // multiply this thread's row of the accumulators by f; rare, kept out of line so that its registers do not weigh on the loop
-__device__ __noinline__ void rescale_row(uint32_t t_o, float f) {
+__device__ __noinline__ void rescale_row(uint32_t t_o, int blocks, float f) {
     tc_fence_after();
 #pragma unroll 1
-    for (int h = 0; h < 8; ++h) {
+    for (int h = 0; h < blocks; ++h) {  // of 32 columns
         float o[32];
         tmem_ld32(t_o + 32 * h, o);
 #pragma unroll
@@ -677,10 +679,12 @@ __device__ __forceinline__ void expand_row(const uint8_t * bytes, uint8_t * out,
     }
 }
 
-template <bool Q8>
+template <bool Q8, int kGroups>
 __global__ void __maxnreg__(128)
 shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedParams p) {
-    constexpr int kSBufs = Tc<Q8>::kSBufs, kSCols = Tc<Q8>::kSCols, kTcOCol = Tc<Q8>::kOCol, kRaw = Q8 ? Tc<Q8>::kRaw : 1;
+    using Z = Tc<Q8, kGroups>;
+    constexpr int kTcStages = Z::kStages, kSBufs = Z::kSBufs, kSCols = Z::kSCols, kTcOCol = Z::kOCol, kRaw = Q8 ? Z::kRaw : 1;
+    constexpr int kSoftmax = 4 * kGroups, kScoreWarp = kSoftmax, kOutWarp = kSoftmax + 1;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1 + 2 * kRaw];
     __shared__ float4   scales[Q8 ? kTcStages : 1][kSub];   // q8_0: of a row's K and V blocks
@@ -689,7 +693,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __shared__ const float2 *  row_rope[kRows];
     __shared__ uint32_t tmem_slot;
     __shared__ int      abort_flag;
-    __shared__ float2   ml[kRows], joined[kRows];
+    __shared__ float2   ml[kGroups * kRows], joined[kRows];
     __shared__ int      rows_at[kRows];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -716,13 +720,13 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
         for (int s = 0; s < kSBufs; ++s) {
             mbar_init(bS0 + 8 * s, 1);
-            mbar_init(bP0 + 8 * s, 4);  // one arrival per softmax warp
+            mbar_init(bP0 + 8 * s, 4);  // one arrival per warp of the group that took the tile
             mbar_init(bF0 + 8 * s, 1);
         }
         mbar_init(bO, 1);
         fence_mbar_init();
     }
-    if (warp == 4) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (warp == kScoreWarp) tmem_alloc(smem_u32(&tmem_slot), 512);
     if (tid < kRows) {  // once per row: the loops below would divide over and over
         const bool live   = tid < w.rows;
         const int  stream = live ? w.streams[tid / p.gqa] : w.streams[0], head = w.kvh * p.gqa + (live ? tid % p.gqa : 0);
@@ -745,7 +749,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     constexpr int kAhead = Q8 ? kRaw : kTcStages;  // tiles on their way
     auto load_tile = [&](int U) {  // one lane
         if constexpr (Q8) {
-            const uint32_t  bar = rfull0 + 8 * (U % kRaw), dst = sRaw + (U % kRaw) * Tc<Q8>::kRawBytes;
+            const uint32_t  bar = rfull0 + 8 * (U % kRaw), dst = sRaw + (U % kRaw) * Z::kRawBytes;
             const uint8_t * src = p.q8_tiles + (size_t) w.prefix * p.q8_nb_stream + (size_t) w.kvh * p.q8_nb_head + q8_tile_off(w.key0 + U * kSub);
             mbar_expect_tx(bar, kQ8TileBytes);
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
@@ -758,26 +762,26 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         tma_load_5d(dst, &map_k, bar, 0, w.key0 + U * kSub, w.kvh, w.prefix, p.layer);
         tma_load_5d(dst + kSub * 128, &map_v, bar, 0, w.key0 + U * kSub, w.kvh, w.prefix, p.layer);
     };
-    if (warp == 5) {
+    if (warp == kOutWarp) {
         if (lane == 0)
             for (int U = 0; U < min(n_sub, kAhead); ++U) load_tile(U);
-    } else if (warp < 4) {
+    } else if (warp < kSoftmax) {
         // Q: 16 threads per row, four head dimensions each; eight loads of a warp in flight.  (Two threads per row, a
         // float2 at a time, took 4 us: every load of a warp touched 16 rows.)
         const int c = lane & 15;
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
+        for (int half = warp >> 2; half < 2; half += kGroups) {
         float4 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float * src = reinterpret_cast<const float *>(row_q[32 * warp + 16 * half + 2 * i + (lane >> 4)]) + 4 * c;
+            const float * src = reinterpret_cast<const float *>(row_q[32 * (warp & 3) + 16 * half + 2 * i + (lane >> 4)]) + 4 * c;
             const float2  a = *reinterpret_cast<const float2 *>(src), b = *reinterpret_cast<const float2 *>(src + 2);
             x[i] = make_float4(a.x, a.y, b.x, b.y);
         }
         if (p.rope != nullptr) {  // elements d and d + 32 are partners: lanes c and c ^ 8
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float2 * tb = row_rope[32 * warp + 16 * half + 2 * i + (lane >> 4)] + 4 * (c & 7);
+                const float2 * tb = row_rope[32 * (warp & 3) + 16 * half + 2 * i + (lane >> 4)] + 4 * (c & 7);
                 const float *  xi = &x[i].x;
                 float          y[4];
 #pragma unroll
@@ -791,7 +795,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int    row = 32 * warp + 16 * half + 2 * i + (lane >> 4);
+            const int    row = 32 * (warp & 3) + 16 * half + 2 * i + (lane >> 4);
             const bool   live = row < w.rows;
             float        h[4], l[4];
             split_hi_lo(live ? x[i].x * p.scale_log2 : 0.0f, h[0], l[0]);
@@ -808,7 +812,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __syncthreads();
 
     bool all_ok = true;  // of the softmax warps
-    if (warp == 4) {
+    if (warp == kScoreWarp) {
         // ------------------------------------------------------------------ scores (all lanes in the loop, one issues)
         constexpr uint32_t idesc = idesc_f16(kSub, false);
         const uint64_t     dQ = smem_desc_sw128(sQ), dQlo = smem_desc_sw128(sQ + kQTile), dK = smem_desc_sw128(sKV);
@@ -830,7 +834,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             __syncwarp();
         }
         if (!ok && lane == 0) give_up();
-    } else if (warp == 5) {
+    } else if (warp == kOutWarp) {
         // ------------------------------------------------------------------ output, and the copies behind it
         constexpr uint32_t idesc = idesc_f16(Q8 ? 32 : kHeadDim, true);
         const uint64_t     dV = smem_desc_sw128_mn(sKV + kSub * 128, 16);
@@ -874,20 +878,22 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
     } else {
         // ------------------------------------------------------------------ softmax: a thread per row
-        const uint32_t t_row = tmem + ((uint32_t) (32 * warp) << 16), t_o = t_row + kTcOCol;
+        const int      group = warp >> 2, row = tid & 127;
+        // accumulators: [parity of the tile][value, remainder][64]; with two groups a group has those of one parity
+        const uint32_t t_row = tmem + ((uint32_t) (32 * (warp & 3)) << 16), t_o = t_row + kTcOCol + (kGroups == 2 ? 2 * kHeadDim * group : 0);
         float          m = -INFINITY, l = 0.0f, v_unit = 1.0f, v_limit = -1.0f;
         bool           ok = true;
-        // q8_0: tile U's bytes to f16, K by the first two warps, V by the others; its scales, and the largest of V's
+        // q8_0: tile U's bytes to f16, K by the group's first two warps, V by the others; its scales, and the largest of V's
         auto expand = [&](int U) {
-            const int rs = U % kRaw, st = U % kTcStages, row = tid & 63, left = n_keys - U * kSub;
+            const int rs = U % kRaw, st = U % kTcStages, key = row & 63, left = n_keys - U * kSub;
             if (!mbar_wait_bounded(rfull0 + 8 * rs, (U / kRaw) & 1) ||
                 (U >= kTcStages && !mbar_wait_bounded(empty0 + 8 * st, ((U / kTcStages) - 1) & 1))) return false;
-            const uint8_t * raw = smem_gen + (sRaw - smem_base) + rs * Tc<true>::kRawBytes;
+            const uint8_t * raw = smem_gen + (sRaw - smem_base) + rs * Z::kRawBytes;
             uint8_t *       out = smem_gen + (sKV - smem_base) + st * kTcStage;
-            const bool      v   = tid >= kSub, here = row < left;
-            expand_row(raw + (v ? kQ8VBytesOff : 0), out + (v ? kSub * 128 : 0), row, here);
-            const uint32_t d  = here ? *reinterpret_cast<const uint32_t *>(raw + (v ? kQ8VScaleOff : kQ8KScaleOff) + row * 4) : 0u;
-            reinterpret_cast<float2 *>(&scales[Q8 ? st : 0][row])[v] = make_float2(half_lo(d), half_hi(d));
+            const bool      v   = row >= kSub, here = key < left;
+            expand_row(raw + (v ? kQ8VBytesOff : 0), out + (v ? kSub * 128 : 0), key, here);
+            const uint32_t d  = here ? *reinterpret_cast<const uint32_t *>(raw + (v ? kQ8VScaleOff : kQ8KScaleOff) + key * 4) : 0u;
+            reinterpret_cast<float2 *>(&scales[Q8 ? st : 0][key])[v] = make_float2(half_lo(d), half_hi(d));
             if (v) {
                 const __half2  a   = __habs2(as_half2(d));
                 const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(a), __high2float(a))));
@@ -901,11 +907,11 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             return true;
         };
-        if (Q8 && n_sub > 0) ok = expand(0);
-        for (int U = 0; U < n_sub && ok; ++U) {
+        if (Q8 && group < n_sub) ok = expand(group);
+        for (int U = group; U < n_sub && (Q8 || ok); U += kGroups) {
             const int sb = U % kSBufs, left = n_keys - U * kSub;  // keys of this tile and after
             // (q8_0: a warp whose wait ran out stays until the barrier at the end of the tile, which the others wait at)
-            if (Q8 && U + 1 < n_sub && !expand(U + 1)) ok = false;
+            if (Q8 && U + kGroups < n_sub && !expand(U + kGroups)) ok = false;
             if (!mbar_wait_bounded(bS0 + 8 * sb, (U / kSBufs) & 1) || (Q8 && !mbar_wait_bounded(full0 + 8 * (U % kTcStages), (U / kTcStages) & 1))) {
                 ok = false;
                 if (!Q8) break;
@@ -936,8 +942,8 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 // rows past the prefix may hold anything, and zero times a NaN is none: V's are cleared
                 const int st = U % kTcStages;
                 if (!mbar_wait_bounded(full0 + 8 * st, (U / kTcStages) & 1)) { ok = false; break; }
-                if (tid >= left && tid < kSub) {
-                    uint4 * v = reinterpret_cast<uint4 *>(smem_gen + (sKV - smem_base) + st * kTcStage + (kSub + tid) * 128);
+                if (row >= left && row < kSub) {
+                    uint4 * v = reinterpret_cast<uint4 *>(smem_gen + (sKV - smem_base) + st * kTcStage + (kSub + row) * 128);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
@@ -960,7 +966,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     v_limit = dm > 0.0f ? now * 8.0f : 0.0f;
                 }
             }
-            if (U == 0) {
+            if (U < kGroups) {
                 m = top;
             } else {
                 const bool raise = top > m + 8.0f;
@@ -968,12 +974,12 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     const float f = raise ? ex2_approx(m - top) : 1.0f;
                     if (raise) m = top;
                     l *= f;
-                    // the accumulators are at rest once P.V of the tile before has retired
-                    if (!mbar_wait_bounded(bF0 + 8 * ((U - 1) % kSBufs), ((U - 1) / kSBufs) & 1)) {
+                    // the accumulators are at rest once P.V of the group's tile before has retired
+                    if (!mbar_wait_bounded(bF0 + 8 * ((U - kGroups) % kSBufs), ((U - kGroups) / kSBufs) & 1)) {
                         ok = false;
                         if (!Q8) break;
                     }
-                    rescale_row(t_o, f * unit);
+                    rescale_row(t_o, 8 / kGroups, f * unit);
                 }
             }
             const float ref = Q8 ? m : m - kTcShift, to_units = 4.0f / v_unit;  // weights up to 2^8 * 8 * 4 = 2^13
@@ -1018,24 +1024,29 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             tmem_wait_st();
             tc_fence_before();
-            if (Q8 && !named_bar_all(1, kJoin, ok)) { ok = false; break; }  // every warp is done with the tile's scales
-            if (Q8 && tid == 0) largest[U % kTcStages] = 0;
+            if (Q8 && !named_bar_all(2 + group, 128, ok)) { ok = false; break; }  // every warp of the group is done with the tile's scales
+            if (Q8 && row == 0) largest[U % kTcStages] = 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(bP0 + 8 * sb);
         }
         if (ok && n_sub > 0 && !mbar_wait_bounded(bO, 0)) ok = false;
         if (!ok) give_up();
-        all_ok = named_bar_all(1, kJoin, ok && !aborted());  // every copy has been consumed: the ring's memory is free
+        all_ok = named_bar_all(1, 128 * kGroups, ok && !aborted());  // every copy and every score has been used: the memory is free
         if (all_ok && n_sub > 0) {
             tc_fence_after();
-            float4 * const part = reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)) + tid * kPartPitch;
-            const float f = Q8 ? v_unit / 4.0f : 1.0f;
+            float4 * const part  = reinterpret_cast<float4 *>(smem_gen) + (group * kRows + row) * kPartPitch;
+            const float    f     = Q8 ? v_unit / 4.0f : 1.0f;
+            const int      parts = group >= n_sub ? 0 : kGroups == 2 || n_sub == 1 ? 2 : 4;  // accumulators with something in them
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t r[32], x[32];
                 tmem_ld32_sync(t_o + 32 * h, r);
+                if (parts == 0) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) r[c] = 0u;
+                }
 #pragma unroll 1
-                for (int o = 1; o < (n_sub > 1 ? 4 : 2); ++o) {
+                for (int o = 1; o < parts; ++o) {
                     tmem_ld32_sync(t_o + kHeadDim * o + 32 * h, x);
 #pragma unroll
                     for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + __uint_as_float(x[c]));
@@ -1045,15 +1056,16 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     part[8 * h + c] = make_float4(__uint_as_float(r[4 * c]) * f, __uint_as_float(r[4 * c + 1]) * f, __uint_as_float(r[4 * c + 2]) * f,
                                                   __uint_as_float(r[4 * c + 3]) * f);
             }
-            ml[tid] = make_float2(Q8 ? m : m - kTcShift, l);
+            ml[group * kRows + row] = make_float2(Q8 ? m : m - kTcShift, l);
         }
+        if (kGroups == 2) named_bar_sync(1, 128 * kGroups);  // the first group joins both
     }
-    // (the queries' tiles are done with: every score has been used)
-    join_and_write(p, w, reinterpret_cast<float4 *>(smem_gen + (sKV - smem_base)), ml, joined, rows_at, reinterpret_cast<float4 *>(smem_gen), 1, kRows, all_ok, tid);
+    float4 * const part = reinterpret_cast<float4 *>(smem_gen);
+    join_and_write(p, w, part, ml, joined, rows_at, part + kRows * kPartPitch, kGroups, kRows, all_ok, tid);
     // common exit: every role has left its loop; release TMEM
     tc_fence_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == kScoreWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -1226,28 +1238,45 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     const size_t            own = aligned(decode_shared_workspace_bytes(a->own.n_streams, a->own.n_heads, HK, a->own.kv_bound));
     const bool              shares = pl != nullptr && a->prefix_bound > 0;
     float2 * const          ml  = shares ? reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + own) : nullptr;
-    rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml, shares}, workspace, own, st);
+    const vox_kv_cache *    pc  = a->prefix;
+    const bool              q8  = a->own.cache->cfg.type == VOX_TYPE_Q8_0, tc = shares && pl->full;
+    const int               sms = std::min(kDecodeMaxSms, e->sm_count), k = !shares || tc ? 0 : small_arrangement(pl, sms, HK, a->prefix_bound);
+    const int               cluster = shares ? cluster_size(sms, pl->n_tiles[k], HK, a->prefix_bound, tc) : 1;
+    // Two softmax groups, beside one decode CTA per SM, where the streams' own 64-row tiles per SM are at most four times the
+    // tiles that a CTA of the prefix kernel walks (the two kernels then end together): under prompts of 4096 rows 256
+    // streams with a row of their own take 21 us against 34 us, with up to 2048 rows 57 us against 49 us.
+    const long long own_tiles = (long long) a->own.n_streams * HK * ((a->own.kv_bound + kKvTile - 1) / kKvTile) / sms;
+    const bool      wide = tc && own_tiles <= 4LL * ((a->prefix_bound + kSub - 1) / kSub) / cluster;
+    rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml, !shares ? 0 : wide ? 1 : 2}, workspace, own, st);
     if (rc != VOX_ATTN_OK || !shares) return rc;
-    const vox_kv_cache * pc = a->prefix;
-    const bool           q8 = pc->cfg.type == VOX_TYPE_Q8_0, tc = pl->full;
     SharedParams         p;
     p.q = reinterpret_cast<const uint8_t *>(a->own.q);
     p.q_nb_head = a->own.q_nb_head; p.q_nb_stream = a->own.q_nb_stream;
     p.rope    = reinterpret_cast<const float2 *>(a->own.rope_table);
-    const int sms = std::min(kDecodeMaxSms, e->sm_count), k = tc ? 0 : small_arrangement(pl, sms, HK, a->prefix_bound);
     p.tiles   = reinterpret_cast<const int2 *>(pl->dev + pl->at[k]);
     p.members = pl->dev + pl->members_at(k);
     p.len     = a->prefix_len;
     p.per_tile = pl->per_tile(k); p.n_kv_heads = HK; p.n_heads = a->own.n_heads; p.gqa = pl->gqa; p.layer = a->own.layer; p.max_len = pc->cfg.max_len;
-    p.cluster    = cluster_size(sms, pl->n_tiles[k], HK, a->prefix_bound, tc);
+    p.cluster    = cluster;
     p.scale_log2 = a->own.scale * 1.4426950408889634f;
     p.q8_tiles   = pc->k_data + (size_t) a->own.layer * pc->nb_layer;
     p.q8_nb_head = pc->nb_head; p.q8_nb_stream = pc->nb_stream;
     p.dst = a->own.dst; p.ml = ml; p.lse = a->lse;
     p.status = e->status_dev;
-    const auto     kernel = tc ? (q8 ? shared_rows_tc_kernel<true> : shared_rows_tc_kernel<false>) : q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
-    const int      smem   = tc ? (q8 ? Tc<true>::kSmem : Tc<false>::kSmem) : q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes;
-    const uint32_t bit    = 1u << (tc ? (q8 ? 28 : 21) : q8 ? 19 : 18);
+    auto     kernel  = q8 ? shared_rows_kernel<true> : shared_rows_kernel<false>;
+    int      smem    = q8 ? Ring<true>::kSmemBytes : Ring<false>::kSmemBytes, threads = kThreads;
+    uint32_t bit     = 1u << (q8 ? 19 : 18);
+    if (wide) {
+        kernel  = q8 ? shared_rows_tc_kernel<true, 2> : shared_rows_tc_kernel<false, 2>;
+        smem    = q8 ? Tc<true, 2>::kSmem : Tc<false, 2>::kSmem;
+        threads = Tc<false, 2>::kThreads;
+        bit     = 1u << (q8 ? 30 : 29);
+    } else if (tc) {
+        kernel  = q8 ? shared_rows_tc_kernel<true, 1> : shared_rows_tc_kernel<false, 1>;
+        smem    = q8 ? Tc<true, 1>::kSmem : Tc<false, 1>::kSmem;
+        threads = Tc<false, 1>::kThreads;
+        bit     = 1u << (q8 ? 28 : 21);
+    }
     if (!(e->attr_mask & bit)) {
         VOX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         // all of the SM's memory as shared memory, so that a CTA fits beside one of the decode kernel's
@@ -1255,7 +1284,7 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
         e->attr_mask |= bit;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) (pl->max_tiles[k] * HK * p.cluster)); cfg.blockDim = dim3(tc ? kTcThreads : kThreads);
+    cfg.gridDim = dim3((unsigned) (pl->max_tiles[k] * HK * p.cluster)); cfg.blockDim = dim3((unsigned) threads);
     cfg.dynamicSmemBytes = (size_t) smem; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -9,7 +9,7 @@ namespace vox {
 struct OwnRows {
     float *  lse;
     float2 * ml;
-    bool     beside;  // the prefix kernel runs beside it: at most two CTAs per SM
+    int      wave;    // CTAs per SM at most, where the prefix kernel is to run beside it (0: all that fit)
 };
 int    check_decode(const vox_engine * e, const vox_decode_args * a, const char * who);
 int    launch_decode_shared(vox_engine * e, const vox_decode_args * a, const OwnRows & rows, void * workspace, size_t workspace_bytes,
