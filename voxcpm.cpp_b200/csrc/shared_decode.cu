@@ -636,11 +636,12 @@ constexpr int kQTile     = kRows * 128;
 constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V, in f16
 template <bool Q8, int kGroups> struct Tc {
     static constexpr int kThreads = (4 * kGroups + 2) * 32;
-    static constexpr int kStages  = 2 + kGroups;
+    // A stage is held from the copy until P.V has retired, about 3500 clocks; beside two decode CTAs there is room for three.
+    static constexpr int kStages  = kGroups == 1 ? 3 : Q8 ? 5 : 6;
     static constexpr int kSCols  = Q8 ? 2 * kSub : kSub;   // TMEM columns of a score tile
     static constexpr int kSBufs  = Q8 ? 2 : 4;             // the accumulators, 4 x 64 columns, lie behind the buffers
     static constexpr int kOCol   = kSBufs * kSCols;
-    static constexpr int kRaw    = Q8 ? kStages : 0;       // q8_0: stages of tiles as the cache holds them
+    static constexpr int kRaw    = Q8 ? 2 + kGroups : 0;   // q8_0: stages of tiles as the cache holds them
     static constexpr int kRawBytes = 8704;
     static constexpr int kSmem   = 2 * kQTile + kStages * kTcStage + kRaw * kRawBytes + 1024;
     // the partial results, and behind those of one group its CTA's share of the rows, take the queries' and the ring's memory
@@ -699,7 +700,9 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t sQ = smem_base, sKV = sQ + 2 * kQTile, sRaw = sKV + kTcStages * kTcStage;
     const int      tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // full: a stage holds its tile in f16; empty: its products have retired; rfull, rempty: a tile's bytes have landed, are expanded
+    // full: a stage holds its tile in f16; S: scores ready; P: weights ready; F: P.V retired (the score buffer is free, f16: the
+    // stage too); q8_0: empty: the stage is free (F of a score buffer may complete twice between two looks at it, that of a stage
+    // cannot); rfull, rempty: a tile's bytes have landed, are expanded
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = full0 + 8 * kTcStages, bS0 = empty0 + 8 * kTcStages, bP0 = bS0 + 8 * kSBufs,
                    bF0 = bP0 + 8 * kSBufs, bO = bF0 + 8 * kSBufs, rfull0 = bO + 8, rempty0 = rfull0 + 8 * kRaw;
     const Item     w = load_item(p);
@@ -746,6 +749,10 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     };
     auto aborted   = [&]() { return *reinterpret_cast<volatile int *>(&abort_flag) != 0; };
     auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0; };
+    auto warp_wait2 = [&](uint32_t a, uint32_t pa, uint32_t b, bool two, uint32_t pb) {
+        return __all_sync(0xffffffffu, mbar_wait_bounded(a, pa) && (!two || mbar_wait_bounded(b, pb))) != 0;
+    };
+    auto retired = [&](int U) { return mbar_wait_bounded(bF0 + 8 * (U % kSBufs), (U / kSBufs) & 1); };  // tile U's P.V
     constexpr int kAhead = Q8 ? kRaw : kTcStages;  // tiles on their way
     auto load_tile = [&](int U) {  // one lane
         if constexpr (Q8) {
@@ -820,7 +827,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         bool               ok = true;
         for (int U = 0; U < n_sub && ok; ++U) {
             const int st = U % kTcStages, sb = U % kSBufs;
-            if (!warp_wait(full0 + 8 * st, (U / kTcStages) & 1) || (U >= kSBufs && !warp_wait(bF0 + 8 * sb, ((U / kSBufs) - 1) & 1))) { ok = false; break; }
+            if (!warp_wait2(full0 + 8 * st, (U / kTcStages) & 1, bF0 + 8 * sb, U >= kSBufs, ((U / kSBufs) - 1) & 1)) { ok = false; break; }
             tc_fence_after();
             if (leader) {
                 const uint32_t dS = tmem + kSCols * sb;
@@ -843,7 +850,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         int                loaded = min(n_sub, kAhead);
         for (int U = 0; U < n_sub && ok; ++U) {
             const int st = U % kTcStages, sb = U % kSBufs;
-            if (!warp_wait(full0 + 8 * st, (U / kTcStages) & 1) || !warp_wait(bP0 + 8 * sb, (U / kSBufs) & 1)) { ok = false; break; }
+            if (!warp_wait2(full0 + 8 * st, (U / kTcStages) & 1, bP0 + 8 * sb, true, (U / kSBufs) & 1)) { ok = false; break; }
             tc_fence_after();
             if (leader) {
                 const uint64_t v0 = dV + (uint64_t) (st * (kTcStage >> 4));
@@ -858,14 +865,14 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO + kHeadDim, tP + kSub / 2 + 8 * k, vb + k * (2048 >> 4), idesc, U > 1 || k > 0);
                 }
                 tc_commit(bF0 + 8 * sb);
-                tc_commit(empty0 + 8 * st);
+                if (Q8) tc_commit(empty0 + 8 * st);
                 if (U == n_sub - 1) tc_commit(bO);
             }
             __syncwarp();
             // f16: the stage of the tile before this one is free as soon as its P.V has retired, which was issued a tile ago;
             // q8_0: the bytes of this tile were expanded before its scores were made
             if ((Q8 || U > 0) && loaded < n_sub) {
-                const bool free = Q8 ? warp_wait(rempty0 + 8 * (U % kRaw), (U / kRaw) & 1) : warp_wait(empty0 + 8 * ((U - 1) % kTcStages), ((U - 1) / kTcStages) & 1);
+                const bool free = Q8 ? warp_wait(rempty0 + 8 * (U % kRaw), (U / kRaw) & 1) : __all_sync(0xffffffffu, retired(U - 1)) != 0;
                 if (!free || __any_sync(0xffffffffu, aborted())) { ok = false; break; }
                 if (lane == 0) load_tile(loaded);
                 ++loaded;
@@ -975,7 +982,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     if (raise) m = top;
                     l *= f;
                     // the accumulators are at rest once P.V of the group's tile before has retired
-                    if (!mbar_wait_bounded(bF0 + 8 * ((U - kGroups) % kSBufs), ((U - kGroups) / kSBufs) & 1)) {
+                    if (!retired(U - kGroups)) {
                         ok = false;
                         if (!Q8) break;
                     }
