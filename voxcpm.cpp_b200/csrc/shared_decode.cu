@@ -621,7 +621,8 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // values and remainders of even and of odd tiles, added up in f32 at the end: the tensor core truncates every sum it
 // makes, and one accumulator for all came out 2.2e-6 too small after 1024 keys.  The reference of a row is raised only
 // when a maximum exceeds it by 2^8 (its accumulators are then rescaled in TMEM).
-//   warps 0 .. 4 kGroups - 1  softmax      then one warp  issues S = Q.K      and one  issues O += P.V and the copies of K and V
+//   warps 0 .. 4 kGroups - 1  softmax      then one warp  issues S = Q.K, one  O += P.V, and that one, or a third of two
+//   groups, the copies of K and V
 // One softmax group (192 threads of 128 registers, 81 KB of shared memory; q8_0 107 KB): the CTA runs beside two CTAs of the decode
 // kernel, whose time is HBM's, and takes about 1.1 us for 64 keys (q8_0 2.3 us), most of it latency that nothing hides.
 // Two groups, which take tiles in turn with a reference and accumulators of their own, need less than two thirds of that,
@@ -635,7 +636,7 @@ constexpr int kSub       = 64;                    // keys of a score tile and of
 constexpr int kQTile     = kRows * 128;
 constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V, in f16
 template <bool Q8, int kGroups> struct Tc {
-    static constexpr int kThreads = (4 * kGroups + 2) * 32;
+    static constexpr int kThreads = (4 * kGroups + 1 + kGroups) * 32;
     // A stage is held from the copy until P.V has retired, about 3500 clocks; beside two decode CTAs there is room for three.
     static constexpr int kStages  = kGroups == 1 ? 3 : Q8 ? 5 : 6;
     static constexpr int kSCols  = Q8 ? 2 * kSub : kSub;   // TMEM columns of a score tile
@@ -685,7 +686,7 @@ __global__ void __maxnreg__(128)
 shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedParams p) {
     using Z = Tc<Q8, kGroups>;
     constexpr int kTcStages = Z::kStages, kSBufs = Z::kSBufs, kSCols = Z::kSCols, kTcOCol = Z::kOCol, kRaw = Q8 ? Z::kRaw : 1;
-    constexpr int kSoftmax = 4 * kGroups, kScoreWarp = kSoftmax, kOutWarp = kSoftmax + 1;
+    constexpr int kSoftmax = 4 * kGroups, kScoreWarp = kSoftmax, kOutWarp = kSoftmax + 1, kCopyWarp = kSoftmax + kGroups;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1 + 2 * kRaw];
     __shared__ float4   scales[Q8 ? kTcStages : 1][kSub];   // q8_0: of a row's K and V blocks
@@ -701,7 +702,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const uint32_t sQ = smem_base, sKV = sQ + 2 * kQTile, sRaw = sKV + kTcStages * kTcStage;
     const int      tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // full: a stage holds its tile in f16; S: scores ready; P: weights ready; F: P.V retired (the score buffer is free, f16: the
-    // stage too); q8_0: empty: the stage is free (F of a score buffer may complete twice between two looks at it, that of a stage
+    // stage too); empty (q8_0, and two groups): the stage is free (F of a score buffer may complete twice between two looks at it, that of a stage
     // cannot); rfull, rempty: a tile's bytes have landed, are expanded
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = full0 + 8 * kTcStages, bS0 = empty0 + 8 * kTcStages, bP0 = bS0 + 8 * kSBufs,
                    bF0 = bP0 + 8 * kSBufs, bO = bF0 + 8 * kSBufs, rfull0 = bO + 8, rempty0 = rfull0 + 8 * kRaw;
@@ -769,7 +770,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         tma_load_5d(dst, &map_k, bar, 0, w.key0 + U * kSub, w.kvh, w.prefix, p.layer);
         tma_load_5d(dst + kSub * 128, &map_v, bar, 0, w.key0 + U * kSub, w.kvh, w.prefix, p.layer);
     };
-    if (warp == kOutWarp) {
+    if (warp == kCopyWarp) {
         if (lane == 0)
             for (int U = 0; U < min(n_sub, kAhead); ++U) load_tile(U);
     } else if (warp < kSoftmax) {
@@ -865,13 +866,13 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     for (int k = 0; k < 4; ++k) tc_mma_f16_ts(tO + kHeadDim, tP + kSub / 2 + 8 * k, vb + k * (2048 >> 4), idesc, U > 1 || k > 0);
                 }
                 tc_commit(bF0 + 8 * sb);
-                if (Q8) tc_commit(empty0 + 8 * st);
+                if (Q8 || kGroups == 2) tc_commit(empty0 + 8 * st);
                 if (U == n_sub - 1) tc_commit(bO);
             }
             __syncwarp();
             // f16: the stage of the tile before this one is free as soon as its P.V has retired, which was issued a tile ago;
             // q8_0: the bytes of this tile were expanded before its scores were made
-            if ((Q8 || U > 0) && loaded < n_sub) {
+            if (kGroups == 1 && (Q8 || U > 0) && loaded < n_sub) {
                 const bool free = Q8 ? warp_wait(rempty0 + 8 * (U % kRaw), (U / kRaw) & 1) : __all_sync(0xffffffffu, retired(U - 1)) != 0;
                 if (!free || __any_sync(0xffffffffu, aborted())) { ok = false; break; }
                 if (lane == 0) load_tile(loaded);
@@ -880,8 +881,23 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
         if (!ok) {
             if (lane == 0) give_up();
-            for (int i = max(0, loaded - kAhead); i < loaded; ++i)  // copies in flight land
+            for (int i = kGroups == 1 ? max(0, loaded - kAhead) : loaded; i < loaded; ++i)  // copies in flight land
                 warp_wait(Q8 ? rfull0 + 8 * (i % kRaw) : full0 + 8 * (i % kTcStages), (i / kAhead) & 1);
+        }
+    } else if (kGroups == 2 && warp == kCopyWarp) {
+        // ------------------------------------------------------------------ copies (issuing one costs the output warp 500 clocks)
+        if (lane == 0) {
+            bool ok = true;
+            int  U  = min(n_sub, kAhead);
+            for (; U < n_sub; ++U) {  // the stage's last tile has retired, q8_0: has been expanded
+                const uint32_t bar = Q8 ? rempty0 + 8 * (U % kRaw) : empty0 + 8 * (U % kTcStages);
+                if (!mbar_wait_bounded(bar, ((U / kAhead) - 1) & 1) || aborted()) { ok = false; break; }
+                load_tile(U);
+            }
+            if (!ok) give_up();
+            if (aborted())
+                for (int i = max(0, U - kAhead); i < U; ++i)  // copies in flight land
+                    mbar_wait_bounded(Q8 ? rfull0 + 8 * (i % kRaw) : full0 + 8 * (i % kTcStages), (i / kAhead) & 1);
         }
     } else {
         // ------------------------------------------------------------------ softmax: a thread per row
