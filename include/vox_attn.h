@@ -388,7 +388,8 @@ void vox_prefix_plan_destroy(vox_prefix_plan * p);
  *                which vox_kv_observe takes
  * prefix, plan and prefix_len all NULL: own rows only (vox_attn_decode with lse).  Results agree with vox_attn_decode over a
  * cache that holds both parts to rounding; q8_0 weights are not rounded to f16 here (error under 1e-5 of the output's RMS).
- * A stream whose rows are all masked (no prefix row, no own row) gives zeros.
+ * A stream without a prefix row and without an own row gives zeros.  Rows past a length may hold anything, NaN included.
+ * dst must not overlap q.  Two launches, the second on the SMs that the first leaves room on.
  * workspace: vox_attn_decode_shared_workspace_bytes, 16-byte aligned.  The engine's device must be the current one. */
 typedef struct {
     vox_decode_args         own;
@@ -420,7 +421,8 @@ int    vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, 
  *              (the same for both); row_pos may be NULL.  Rows at kv_len and beyond are left as they are.
  *   n_seen     device array [n_streams]: tokens every stream has seen, the new ones included (NULL: kv_len)
  *   kv_bound   host-known upper bound of every kv_len; a longer stream raises VOX_ATTN_DEVICE_STATE and is left alone
- * No atomics: the same call gives the same bits.  workspace: vox_kv_observe_workspace_bytes, 16-byte aligned. */
+ * The same call gives the same bits.  workspace: vox_kv_observe_workspace_bytes (0 for most calls with n_q == 1), 16-byte
+ * aligned. */
 typedef struct {
     const vox_kv_cache * cache;
     int32_t         layer;
@@ -454,9 +456,9 @@ int    vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * work
  * to index new_len; its rotary position is its count of tokens, which kv_len no longer is.
  *   kv_len     device array [n_streams]; kv_bound its host-known upper bound (a longer stream raises
  *              VOX_ATTN_DEVICE_STATE and is left alone, its new_len its kv_len)
- *   n_sink + n_recent <= budget;  budget >= 1
+ *   n_sink + n_recent <= budget;  budget >= 1;  kv_bound <= 49152 (VOX_ATTN_UNSUPPORTED beyond)
  *   score, row_pos  as vox_kv_observe leaves them, layers nb_layer bytes apart
- *   new_len    device out [n_streams]: min(kv_len, budget); not kv_len itself
+ *   new_len    device out [n_streams]: min(kv_len, budget); must not overlap kv_len or n_seen
  *   kept       optional out [budget, HK, n_streams, n_layers] int32 contiguous: for every row below new_len the index it had
  *              (rows beyond are left as they are)
  * Rows at new_len and beyond are left as they are. */

@@ -769,6 +769,7 @@ def test_refusals(engine, pkg):
     refused("INVALID_ARGUMENT", "heads per kv head", shared(plan=pkg.PrefixPlan(engine, [0, 0], 1, 8, 2)))
     refused("WORKSPACE_TOO_SMALL", "workspace", shared(workspace=torch.empty(16, dtype=torch.uint8, device="cuda")))
     refused("INVALID_ARGUMENT", "kv_bound", shared(kv_bound=5000))
+    refused("INVALID_ARGUMENT", "overlap", shared(dst=c.q))
     for of, G in (([0, 1], 1), ([-2, 0], 1)):
         refused("INVALID_ARGUMENT", "prefix_of", lambda: pkg.PrefixPlan(engine, of, G))
     refused("INVALID_ARGUMENT", "must be in", lambda: pkg.PrefixPlan(engine, [], 1))
@@ -808,7 +809,9 @@ def test_refusals(engine, pkg):
     refused("INVALID_ARGUMENT", "budget", evict(n_sink=2**31 - 1, n_recent=2**31 - 1))
     refused("INVALID_ARGUMENT", "layers", evict(layer0=1))
     refused("INVALID_ARGUMENT", "kv_bound", evict(kv_bound=33))
-    refused("INVALID_ARGUMENT", "kv_len itself", evict(new_len=v.kv_len))
+    refused("INVALID_ARGUMENT", "overlap", evict(new_len=v.kv_len))
+    refused("INVALID_ARGUMENT", "overlap", evict(new_len=v.n_seen))
+    refused("INVALID_ARGUMENT", "overlap", evict(new_len=v.kv_len[1:]))
     other_engine.close()
     out, lse = c.run()
     engine.sync_status()

@@ -387,7 +387,9 @@ int check_evict(const vox_engine * e, const vox_kv_evict_args * a) {
                 a->kv_bound, c->cfg.max_len);
     VOX_REQUIRE(a->budget >= 1 && a->n_sink >= 0 && a->n_recent >= 0 && a->n_sink <= a->budget - a->n_recent, VOX_ATTN_INVALID_ARGUMENT,
                 "budget %d must be positive and hold n_sink %d + n_recent %d", a->budget, a->n_sink, a->n_recent);
-    VOX_REQUIRE(a->new_len != a->kv_len, VOX_ATTN_INVALID_ARGUMENT, "new_len must not be kv_len itself");
+    for (const int32_t * in : {a->kv_len, a->n_seen})  // read by every CTA of the launch, while one of them writes new_len
+        VOX_REQUIRE(in == nullptr || a->new_len + a->n_streams <= in || in + a->n_streams <= a->new_len, VOX_ATTN_INVALID_ARGUMENT,
+                    "new_len must not overlap kv_len or n_seen");
     VOX_REQUIRE(a->kv_bound <= kMaxRows, VOX_ATTN_UNSUPPORTED, "kv_bound %d: at most %d rows a stream", a->kv_bound, kMaxRows);
     VOX_REQUIRE(((reinterpret_cast<uintptr_t>(a->score) | reinterpret_cast<uintptr_t>(a->row_pos) | reinterpret_cast<uintptr_t>(a->new_len) |
                   reinterpret_cast<uintptr_t>(a->kept)) & 3) == 0 && a->nb_head % 4 == 0 && a->nb_stream % 4 == 0 && a->nb_layer % 4 == 0,

@@ -1163,6 +1163,13 @@ int check_shared(const vox_engine * e, const vox_decode_shared_args * a) {
     VOX_REQUIRE(a->own.stream_order == nullptr, VOX_ATTN_UNSUPPORTED, "vox_attn_decode_shared takes no stream_order");
     VOX_REQUIRE((reinterpret_cast<uintptr_t>(a->lse) & 3) == 0, VOX_ATTN_INVALID_ARGUMENT, "lse must be 4-byte aligned");
     if (a->prefix == nullptr && a->plan == nullptr) return VOX_ATTN_OK;  // own rows only
+    {
+        // the prefix kernel reads the queries while the decode kernel writes its results: they must not share memory
+        const uintptr_t q0 = reinterpret_cast<uintptr_t>(a->own.q), d0 = reinterpret_cast<uintptr_t>(a->own.dst);
+        const size_t    q_bytes = (size_t) (a->own.n_streams - 1) * a->own.q_nb_stream + (size_t) (a->own.n_heads - 1) * a->own.q_nb_head + kHeadDim * sizeof(float);
+        const size_t    d_bytes = (size_t) a->own.n_streams * a->own.n_heads * kHeadDim * sizeof(float);
+        VOX_REQUIRE(q0 + q_bytes <= d0 || d0 + d_bytes <= q0, VOX_ATTN_INVALID_ARGUMENT, "dst and q must not overlap");
+    }
     VOX_REQUIRE(a->prefix && a->plan && a->prefix_len, VOX_ATTN_INVALID_ARGUMENT, "prefix, plan and prefix_len must be given together");
     VOX_REQUIRE(a->prefix->e == e && a->plan->e == e, VOX_ATTN_INVALID_ARGUMENT, "the prefix cache or the plan belongs to another engine");
     const vox_kv_config & pc = a->prefix->cfg;
