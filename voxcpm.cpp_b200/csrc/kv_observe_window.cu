@@ -39,6 +39,7 @@ template <bool Q8> struct Shape {
 
 struct Part {
     int stream, kvh, len, tile0, tiles, first_slot, slots;  // tiles of this part; the slots of the pair's statistics
+    int parts;                                              // of the whole cut
 };
 
 // Part `b` of the cut, by one warp (each lane holds the tile counts of every 32nd stream); false past the last part.
@@ -60,10 +61,12 @@ __device__ bool find_part(const ObserveParams & p, int b, int n_ctas, Part & w) 
     most  = __reduce_max_sync(0xffffffffu, most);
     if (total == 0) return false;
     int r = live >= n_ctas ? most : (total + n_ctas - 1) / n_ctas;
+    w.parts = live;  // r == most
     for (; r < most; ++r) {
         int parts = 0;
         for (int i = 0; i < rounds; ++i) parts += 32 * i + lane < n ? (tiles_of(p, 32 * i + lane) + r - 1) / r : 0;
-        if (__reduce_add_sync(0xffffffffu, parts) * HK <= n_ctas) break;
+        parts = __reduce_add_sync(0xffffffffu, parts) * HK;
+        if (parts <= n_ctas) { w.parts = parts; break; }
     }
     int before = 0;  // parts of the streams before this round's
     for (int i = 0; i < rounds; ++i) {
@@ -133,8 +136,13 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_wait();
-    pdl_launch_dependents();
+    // The second launch reads one thing that the first has written, the statistics: it waits for it when its queries are ready.
+    // (All else it reads was there before the first launch began, and that one has begun.)
+    bool waits = kWeights;
+    if (!kWeights) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&tmem_slot);
     const int rows = p.n_q * p.gqa, n_m = (rows + 127) / 128, n_b = (rows + kSub - 1) / kSub;
     const int per_tile = kWeights ? n_b : 2 * n_m;  // score tiles per key tile
@@ -150,7 +158,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
     int issued = 0;    // copies of key tiles, by the warp that issues them
     int T = 0, U = 0;  // key tiles and score tiles so far, over all parts of this CTA: they fix the phase of every barrier
 
-    for (int b = blockIdx.x;; b += gridDim.x) {
+    for (int b = blockIdx.x, n_parts = 0x7fffffff; b < n_parts; b += gridDim.x) {
         if (warp == 0) {
             Part      w{};
             const bool have = find_part(p, b, gridDim.x, w);
@@ -159,6 +167,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
         __syncthreads();
         if (!have_part) break;
         const Part w = part;
+        n_parts = w.parts;
 
         auto copy_tile = [&](int t) {  // one lane
             const int n = T + t, key = (w.tile0 + t) * kKeys, boxes = w.len - key > kKvTile ? 2 : 1;
@@ -220,21 +229,40 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                     *reinterpret_cast<uint2 *>(dst + kQTile) = lo;
                 }
             }
-            if (kWeights) {
-                const float2 * all = p.stats + (size_t) w.first_slot * rows;
-                for (int r = tid; r < n_b * kSub; r += 256) {
-                    float M = -INFINITY, L = 0.0f;
-                    if (r < rows) {
-                        for (int s = 0; s < w.slots; ++s) M = fmaxf(M, __ldcg(all + (size_t) s * rows + r).x);
-                        for (int s = 0; s < w.slots; ++s) {
-                            const float2 x = __ldcg(all + (size_t) s * rows + r);
-                            L = fmaf(x.y, x.x == -INFINITY ? (x.y == 0.0f ? 0.0f : 1.0f) : exp2f(x.x - M), L);
-                        }
-                    }
-                    row_stat[r] = L == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(M, 1.0f / L);  // a row that sees nothing adds nothing
-                }
-            }
             fence_proxy_async_smem();
+        }
+        if (kWeights) {
+            if (waits) {
+                pdl_wait();
+                pdl_launch_dependents();
+                waits = false;
+            }
+            if (warp < 8) {  // the rows' statistics: two rows of a thread, eight parts of both in flight
+                constexpr int  kParts = 8;
+                const float2 * all = p.stats + (size_t) w.first_slot * rows;
+                float          M[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f};
+                for (int s0 = 0; s0 < w.slots; s0 += kParts) {
+                    float2 x[2][kParts];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int s = 0; s < kParts; ++s)
+                            x[h][s] = s0 + s < w.slots && tid + 256 * h < rows ? __ldcg(all + (size_t) (s0 + s) * rows + tid + 256 * h) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float most = M[h];
+#pragma unroll
+                        for (int s = 0; s < kParts; ++s) most = fmaxf(most, x[h][s].x);
+                        if (M[h] != -INFINITY) L[h] *= exp2f(M[h] - most);
+                        M[h] = most;
+#pragma unroll
+                        for (int s = 0; s < kParts; ++s) L[h] = fmaf(x[h][s].y, x[h][s].x == -INFINITY ? (x[h][s].y == 0.0f ? 0.0f : 1.0f) : exp2f(x[h][s].x - most), L[h]);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (tid + 256 * h < n_b * kSub) row_stat[tid + 256 * h] = L[h] == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(M[h], 1.0f / L[h]);  // a row that sees nothing adds nothing
+            }
         }
         __syncthreads();
 
@@ -466,6 +494,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
         U += w.tiles * per_tile;
         __syncthreads();  // the queries' tiles and the part's description are free
     }
+    if (kWeights && waits) pdl_wait();  // no launch of the next call ends before the first one of this call
     if (warp == 8 && lane == 0 && aborted()) {  // copies in flight land before the CTA retires
         constexpr int      n_stages = Q8 ? kRawStages : Z::kStages;
         const uint32_t     bar0 = Q8 ? rfull0 : full0;
