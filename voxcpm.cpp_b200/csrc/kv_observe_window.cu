@@ -29,9 +29,12 @@ constexpr int kQTile    = kMaxRows * 128;       // the queries' f16 values; thei
 constexpr int kKTile    = kKeys * 128;
 constexpr int kRawStage = 2 * (kKvTile * 64 + kKvTile * 4);  // q8_0: bytes and scales of 128 rows of K
 constexpr int kRawStages = 4;
+constexpr int kGroups   = 4;                    // groups of four warps that take score tiles
+constexpr int kTakers   = kGroups * 128;
+static_assert(kMaxRows == kTakers, "a thread joins the statistics of one row");
 template <bool Q8> struct Shape {
     static constexpr int kStages  = Q8 ? 2 : 4;    // f16 tiles of K
-    static constexpr int kThreads = (Q8 ? 12 : 10) * 32;
+    static constexpr int kThreads = kTakers + (Q8 ? 4 : 2) * 32;
     static constexpr int kCols    = Q8 ? 2 * kSub : kSub;  // TMEM columns of a score tile: q8_0 has an accumulator per block
     static constexpr int kBufs    = 512 / kCols;
     static constexpr int kSmem    = 2 * kQTile + kStages * kKTile + (Q8 ? kRawStages * kRawStage : 0) + 1024;
@@ -109,18 +112,19 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
     __shared__ Part     part;
     __shared__ __align__(16) float2 row_stat[kMaxRows];         // kWeights: (max, 1 / sum); otherwise what the second group found
     __shared__ float2   scales[Z::kStages][kKeys];  // q8_0: of the f16 tile of a stage
-    __shared__ float    half_sum[2][kKeys];         // kWeights: the second group's sums of a key tile
+    __shared__ float    group_sum[2][kGroups][kKeys];  // kWeights: the groups' sums of a key tile (two buffers in turn)
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *      smem_gen  = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t sQ = smem_base, sK = sQ + 2 * kQTile, sRaw = sK + Z::kStages * kKTile;
     const int      tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int  kCopyWarp = kTakers / 32, kIssueWarp = kCopyWarp + 1;  // behind them the converting warps
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = full0 + 8 * Z::kStages, rfull0 = empty0 + 8 * Z::kStages, rempty0 = rfull0 + 8 * kRawStages,
                    bS0 = rempty0 + 8 * kRawStages, bE0 = bS0 + 8 * Z::kBufs;
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < Z::kStages; ++s) {
             mbar_init(full0 + 8 * s, Q8 ? 2 : 1);  // the converting warps, or the copy
-            mbar_init(empty0 + 8 * s, Q8 ? 9 : 1); // the products have retired (and the eight warps that read the scales are done)
+            mbar_init(empty0 + 8 * s, Q8 ? 1 + kTakers / 32 : 1);  // the products have retired (and the warps that read the scales are done)
         }
         for (int s = 0; s < kRawStages; ++s) {
             mbar_init(rfull0 + 8 * s, 1);
@@ -132,7 +136,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
         }
         fence_mbar_init();
     }
-    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (warp == kIssueWarp) tmem_alloc(smem_u32(&tmem_slot), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -197,16 +201,16 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
             return true;
         };
         bool first_ok = true;
-        if (warp == 8 && lane == 0)  // the first two while the queries are made ready
+        if (warp == kCopyWarp && lane == 0)  // the first two while the queries are made ready
             for (int t = 0; t < min(w.tiles, 2) && first_ok; ++t) first_ok = copy_tile(t);
 
-        // ---- the queries of the pair, by all but the copying and issuing warps; in the second launch their statistics too
-        if (warp < 8) {
+        // ---- the queries of the pair, by the warps that will take score tiles; in the second launch their statistics too
+        if (warp < kCopyWarp) {
             const int       c = lane & 15, n_rows = n_m * 128;
             const uint8_t * q_base = p.q + (size_t) w.stream * p.q_nb_stream + (size_t) (w.kvh * p.gqa) * p.q_nb_head + 16 * c;
             constexpr int kLoads = 8;  // rows of a lane in flight
 #pragma unroll 1
-            for (int r0 = 2 * warp * kLoads; r0 < n_rows; r0 += 16 * kLoads) {
+            for (int r0 = 2 * warp * kLoads; r0 < n_rows; r0 += kTakers / 16 * kLoads) {
                 float4 x[kLoads];
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
@@ -237,36 +241,29 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                 pdl_launch_dependents();
                 waits = false;
             }
-            if (warp < 8) {  // the rows' statistics: two rows of a thread, eight parts of both in flight
+            if (warp < kCopyWarp) {  // the rows' statistics: a row of a thread, eight parts in flight
                 constexpr int  kParts = 8;
-                const float2 * all = p.stats + (size_t) w.first_slot * rows;
-                float          M[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f};
-                for (int s0 = 0; s0 < w.slots; s0 += kParts) {
-                    float2 x[2][kParts];
+                const float2 * all = p.stats + (size_t) w.first_slot * rows + tid;
+                float          M = -INFINITY, L = 0.0f;
+                if (tid < rows)
+                    for (int s0 = 0; s0 < w.slots; s0 += kParts) {
+                        float2 x[kParts];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                        for (int s = 0; s < kParts; ++s) x[s] = s0 + s < w.slots ? __ldcg(all + (size_t) (s0 + s) * rows) : make_float2(-INFINITY, 0.0f);
+                        float most = M;
 #pragma unroll
-                        for (int s = 0; s < kParts; ++s)
-                            x[h][s] = s0 + s < w.slots && tid + 256 * h < rows ? __ldcg(all + (size_t) (s0 + s) * rows + tid + 256 * h) : make_float2(-INFINITY, 0.0f);
+                        for (int s = 0; s < kParts; ++s) most = fmaxf(most, x[s].x);
+                        if (M != -INFINITY) L *= exp2f(M - most);
+                        M = most;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float most = M[h];
-#pragma unroll
-                        for (int s = 0; s < kParts; ++s) most = fmaxf(most, x[h][s].x);
-                        if (M[h] != -INFINITY) L[h] *= exp2f(M[h] - most);
-                        M[h] = most;
-#pragma unroll
-                        for (int s = 0; s < kParts; ++s) L[h] = fmaf(x[h][s].y, x[h][s].x == -INFINITY ? (x[h][s].y == 0.0f ? 0.0f : 1.0f) : exp2f(x[h][s].x - most), L[h]);
+                        for (int s = 0; s < kParts; ++s) L = fmaf(x[s].y, x[s].x == -INFINITY ? (x[s].y == 0.0f ? 0.0f : 1.0f) : exp2f(x[s].x - most), L);
                     }
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (tid + 256 * h < n_b * kSub) row_stat[tid + 256 * h] = L[h] == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(M[h], 1.0f / L[h]);  // a row that sees nothing adds nothing
+                row_stat[tid] = L == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(M, 1.0f / L);  // a row that sees nothing adds nothing
             }
         }
         __syncthreads();
 
-        if (warp == 8) {
+        if (warp == kCopyWarp) {
             // ------------------------------------------------------------------ copies
             if (lane == 0) {
                 bool ok = first_ok;
@@ -275,7 +272,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                 else    give_up();
             }
             __syncwarp();
-        } else if (warp == 9) {
+        } else if (warp == kIssueWarp) {
             // ------------------------------------------------------------------ products (all lanes in the loop, one issues)
             constexpr uint32_t idesc = idesc_f16(kSub, false);
             const uint64_t     dQ = smem_desc_sw128(sQ), dK = smem_desc_sw128(sK);
@@ -311,30 +308,36 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                 }
             }
             if (!ok && lane == 0) give_up();
-        } else if (warp < 8) {
-            // ------------------------------------------------------------------ scores out: warps 0-3 the even tiles, 4-7 the odd ones
+        } else if (warp < kCopyWarp) {
+            // ------------------------------------------------------------------ scores out, by groups of four warps.  First launch:
+            // group g has half g % 2 of a tile's keys and every other 128 query rows from g / 2 on; second: 64 query rows of every four
             const int      group = warp >> 2, row = tid & 127, first_cut = w.len - p.n_q;  // first key that not every query sees
             const uint32_t t_row = tmem + ((uint32_t) (32 * (warp & 3)) << 16);
+            constexpr int  kMine = kMaxRows / 256;
             bool           ok = true;
             int            u = U;
-            float          m[kMaxRows / 128], l[kMaxRows / 128];
+            float          m[kMine], l[kMine];
             if (!kWeights) {
 #pragma unroll
-                for (int i = 0; i < kMaxRows / 128; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
+                for (int i = 0; i < kMine; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
             }
             for (int t = 0; t < w.tiles && ok; ++t) {
-                const int n = T + t, st = n % Z::kStages, key0 = (w.tile0 + t) * kKeys;
-                float     sum = 0.0f, d0 = 1.0f, d1 = 1.0f;
+                const int n = T + t, st = n % Z::kStages, key0 = (w.tile0 + t) * kKeys, key = key0 + row;
+                float     sum = 0.0f, d0 = 1.0f, d1 = 1.0f, old = 0.0f;
+                float *   score = nullptr;
                 if (Q8) {  // the scales are the converting warps'
                     // (a warp whose wait ran out stays until the barrier at the end of the tile, which the others wait at)
                     if (!mbar_wait_bounded(full0 + 8 * st, (n / Z::kStages) & 1)) ok = false;
                     if (kWeights) { d0 = scales[st][row].x; d1 = scales[st][row].y; }
                 }
-                auto take = [&](int uu, uint32_t (&r)[kSub]) {  // a score tile out of TMEM, and its buffer back
-                    const int sb = uu % Z::kBufs;
-                    if (!mbar_wait_bounded(bS0 + 8 * sb, (uu / Z::kBufs) & 1)) return false;
+                const bool mine = kWeights && group == (t & (kGroups - 1)) && key < w.len, fresh = key >= w.len - p.n_new;  // who writes this tile's scores
+                if (mine) {
+                    score = reinterpret_cast<float *>(p.score + (size_t) w.stream * p.nb_stream + (size_t) w.kvh * p.nb_head) + key;
+                    if (!fresh) old = *score;
+                }
+                auto take = [&](int uu) {  // a score tile is there
+                    if (!mbar_wait_bounded(bS0 + 8 * (uu % Z::kBufs), (uu / Z::kBufs) & 1)) return false;
                     tc_fence_after();
-                    tmem_ld64_sync(t_row + Z::kCols * sb, r);
                     return true;
                 };
                 auto give_back = [&](int uu) {
@@ -343,87 +346,90 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                     if (lane == 0) mbar_arrive(bE0 + 8 * (uu % Z::kBufs));
                 };
                 if constexpr (!kWeights) {
+                    constexpr int kCols = Q8 ? 32 : kSub;  // scores at a time
 #pragma unroll
-                    for (int i = 0; i < kMaxRows / 128; ++i) {
-                        if (i >= n_m || !ok) break;
-                        const int uu = u + 2 * i + group, k0 = key0 + kSub * group;
-                        uint32_t  r[kSub];
-                        if (!take(uu, r)) { ok = false; break; }
-                        if constexpr (Q8) {
-                            const float2 * ds = scales[st] + kSub * group;
+                    for (int i = 0; i < kMine; ++i) {
+                        const int mt = 2 * i + (group >> 1), uu = u + 2 * mt + (group & 1), k0 = key0 + kSub * (group & 1);
+                        if (mt >= n_m || !ok) break;
+                        if (!take(uu)) { ok = false; break; }
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
+                        for (int h = 0; h < kSub; h += kCols) {
+                            uint32_t r[kCols];
+                            if constexpr (Q8) {
                                 uint32_t x[32];
-                                tmem_ld32_sync(t_row + Z::kCols * (uu % Z::kBufs) + kSub + 32 * h, x);
+                                tmem_ld32_sync(t_row + Z::kCols * (uu % Z::kBufs) + h, r);
+                                tmem_ld32_sync(t_row + Z::kCols * (uu % Z::kBufs) + kSub + h, x);
+                                const float2 * ds = scales[st] + kSub * (group & 1) + h;
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) {
-                                    const float2 d = ds[32 * h + e];
-                                    r[32 * h + e] = __float_as_uint(fmaf(__uint_as_float(x[e]), d.y, __uint_as_float(r[32 * h + e]) * d.x));
+                                    const float2 d = ds[e];
+                                    r[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), d.y, __uint_as_float(r[e]) * d.x));
                                 }
+                            } else {
+                                tmem_ld64_sync(t_row + Z::kCols * (uu % Z::kBufs), r);
                             }
-                        }
-                        give_back(uu);
-                        if (k0 + kSub > first_cut) {  // keys that this row's query does not see, and keys past the end
-                            const int last = first_cut + (int) ((uint32_t) (128 * i + row) * p.gqa_magic >> 16) - k0;
+                            if (h + kCols == kSub) give_back(uu);
+                            if (k0 + kSub > first_cut) {  // keys that this row's query does not see, and keys past the end
+                                const int last = first_cut + (int) ((uint32_t) (128 * mt + row) * p.gqa_magic >> 16) - k0 - h;
 #pragma unroll
-                            for (int e = 0; e < kSub; ++e)
-                                if (e > last) r[e] = 0xff800000u;
-                        }
-                        float t0 = m[i], t1 = -INFINITY;
+                                for (int e = 0; e < kCols; ++e)
+                                    if (e > last) r[e] = 0xff800000u;
+                            }
+                            float t0 = m[i], t1 = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < kSub; e += 4) {
-                            t0 = max3(t0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
-                            t1 = max3(t1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
-                        }
-                        const float mn = fmaxf(t0, t1), ref = mn == -INFINITY ? 0.0f : mn;
-                        float s0 = m[i] == -INFINITY ? l[i] : l[i] * ex2_approx(m[i] - ref), s1 = 0.0f;
+                            for (int e = 0; e < kCols; e += 4) {
+                                t0 = max3(t0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+                                t1 = max3(t1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+                            }
+                            const float mn = fmaxf(t0, t1), ref = mn == -INFINITY ? 0.0f : mn;
+                            float s0 = m[i] == -INFINITY ? l[i] : l[i] * ex2_approx(m[i] - ref), s1 = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < kSub; e += 2) {
-                            s0 += ex2_approx(__uint_as_float(r[e]) - ref);
-                            s1 += ex2_approx(__uint_as_float(r[e + 1]) - ref);
+                            for (int e = 0; e < kCols; e += 2) {
+                                s0 += ex2_approx(__uint_as_float(r[e]) - ref);
+                                s1 += ex2_approx(__uint_as_float(r[e + 1]) - ref);
+                            }
+                            m[i] = mn;
+                            l[i] = s0 + s1;
                         }
-                        m[i] = mn;
-                        l[i] = s0 + s1;
                     }
                 } else {
-                    const int key = key0 + row, hidden = (key - first_cut) * p.gqa;  // rows before this one do not see the key
+                    const int hidden = (key - first_cut) * p.gqa;  // rows before this one do not see the key
                     float     s1 = 0.0f;
-                    for (int i = group; i < n_b && ok; i += 2) {
-                        uint32_t r[kSub];
-                        if (!take(u + i, r)) { ok = false; break; }
-                        if constexpr (Q8) {
+                    for (int i = group; i < n_b && ok; i += kGroups) {
+                        if (!take(u + i)) { ok = false; break; }
+                        const bool cut = key0 + kKeys > first_cut;
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
+                        for (int h = 0; h < kSub; h += 32) {
+                            uint32_t r[32];
+                            tmem_ld32_sync(t_row + Z::kCols * ((u + i) % Z::kBufs) + h, r);
+                            if constexpr (Q8) {
                                 uint32_t x[32];
-                                tmem_ld32_sync(t_row + Z::kCols * ((u + i) % Z::kBufs) + kSub + 32 * h, x);
+                                tmem_ld32_sync(t_row + Z::kCols * ((u + i) % Z::kBufs) + kSub + h, x);
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) r[32 * h + e] = __float_as_uint(fmaf(__uint_as_float(x[e]), d1, __uint_as_float(r[32 * h + e]) * d0));
+                                for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), d1, __uint_as_float(r[e]) * d0));
                             }
-                        }
-                        give_back(u + i);
-                        const float4 * st4 = reinterpret_cast<const float4 *>(row_stat + kSub * i);
-                        const bool     cut = key0 + kKeys > first_cut;
+                            if (h + 32 == kSub) give_back(u + i);
+                            const float4 * st4 = reinterpret_cast<const float4 *>(row_stat + kSub * i + h);
 #pragma unroll
-                        for (int e = 0; e < kSub; e += 2) {
-                            const float4 q = st4[e >> 1];  // two rows' (max, 1 / sum), the same for all threads
-                            float        a = ex2_approx(__uint_as_float(r[e]) - q.x), c = ex2_approx(__uint_as_float(r[e + 1]) - q.z);
-                            if (cut) {
-                                if (kSub * i + e < hidden) a = 0.0f;
-                                if (kSub * i + e + 1 < hidden) c = 0.0f;
+                            for (int e = 0; e < 32; e += 2) {
+                                const float4 q = st4[e >> 1];  // two rows' (max, 1 / sum), the same for all threads
+                                float        a = ex2_approx(__uint_as_float(r[e]) - q.x), c = ex2_approx(__uint_as_float(r[e + 1]) - q.z);
+                                if (cut) {
+                                    if (kSub * i + h + e < hidden) a = 0.0f;
+                                    if (kSub * i + h + e + 1 < hidden) c = 0.0f;
+                                }
+                                sum = fmaf(a, q.y, sum);
+                                s1  = fmaf(c, q.w, s1);
                             }
-                            sum = fmaf(a, q.y, sum);
-                            s1  = fmaf(c, q.w, s1);
                         }
                     }
-                    sum += s1;
-                    // the second group's half goes through shared memory (two buffers in turn)
-                    if (group == 1) half_sum[t & 1][row] = sum;
-                    if (!named_bar_all(1, 256, ok)) { ok = false; break; }
-                    if (group == 0 && key < w.len) {
-                        sum += half_sum[t & 1][row];
-                        float *   score = reinterpret_cast<float *>(p.score + (size_t) w.stream * p.nb_stream + (size_t) w.kvh * p.nb_head) + key;
-                        const bool fresh = key >= w.len - p.n_new;
-                        *score = fresh ? sum : fmaf(p.decay, *score, sum);
+                    group_sum[t & 1][group][row] = sum + s1;
+                    if (!named_bar_all(1, kTakers, ok)) { ok = false; break; }
+                    if (mine) {
+                        sum = 0.0f;
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g) sum += group_sum[t & 1][g][row];
+                        *score = fresh ? sum : fmaf(p.decay, old, sum);
                         if (fresh && p.row_pos != nullptr)
                             *(reinterpret_cast<int32_t *>(p.row_pos + (size_t) w.stream * p.nb_stream + (size_t) w.kvh * p.nb_head) + key) =
                                 (p.n_seen ? p.n_seen[w.stream] : w.len) - w.len + key;
@@ -437,15 +443,15 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
             }
             if (!ok) give_up();
             if (!kWeights) {
-                // both groups have seen half of the keys of every row: the second one's statistics through shared memory
-                if (group == 1)
+                // a row's two halves of the keys meet through shared memory
+                if (group & 1)
 #pragma unroll
-                    for (int i = 0; i < kMaxRows / 128; ++i) row_stat[128 * i + row] = make_float2(m[i], l[i]);
-                ok = named_bar_all(1, 256, ok && !aborted());
-                if (ok && group == 0) {
+                    for (int i = 0; i < kMine; ++i) row_stat[256 * i + 128 * (group >> 1) + row] = make_float2(m[i], l[i]);
+                ok = named_bar_all(1, kTakers, ok && !aborted());
+                if (ok && !(group & 1)) {
 #pragma unroll
-                    for (int i = 0; i < kMaxRows / 128; ++i) {
-                        const int at = 128 * i + row;
+                    for (int i = 0; i < kMine; ++i) {
+                        const int at = 256 * i + 128 * (group >> 1) + row;
                         if (at >= rows) break;
                         const float2 o = row_stat[at];
                         const float  M = fmaxf(m[i], o.x), fa = m[i] == -INFINITY ? 1.0f : ex2_approx(m[i] - M), fb = o.x == -INFINITY ? 1.0f : ex2_approx(o.x - M);
@@ -462,7 +468,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                     (n >= Z::kStages && !mbar_wait_bounded(empty0 + 8 * st, ((n / Z::kStages) - 1) & 1))) { ok = false; break; }
                 const uint8_t * raw = smem_gen + (sRaw - smem_base) + rs * kRawStage;
 #pragma unroll 1
-                for (int row = tid - 10 * 32; row < kKeys; row += 64) {
+                for (int row = tid - (kIssueWarp + 1) * 32; row < kKeys; row += 64) {
                 uint8_t *  out = smem_gen + (sK - smem_base) + st * kKTile + row * 128;
                 const bool here = row < left;  // rows past the end: zeros, whatever the cache holds there
 #pragma unroll
@@ -495,14 +501,14 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
         __syncthreads();  // the queries' tiles and the part's description are free
     }
     if (kWeights && waits) pdl_wait();  // no launch of the next call ends before the first one of this call
-    if (warp == 8 && lane == 0 && aborted()) {  // copies in flight land before the CTA retires
+    if (warp == kCopyWarp && lane == 0 && aborted()) {  // copies in flight land before the CTA retires
         constexpr int      n_stages = Q8 ? kRawStages : Z::kStages;
         const uint32_t     bar0 = Q8 ? rfull0 : full0;
         for (int i = max(0, issued - n_stages); i < issued; ++i) mbar_wait_bounded(bar0 + 8 * (i % n_stages), (i / n_stages) & 1);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kIssueWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
