@@ -134,21 +134,26 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
         if (len > 0 && tid == 0 && kvh == 0 && chunk == 0) atomicOr(p.status, kStatusBadState);
         return;
     }
-    const int first = chunk * kChunk + warp * kWarpKeys;
-    if (kMode != kCluster && chunk * kChunk >= len) return;
+    // Given the log-sum-exp, a CTA takes p.run chunks one after the other; the next one's keys are asked for as soon as the products
+    // have taken this one's.
+    const int chunk0 = kMode == kGiven ? chunk * p.run : chunk, end = kMode == kGiven ? min(len, (chunk0 + p.run) * kChunk) : len;
+    int       first  = chunk0 * kChunk + warp * kWarpKeys;
+    if (kMode != kCluster && chunk0 * kChunk >= len) return;
     // everything the CTA reads is asked for before anything is waited for
     KeyTile<Q8>     keys[kWarpKeys / 8];
     const uint8_t * pair = p.k + (size_t) stream * p.k_nb_stream + (size_t) kvh * p.k_nb_head;
+    float * const   score = reinterpret_cast<float *>(p.score + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head);
+    float           old[2], next_old[2] = {0.0f, 0.0f};
+    auto ask = [&](int from) {
 #pragma unroll
-    for (int n = 0; n < kWarpKeys / 8; ++n) keys[n] = load_keys<Q8>(pair, first + 8 * n + g, t, first + 8 * n + g < len);
-    float * const score = reinterpret_cast<float *>(p.score + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head);
-    const int     mine = first + 8 * g + 2 * t;  // the two keys whose scores this lane writes
-    float         old[2] = {0.0f, 0.0f};
-    if (kMode != kFind) {
+        for (int n = 0; n < kWarpKeys / 8; ++n) keys[n] = load_keys<Q8>(pair, from + 8 * n + g, t, from + 8 * n + g < len);
+        if (kMode != kFind) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (mine + e < len - p.n_new) old[e] = score[mine + e];
-    }
+            for (int e = 0; e < 2; ++e)
+                if (from + 8 * g + 2 * t + e < len - p.n_new) next_old[e] = score[from + 8 * g + 2 * t + e];
+        }
+    };
+    ask(first);
     if (kMode == kGiven && tid < p.gqa) {
         // kept as the scores are, in units of log2, in two parts: one would lose 2^-24 of its size
         const float x = p.lse[(size_t) stream * p.n_heads + kvh * p.gqa + tid], hi = x * 1.4426950408889634f;
@@ -163,78 +168,87 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
     }
     uint32_t q[4][4];
     load_query(p, stream, kvh, lane, q);
-    float sc[kWarpKeys / 8][2];
+    if (kMode == kGiven) __syncthreads();
+    for (;; first += kChunk) {
+        const int mine = first + 8 * g + 2 * t;  // the two keys whose scores this lane writes
+        float sc[kWarpKeys / 8][2];
 #pragma unroll
-    for (int n = 0; n < kWarpKeys / 8; ++n) {
-        score_tile<Q8>(sc[n], q, keys[n], lane);
+        for (int n = 0; n < kWarpKeys / 8; ++n) {
+            score_tile<Q8>(sc[n], q, keys[n], lane);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (first + 8 * n + 2 * t + e >= len) sc[n][e] = -INFINITY;
-    }
-    if (kMode == kFind || kMode == kCluster) {
-        float m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int n = 0; n < kWarpKeys / 8; ++n) m = fmaxf(m, fmaxf(sc[n][0], sc[n][1]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int n = 0; n < kWarpKeys / 8; ++n) l += ex2_approx(sc[n][0] - ref) + ex2_approx(sc[n][1] - ref);
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) warp_stat[warp][g] = make_float2(m, l);
-        __syncthreads();
-        if (tid < p.gqa) {
-            float2 s = warp_stat[0][tid];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) s = join_stats(s, warp_stat[w][tid]);
-            if (kMode == kFind) p.stats[((size_t) blockIdx.y * p.n_chunks + chunk) * p.gqa + tid] = s;
-            else                cta_stat[tid] = s;
+            for (int e = 0; e < 2; ++e)
+                if (first + 8 * n + 2 * t + e >= len) sc[n][e] = -INFINITY;
         }
-        if (kMode == kFind) return;
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (tid < p.gqa) {
-            const uint32_t at = smem_u32(&cta_stat[tid]);
-            float2         all[kMaxCluster], s = make_float2(-INFINITY, 0.0f);
+        old[0] = next_old[0];
+        old[1] = next_old[1];
+        if (kMode == kGiven && first + kChunk < end) ask(first + kChunk);
+        if (kMode == kFind || kMode == kCluster) {
+            float m = -INFINITY, l = 0.0f;
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) {  // all on their way together
-                all[r] = s;
-                if (r < p.n_chunks) {
-                    uint32_t peer;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(r));
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(all[r].x), "=f"(all[r].y) : "r"(peer) : "memory");
-                }
+            for (int n = 0; n < kWarpKeys / 8; ++n) m = fmaxf(m, fmaxf(sc[n][0], sc[n][1]));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int n = 0; n < kWarpKeys / 8; ++n) l += ex2_approx(sc[n][0] - ref) + ex2_approx(sc[n][1] - ref);
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (t == 0) warp_stat[warp][g] = make_float2(m, l);
+            __syncthreads();
+            if (tid < p.gqa) {
+                float2 s = warp_stat[0][tid];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) s = join_stats(s, warp_stat[w][tid]);
+                if (kMode == kFind) p.stats[((size_t) blockIdx.y * p.n_chunks + chunk) * p.gqa + tid] = s;
+                else                cta_stat[tid] = s;
             }
+            if (kMode == kFind) return;
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            if (tid < p.gqa) {
+                const uint32_t at = smem_u32(&cta_stat[tid]);
+                float2         all[kMaxCluster], s = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) s = join_stats(s, all[r]);
-            row_stat[tid] = as_weights(s);
+                for (int r = 0; r < kMaxCluster; ++r) {  // all on their way together
+                    all[r] = s;
+                    if (r < p.n_chunks) {
+                        uint32_t peer;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(r));
+                        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(all[r].x), "=f"(all[r].y) : "r"(peer) : "memory");
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) s = join_stats(s, all[r]);
+                row_stat[tid] = as_weights(s);
+            }
+            __syncthreads();
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for at the end: nobody leaves while its memory is read
+        } else if (kMode == kJoin) {
+            __syncthreads();
         }
-        __syncthreads();
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for at the end: nobody leaves while its memory is read
-    } else {
-        __syncthreads();
-    }
-    const float2 st = g < p.gqa ? row_stat[g] : make_float2(0.0f, 0.0f);
-    float        w0 = 0.0f, w1 = 0.0f;
+        const float2 st = g < p.gqa ? row_stat[g] : make_float2(0.0f, 0.0f);
+        // the sums over the rows of the group, g: halving the keys as it halves the rows, so that lane (g, t) ends with keys 2t and
+        // 2t + 1 of tile g (14 shuffles; each sum by itself in every lane would be 48)
+        static_assert(kWarpKeys == 64, "a tile of keys to a row of lanes");
+        float w[16];
 #pragma unroll
-    for (int n = 0; n < kWarpKeys / 8; ++n)
+        for (int n = 0; n < 16; ++n) w[n] = ex2_approx(sc[n >> 1][n & 1] - st.x) * st.y;
+#pragma unroll
+        for (int half = 8; half >= 2; half >>= 1) {
+            const bool upper = g & (half >> 1);
+#pragma unroll
+            for (int n = 0; n < half; ++n) w[n] = (upper ? w[n + half] : w[n]) + __shfl_xor_sync(0xffffffffu, upper ? w[n] : w[n + half], 2 * half);
+        }
+        int32_t * row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float w = ex2_approx(sc[n][e] - st.x) * st.y;  // over the rows of the group:
-            w += __shfl_xor_sync(0xffffffffu, w, 4);
-            w += __shfl_xor_sync(0xffffffffu, w, 8);
-            w += __shfl_xor_sync(0xffffffffu, w, 16);
-            if (g == n) (e ? w1 : w0) = w;  // every row of lanes has the sums: each writes one tile
+            const int key = mine + e;
+            if (key >= len) break;
+            const bool fresh = key >= len - p.n_new;
+            score[key] = fresh ? w[e] : fmaf(p.decay, old[e], w[e]);
+            if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
         }
-    int32_t * row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int key = mine + e;
-        if (key >= len) break;
-        const bool fresh = key >= len - p.n_new;
-        score[key] = fresh ? (e ? w1 : w0) : fmaf(p.decay, old[e], e ? w1 : w0);
-        if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
+        if (kMode != kGiven || first + kChunk >= end) break;
     }
     if (kMode == kCluster) {
         __syncwarp();
@@ -281,7 +295,7 @@ int launch_observe(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
         return check_launch(e, "observe_kernel<weights>");
     }
     if (p.lse != nullptr) {
-        launch_pdl(observe_kernel<Q8, kGiven>, grid, dim3(kThreads), 0, st, p);
+        launch_pdl(observe_kernel<Q8, kGiven>, dim3((grid.x + p.run - 1) / p.run, grid.y), dim3(kThreads), 0, st, p);
         return check_launch(e, "observe_kernel<given>");
     }
     cudaLaunchConfig_t cfg = {};
@@ -334,6 +348,12 @@ int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspa
     p.n_q = a->n_q; p.n_new = a->n_new; p.kv_bound = a->kv_bound; p.n_chunks = chunks_of(a->kv_bound);
     p.score = reinterpret_cast<uint8_t *>(a->score); p.row_pos = reinterpret_cast<uint8_t *>(a->row_pos);
     p.nb_head = a->nb_head; p.nb_stream = a->nb_stream;
+    {   // given the log-sum-exp, chunks of a CTA: up to eight, while every SM is left three rounds of its two CTAs.  256 streams of 4096
+        // rows: 1 / 2 / 4 / 8 chunks 41.5 / 35.6 / 33.9 / 36.2 us
+        const long long chunks = (long long) p.n_chunks * a->n_streams * p.n_kv_heads;
+        const int       most = (int) std::max(1LL, std::min<long long>(8, chunks / (6LL * e->sm_count))), ctas = (p.n_chunks + most - 1) / most;
+        p.run = (p.n_chunks + ctas - 1) / ctas;
+    }
     p.stats = static_cast<float2 *>(workspace);
     p.status = e->status_dev;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
