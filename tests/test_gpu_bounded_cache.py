@@ -423,6 +423,14 @@ def test_weights_against_a_given_log_sum_exp(case, engine, pkg):
     ObserveCase(engine, pkg, case, given_lse=True).check()
 
 
+@pytest.mark.parametrize("given_lse", [True, False])
+@pytest.mark.parametrize("kind,streams,rows", [("f16", 128, 4700), ("q8_0", 64, 9300)])
+def test_weights_of_many_long_streams(kind, streams, rows, given_lse, engine, pkg):
+    """Enough keys for a block to take several chunks of a stream one after the other: lengths on both sides of every chunk's end."""
+    lens = [min(rows, max(0, 512 * (i % 11) + (0, 1, -1, 64, 257)[i % 5])) for i in range(streams - 2)] + [rows, rows - 1]
+    ObserveCase(engine, pkg, (kind, lens, 1, 4, 2), given_lse=given_lse).check(decay=0.5)
+
+
 @pytest.mark.parametrize("n_new", [0, 3, 1000])
 def test_new_rows_start_from_nothing(n_new, engine, pkg):
     """n_new rows (none, some, all of them) take the weight alone, whatever their score held: NaN included."""

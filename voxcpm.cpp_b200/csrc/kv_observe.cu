@@ -134,9 +134,9 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
         if (len > 0 && tid == 0 && kvh == 0 && chunk == 0) atomicOr(p.status, kStatusBadState);
         return;
     }
-    // Given the log-sum-exp, a CTA takes p.run chunks one after the other; the next one's keys are asked for as soon as the products
-    // have taken this one's.
-    const int chunk0 = kMode == kGiven ? chunk * p.run : chunk, end = kMode == kGiven ? min(len, (chunk0 + p.run) * kChunk) : len;
+    // A CTA takes p.run chunks one after the other (of a cluster: one); the next one's keys are asked for as soon as the products have
+    // taken this one's.
+    const int chunk0 = chunk * p.run, end = min(len, (chunk0 + p.run) * kChunk);
     int       first  = chunk0 * kChunk + warp * kWarpKeys;
     if (kMode != kCluster && chunk0 * kChunk >= len) return;
     // everything the CTA reads is asked for before anything is waited for
@@ -161,14 +161,16 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
         row_stat[tid] = make_float2(hi, isinf(hi) ? 1.0f : ex2_approx(-rest));
     }
     if (kMode == kJoin && tid < p.gqa) {
-        const float2 * all = p.stats + (size_t) blockIdx.y * p.n_chunks * p.gqa + tid;
+        const float2 * all = p.stats + (size_t) blockIdx.y * gridDim.x * p.gqa + tid;
         float2         s = make_float2(-INFINITY, 0.0f);
-        for (int c = 0; c * kChunk < len; ++c) s = join_stats(s, __ldcg(all + (size_t) c * p.gqa));
+#pragma unroll 4
+        for (int c = 0; c * p.run * kChunk < len; ++c) s = join_stats(s, __ldcg(all + (size_t) c * p.gqa));
         row_stat[tid] = as_weights(s);
     }
     uint32_t q[4][4];
     load_query(p, stream, kvh, lane, q);
-    if (kMode == kGiven) __syncthreads();
+    if (kMode == kGiven || kMode == kJoin) __syncthreads();
+    float m = -INFINITY, l = 0.0f;  // kFind, kCluster: of the row's keys in this lane
     for (;; first += kChunk) {
         const int mine = first + 8 * g + 2 * t;  // the two keys whose scores this lane writes
         float sc[kWarpKeys / 8][2];
@@ -181,16 +183,19 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
         }
         old[0] = next_old[0];
         old[1] = next_old[1];
-        if (kMode == kGiven && first + kChunk < end) ask(first + kChunk);
+        const bool more = kMode != kCluster && first + kChunk < end;
+        if (more) ask(first + kChunk);
         if (kMode == kFind || kMode == kCluster) {
-            float m = -INFINITY, l = 0.0f;
+            const float before = m;
 #pragma unroll
             for (int n = 0; n < kWarpKeys / 8; ++n) m = fmaxf(m, fmaxf(sc[n][0], sc[n][1]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             const float ref = m == -INFINITY ? 0.0f : m;
+            if (before != -INFINITY) l *= ex2_approx(before - ref);
 #pragma unroll
             for (int n = 0; n < kWarpKeys / 8; ++n) l += ex2_approx(sc[n][0] - ref) + ex2_approx(sc[n][1] - ref);
+            if (kMode == kFind && more) continue;
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if (t == 0) warp_stat[warp][g] = make_float2(m, l);
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
                 float2 s = warp_stat[0][tid];
 #pragma unroll
                 for (int w = 1; w < kWarps; ++w) s = join_stats(s, warp_stat[w][tid]);
-                if (kMode == kFind) p.stats[((size_t) blockIdx.y * p.n_chunks + chunk) * p.gqa + tid] = s;
+                if (kMode == kFind) p.stats[((size_t) blockIdx.y * gridDim.x + chunk) * p.gqa + tid] = s;
                 else                cta_stat[tid] = s;
             }
             if (kMode == kFind) return;
@@ -223,8 +228,6 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
             }
             __syncthreads();
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for at the end: nobody leaves while its memory is read
-        } else if (kMode == kJoin) {
-            __syncthreads();
         }
         const float2 st = g < p.gqa ? row_stat[g] : make_float2(0.0f, 0.0f);
         // the sums over the rows of the group, g: halving the keys as it halves the rows, so that lane (g, t) ends with keys 2t and
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
             score[key] = fresh ? w[e] : fmaf(p.decay, old[e], w[e]);
             if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
         }
-        if (kMode != kGiven || first + kChunk >= end) break;
+        if (!more) break;
     }
     if (kMode == kCluster) {
         __syncwarp();
@@ -286,7 +289,7 @@ int chunks_of(int kv_bound) { return (std::max(kv_bound, 1) + kChunk - 1) / kChu
 
 template <bool Q8>
 int launch_observe(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
-    const dim3 grid((unsigned) p.n_chunks, (unsigned) (p.n_streams * p.n_kv_heads));
+    const dim3 grid((unsigned) ((p.n_chunks + p.run - 1) / p.run), (unsigned) (p.n_streams * p.n_kv_heads));
     if (p.lse == nullptr && p.n_chunks > kMaxCluster) {
         launch_pdl(observe_kernel<Q8, kFind>, grid, dim3(kThreads), 0, st, p);
         const int rc = check_launch(e, "observe_kernel<statistics>");
@@ -295,7 +298,7 @@ int launch_observe(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
         return check_launch(e, "observe_kernel<weights>");
     }
     if (p.lse != nullptr) {
-        launch_pdl(observe_kernel<Q8, kGiven>, dim3((grid.x + p.run - 1) / p.run, grid.y), dim3(kThreads), 0, st, p);
+        launch_pdl(observe_kernel<Q8, kGiven>, grid, dim3(kThreads), 0, st, p);
         return check_launch(e, "observe_kernel<given>");
     }
     cudaLaunchConfig_t cfg = {};
@@ -348,8 +351,10 @@ int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspa
     p.n_q = a->n_q; p.n_new = a->n_new; p.kv_bound = a->kv_bound; p.n_chunks = chunks_of(a->kv_bound);
     p.score = reinterpret_cast<uint8_t *>(a->score); p.row_pos = reinterpret_cast<uint8_t *>(a->row_pos);
     p.nb_head = a->nb_head; p.nb_stream = a->nb_stream;
-    {   // given the log-sum-exp, chunks of a CTA: up to eight, while every SM is left three rounds of its two CTAs.  256 streams of 4096
-        // rows: 1 / 2 / 4 / 8 chunks 41.5 / 35.6 / 33.9 / 36.2 us
+    p.run = 1;
+    if (p.lse != nullptr || p.n_chunks > kMaxCluster) {
+        // chunks of a CTA: up to eight, while every SM is left three rounds of its two CTAs.  256 streams of 4096 rows, given the
+        // log-sum-exp: 1 / 2 / 4 / 8 chunks 41.5 / 35.6 / 33.9 / 36.2 us
         const long long chunks = (long long) p.n_chunks * a->n_streams * p.n_kv_heads;
         const int       most = (int) std::max(1LL, std::min<long long>(8, chunks / (6LL * e->sm_count))), ctas = (p.n_chunks + most - 1) / most;
         p.run = (p.n_chunks + ctas - 1) / ctas;

@@ -20,7 +20,7 @@ struct ObserveParams {
     const float *   lse;
     float           scale_log2, decay;
     int             n_streams, n_heads, n_kv_heads, gqa, layer, n_q, n_new, kv_bound, n_chunks;
-    int             run;       // one query, given its log-sum-exp: chunks of a CTA
+    int             run;       // one query: chunks of a CTA
     uint8_t *       score;
     uint8_t *       row_pos;
     size_t          nb_head, nb_stream;
