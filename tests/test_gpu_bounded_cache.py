@@ -347,6 +347,8 @@ OBSERVE = {  # kind, lengths, n_q, heads, kv heads
     "empty and short": ("f16", [0, 1, 2, 63, 64, 65, 0], 1, 16, 2),
     "chunk edges": ("f16", [511, 512, 513, 1024, 1500], 1, 16, 2),
     "long": ("f16", [9001], 1, 16, 2),
+    "longer than a cluster takes": ("f16", [24577, 600, 25100], 1, 16, 2),
+    "as long as a cluster takes": ("q8_0", [24576, 20000, 1, 3000], 1, 8, 1),
     "many": ("f16", [3 * i for i in range(200)], 1, 16, 2),
     "one head each": ("f16", [100, 700], 1, 4, 4),
     "six heads": ("f16", [100, 700], 1, 6, 1),

@@ -6,8 +6,8 @@
 // (stream, kv head), a warp 64 of them, from global memory straight into the operands of the products (a lane's 16-byte
 // loads; nothing is shared between warps, so nothing passes through shared memory).  The softmax's (max, sum) are
 //   given:    the log-sum-exp is an input; every CTA for itself;
-//   cluster:  up to 4096 keys: the CTAs of a pair are a cluster and exchange (max, sum) through distributed shared memory
-//             while the scores wait in registers: K is read once, in one launch;
+//   cluster:  up to 24576 keys: the CTAs of a pair are a cluster and exchange (max, sum) through distributed shared memory
+//             while the scores wait in registers and shared memory: K is read once, in one launch;
 //   two:      longer streams: a launch that finds the (max, sum) of every CTA's keys, and one that joins them.
 #include "kv_observe.cuh"
 
@@ -21,6 +21,7 @@ constexpr int kWarpKeys  = 64;                  // keys a warp keeps as operands
 constexpr int kChunk     = kWarps * kWarpKeys;  // keys of a CTA
 constexpr int kMaxGroup  = 8;                   // query heads of a kv head
 constexpr int kMaxCluster = 8;
+constexpr int kMaxRun     = 6;                   // chunks of a CTA of a cluster: the scores of two CTAs fit an SM
 
 enum { kGiven, kCluster, kFind, kJoin };        // which launch (see above); kFind and kJoin are the two
 
@@ -124,6 +125,7 @@ __device__ __forceinline__ float2 as_weights(float2 s) { return s.y == 0.0f ? ma
 
 template <bool Q8, int kMode>
 __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParams p) {
+    extern __shared__ float4 kept_scores[];  // kCluster: [chunk][4][thread], of all chunks of a CTA but the last
     __shared__ float2 row_stat[kMaxGroup], cta_stat[kMaxGroup], warp_stat[kWarps][kMaxGroup];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int chunk = blockIdx.x, kvh = blockIdx.y % p.n_kv_heads, stream = blockIdx.y / p.n_kv_heads;
@@ -134,8 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
         if (len > 0 && tid == 0 && kvh == 0 && chunk == 0) atomicOr(p.status, kStatusBadState);
         return;
     }
-    // A CTA takes p.run chunks one after the other (of a cluster: one); the next one's keys are asked for as soon as the products have
-    // taken this one's.
+    // A CTA takes p.run chunks one after the other; the next one's keys are asked for as soon as the products have taken this one's.
     const int chunk0 = chunk * p.run, end = min(len, (chunk0 + p.run) * kChunk);
     int       first  = chunk0 * kChunk + warp * kWarpKeys;
     if (kMode != kCluster && chunk0 * kChunk >= len) return;
@@ -147,13 +148,14 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
     auto ask = [&](int from) {
 #pragma unroll
         for (int n = 0; n < kWarpKeys / 8; ++n) keys[n] = load_keys<Q8>(pair, from + 8 * n + g, t, from + 8 * n + g < len);
-        if (kMode != kFind) {
+    };
+    auto ask_old = [&](int from) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (from + 8 * g + 2 * t + e < len - p.n_new) next_old[e] = score[from + 8 * g + 2 * t + e];
-        }
+        for (int e = 0; e < 2; ++e)
+            if (from + 8 * g + 2 * t + e < len - p.n_new) next_old[e] = score[from + 8 * g + 2 * t + e];
     };
     ask(first);
+    if (kMode == kGiven || kMode == kJoin || first + kChunk >= end) ask_old(first);
     if (kMode == kGiven && tid < p.gqa) {
         // kept as the scores are, in units of log2, in two parts: one would lose 2^-24 of its size
         const float x = p.lse[(size_t) stream * p.n_heads + kvh * p.gqa + tid], hi = x * 1.4426950408889634f;
@@ -170,9 +172,31 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
     uint32_t q[4][4];
     load_query(p, stream, kvh, lane, q);
     if (kMode == kGiven || kMode == kJoin) __syncthreads();
+    int32_t * const row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
+    auto write = [&](const float (&sc)[kWarpKeys / 8][2], float2 st, int from, const float (&old)[2]) {
+        // the sums over the rows of the group, g: halving the keys as it halves the rows, so that lane (g, t) ends with keys 2t and
+        // 2t + 1 of tile g (14 shuffles; each sum by itself in every lane would be 48)
+        static_assert(kWarpKeys == 64, "a tile of keys to a row of lanes");
+        float w[16];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) w[n] = ex2_approx(sc[n >> 1][n & 1] - st.x) * st.y;
+#pragma unroll
+        for (int half = 8; half >= 2; half >>= 1) {
+            const bool upper = g & (half >> 1);
+#pragma unroll
+            for (int n = 0; n < half; ++n) w[n] = (upper ? w[n + half] : w[n]) + __shfl_xor_sync(0xffffffffu, upper ? w[n] : w[n + half], 2 * half);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int key = from + 8 * g + 2 * t + e;
+            if (key >= len) break;
+            const bool fresh = key >= len - p.n_new;
+            score[key] = fresh ? w[e] : fmaf(p.decay, old[e], w[e]);
+            if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
+        }
+    };
     float m = -INFINITY, l = 0.0f;  // kFind, kCluster: of the row's keys in this lane
-    for (;; first += kChunk) {
-        const int mine = first + 8 * g + 2 * t;  // the two keys whose scores this lane writes
+    for (int n_kept = 0;; first += kChunk) {
         float sc[kWarpKeys / 8][2];
 #pragma unroll
         for (int n = 0; n < kWarpKeys / 8; ++n) {
@@ -183,8 +207,11 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
         }
         old[0] = next_old[0];
         old[1] = next_old[1];
-        const bool more = kMode != kCluster && first + kChunk < end;
-        if (more) ask(first + kChunk);
+        const bool more = first + kChunk < end;
+        if (more) {
+            ask(first + kChunk);
+            if (kMode == kGiven || kMode == kJoin || (kMode == kCluster && first + 2 * kChunk >= end)) ask_old(first + kChunk);
+        }
         if (kMode == kFind || kMode == kCluster) {
             const float before = m;
 #pragma unroll
@@ -195,7 +222,14 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
             if (before != -INFINITY) l *= ex2_approx(before - ref);
 #pragma unroll
             for (int n = 0; n < kWarpKeys / 8; ++n) l += ex2_approx(sc[n][0] - ref) + ex2_approx(sc[n][1] - ref);
-            if (kMode == kFind && more) continue;
+            if (more) {
+                if (kMode == kCluster) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) kept_scores[(4 * n_kept + n) * kThreads + tid] = make_float4(sc[2 * n][0], sc[2 * n][1], sc[2 * n + 1][0], sc[2 * n + 1][1]);
+                    ++n_kept;
+                }
+                continue;
+            }
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if (t == 0) warp_stat[warp][g] = make_float2(m, l);
@@ -216,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
 #pragma unroll
                 for (int r = 0; r < kMaxCluster; ++r) {  // all on their way together
                     all[r] = s;
-                    if (r < p.n_chunks) {
+                    if (r < (int) gridDim.x) {
                         uint32_t peer;
                         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(r));
                         asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(all[r].x), "=f"(all[r].y) : "r"(peer) : "memory");
@@ -230,27 +264,22 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for at the end: nobody leaves while its memory is read
         }
         const float2 st = g < p.gqa ? row_stat[g] : make_float2(0.0f, 0.0f);
-        // the sums over the rows of the group, g: halving the keys as it halves the rows, so that lane (g, t) ends with keys 2t and
-        // 2t + 1 of tile g (14 shuffles; each sum by itself in every lane would be 48)
-        static_assert(kWarpKeys == 64, "a tile of keys to a row of lanes");
-        float w[16];
+        if (kMode == kCluster) {  // the last chunk's scores are here; back over the others
+            while (n_kept > 0) {
+                --n_kept;
+                ask_old(first - kChunk);
+                write(sc, st, first, old);
+                first -= kChunk;
 #pragma unroll
-        for (int n = 0; n < 16; ++n) w[n] = ex2_approx(sc[n >> 1][n & 1] - st.x) * st.y;
-#pragma unroll
-        for (int half = 8; half >= 2; half >>= 1) {
-            const bool upper = g & (half >> 1);
-#pragma unroll
-            for (int n = 0; n < half; ++n) w[n] = (upper ? w[n + half] : w[n]) + __shfl_xor_sync(0xffffffffu, upper ? w[n] : w[n + half], 2 * half);
+                for (int n = 0; n < 4; ++n) {
+                    const float4 x = kept_scores[(4 * n_kept + n) * kThreads + tid];
+                    sc[2 * n][0] = x.x; sc[2 * n][1] = x.y; sc[2 * n + 1][0] = x.z; sc[2 * n + 1][1] = x.w;
+                }
+                old[0] = next_old[0];
+                old[1] = next_old[1];
+            }
         }
-        int32_t * row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int key = mine + e;
-            if (key >= len) break;
-            const bool fresh = key >= len - p.n_new;
-            score[key] = fresh ? w[e] : fmaf(p.decay, old[e], w[e]);
-            if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
-        }
+        write(sc, st, first, old);
         if (!more) break;
     }
     if (kMode == kCluster) {
@@ -290,7 +319,7 @@ int chunks_of(int kv_bound) { return (std::max(kv_bound, 1) + kChunk - 1) / kChu
 template <bool Q8>
 int launch_observe(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
     const dim3 grid((unsigned) ((p.n_chunks + p.run - 1) / p.run), (unsigned) (p.n_streams * p.n_kv_heads));
-    if (p.lse == nullptr && p.n_chunks > kMaxCluster) {
+    if (p.lse == nullptr && p.n_chunks > kMaxCluster * kMaxRun) {
         launch_pdl(observe_kernel<Q8, kFind>, grid, dim3(kThreads), 0, st, p);
         const int rc = check_launch(e, "observe_kernel<statistics>");
         if (rc != VOX_ATTN_OK) return rc;
@@ -301,8 +330,15 @@ int launch_observe(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
         launch_pdl(observe_kernel<Q8, kGiven>, grid, dim3(kThreads), 0, st, p);
         return check_launch(e, "observe_kernel<given>");
     }
+    const size_t   most = (size_t) (kMaxRun - 1) * kChunk * kMaxGroup * sizeof(float);
+    const uint32_t bit  = 1u << (Q8 ? 11 : 10);
+    if (!(e->attr_mask & bit)) {
+        VOX_CUDA_TRY(cudaFuncSetAttribute(observe_kernel<Q8, kCluster>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most));
+        e->attr_mask |= bit;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = dim3(kThreads); cfg.stream = st;
+    cfg.dynamicSmemBytes = (size_t) (p.run - 1) * kChunk * kMaxGroup * sizeof(float);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = grid.x; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -323,7 +359,7 @@ size_t vox_kv_observe_workspace_bytes(const vox_kv_observe_args * a) {
     const int HK = a->cache->cfg.n_kv_heads;
     if (a->n_q > 1) return observe_window_bytes(a->n_streams, HK, a->n_heads / HK * a->n_q, a->kv_bound);
     const int chunks = chunks_of(a->kv_bound);
-    return chunks <= kMaxCluster ? 0 : (size_t) a->n_streams * a->n_heads * chunks * sizeof(float2);
+    return chunks <= kMaxCluster * kMaxRun ? 0 : (size_t) a->n_streams * a->n_heads * chunks * sizeof(float2);
 }
 
 int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspace, size_t workspace_bytes, void * stream) {
@@ -351,14 +387,16 @@ int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspa
     p.n_q = a->n_q; p.n_new = a->n_new; p.kv_bound = a->kv_bound; p.n_chunks = chunks_of(a->kv_bound);
     p.score = reinterpret_cast<uint8_t *>(a->score); p.row_pos = reinterpret_cast<uint8_t *>(a->row_pos);
     p.nb_head = a->nb_head; p.nb_stream = a->nb_stream;
-    p.run = 1;
-    if (p.lse != nullptr || p.n_chunks > kMaxCluster) {
-        // chunks of a CTA: up to eight, while every SM is left three rounds of its two CTAs.  256 streams of 4096 rows, given the
-        // log-sum-exp: 1 / 2 / 4 / 8 chunks 41.5 / 35.6 / 33.9 / 36.2 us
-        const long long chunks = (long long) p.n_chunks * a->n_streams * p.n_kv_heads;
-        const int       most = (int) std::max(1LL, std::min<long long>(8, chunks / (6LL * e->sm_count))), ctas = (p.n_chunks + most - 1) / most;
-        p.run = (p.n_chunks + ctas - 1) / ctas;
-    }
+    // Chunks of a CTA, 256 streams of 4096 rows.  Given the log-sum-exp: several while every SM is left two rounds of its two CTAs (1 / 2
+    // / 4 / 8 chunks 41.5 / 35.6 / 33.9 / 36.2 us).  In a cluster a CTA waits for the others once, whatever it holds: as many as make
+    // one round of all CTAs, if they fit (1 / 4 / 6 chunks 86.7 / 53.4 / 53.4 us; 64 streams 1 / 4 chunks 23.8 / 15.9 us), and what
+    // eight CTAs need.
+    const long long chunks  = (long long) p.n_chunks * a->n_streams * p.n_kv_heads, slots = 2LL * e->sm_count;
+    const bool      cluster = p.lse == nullptr && p.n_chunks <= kMaxCluster * kMaxRun;
+    const int       most    = cluster ? std::max((p.n_chunks + kMaxCluster - 1) / kMaxCluster, (int) std::min<long long>(kMaxRun, (chunks + slots - 1) / slots))
+                                      : (int) std::max(1LL, std::min<long long>(8, chunks / (2 * slots)));
+    const int       ctas    = (p.n_chunks + most - 1) / most;
+    p.run = (p.n_chunks + ctas - 1) / ctas;
     p.stats = static_cast<float2 *>(workspace);
     p.status = e->status_dev;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
