@@ -14,9 +14,10 @@
 // head) is the work of one thread-block cluster of up to eight CTAs, which share out the prefix's 128-key tiles; their
 // partial results meet through distributed shared memory, every CTA joining a share of the rows.  Nothing goes through
 // global memory but the inputs and the result.
-// (Measured against it: the prefix kernel first, partials in global memory, folded by the decode kernel as it wrote every
-// result: 61.7 us for 256 streams under two prompts of 4096 rows and up to 2048 rows of their own, 16.9 us for 32 streams
-// under four of 700; the folds' round trips to L2 and the decode kernel's late start were a third of it.)
+// 256 streams under two prompts of 4096 rows with up to 2048 rows of their own: 49 us, of which the own rows (151 MB) are the bound: 3.1
+// TB/s; each stream reading its prefix would be 690 MB.  32 streams under four of 700: 11.4 us, latency.
+// (Built first: the prefix kernel in front, partials in global memory, folded by the decode kernel as it wrote every result: 61.7 and
+// 16.9 us; the folds' round trips to L2 and the decode kernel's late start were a third of it.)
 #include "shared_prefix.cuh"
 #include "tcgen05.cuh"
 
@@ -624,10 +625,10 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 //   warps 0 .. 4 kGroups - 1  softmax      then one warp  issues S = Q.K, one  O += P.V, and that one, or a third of two
 //   groups, the copies of K and V
 // One softmax group (192 threads of 128 registers, 81 KB of shared memory; q8_0 107 KB): the CTA runs beside two CTAs of the decode
-// kernel, whose time is HBM's, and takes about 1.1 us for 64 keys (q8_0 2.3 us), most of it latency that nothing hides.
-// Two groups, which take tiles in turn with a reference and accumulators of their own, need less than two thirds of that,
-// but leave room for one decode CTA per SM only: taken where the streams' own rows are few against the prefix (see
-// vox_attn_decode_shared).
+// kernel, whose time is HBM's, and takes about 1.1 us for 64 keys (q8_0 2.3 us), most of it latency that nothing hides: 0.5 us of
+// it are products and exponentials.  Two groups, which take tiles in turn with a reference and accumulators of their own, hide
+// some of it (256 streams under two prompts of 2048 / 4096 rows, one row of their own: 25.2 / 34.2 -> 20.3 / 28.4 us), but leave
+// room for one decode CTA per SM only: taken where the streams' own rows are few against the prefix (see vox_attn_decode_shared).
 //
 // q8_0: the softmax warps turn a tile's bytes into f16 numbers q (exact; a tile ahead of the scores they work on) and keep the
 // scales apart.  Either 32-value block has a score accumulator of its own (s = d0 S0 + d1 S1), and its 32 output columns have
@@ -1272,11 +1273,12 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     const bool              q8  = a->own.cache->cfg.type == VOX_TYPE_Q8_0, tc = shares && pl->full;
     const int               sms = std::min(kDecodeMaxSms, e->sm_count), k = !shares || tc ? 0 : small_arrangement(pl, sms, HK, a->prefix_bound);
     const int               cluster = shares ? cluster_size(sms, pl->n_tiles[k], HK, a->prefix_bound, tc) : 1;
-    // Two softmax groups, beside one decode CTA per SM, where the streams' own 64-row tiles per SM are at most four times the
-    // tiles that a CTA of the prefix kernel walks (the two kernels then end together): under prompts of 4096 rows 256
-    // streams with a row of their own take 21 us against 34 us, with up to 2048 rows 57 us against 49 us.
+    // Two softmax groups, beside one decode CTA per SM, where the streams' own 64-row tiles per SM are few against the tiles that a
+    // CTA of the prefix kernel walks: then the prefix kernel is what the call waits for.  256 streams under two prompts of 4096
+    // rows, own rows 1 / 128 / 512 / 1024 / 2048: f16 28 / 25 / 38 / 47 / 68 us against 34 / 35 / 33 / 37 / 49 us with one group;
+    // q8_0, whose scores cost more, 44 / 45 / 51 / 59 / 77 against 56 / 58 / 62 / 67 / 71 us.
     const long long own_tiles = (long long) a->own.n_streams * HK * ((a->own.kv_bound + kKvTile - 1) / kKvTile) / sms;
-    const bool      wide = tc && own_tiles <= 4LL * ((a->prefix_bound + kSub - 1) / kSub) / cluster;
+    const bool      wide = tc && 4 * own_tiles <= (q8 ? 20LL : 5LL) * ((a->prefix_bound + kSub - 1) / kSub) / cluster;
     rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml, !shares ? 0 : wide ? 1 : 2}, workspace, own, st);
     if (rc != VOX_ATTN_OK || !shares) return rc;
     SharedParams         p;
