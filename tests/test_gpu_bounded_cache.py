@@ -568,6 +568,8 @@ class EvictCase:
     ([5, 4, 3, 2, 1, 0], 1, 0, 0),
     ([1025, 1026, 1027, 1028], 1024, 4, 32),
     ([5000, 2100], 900, 4, 32),
+    ([4, 5, 6, 7] * 12, 3, 0, 0),
+    ([36, 35, 34, 33] * 6, 32, 0, 0),
 ])
 def test_eviction_matches_the_definition(kind, lens, budget, n_sink, n_recent, engine, pkg):
     EvictCase(engine, pkg, kind, lens, 2, 2, max(lens) + 9).check(budget, n_sink, n_recent)

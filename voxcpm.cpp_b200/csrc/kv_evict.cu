@@ -50,12 +50,18 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 
 // one of the eight 16-byte pieces of a q8_0 row: four of K, four of V; the first of either also takes its two scales
-__device__ __forceinline__ void move_q8_piece(uint8_t * pair, int from, int to, int piece) {
-    const uint32_t  bytes = piece & 4 ? kQ8VBytesOff : 0, scales = piece & 4 ? kQ8VScaleOff : kQ8KScaleOff;
-    const uint8_t * a = pair + q8_tile_off(from);
-    uint8_t *       b = pair + q8_tile_off(to);
-    *reinterpret_cast<uint4 *>(b + bytes + q8_byte_off(to, 16 * (piece & 3))) = *reinterpret_cast<const uint4 *>(a + bytes + q8_byte_off(from, 16 * (piece & 3)));
-    if ((piece & 3) == 0) *reinterpret_cast<uint32_t *>(b + scales + q8_scale_off(to, 0)) = *reinterpret_cast<const uint32_t *>(a + scales + q8_scale_off(from, 0));
+struct Q8Piece { uint4 bytes; uint32_t scales; };
+__device__ __forceinline__ Q8Piece load_q8_piece(const uint8_t * pair, int row, int piece) {
+    const uint8_t * a = pair + q8_tile_off(row);
+    Q8Piece         x;
+    x.bytes  = *reinterpret_cast<const uint4 *>(a + (piece & 4 ? kQ8VBytesOff : 0) + q8_byte_off(row, 16 * (piece & 3)));
+    x.scales = (piece & 3) == 0 ? *reinterpret_cast<const uint32_t *>(a + (piece & 4 ? kQ8VScaleOff : kQ8KScaleOff) + q8_scale_off(row, 0)) : 0u;
+    return x;
+}
+__device__ __forceinline__ void store_q8_piece(uint8_t * pair, int row, int piece, const Q8Piece & x) {
+    uint8_t * b = pair + q8_tile_off(row);
+    *reinterpret_cast<uint4 *>(b + (piece & 4 ? kQ8VBytesOff : 0) + q8_byte_off(row, 16 * (piece & 3))) = x.bytes;
+    if ((piece & 3) == 0) *reinterpret_cast<uint32_t *>(b + (piece & 4 ? kQ8VScaleOff : kQ8KScaleOff) + q8_scale_off(row, 0)) = x.scales;
 }
 
 // Exclusive prefix sums over the block, and their total.  Two buffers of warp sums in turn, so that one barrier is enough.
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
         }
     } else {      // 8 lanes a row
 #pragma unroll 2
-        for (int i = 4 * (rank * kWarps + warp) + (lane >> 3); i < n_move; i += 4 * kWarps * p.cluster) move_q8_piece(p.k_data + pair, src[i], dst[i], lane & 7);
+        for (int i = 4 * (rank * kWarps + warp) + (lane >> 3); i < n_move; i += 4 * kWarps * p.cluster) store_q8_piece(p.k_data + pair, dst[i], lane & 7, load_q8_piece(p.k_data + pair, src[i], lane & 7));
     }
 }
 
@@ -276,6 +282,7 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
 // index first, so the next is the least of those after the last.
 constexpr int kFew        = 4;
 constexpr int kFewThreads = 128;
+static_assert(kFewThreads / 32 >= kFew, "a warp for each row behind the budget");
 __global__ void __launch_bounds__(kFewThreads, 16) evict_few_kernel(const EvictParams p) {
     __shared__ uint32_t least_key[2][kFewThreads / 32];
     __shared__ int      least_row[2][kFewThreads / 32];
@@ -295,44 +302,59 @@ __global__ void __launch_bounds__(kFewThreads, 16) evict_few_kernel(const EvictP
     float *   const score = reinterpret_cast<float *>(p.score + at);
     int32_t * const pos   = reinterpret_cast<int32_t *>(p.row_pos + at);
     const int recent = (p.n_seen ? p.n_seen[stream] : len) - p.n_recent, n_go = len - p.budget;
-    int       gone[kFew];
-    uint32_t  last_key = 0;
-    int       last_row = 0x7fffffff;
+    if (n_go <= 0) {
+        if (kept) for (int j = tid; j < len; j += kFewThreads) kept[j] = j;
+        return;
+    }
+    // the rows behind the budget are at most kFew: a warp asks for each, wherever it may have to go
+    const size_t    pair = (size_t) (p.layer0 + layer) * p.c_nb_layer + (size_t) stream * p.c_nb_stream + (size_t) kvh * p.c_nb_head;
+    uint8_t * const base = (lane & 8 ? p.v_data : p.k_data) + pair + (lane & 7) * 16;
+    const int       from = p.budget + warp;
+    Q8Piece         row = {};
+    float           row_score = 0.0f;
+    int             row_at = 0;
+    if (warp < n_go) {
+        if (lane == 31) {
+            row_score = score[from];
+            row_at    = pos[from];
+        } else if (!p.q8 && lane < 16) {
+            row.bytes = *reinterpret_cast<const uint4 *>(base + (size_t) from * 128);
+        } else if (p.q8 && lane < 8) {
+            row = load_q8_piece(p.k_data + pair, from, lane);
+        }
+    }
+    int      gone[kFew];
+    uint32_t last_key = 0;
+    int      last_row = 0x7fffffff;
 #pragma unroll
     for (int g = 0; g < kFew; ++g) {
         gone[g] = 0x7fffffff;
         if (g >= n_go) continue;
         uint32_t key = 0xffffffffu;
-        int      row = -1;
+        int      at = -1;
 #pragma unroll 8
-        for (int j = tid; j < len; j += kFewThreads) {
+        for (int j = tid; j < len; j += kFewThreads) {  // of equal keys the last
             const int      q = pos[j];
             const float    w = score[j];
             const uint32_t k = q < p.n_sink || q >= recent ? 0xffffffffu : ordered(w);
-            const bool     later = k > last_key || (k == last_key && j < last_row);
-            if (later && (k < key || (k == key && j > row))) { key = k; row = j; }
+            const bool     later = g == 0 || k > last_key || (k == last_key && j < last_row);
+            if (later && k <= key) { key = k; at = j; }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const uint32_t k = __shfl_xor_sync(0xffffffffu, key, o);
-            const int      r = __shfl_xor_sync(0xffffffffu, row, o);
-            if (k < key || (k == key && r > row)) { key = k; row = r; }
-        }
-        if (lane == 0) { least_key[g & 1][warp] = key; least_row[g & 1][warp] = row; }
+        const uint32_t least = __reduce_min_sync(0xffffffffu, key);
+        at = __reduce_max_sync(0xffffffffu, key == least ? at : -1);
+        if (lane == 0) { least_key[g & 1][warp] = least; least_row[g & 1][warp] = at; }
         __syncthreads();
+        key = least_key[g & 1][0];
+        at  = least_row[g & 1][0];
 #pragma unroll
-        for (int o = 0; o < kFewThreads / 32; ++o) {
+        for (int o = 1; o < kFewThreads / 32; ++o) {
             const uint32_t k = least_key[g & 1][o];
             const int      r = least_row[g & 1][o];
-            if (o == 0 || k < key || (k == key && r > row)) { key = k; row = r; }
+            if (k < key || (k == key && r > at)) { key = k; at = r; }
         }
         last_key = key;
-        last_row = row;
-        gone[g]  = row;
-    }
-    if (n_go <= 0) {
-        if (kept) for (int j = tid; j < len; j += kFewThreads) kept[j] = j;
-        return;
+        last_row = at;
+        gone[g]  = at;
     }
 #pragma unroll
     for (int a = 0; a + 1 < kFew; ++a)  // by index
@@ -342,36 +364,31 @@ __global__ void __launch_bounds__(kFewThreads, 16) evict_few_kernel(const EvictP
             gone[b] = lo;
             gone[b + 1] = hi;
         }
-    auto goes = [&](int j) {
-        bool g = false;
-#pragma unroll
-        for (int i = 0; i < kFew; ++i) g |= gone[i] == j;
-        return g;
-    };
     if (kept)
-        for (int j = tid; j < p.budget; j += kFewThreads)
-            if (!goes(j)) kept[j] = j;
-    __syncthreads();  // every thread has read the scores
-    const size_t pair = (size_t) (p.layer0 + layer) * p.c_nb_layer + (size_t) stream * p.c_nb_stream + (size_t) kvh * p.c_nb_head;
-    int from = p.budget;
+        for (int j = tid; j < p.budget; j += kFewThreads) kept[j] = j;
+    __syncthreads();  // every thread has read the scores; and the rows that go are written over in `kept`
+    if (warp >= n_go) return;
+    // the i-th row behind the budget that stays moves to the i-th place below it whose row goes
+    int nth = 0, to = p.budget;
 #pragma unroll
-    for (int g = 0; g < kFew; ++g) {
-        const int to = gone[g];
-        if (to >= p.budget) break;  // the rows that go above the budget are left behind
-        while (goes(from)) ++from;
-        if (warp == g % (kFewThreads / 32)) {  // a warp a row
-            if (lane == 31) {
-                score[to] = score[from];
-                pos[to]   = pos[from];
-                if (kept) kept[to] = from;
-            } else if (!p.q8 && lane < 16) {
-                uint8_t * const base = (lane & 8 ? p.v_data : p.k_data) + pair + (lane & 7) * 16;
-                *reinterpret_cast<uint4 *>(base + (size_t) to * 128) = *reinterpret_cast<const uint4 *>(base + (size_t) from * 128);
-            } else if (p.q8 && lane < 8) {
-                move_q8_piece(p.k_data + pair, from, to, lane);
-            }
-        }
-        ++from;
+    for (int i = 0; i < kFew; ++i) {
+        if (gone[i] == from) return;
+        if (p.budget + i < from) ++nth;
+    }
+#pragma unroll
+    for (int i = 0; i < kFew; ++i)
+        if (gone[i] >= p.budget && gone[i] < from) --nth;
+#pragma unroll
+    for (int i = 0; i < kFew; ++i)
+        if (i == nth) to = gone[i];
+    if (lane == 31) {
+        score[to] = row_score;
+        pos[to]   = row_at;
+        if (kept) kept[to] = from;
+    } else if (!p.q8 && lane < 16) {
+        *reinterpret_cast<uint4 *>(base + (size_t) to * 128) = row.bytes;
+    } else if (p.q8 && lane < 8) {
+        store_q8_piece(p.k_data + pair, to, lane, row);
     }
 }
 
