@@ -422,7 +422,7 @@ int    vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, 
  *   n_seen     device array [n_streams]: tokens every stream has seen, the new ones included (NULL: kv_len)
  *   kv_bound   host-known upper bound of every kv_len; a longer stream raises VOX_ATTN_DEVICE_STATE and is left alone
  * The same call gives the same bits.  workspace: vox_kv_observe_workspace_bytes (0 for most calls with n_q == 1), 16-byte
- * aligned. */
+ * aligned.  The engine's device must be the current one. */
 typedef struct {
     const vox_kv_cache * cache;
     int32_t         layer;
@@ -461,7 +461,7 @@ int    vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * work
  *   new_len    device out [n_streams]: min(kv_len, budget); must not overlap kv_len or n_seen
  *   kept       optional out [budget, HK, n_streams, n_layers] int32 contiguous: for every row below new_len the index it had
  *              (rows beyond are left as they are)
- * Rows at new_len and beyond are left as they are. */
+ * Rows at new_len and beyond are left as they are.  The engine's device must be the current one. */
 typedef struct {
     vox_kv_cache *  cache;
     int32_t         layer0, n_layers;

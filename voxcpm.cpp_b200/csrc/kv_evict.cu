@@ -10,6 +10,9 @@
 // hundred keys of the bin it falls in against one another; only a bin with more keys than that (many equal scores) is cut
 // further, 11 and 10 bits at a time.  Lists are few when one stream is cut: then a cluster of CTAs takes each, every CTA
 // selecting for itself (the scores are in L2) and moving a share of the rows.
+// 1440 lists of up to 2048 f16 rows cut to 512 (194 MB read and written): 48 us, 4.0 TB/s, bound by the chain of phases of a CTA and by
+// what unequal lists leave idle (one round of CTAs and a part); 128, 192 and 512 threads, and fewer CTAs with more loads in flight,
+// came out equal or slower.  Six lists of 300 rows: 10 us, latency.
 #include "kv_cache.cuh"
 
 #include <algorithm>
@@ -279,7 +282,8 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
 
 // Few rows to give up (a stream that gains a row a step gives one up a step): no border is looked for, the rows that go are,
 // one after the other, by reductions over the block.  They go in the order of their keys, of equal ones the highest
-// index first, so the next is the least of those after the last.
+// index first, so the next is the least of those after the last.  1920 lists that give up one row of 1025: 12 us for 16.4 MB, bound by
+// the 25 instructions of a key (issue slots 42 % in use).
 constexpr int kFew        = 4;
 constexpr int kFewThreads = 128;
 static_assert(kFewThreads / 32 >= kFew, "a warp for each row behind the budget");

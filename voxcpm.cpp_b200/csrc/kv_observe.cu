@@ -9,6 +9,11 @@
 //   cluster:  up to 24576 keys: the CTAs of a pair are a cluster and exchange (max, sum) through distributed shared memory
 //             while the scores wait in registers and shared memory: K is read once, in one launch;
 //   two:      longer streams: a launch that finds the (max, sum) of every CTA's keys, and one that joins them.
+// 256 streams of 4096 f16 rows, given the log-sum-exp: 32.5 us = 5.5 TB/s, 84 % of the copy bandwidth; without it 53.4 us (a CTA
+// waits for its cluster with its loads done); 64 streams 12.7 / 15.9 us.  Four streams of 300 rows: 4.7 us, the latency of a launch.
+// q8_0 rows cost the conversion of every byte: 34.3 us at 256 x 4096, 2.9 TB/s.
+// (For smaller pieces and more CTAs of fewer registers: 32 keys of a warp 42 - 53 us, three CTAs per SM 43 us, against 40.4 us before a
+// CTA took several chunks.)
 #include "kv_observe.cuh"
 
 using namespace vox;
