@@ -745,6 +745,33 @@ def test_streams_of_one_voice_in_a_bounded_cache(kind, engine, pkg):
     assert n.max() == budget and seen.max() > budget
 
 
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("streams", [1, 2, 12])
+def test_lengths_of_an_eviction_feed_the_next_call_directly(streams, shared, engine, pkg):
+    """new_len as the kv_len of the launch behind it, which may be scheduled while the eviction still runs: few f16 streams (a
+    cluster per pair) and more."""
+    import torch
+    g = gen(6)
+    cache = new_cache(engine, pkg, "f16", 1, streams, 2, 2048)
+    cache.append(0, randn(g, streams, 2048, 2, D), randn(g, streams, 2048, 2, D))
+    q, full, cut = randn(g, streams, 16, D), ints([2000] * streams), ints([1500] * streams)
+    score = torch.rand((1, streams, 2, 2048), generator=g, device="cuda")
+    pos = torch.arange(2048, dtype=torch.int32, device="cuda").expand(1, streams, 2, 2048).contiguous()
+    new_len = ints([0] * streams)
+
+    def decode(n):
+        return cache.decode_shared(0, q, n, 2048) if shared else cache.decode(0, q, n, 2048)
+
+    for _ in range(20):
+        new_len.fill_(40)
+        torch.cuda.synchronize()
+        cache.evict(full, 2048, 1500, score, pos, None, new_len)
+        out = decode(new_len)
+        engine.sync_status()
+        assert new_len.tolist() == [1500] * streams
+        assert torch.equal(out, decode(cut))
+
+
 # ----------------------------------------------------------------------------------------------------------------- refusals
 
 def test_refusals(engine, pkg):

@@ -522,13 +522,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         // One cluster per pair: no list to cut.  The pair's tiles are split into nearly equal parts of four tiles or
         // more, one per CTA of the cluster as far as they go; the other CTAs of the cluster have nothing to do.
         asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-        const int pair = (int) blockIdx.x / p.cluster;
-        w.i = pair / p.n_kv_heads; w.kvh = pair - w.i * p.n_kv_heads;
-        walk_load(p, w);
-        parts   = max(1, min(p.cluster, w.tiles >> 2));
-        w.t     = rank < parts ? (rank * w.tiles) / parts : 0;
-        n_tiles = rank < parts ? ((rank + 1) * w.tiles) / parts - w.t : 0;
-        if (tid == 0) mbar_init(smem_u32(&xbar), parts);
+        // (as many arrivals as the cluster has CTAs: how many take part is known only once the length may be read)
+        if (tid == 0) mbar_init(smem_u32(&xbar), p.cluster);
         fence_mbar_init();
         __syncthreads();
         // every CTA's barrier is initialised before anyone can reach it
@@ -538,6 +533,14 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             pdl_wait();
             pdl_launch_dependents();
         }
+        const int pair = (int) blockIdx.x / p.cluster;
+        w.i = pair / p.n_kv_heads; w.kvh = pair - w.i * p.n_kv_heads;
+        walk_load(p, w);
+        parts   = max(1, min(p.cluster, w.tiles >> 2));
+        w.t     = rank < parts ? (rank * w.tiles) / parts : 0;
+        n_tiles = rank < parts ? ((rank + 1) * w.tiles) / parts - w.t : 0;
+        if (tid == 0 && rank == 0 && parts < p.cluster)  // for the CTAs that have nothing to do
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&xbar)), "r"(p.cluster - parts) : "memory");
         if (tid == 0) DECODE_TRACE(1);
         if (rank >= parts) {
             if (p.early) {  // every CTA of the grid passes the dependency wait
