@@ -382,7 +382,8 @@ void vox_prefix_plan_destroy(vox_prefix_plan * p);
  *                the table is built for positions that count the prefix).  stream_order must be NULL.
  *   prefix       the cache that holds the prefixes: same type and kv heads as own.cache, own.layer is taken of both; it may
  *                be own.cache itself (streams of it that the call does not decode)
- *   prefix_len   device array [streams of the prefix cache]: rows of each prefix
+ *   prefix_len   device array [streams of the prefix cache]: rows of each prefix (more than its capacity: cut off there, and
+ *                VOX_ATTN_DEVICE_STATE raised)
  *   prefix_bound host-known upper bound of every prefix_len in use (sizes the grid and the workspace; 0: no prefix is read)
  *   lse          optional, [H, n_streams] f32: the natural log-sum-exp of every row's scores (-inf: nothing visible),
  *                which vox_kv_observe takes

@@ -772,6 +772,16 @@ def test_lengths_of_an_eviction_feed_the_next_call_directly(streams, shared, eng
         assert torch.equal(out, decode(cut))
 
 
+def test_a_prefix_longer_than_its_cache_is_reported(engine, pkg):
+    c = SharedCase(engine, pkg, ("f16", [0, 0], [20], [5, 9], 16, 2))
+    c.prefix_len.fill_(c.prefix.cfg.max_len + 1)
+    with pytest.raises(pkg.VoxError) as err:
+        c.run()
+        engine.sync_status()
+    assert err.value.status_name == "DEVICE_STATE"
+    engine.sync_status()
+
+
 # ----------------------------------------------------------------------------------------------------------------- refusals
 
 def test_refusals(engine, pkg):

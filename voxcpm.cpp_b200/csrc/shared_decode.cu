@@ -88,7 +88,8 @@ __device__ __forceinline__ Item load_item(const SharedParams & p) {
     w.prefix  = t.x;
     w.rows    = t.y * p.gqa;
     w.streams = p.members + (size_t) tile * p.per_tile;
-    const int len = t.y > 0 ? max(0, min(p.len[t.x], p.max_len)) : 0, n = (len + kKeys - 1) / kKeys;
+    const int given = t.y > 0 ? p.len[t.x] : 0, len = max(0, min(given, p.max_len)), n = (len + kKeys - 1) / kKeys;
+    if (given > p.max_len && threadIdx.x == 0) atomicOr(p.status, kStatusBadState);
     if (len == 0) w.rows = 0;
     w.key0 = (w.rank * n / p.cluster) * kKeys;
     w.key1 = min(len, ((w.rank + 1) * n / p.cluster) * kKeys);
