@@ -772,6 +772,27 @@ def test_lengths_of_an_eviction_feed_the_next_call_directly(streams, shared, eng
         assert torch.equal(out, decode(cut))
 
 
+def test_a_captured_call_outlives_a_larger_workspace(pkg):
+    """A graph captured with the engine's workspace is replayed after a larger call has made the engine take another one."""
+    import torch
+    engine = pkg.Engine(0)
+    c = SharedCase(engine, pkg, ("f16", [0, 0, 0], [300], [500, 9, 0], 16, 2))
+    want, lse = c.run()
+    dst, graph, side = torch.empty_like(want), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        c.run(dst=dst, lse=lse)
+    before = engine.workspace(0)
+    size, at = before.numel(), before.data_ptr()
+    del before
+    assert engine.workspace(size + 1).data_ptr() != at
+    others = [torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    assert all(o.data_ptr() >= at + size or o.data_ptr() + size <= at for o in others)
+    graph.replay()
+    engine.sync_status()
+    assert torch.equal(dst, want) and not any(bool(o.any()) for o in others)
+
+
 def test_a_prefix_longer_than_its_cache_is_reported(engine, pkg):
     c = SharedCase(engine, pkg, ("f16", [0, 0], [20], [5, 9], 16, 2))
     c.prefix_len.fill_(c.prefix.cfg.max_len + 1)

@@ -270,7 +270,7 @@ class Engine:
         _check(lib().vox_engine_create(device, C.byref(h)))
         self.h = h
         self.device = device
-        self._ws = None
+        self._ws, self._outgrown = None, []
         self._children = weakref.WeakSet()  # caches and groups created from this engine: they go before it does
 
     def close(self):
@@ -307,8 +307,13 @@ class Engine:
         _check(lib().vox_engine_selftest_wait(self.h, limit_cycles, _stream_ptr(stream)))
 
     def workspace(self, nbytes: int):
+        """The engine's workspace, for calls that are given none.  It grows; smaller ones before it stay allocated, since a
+        captured call may hold their addresses.  Calls that may run at the same time need workspaces of their own."""
         import torch
         if self._ws is None or self._ws.numel() < nbytes:
+            if self._ws is not None:
+                nbytes = max(nbytes, self._ws.numel() + min(self._ws.numel(), 64 << 20))
+                self._outgrown.append(self._ws)
             self._ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=f"cuda:{self.device}")
         return self._ws
 
@@ -542,7 +547,8 @@ class KVCache:
                       dst=None, k_new=None, v_new=None, cache_stable=False, rope_table=None, lse=None, workspace=None):
         """``vox_attn_decode_shared``: as ``decode``, over the rows of a prefix that several streams share and the streams' own.
         ``prefix``: the KVCache that holds the prefixes; ``plan``: a PrefixPlan; ``prefix_len`` int32 device [prefixes];
-        ``lse`` [n_streams, H] f32 receives the log-sum-exp.  Returns [n_streams, H, 64]."""
+        ``lse`` [n_streams, H] f32 receives the log-sum-exp; ``workspace``: a uint8 tensor (None: the engine's, for calls on
+        one stream).  Returns [n_streams, H, 64]."""
         S, H, D = q.shape
         if dst is None:
             dst = q.new_empty((S, H, D))
