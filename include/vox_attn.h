@@ -419,7 +419,7 @@ int    vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, 
  *   n_new      the last n_new rows of every stream are new: their score starts here, and row_pos[j] becomes
  *              n_seen - kv_len + j, the token's position in its stream
  *   score, row_pos  [max_len, HK, n_streams] f32 / int32 on the device, rows contiguous, strides nb_head, nb_stream in bytes
- *              (the same for both); row_pos may be NULL.  Rows at kv_len and beyond are left as they are.
+ *              (the same for both, no row list over another); row_pos may be NULL.  Rows at kv_len and beyond are left as they are.
  *   n_seen     device array [n_streams]: tokens every stream has seen, the new ones included (NULL: kv_len)
  *   kv_bound   host-known upper bound of every kv_len; a longer stream raises VOX_ATTN_DEVICE_STATE and is left alone
  * The same call gives the same bits.  workspace: vox_kv_observe_workspace_bytes (0 for most calls with n_q == 1), 16-byte

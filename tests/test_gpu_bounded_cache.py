@@ -867,6 +867,9 @@ def test_refusals(engine, pkg):
     refused("INVALID_ARGUMENT", "8-byte aligned", observe(q=randn(gen(0), 2, 1, 16, D + 1)[..., 1:]))
     refused("WORKSPACE_TOO_SMALL", "workspace", observe(n_q=2, workspace=torch.empty(8, dtype=torch.uint8, device="cuda")))
 
+    for view in (o.score[:, :1].expand(2, 2, -1), o.score[:1].expand(2, 2, -1), o.score.as_strided(o.score.shape, (o.score.stride(0), 4, 1))):
+        refused("INVALID_ARGUMENT", "rows overlap", observe(score=view))
+
     v = EvictCase(engine, pkg, "f16", [30, 20], 2, 2, 32)
     n2 = ints([0, 0])
 
@@ -879,6 +882,9 @@ def test_refusals(engine, pkg):
     refused("INVALID_ARGUMENT", "budget", evict(n_sink=2**31 - 1, n_recent=2**31 - 1))
     refused("INVALID_ARGUMENT", "layers", evict(layer0=1))
     refused("INVALID_ARGUMENT", "kv_bound", evict(kv_bound=33))
+    for dim in range(3):
+        score, pos = (x.narrow(dim, 0, 1).expand_as(x) for x in (v.score, v.row_pos))
+        refused("INVALID_ARGUMENT", "rows overlap", lambda: v.cache.evict(v.kv_len, 30, 10, score, pos, v.n_seen, n2, n_sink=0, n_recent=0))
     refused("INVALID_ARGUMENT", "overlap", evict(new_len=v.kv_len))
     refused("INVALID_ARGUMENT", "overlap", evict(new_len=v.n_seen))
     refused("INVALID_ARGUMENT", "overlap", evict(new_len=v.kv_len[1:]))

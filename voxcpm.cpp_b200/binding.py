@@ -553,7 +553,9 @@ class KVCache:
         if dst is None:
             dst = q.new_empty((S, H, D))
         q_s = q.stride()
-        n_s = k_new.stride() if k_new is not None else (0, 0)
+        n_s = k_new.stride() if k_new is not None else (0, 0, 1)
+        assert D == 64 and q_s[2] == n_s[2] == 1 and q.element_size() == kv_len.element_size() == 4
+        assert k_new is None or v_new is None or v_new.stride() == n_s
         own = DecodeArgs(self.h, layer, S, H, kv_len.data_ptr(), kv_bound, q.data_ptr(), q_s[1] * 4, q_s[0] * 4, dst.data_ptr(), scale,
                          _addr(k_new), _addr(v_new), n_s[1] * 4, n_s[0] * 4, 1 if cache_stable else 0, _addr(rope_table), None)
         a = DecodeSharedArgs(own, prefix.h if prefix is not None else None, plan.h if plan is not None else None, _addr(prefix_len),
@@ -569,7 +571,8 @@ class KVCache:
         (int32, the same shape and strides)."""
         S, n_q, H, D = q.shape
         q_s, s_s = q.stride(), score.stride()
-        assert s_s[-1] == 1 and (row_pos is None or row_pos.stride() == s_s)
+        assert D == 64 and q_s[3] == 1 and q.element_size() == kv_len.element_size() == score.element_size() == 4
+        assert s_s[2] == 1 and (row_pos is None or row_pos.stride() == s_s)
         a = ObserveArgs(self.h, layer, S, H, n_q, kv_len.data_ptr(), _addr(n_seen), kv_bound, q.data_ptr(), q_s[2] * 4, q_s[1] * 4, q_s[0] * 4,
                         _addr(rope_table), _addr(lse), scale, decay, n_new, score.data_ptr(), _addr(row_pos), s_s[-2] * 4, s_s[-3] * 4)
         L = lib()
@@ -581,6 +584,7 @@ class KVCache:
         [n_layers, n_streams, HK, budget], optional) the rows' former indices."""
         s_s = score.stride()
         assert s_s[3] == 1 and row_pos.stride() == s_s and (kept is None or kept.is_contiguous())
+        assert score.element_size() == row_pos.element_size() == kv_len.element_size() == new_len.element_size() == 4
         a = EvictArgs(self.h, layer0, score.shape[0], score.shape[1], kv_len.data_ptr(), _addr(n_seen), kv_bound, budget, n_sink, n_recent,
                       score.data_ptr(), row_pos.data_ptr(), s_s[2] * 4, s_s[1] * 4, s_s[0] * 4, new_len.data_ptr(), _addr(kept))
         st = _raw_stream(self.engine.device) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream

@@ -415,6 +415,10 @@ int check_evict(const vox_engine * e, const vox_kv_evict_args * a) {
     VOX_REQUIRE(((reinterpret_cast<uintptr_t>(a->score) | reinterpret_cast<uintptr_t>(a->row_pos) | reinterpret_cast<uintptr_t>(a->new_len) |
                   reinterpret_cast<uintptr_t>(a->kept)) & 3) == 0 && a->nb_head % 4 == 0 && a->nb_stream % 4 == 0 && a->nb_layer % 4 == 0,
                 VOX_ATTN_INVALID_ARGUMENT, "score, row_pos, new_len and kept must be 4-byte aligned");
+    const size_t row_bytes = (size_t) a->kv_bound * sizeof(float);
+    VOX_REQUIRE((c->cfg.n_kv_heads == 1 || a->nb_head >= row_bytes) && (a->n_streams == 1 || a->nb_stream >= row_bytes) &&
+                    (a->n_layers == 1 || a->nb_layer >= row_bytes),
+                VOX_ATTN_INVALID_ARGUMENT, "the scores of %d rows overlap (strides %zu, %zu, %zu bytes)", a->kv_bound, a->nb_head, a->nb_stream, a->nb_layer);
     VOX_REQUIRE((long long) a->n_layers * a->n_streams * c->cfg.n_kv_heads < (1LL << 31), VOX_ATTN_UNSUPPORTED, "more than 2^31 row lists in one call");
     return VOX_ATTN_OK;
 }

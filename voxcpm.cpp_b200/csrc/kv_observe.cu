@@ -315,6 +315,9 @@ int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
     VOX_REQUIRE(((reinterpret_cast<uintptr_t>(a->score) | reinterpret_cast<uintptr_t>(a->row_pos) | reinterpret_cast<uintptr_t>(a->lse)) & 3) == 0 &&
                     a->nb_head % 4 == 0 && a->nb_stream % 4 == 0,
                 VOX_ATTN_INVALID_ARGUMENT, "score, row_pos and lse must be 4-byte aligned");
+    const size_t row_bytes = (size_t) a->kv_bound * sizeof(float);
+    VOX_REQUIRE((c->cfg.n_kv_heads == 1 || a->nb_head >= row_bytes) && (a->n_streams == 1 || a->nb_stream >= row_bytes), VOX_ATTN_INVALID_ARGUMENT,
+                "the scores of %d rows overlap (strides %zu, %zu bytes)", a->kv_bound, a->nb_head, a->nb_stream);
     VOX_REQUIRE((long long) a->n_streams * c->cfg.n_kv_heads <= 65535, VOX_ATTN_UNSUPPORTED, "more than 65535 (stream, kv head) pairs in one call");
     return VOX_ATTN_OK;
 }
