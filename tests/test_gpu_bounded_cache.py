@@ -772,6 +772,61 @@ def test_lengths_of_an_eviction_feed_the_next_call_directly(streams, shared, eng
         assert torch.equal(out, decode(cut))
 
 
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("streams", [2, 40])
+def test_a_captured_step_follows_its_inputs(kind, streams, engine, pkg):
+    """Decode, the weights of a step and of a window, eviction and the next decode as one graph, each launch right behind the one whose
+    results it takes; replayed with other lengths and queries it gives what the calls give one at a time."""
+    import torch
+    rows, budget = 900, 500
+
+    def start(seed):
+        g = gen(seed)
+        c = new_cache(engine, pkg, kind, 1, streams, 2, rows)
+        c.append(0, randn(g, streams, c.cfg.max_len, 2, D), randn(g, streams, c.cfg.max_len, 2, D))
+        n = torch.randint(1, rows + 1, (streams,), generator=g, device="cuda", dtype=torch.int32)
+        return {"cache": c, "q": randn(g, streams, 16, D), "window": randn(g, streams, 20, 16, D), "n": n,
+                "score": torch.rand((1, streams, 2, rows + 4), generator=g, device="cuda"),
+                "pos": torch.arange(rows + 4, device="cuda", dtype=torch.int32).expand(1, streams, 2, -1).contiguous(),
+                "new": torch.full((streams,), 7, dtype=torch.int32, device="cuda"), "lse": torch.zeros((streams, 16), device="cuda"),
+                "ws": torch.zeros(1 << 24, dtype=torch.uint8, device="cuda")}
+
+    def step(s, wait):
+        def then():
+            if wait:
+                engine.sync_status()
+        c, out = s["cache"], []
+        out.append(c.decode_shared(0, s["q"], s["n"], rows, lse=s["lse"], workspace=s["ws"])); then()
+        c.observe(0, s["q"][:, None], s["n"], rows, s["score"][0], row_pos=s["pos"][0], lse=s["lse"], workspace=s["ws"]); then()
+        c.observe(0, s["window"], s["n"], rows, s["score"][0], n_new=0, workspace=s["ws"]); then()
+        c.evict(s["n"], rows, budget, s["score"], s["pos"], None, s["new"]); then()
+        c.observe(0, s["window"], s["new"], rows, s["score"][0], n_new=0, decay=0.5, workspace=s["ws"]); then()
+        c.observe(0, s["q"][:, None], s["new"], rows, s["score"][0], n_new=0, workspace=s["ws"]); then()
+        out.append(c.decode_shared(0, s["q"], s["new"], rows, lse=s["lse"], workspace=s["ws"])); then()
+        return out
+
+    captured = start(0)
+    step(captured, True)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        out = step(captured, False)
+    for seed in (1, 2, 3):
+        fresh, refill = start(seed), start(seed)
+        want = step(fresh, True)
+        for name in ("q", "window", "n", "score", "pos", "lse"):
+            captured[name].copy_(refill[name])
+        captured["new"].fill_(3)
+        g = gen(seed)
+        captured["cache"].append(0, randn(g, streams, fresh["cache"].cfg.max_len, 2, D), randn(g, streams, fresh["cache"].cfg.max_len, 2, D))
+        torch.cuda.synchronize()
+        graph.replay()
+        engine.sync_status()
+        assert torch.equal(captured["new"], fresh["new"]) and torch.equal(captured["pos"], fresh["pos"])
+        assert torch.equal(captured["score"], fresh["score"]) and torch.equal(captured["lse"], fresh["lse"])
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_a_captured_call_outlives_a_larger_workspace(pkg):
     """A graph captured with the engine's workspace is replayed after a larger call has made the engine take another one."""
     import torch
