@@ -6,13 +6,14 @@
 // rows move in place and in any order.
 //
 // One CTA per row list, keys in shared memory.  The border between what stays and what goes is found by a histogram of the
-// keys' top 11 bits (sign, exponent and two bits of the mantissa: a bin is a quarter of an octave) and, as a rule, by ranking the few
-// hundred keys of the bin it falls in against one another; only a bin with more keys than that (many equal scores) is cut
-// further, 11 and 10 bits at a time.  Lists are few when one stream is cut: then a cluster of CTAs takes each, every CTA
+// keys' top 11 bits (sign, exponent and two bits of the mantissa: a bin is a quarter of an octave) and, as a rule, by ranking the
+// keys of the bin it falls in against one another; only a bin with more keys than threads (many equal scores) is cut further, 11 and
+// 10 bits at a time.  Lists are few when one stream is cut: then a cluster of CTAs takes each, every CTA
 // selecting for itself (the scores are in L2) and moving a share of the rows.
-// 1440 lists of up to 2048 f16 rows cut to 512 (194 MB read and written): 48 us, 4.0 TB/s, bound by the chain of phases of a CTA and by
-// what unequal lists leave idle (one round of CTAs and a part); 128, 192 and 512 threads, and fewer CTAs with more loads in flight,
-// came out equal or slower.  Six lists of 300 rows: 10 us, latency.
+// 1440 lists of up to 2048 f16 rows cut to 512 (194 MB read and written): 48 us, 4.0 TB/s.  The rows move at HBM's rate (29 us); what
+// comes before is a chain of short phases (keys 9, border 5, places 4 us, over one round of CTAs and a part); 128, 192 and 512 threads,
+// and fewer CTAs with more loads in flight, came out equal or slower.  Six lists of 300 rows: 6 us, latency (10 us when a bin of more than
+// 96 keys took another histogram and the others were ranked a key at a time).
 #include "kv_cache.cuh"
 
 #include <algorithm>
@@ -25,7 +26,7 @@ constexpr int kThreads   = 256;
 constexpr int kWarps     = kThreads / 32;
 constexpr int kBits      = 11;
 constexpr int kBins      = 1 << kBits;
-constexpr int kRanked    = 96;       // keys of a bin that are ranked against one another
+constexpr int kRanked    = kThreads; // keys of a bin that are ranked against one another, one of a thread
 constexpr int kMaxRows   = 49152;    // rows are numbered in 16 bits in the lists of moving rows
 constexpr size_t kSmemMost = 200 * 1024;  // keys that fit stay in shared memory; those of longer row lists are made again
 constexpr int kMaxCluster = 8;
@@ -91,8 +92,9 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t (*warp_sums)
 }
 
 __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p) {
-    extern __shared__ uint32_t smem[];  // keys (if they are kept), then sources and destinations of the rows that move
-    __shared__ uint32_t hist[kBins], warp_sums[2][kWarps], found[3];
+    extern __shared__ __align__(16) uint32_t smem[];  // keys (if they are kept), then sources and destinations of the rows that move
+    __shared__ __align__(16) uint32_t hist[kBins];
+    __shared__ uint32_t warp_sums[2][kWarps], found[3];
     uint32_t * const keys = smem;
     uint16_t * const src  = reinterpret_cast<uint16_t *>(smem + (p.keys_kept ? (p.kv_bound + 3) / 4 * 4 : 0)), * const dst = src + p.n_list;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -140,11 +142,11 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
     int      last = len, need = p.budget;
     for (int shift = 32 - kBits;;) {
         // the bin, from the top, in which the count reaches `need`
-        const int bits = min(kBits, 32 - __popc(mask)), bins = 1 << bits, per = max(1, bins / kThreads);
-        const int top  = bins - 1 - tid * per;
-        uint32_t  mine = 0, total;
-        if (top >= 0)
-            for (int i = 0; i < per; ++i) mine += hist[top - i];
+        constexpr int kPer = kBins / kThreads;  // (fewer bins: the others are zeros)
+        static_assert(kPer == 8, "two vectors of a thread");
+        const int bits = min(kBits, 32 - __popc(mask)), bins = 1 << bits, top = kBins - 1 - tid * kPer;
+        const uint4 b0 = *reinterpret_cast<const uint4 *>(hist + top - 7), b1 = *reinterpret_cast<const uint4 *>(hist + top - 3);
+        uint32_t  mine = (b0.x + b0.y) + (b0.z + b0.w) + (b1.x + b1.y) + (b1.z + b1.w), total;
         uint32_t before = block_scan(mine, warp_sums, turn, total);
         if (before < (uint32_t) need && before + mine >= (uint32_t) need) {
             int bin = top;
@@ -181,25 +183,32 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
         }
         __syncthreads();
         if (n_bin <= kRanked) {  // rank the keys of the bin against one another; the histogram's memory holds them
-            uint32_t * const bin_key = hist, * const bin_row = hist + kRanked;
-            if (tid == 0) found[2] = 0;
+            // a key, and of equal ones the lower index first, as one number; none is 0, which fills the last pair
+            unsigned long long * const of_bin = reinterpret_cast<unsigned long long *>(hist);
+            if (tid == 0) {
+                found[2] = 0;
+                of_bin[n_bin] = 0;
+            }
             __syncthreads();
             for (int j = tid; j < len; j += kThreads) {
                 const uint32_t k = key_of(j);
                 if ((k & mask) == edge) {
                     const uint32_t i = atomicAdd(&found[2], 1u);
-                    bin_key[i] = k;
-                    bin_row[i] = (uint32_t) j;
+                    of_bin[i] = (unsigned long long) k << 32 | (0xffffffffu - (uint32_t) j);
                 }
             }
             __syncthreads();
-            for (int i = tid; i < n_bin; i += kThreads) {
-                const uint32_t k = bin_key[i], j = bin_row[i];
-                int            above = 0;
-                for (int o = 0; o < n_bin; ++o) above += bin_key[o] > k || (bin_key[o] == k && bin_row[o] < j);
+            if (tid < n_bin) {
+                const unsigned long long own = of_bin[tid];
+                int                      above = 0;
+#pragma unroll 4
+                for (int o = 0; o < n_bin; o += 2) {
+                    const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(of_bin + o);
+                    above += (x.x > own) + (x.y > own);
+                }
                 if (above == need - 1) {  // the last one that stays
-                    found[0] = k;
-                    found[1] = j;
+                    found[0] = (uint32_t) (own >> 32);
+                    found[1] = 0xffffffffu - (uint32_t) own;
                 }
             }
             __syncthreads();
@@ -208,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
             break;
         }
         const int next = max(0, shift - kBits), width = shift - next;
-        for (int i = tid; i < (1 << width); i += kThreads) hist[i] = 0;
+        for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
         __syncthreads();
         for (int j = tid; j < len; j += kThreads) {
             const uint32_t k = key_of(j);
@@ -222,11 +231,15 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
     uint32_t marks = 0;  // places in the low half, rows in the high half
     for (int j0 = 0; j0 < len; j0 += 4 * kThreads) {
         const int j = j0 + 4 * tid;
-        uint32_t  flags = 0, count = 0, n;
+        uint32_t  flags = 0, count = 0, n, four[4];
+        if (p.keys_kept && j < len) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(keys + j);
+            four[0] = x.x; four[1] = x.y; four[2] = x.z; four[3] = x.w;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (j + e >= len) continue;
-            const uint32_t k = key_of(j + e);
+            const uint32_t k = p.keys_kept ? four[e] : make_key(j + e);
             const bool     stays = k > edge || (k == edge && j + e <= last), low = j + e < p.budget;
             if (stays != low) {
                 flags |= 1u << e;
