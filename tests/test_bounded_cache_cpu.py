@@ -29,3 +29,33 @@ def test_size_queries_of_nothing(pkg, L):
     assert L.vox_attn_decode_shared_workspace_bytes(C.byref(pkg.DecodeSharedArgs())) == 0
     assert L.vox_kv_observe_workspace_bytes(None) == 0
     assert L.vox_kv_observe_workspace_bytes(C.byref(pkg.ObserveArgs())) == 0
+
+
+@pytest.mark.parametrize("name", ["DecodeSharedArgs", "ObserveArgs", "EvictArgs"])
+def test_packed_argument_blocks_are_the_structures(pkg, name):
+    """The bytes that the binding packs are those of the ctypes structure with the same values."""
+    cls = getattr(pkg, name)
+
+    def fill(c, values):
+        x = c()
+        for field, t in c._fields_:
+            if issubclass(t, C.Structure):
+                setattr(x, field, fill(t, values))
+            else:
+                values.append(len(values) + (0.25 if t is C.c_float else 3))
+                setattr(x, field, values[-1])
+        return x
+    values = []
+    want = fill(cls, values)
+    binding = __import__("sys").modules[pkg.__name__ + ".binding"]
+    got = cls.from_buffer_copy(binding._packer(cls)(*values))
+
+    def same(a, b):
+        for field, t in a._fields_:
+            x, y = getattr(a, field), getattr(b, field)
+            same(x, y) if issubclass(t, C.Structure) else _equal(x, y)
+    same(got, want)
+
+
+def _equal(x, y):
+    assert x == y
