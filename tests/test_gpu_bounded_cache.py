@@ -361,6 +361,12 @@ OBSERVE = {  # kind, lengths, n_q, heads, kv heads
     "three heads, odd window": ("f16", [90, 600], 7, 9, 3),
     "q8_0 window": ("q8_0", [17, 64, 700], 17, 16, 2),
     "q8_0 largest window": ("q8_0", [1000], 64, 16, 2),
+    "few rows": ("f16", [0, 1, 3, 4, 511, 514, 4700], 4, 16, 2),
+    "few rows, one head each": ("f16", [40, 600, 3000, 1], 64, 4, 4),
+    "few rows, more queries than rows": ("f16", [3, 0, 9, 700], 10, 6, 1),
+    "q8_0 few rows": ("q8_0", [0, 2, 17, 64, 700, 1300], 3, 16, 2),
+    "q8_0 few rows, six heads": ("q8_0", [130, 5, 2100], 10, 6, 1),
+    "nine heads, just too many rows": ("f16", [130, 700], 22, 9, 3),
 }
 
 
@@ -431,6 +437,12 @@ def test_weights_of_many_long_streams(kind, streams, rows, given_lse, engine, pk
     """Enough keys for a block to take several chunks of a stream one after the other: lengths on both sides of every chunk's end."""
     lens = [min(rows, max(0, 512 * (i % 11) + (0, 1, -1, 64, 257)[i % 5])) for i in range(streams - 2)] + [rows, rows - 1]
     ObserveCase(engine, pkg, (kind, lens, 1, 4, 2), given_lse=given_lse).check(decay=0.5)
+
+
+@pytest.mark.parametrize("kind,streams,rows", [("f16", 128, 4700), ("q8_0", 64, 9300)])
+def test_few_query_rows_over_many_long_streams(kind, streams, rows, engine, pkg):
+    lens = [min(rows, max(0, 512 * (i % 11) + (0, 1, -1, 64, 257)[i % 5])) for i in range(streams - 2)] + [rows, rows - 1]
+    ObserveCase(engine, pkg, (kind, lens, 3, 4, 2)).check(n_new=2, decay=0.5)
 
 
 @pytest.mark.parametrize("n_new", [0, 3, 1000])

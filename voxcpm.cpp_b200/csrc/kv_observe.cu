@@ -25,6 +25,7 @@ constexpr int kThreads   = kWarps * 32;
 constexpr int kWarpKeys  = 64;                  // keys a warp keeps as operands
 constexpr int kChunk     = kWarps * kWarpKeys;  // keys of a CTA
 constexpr int kMaxGroup  = 8;                   // query heads of a kv head
+constexpr int kFewRows    = 64;                  // query rows of a group up to which a window is taken here
 constexpr int kMaxCluster = 8;
 constexpr int kMaxRun     = 6;                   // chunks of a CTA of a cluster: the scores of two CTAs fit an SM
 
@@ -128,6 +129,28 @@ __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
 // as the weights take them: (max, 1 / sum); a row that saw nothing adds nothing
 __device__ __forceinline__ float2 as_weights(float2 s) { return s.y == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(s.x, 1.0f / s.y); }
 
+// A warp's 64 keys from `from` on: the weights w (of keys 8n + 2t + e, n and e the index's parts, by the row g of this lane) are added up
+// over the rows and go to the scores.  Halving the keys as it halves the rows: lane (g, t) ends with keys 2t and 2t + 1 of tile g (14
+// shuffles; each sum by itself in every lane would be 48).
+__device__ __forceinline__ void add_weights(const ObserveParams & p, float (&w)[16], float * score, int32_t * row_pos, int stream, int len, int from,
+                                            const float (&old)[2], int g, int t) {
+    static_assert(kWarpKeys == 64, "a tile of keys to a row of lanes");
+#pragma unroll
+    for (int half = 8; half >= 2; half >>= 1) {
+        const bool upper = g & (half >> 1);
+#pragma unroll
+        for (int n = 0; n < half; ++n) w[n] = (upper ? w[n + half] : w[n]) + __shfl_xor_sync(0xffffffffu, upper ? w[n] : w[n + half], 2 * half);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int key = from + 8 * g + 2 * t + e;
+        if (key >= len) break;
+        const bool fresh = key >= len - p.n_new;
+        score[key] = fresh ? w[e] : fmaf(p.decay, old[e], w[e]);
+        if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
+    }
+}
+
 template <bool Q8, int kMode>
 __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParams p) {
     extern __shared__ float4 kept_scores[];  // kCluster: [chunk][4][thread], of all chunks of a CTA but the last
@@ -179,26 +202,10 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
     if (kMode == kGiven || kMode == kJoin) __syncthreads();
     int32_t * const row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
     auto write = [&](const float (&sc)[kWarpKeys / 8][2], float2 st, int from, const float (&old)[2]) {
-        // the sums over the rows of the group, g: halving the keys as it halves the rows, so that lane (g, t) ends with keys 2t and
-        // 2t + 1 of tile g (14 shuffles; each sum by itself in every lane would be 48)
-        static_assert(kWarpKeys == 64, "a tile of keys to a row of lanes");
         float w[16];
 #pragma unroll
         for (int n = 0; n < 16; ++n) w[n] = ex2_approx(sc[n >> 1][n & 1] - st.x) * st.y;
-#pragma unroll
-        for (int half = 8; half >= 2; half >>= 1) {
-            const bool upper = g & (half >> 1);
-#pragma unroll
-            for (int n = 0; n < half; ++n) w[n] = (upper ? w[n + half] : w[n]) + __shfl_xor_sync(0xffffffffu, upper ? w[n] : w[n + half], 2 * half);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int key = from + 8 * g + 2 * t + e;
-            if (key >= len) break;
-            const bool fresh = key >= len - p.n_new;
-            score[key] = fresh ? w[e] : fmaf(p.decay, old[e], w[e]);
-            if (fresh && row_pos != nullptr) row_pos[key] = (p.n_seen ? p.n_seen[stream] : len) - len + key;
-        }
+        add_weights(p, w, score, row_pos, stream, len, from, old, g, t);
     };
     float m = -INFINITY, l = 0.0f;  // kFind, kCluster: of the row's keys in this lane
     for (int n_kept = 0;; first += kChunk) {
@@ -293,6 +300,127 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
     }
 }
 
+// A window of few query rows (at most kFewRows, queries times the heads of a group): as above, with the rows in groups of eight.  A
+// warp's keys stay in its registers while the groups' operands come from shared memory one after the other.  Two launches: the
+// rows' (max, sum) over every CTA's keys, and the weights.
+template <bool Q8, bool kWeights>
+__global__ void __launch_bounds__(kThreads, 2) observe_rows_kernel(const ObserveParams p) {
+    __shared__ uint4  q_op[kFewRows / 8][4][32];
+    __shared__ float2 row_stat[kFewRows], warp_stat[kWarps][kFewRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int chunk = blockIdx.x, kvh = blockIdx.y % p.n_kv_heads, stream = blockIdx.y / p.n_kv_heads;
+    const int rows = p.n_q * p.gqa, n_groups = (rows + 7) >> 3;
+    // (the second launch reads one thing that the first has written, the statistics: it waits for them alone)
+    if (!kWeights) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
+    const int len = p.kv_len[stream], first0 = chunk * p.run * kChunk, end = min(len, first0 + p.run * kChunk);
+    if (len > p.kv_bound || first0 >= len) {
+        if (kWeights) pdl_wait();  // no launch of the next call ends before the first one of this call
+        else if (len > p.kv_bound && tid == 0 && kvh == 0 && chunk == 0) atomicOr(p.status, kStatusBadState);
+        return;
+    }
+    int             first = first0 + warp * kWarpKeys;
+    KeyTile<Q8>     keys[kWarpKeys / 8];
+    const uint8_t * pair = p.k + (size_t) stream * p.k_nb_stream + (size_t) kvh * p.k_nb_head;
+    float * const   score = reinterpret_cast<float *>(p.score + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head);
+    int32_t * const row_pos = p.row_pos ? reinterpret_cast<int32_t *>(p.row_pos + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head) : nullptr;
+    auto ask = [&](int from) {
+#pragma unroll
+        for (int n = 0; n < kWarpKeys / 8; ++n) keys[n] = load_keys<Q8>(pair, from + 8 * n + g, t, from + 8 * n + g < len);
+    };
+    ask(first);
+    for (int i = warp; i < n_groups; i += kWarps) {
+        const int     row = 8 * i + g, at = min(row, rows - 1), q = (int) ((uint32_t) at * p.gqa_magic >> 16);
+        const float * src = reinterpret_cast<const float *>(p.q + (size_t) stream * p.q_nb_stream + (size_t) q * p.q_nb_tok +
+                                                            (size_t) (kvh * p.gqa + at - q * p.gqa) * p.q_nb_head);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float2 a = *reinterpret_cast<const float2 *>(src + step_d(c, t)), b = *reinterpret_cast<const float2 *>(src + step_d(c, t) + 2);
+            const float  x[4] = {a.x, a.y, b.x, b.y};
+            float        h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split_hi_lo(row < rows ? x[e] * p.scale_log2 : 0.0f, h[e], l[e]);
+            q_op[i][c][lane] = make_uint4(pack_half2(h[0], h[1]), pack_half2(l[0], l[1]), pack_half2(h[2], h[3]), pack_half2(l[2], l[3]));
+        }
+    }
+    if (kWeights) {
+        pdl_wait();
+        pdl_launch_dependents();
+        if (tid < kFewRows) {
+            const float2 * all = p.stats + (size_t) blockIdx.y * gridDim.x * rows + tid;
+            float2         s = make_float2(-INFINITY, 0.0f);
+            if (tid < rows)
+#pragma unroll 4
+                for (int c = 0; c * p.run * kChunk < len; ++c) s = join_stats(s, __ldcg(all + (size_t) c * rows));
+            row_stat[tid] = as_weights(s);
+        }
+    } else if (t == 0) {
+        for (int i = 0; i < n_groups; ++i) warp_stat[warp][8 * i + g] = make_float2(-INFINITY, 0.0f);
+    }
+    __syncthreads();
+    for (;; first += kChunk) {
+        const bool cut = first + kWarpKeys > len - p.n_q;  // keys that not every query sees, and keys past the end
+        float      w[16], old[2] = {0.0f, 0.0f};
+        if (kWeights) {
+#pragma unroll
+            for (int n = 0; n < 16; ++n) w[n] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (first + 8 * g + 2 * t + e < len - p.n_new) old[e] = score[first + 8 * g + 2 * t + e];
+        }
+#pragma unroll 1
+        for (int i = 0; i < n_groups; ++i) {
+            uint32_t q[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint4 x = q_op[i][c][lane];
+                q[c][0] = x.x; q[c][1] = x.y; q[c][2] = x.z; q[c][3] = x.w;
+            }
+            float sc[kWarpKeys / 8][2];
+#pragma unroll
+            for (int n = 0; n < kWarpKeys / 8; ++n) score_tile<Q8>(sc[n], q, keys[n], lane);
+            if (cut) {
+                const int last = len - p.n_q + (int) ((uint32_t) (8 * i + g) * p.gqa_magic >> 16) - first - 2 * t;
+#pragma unroll
+                for (int n = 0; n < 16; ++n)
+                    if (8 * (n >> 1) + (n & 1) > last) sc[n >> 1][n & 1] = -INFINITY;
+            }
+            if (kWeights) {
+                const float2 st = row_stat[8 * i + g];
+#pragma unroll
+                for (int n = 0; n < 16; ++n) w[n] = fmaf(ex2_approx(sc[n >> 1][n & 1] - st.x), st.y, w[n]);
+            } else {
+                float m = -INFINITY, l = 0.0f;
+#pragma unroll
+                for (int n = 0; n < kWarpKeys / 8; ++n) m = fmaxf(m, fmaxf(sc[n][0], sc[n][1]));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int n = 0; n < 16; ++n) l += ex2_approx(sc[n >> 1][n & 1] - ref);
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                if (t == 0) warp_stat[warp][8 * i + g] = join_stats(warp_stat[warp][8 * i + g], make_float2(m, l));
+            }
+        }
+        const bool more = first + kChunk < end;
+        if (more) ask(first + kChunk);
+        if (kWeights) add_weights(p, w, score, row_pos, stream, len, first, old, g, t);
+        if (!more) break;
+    }
+    if (!kWeights) {
+        __syncthreads();
+        if (tid < rows) {
+            float2 s = warp_stat[0][tid];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) s = join_stats(s, warp_stat[w][tid]);
+            p.stats[((size_t) blockIdx.y * gridDim.x + chunk) * rows + tid] = s;
+        }
+    }
+}
+
 int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
     VOX_REQUIRE(e && a && a->cache && a->q && a->score && a->kv_len, VOX_ATTN_INVALID_ARGUMENT, "vox_kv_observe: null argument");
     const vox_kv_cache * c = a->cache;
@@ -323,6 +451,17 @@ int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
 }
 
 int chunks_of(int kv_bound) { return (std::max(kv_bound, 1) + kChunk - 1) / kChunk; }
+bool few_rows(const vox_kv_observe_args * a) { return a->n_heads / a->cache->cfg.n_kv_heads * a->n_q <= kFewRows; }
+
+template <bool Q8>
+int launch_rows(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
+    const dim3 grid((unsigned) ((p.n_chunks + p.run - 1) / p.run), (unsigned) (p.n_streams * p.n_kv_heads));
+    launch_pdl(observe_rows_kernel<Q8, false>, grid, dim3(kThreads), 0, st, p);
+    const int rc = check_launch(e, "observe_rows_kernel<statistics>");
+    if (rc != VOX_ATTN_OK) return rc;
+    launch_pdl(observe_rows_kernel<Q8, true>, grid, dim3(kThreads), 0, st, p);
+    return check_launch(e, "observe_rows_kernel<weights>");
+}
 
 template <bool Q8>
 int launch_observe(vox_engine * e, const ObserveParams & p, cudaStream_t st) {
@@ -365,6 +504,7 @@ extern "C" {
 size_t vox_kv_observe_workspace_bytes(const vox_kv_observe_args * a) {
     if (a == nullptr || a->cache == nullptr || a->n_streams <= 0 || a->n_heads <= 0 || a->n_q <= 0 || a->kv_bound < 0 || a->lse != nullptr) return 0;
     const int HK = a->cache->cfg.n_kv_heads;
+    if (a->n_q > 1 && few_rows(a)) return (size_t) a->n_streams * a->n_heads * a->n_q * chunks_of(a->kv_bound) * sizeof(float2);
     if (a->n_q > 1) return observe_window_bytes(a->n_streams, HK, a->n_heads / HK * a->n_q, a->kv_bound);
     const int chunks = chunks_of(a->kv_bound);
     return chunks <= kMaxCluster * kMaxRun ? 0 : (size_t) a->n_streams * a->n_heads * chunks * sizeof(float2);
@@ -400,7 +540,7 @@ int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspa
     // one round of all CTAs, if they fit (1 / 4 / 6 chunks 86.7 / 53.4 / 53.4 us; 64 streams 1 / 4 chunks 23.8 / 15.9 us), and what
     // eight CTAs need.
     const long long chunks  = (long long) p.n_chunks * a->n_streams * p.n_kv_heads, slots = 2LL * e->sm_count;
-    const bool      cluster = p.lse == nullptr && p.n_chunks <= kMaxCluster * kMaxRun;
+    const bool      cluster = p.n_q == 1 && p.lse == nullptr && p.n_chunks <= kMaxCluster * kMaxRun;
     const int       most    = cluster ? std::max((p.n_chunks + kMaxCluster - 1) / kMaxCluster, (int) std::min<long long>(kMaxRun, (chunks + slots - 1) / slots))
                                       : (int) std::max(1LL, std::min<long long>(8, chunks / (2 * slots)));
     const int       ctas    = (p.n_chunks + most - 1) / most;
@@ -408,6 +548,7 @@ int vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * workspa
     p.stats = static_cast<float2 *>(workspace);
     p.status = e->status_dev;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->n_q > 1 && few_rows(a)) return q8 ? launch_rows<true>(e, p, st) : launch_rows<false>(e, p, st);
     if (a->n_q > 1) return launch_observe_window(e, c, p, st);
     return q8 ? launch_observe<true>(e, p, st) : launch_observe<false>(e, p, st);
 }
