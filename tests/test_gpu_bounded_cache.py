@@ -443,6 +443,8 @@ def test_weights_of_many_long_streams(kind, streams, rows, given_lse, engine, pk
 def test_few_query_rows_over_many_long_streams(kind, streams, rows, engine, pkg):
     lens = [min(rows, max(0, 512 * (i % 11) + (0, 1, -1, 64, 257)[i % 5])) for i in range(streams - 2)] + [rows, rows - 1]
     ObserveCase(engine, pkg, (kind, lens, 3, 4, 2)).check(n_new=2, decay=0.5)
+    ObserveCase(engine, pkg, (kind, lens, 46, 4, 2)).check(n_new=46)
+    ObserveCase(engine, pkg, (kind, lens, 49, 4, 2)).check(n_new=46)
 
 
 @pytest.mark.parametrize("n_new", [0, 3, 1000])

@@ -25,7 +25,7 @@ constexpr int kThreads   = kWarps * 32;
 constexpr int kWarpKeys  = 64;                  // keys a warp keeps as operands
 constexpr int kChunk     = kWarps * kWarpKeys;  // keys of a CTA
 constexpr int kMaxGroup  = 8;                   // query heads of a kv head
-constexpr int kFewRows    = 64;                  // query rows of a group up to which a window is taken here
+constexpr int kFewRows    = 96;                  // query rows of a kv head up to which a window is taken here
 constexpr int kMaxCluster = 8;
 constexpr int kMaxRun     = 6;                   // chunks of a CTA of a cluster: the scores of two CTAs fit an SM
 
@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
 
 // A window of few query rows (at most kFewRows, queries times the heads of a group): as above, with the rows in groups of eight.  A
 // warp's keys stay in its registers while the groups' operands come from shared memory one after the other.  Two launches: the
-// rows' (max, sum) over every CTA's keys, and the weights.
+// rows' (max, sum) over every CTA's keys, and the weights.  Bound by the rows: 0.3 us a group and launch where nothing else runs, the
+// issue of products and exponentials where much does (128 streams of 4096 rows, 4 queries of 8 heads: 60 us, of which K twice
+// from HBM or L2 would be 28; q8_0, whose bytes are converted for every group, 86 us).
 template <bool Q8, bool kWeights>
 __global__ void __launch_bounds__(kThreads, 2) observe_rows_kernel(const ObserveParams p) {
     __shared__ uint4  q_op[kFewRows / 8][4][32];
@@ -451,7 +453,15 @@ int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
 }
 
 int chunks_of(int kv_bound) { return (std::max(kv_bound, 1) + kChunk - 1) / kChunk; }
-bool few_rows(const vox_kv_observe_args * a) { return a->n_heads / a->cache->cfg.n_kv_heads * a->n_q <= kFewRows; }
+// Windows of few query rows are this file's: up to 40 rows, or 96 where there is work for more than two rounds of CTAs (the kernel for
+// the others takes a pair or a part of one per SM, with nothing beside it to hide its latency).  24 / 48 / 64 / 96 / 128 rows, f16:
+// 4 streams of 4096 rows 9.8 / 13.0 / 15.6 / 20.3 / 25.1 us against 13.9 / 13.9 / 13.9 / 14.5 / 14.5 us there; 128 streams of
+// 2048 rows 35 / 49 / 59 / 80 / 100 against 74 / 74 / 74 / 83 / 84 us.  q8_0: 11.8 / 16.8 / 19.9 / 26.2 / 32.3 against 18.6 / 18.8 /
+// 18.6 / 19.3 / 19.5 us, and 46 / 66 / 79 / 108 / 135 against 113 / 114 / 114 / 125 / 126 us.
+bool few_rows(const vox_kv_observe_args * a) {
+    const int HK = a->cache->cfg.n_kv_heads;
+    return a->n_heads / HK * a->n_q <= ((long long) chunks_of(a->kv_bound) * a->n_streams * HK > 4LL * a->cache->e->sm_count ? kFewRows : 40);
+}
 
 template <bool Q8>
 int launch_rows(vox_engine * e, const ObserveParams & p, cudaStream_t st) {

@@ -1,4 +1,4 @@
-// vox_kv_observe: what its kernels share.  One query per stream: kv_observe.cu; a window of queries: kv_observe_window.cu.
+// vox_kv_observe: what its kernels share.  One query per stream, windows of few query rows: kv_observe.cu; others: kv_observe_window.cu.
 #pragma once
 
 #include "kv_cache.cuh"
