@@ -472,6 +472,24 @@ def test_weights_with_a_rotary_table_and_strided_queries(engine, pkg):
     assert bool(((c.score.double() - score).abs() <= WEIGHT * score.abs() + 1e-9).all())
 
 
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("n_q", [1, 3, 20])
+def test_a_query_of_nan_touches_the_keys_it_sees(n_q, kind, engine, pkg):
+    """Weights of a NaN query are NaN for the keys that it sees; later keys and other streams have the others' weights."""
+    import torch
+    c = ObserveCase(engine, pkg, (kind, [200, 700, 5], n_q, 16, 2))
+    score, _ = c.want(1, 1.0)
+    c.q[1, 0] = float("nan")
+    seen = 700 - n_q + 1  # rows that the first query sees
+    c.run()
+    engine.sync_status()
+    assert bool(c.score[1, :, :seen].isnan().all()) and not bool(c.score[1, :, seen:].isnan().any())
+    for s in (0, 2):
+        assert bool(((c.score[s].double() - score[s]).abs() <= WEIGHT * score[s].abs() + 1e-9).all())
+    later = slice(seen, None)  # rows that the first query does not see: they never had its weight
+    assert bool(((c.score[1, :, later].double() - score[1, :, later]).abs() <= WEIGHT * score[1, :, later].abs() + 1e-9).all())
+
+
 def test_weights_of_every_stream_add_up_to_its_heads(engine, pkg):
     """Over a whole softmax the weights of a query sum to one: 8 heads give 8 per kv head."""
     c = ObserveCase(engine, pkg, ("f16", [700, 64, 9], 1, 16, 2))

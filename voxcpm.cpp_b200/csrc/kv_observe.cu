@@ -383,16 +383,22 @@ __global__ void __launch_bounds__(kThreads, 2) observe_rows_kernel(const Observe
             float sc[kWarpKeys / 8][2];
 #pragma unroll
             for (int n = 0; n < kWarpKeys / 8; ++n) score_tile<Q8>(sc[n], q, keys[n], lane);
+            const int last = len - p.n_q + (int) ((uint32_t) (8 * i + g) * p.gqa_magic >> 16) - first - 2 * t;
             if (cut) {
-                const int last = len - p.n_q + (int) ((uint32_t) (8 * i + g) * p.gqa_magic >> 16) - first - 2 * t;
 #pragma unroll
                 for (int n = 0; n < 16; ++n)
                     if (8 * (n >> 1) + (n & 1) > last) sc[n >> 1][n & 1] = -INFINITY;
             }
             if (kWeights) {
                 const float2 st = row_stat[8 * i + g];
+                if (cut) {  // (the sum of a row that does not see a key may be NaN)
 #pragma unroll
-                for (int n = 0; n < 16; ++n) w[n] = fmaf(ex2_approx(sc[n >> 1][n & 1] - st.x), st.y, w[n]);
+                    for (int n = 0; n < 16; ++n)
+                        if (8 * (n >> 1) + (n & 1) <= last) w[n] = fmaf(ex2_approx(sc[n >> 1][n & 1] - st.x), st.y, w[n]);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) w[n] = fmaf(ex2_approx(sc[n >> 1][n & 1] - st.x), st.y, w[n]);
+                }
             } else {
                 float m = -INFINITY, l = 0.0f;
 #pragma unroll

@@ -416,11 +416,11 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                             const float4 * st4 = reinterpret_cast<const float4 *>(row_stat + kSub * i + h);
 #pragma unroll
                             for (int e = 0; e < 32; e += 2) {
-                                const float4 q = st4[e >> 1];  // two rows' (max, 1 / sum), the same for all threads
+                                float4 q = st4[e >> 1];  // two rows' (max, 1 / sum), the same for all threads
                                 float        a = ex2_approx(__uint_as_float(r[e]) - q.x), c = ex2_approx(__uint_as_float(r[e + 1]) - q.z);
-                                if (cut) {
-                                    if (kSub * i + h + e < hidden) a = 0.0f;
-                                    if (kSub * i + h + e + 1 < hidden) c = 0.0f;
+                                if (cut) {  // (the sum of a row that does not see the key may be NaN)
+                                    if (kSub * i + h + e < hidden) a = q.y = 0.0f;
+                                    if (kSub * i + h + e + 1 < hidden) c = q.w = 0.0f;
                                 }
                                 sum = fmaf(a, q.y, sum);
                                 s1  = fmaf(c, q.w, s1);
