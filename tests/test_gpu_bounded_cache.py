@@ -607,6 +607,20 @@ def test_eviction_matches_the_definition(kind, lens, budget, n_sink, n_recent, e
     EvictCase(engine, pkg, kind, lens, 2, 2, max(lens) + 9).check(budget, n_sink, n_recent)
 
 
+@pytest.mark.parametrize("pad,offset", [(1, 0), (4, 1), (4, 2), (2, 1)])
+@pytest.mark.parametrize("lens,budget", [([700, 64, 300, 513, 1026], 256), ([1025, 1026, 1027, 1028, 7], 1024), ([5000, 4100, 3, 4099], 900)])
+def test_eviction_of_scores_off_the_vector_grid(lens, budget, pad, offset, engine, pkg):
+    """Row lists of scores and positions that do not start on 16 bytes, some or all of them."""
+    import torch
+    c = EvictCase(engine, pkg, "f16", lens, 2, 2, max(lens) + 9)
+    for name in ("score", "row_pos"):
+        x = getattr(c, name)
+        wide = torch.zeros((*x.shape[:3], x.shape[3] + pad), dtype=x.dtype, device="cuda")
+        wide[..., offset: offset + x.shape[3]] = x
+        setattr(c, name, wide[..., offset: offset + x.shape[3]])
+    c.check(budget, 4, 32)
+
+
 @pytest.mark.parametrize("budget", [24000, 49000, 50])
 @pytest.mark.parametrize("spread", ["ties", "close", "wide"])
 def test_eviction_from_the_longest_row_lists(budget, spread, engine, pkg):

@@ -10,9 +10,9 @@
 // keys of the bin it falls in against one another; only a bin with more keys than threads (many equal scores) is cut further, 11 and
 // 10 bits at a time.  Lists are few when one stream is cut: then a cluster of CTAs takes each, every CTA
 // selecting for itself (the scores are in L2) and moving a share of the rows.
-// 1440 lists of up to 2048 f16 rows cut to 512 (194 MB read and written): 48 us, 4.0 TB/s.  The rows move at HBM's rate (29 us); what
-// comes before is a chain of short phases (keys 9, border 5, places 4 us, over one round of CTAs and a part); 128, 192 and 512 threads,
-// and fewer CTAs with more loads in flight, came out equal or slower.  Six lists of 300 rows: 6 us, latency (10 us when a bin of more than
+// 1440 lists of up to 2048 f16 rows cut to 512 (194 MB read and written): 46 us, 4.2 TB/s.  The rows move at HBM's rate (29 us); what
+// comes before is a chain of short phases (keys 8, border 5, places 4 us, over one round of CTAs and a part); 128, 192 and 512 threads,
+// and fewer CTAs with more loads in flight, came out equal or slower.  Six lists of 300 rows: 5 us, latency (10 us when a bin of more than
 // 96 keys took another histogram and the others were ranked a key at a time).
 #include "kv_cache.cuh"
 
@@ -49,8 +49,18 @@ struct EvictParams {
 // f32 -> unsigned in the order of the numbers: -0 as 0, NaN lowest (0), every number between 1 and 2^32 - 2
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
-    if (isnan(x)) return 0u;
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return isnan(x) ? 0u : b ^ ((uint32_t) ((int32_t) b >> 31) | 0x80000000u);
+}
+// The positions that are not protected: n_sink and `free_rows(..)` from there on, so that one comparison tells.
+__device__ __forceinline__ uint32_t free_rows(int n_seen, int n_sink, int n_recent) {
+    return (uint32_t) max(0LL, (long long) n_seen - n_recent - n_sink);
+}
+__device__ __forceinline__ uint32_t key_of_row(int pos, float score, int n_sink, uint32_t n_free) {
+    return (uint32_t) pos - (uint32_t) n_sink < n_free ? ordered(score) : 0xffffffffu;
+}
+// four rows of scores and positions, wherever they lie; both come in vectors if every fourth row starts on 16 bytes
+__device__ __forceinline__ bool in_vectors(const float * score, const int32_t * pos) {
+    return ((reinterpret_cast<uintptr_t>(score) | reinterpret_cast<uintptr_t>(pos)) & 15) == 0;
 }
 
 // one of the eight 16-byte pieces of a q8_0 row: four of K, four of V; the first of either also takes its two scales
@@ -122,15 +132,28 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
     const size_t at = (size_t) layer * p.nb_layer + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head;
     float *   const score = reinterpret_cast<float *>(p.score + at);
     int32_t * const pos   = reinterpret_cast<int32_t *>(p.row_pos + at);
-    const int recent = (p.n_seen ? p.n_seen[stream] : len) - p.n_recent;
-    auto make_key = [&](int j) {
-        const int q = pos[j];
-        return q < p.n_sink || q >= recent ? 0xffffffffu : ordered(score[j]);
-    };
+    const uint32_t n_free = free_rows(p.n_seen ? p.n_seen[stream] : len, p.n_sink, p.n_recent);
+    auto make_key = [&](int j) { return key_of_row(pos[j], score[j], p.n_sink, n_free); };
     auto key_of = [&](int j) { return p.keys_kept ? keys[j] : make_key(j); };
     __syncthreads();
+    int done = 0;
+    if (p.keys_kept && in_vectors(score, pos)) {
+        done = len & ~3;
+#pragma unroll 2
+        for (int j = 4 * tid; j < done; j += 4 * kThreads) {
+            const int4   q = *reinterpret_cast<const int4 *>(pos + j);
+            const float4 w = *reinterpret_cast<const float4 *>(score + j);
+            const uint4  k = make_uint4(key_of_row(q.x, w.x, p.n_sink, n_free), key_of_row(q.y, w.y, p.n_sink, n_free),
+                                        key_of_row(q.z, w.z, p.n_sink, n_free), key_of_row(q.w, w.w, p.n_sink, n_free));
+            *reinterpret_cast<uint4 *>(keys + j) = k;
+            atomicAdd(&hist[k.x >> (32 - kBits)], 1u);
+            atomicAdd(&hist[k.y >> (32 - kBits)], 1u);
+            atomicAdd(&hist[k.z >> (32 - kBits)], 1u);
+            atomicAdd(&hist[k.w >> (32 - kBits)], 1u);
+        }
+    }
 #pragma unroll 4
-    for (int j = tid; j < len; j += kThreads) {
+    for (int j = done + tid; j < len; j += kThreads) {
         const uint32_t k = make_key(j);
         if (p.keys_kept) keys[j] = k;
         atomicAdd(&hist[k >> (32 - kBits)], 1u);
@@ -295,8 +318,8 @@ __global__ void __launch_bounds__(kThreads, 7) evict_kernel(const EvictParams p)
 
 // Few rows to give up (a stream that gains a row a step gives one up a step): no border is looked for, the rows that go are,
 // one after the other, by reductions over the block.  They go in the order of their keys, of equal ones the highest
-// index first, so the next is the least of those after the last.  1920 lists that give up one row of 1025: 12 us for 16.4 MB, bound by
-// the 25 instructions of a key (issue slots 42 % in use).
+// index first, so the next is the least of those after the last.  1920 lists that give up one row of 1025: 10 us for 16.4 MB, bound by
+// instructions and by the chain from the length to the row that moves (12 us before vectors and one comparison for protection).
 constexpr int kFew        = 4;
 constexpr int kFewThreads = 128;
 static_assert(kFewThreads / 32 >= kFew, "a warp for each row behind the budget");
@@ -318,7 +341,8 @@ __global__ void __launch_bounds__(kFewThreads, 16) evict_few_kernel(const EvictP
     const size_t at = (size_t) layer * p.nb_layer + (size_t) stream * p.nb_stream + (size_t) kvh * p.nb_head;
     float *   const score = reinterpret_cast<float *>(p.score + at);
     int32_t * const pos   = reinterpret_cast<int32_t *>(p.row_pos + at);
-    const int recent = (p.n_seen ? p.n_seen[stream] : len) - p.n_recent, n_go = len - p.budget;
+    const uint32_t n_free = free_rows(p.n_seen ? p.n_seen[stream] : len, p.n_sink, p.n_recent);
+    const int      n_go = len - p.budget;
     if (n_go <= 0) {
         if (kept) for (int j = tid; j < len; j += kFewThreads) kept[j] = j;
         return;
@@ -340,6 +364,7 @@ __global__ void __launch_bounds__(kFewThreads, 16) evict_few_kernel(const EvictP
             row = load_q8_piece(p.k_data + pair, from, lane);
         }
     }
+    const bool vectors = in_vectors(score, pos);
     int      gone[kFew];
     uint32_t last_key = 0;
     int      last_row = 0x7fffffff;
@@ -349,14 +374,26 @@ __global__ void __launch_bounds__(kFewThreads, 16) evict_few_kernel(const EvictP
         if (g >= n_go) continue;
         uint32_t key = 0xffffffffu;
         int      at = -1;
-#pragma unroll 8
-        for (int j = tid; j < len; j += kFewThreads) {  // of equal keys the last
-            const int      q = pos[j];
-            const float    w = score[j];
-            const uint32_t k = q < p.n_sink || q >= recent ? 0xffffffffu : ordered(w);
+        auto look = [&](int j, int q, float w) {  // of equal keys the last
+            const uint32_t k = key_of_row(q, w, p.n_sink, n_free);
             const bool     later = g == 0 || k > last_key || (k == last_key && j < last_row);
             if (later && k <= key) { key = k; at = j; }
+        };
+        int done = 0;
+        if (vectors) {
+            done = len & ~3;
+#pragma unroll 2
+            for (int j = 4 * tid; j < done; j += 4 * kFewThreads) {
+                const int4   q = *reinterpret_cast<const int4 *>(pos + j);
+                const float4 w = *reinterpret_cast<const float4 *>(score + j);
+                look(j, q.x, w.x);
+                look(j + 1, q.y, w.y);
+                look(j + 2, q.z, w.z);
+                look(j + 3, q.w, w.w);
+            }
         }
+#pragma unroll 8
+        for (int j = done + tid; j < len; j += kFewThreads) look(j, pos[j], score[j]);
         const uint32_t least = __reduce_min_sync(0xffffffffu, key);
         at = __reduce_max_sync(0xffffffffu, key == least ? at : -1);
         if (lane == 0) { least_key[g & 1][warp] = least; least_row[g & 1][warp] = at; }
