@@ -156,3 +156,35 @@ def test_the_border_leaves_the_largest_keys(seed):
     want[np.lexsort((i, -key.astype(np.int64)))[:budget]] = True
     assert stays.sum() == budget and np.array_equal(stays, want)
     assert stays[safe].all()
+
+
+# ------------------------------------------------------- vox_kv_observe, windows: score tiles of the groups of warps
+
+def score_tiles(q8, weights, rows, key_tiles, groups=4):
+    """The score tiles that each group of warps of kv_observe_window.cu takes, in order, and how many there are."""
+    n_b, blocks = -(-rows // 64), -(-rows // 128)
+    n_m = 4 if q8 and not weights and blocks == 3 else blocks
+    per_tile = n_b if weights else 2 * n_m
+    taken = [[] for _ in range(groups)]
+    for t in range(key_tiles):
+        u = t * per_tile
+        for g in range(groups):
+            if weights:
+                taken[g] += [u + i for i in range((g - u) % groups, n_b, groups)]
+            else:
+                taken[g] += [u + 2 * mt + (g & 1) for mt in range(g >> 1, n_m, 2)]
+    return taken, per_tile * key_tiles
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("weights", [False, True])
+def test_a_wait_for_a_score_tile_is_never_two_uses_of_its_buffer_away(q8, weights):
+    """A barrier tells even uses of a buffer from odd ones.  When a group waits for tile u, the use of its buffer before that, tile
+    u - buffers, must be over: that is so if the group has taken a tile from there on."""
+    buffers = 4 if q8 else 8
+    for rows in range(2, 513):
+        taken, total = score_tiles(q8, weights, rows, 11)
+        assert sorted(u for g in taken for u in g) == list(range(total))
+        for g in taken:
+            for last, u in zip([-1] + g, g):
+                assert u - buffers <= last, (rows, last, u)

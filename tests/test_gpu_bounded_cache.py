@@ -447,6 +447,15 @@ def test_few_query_rows_over_many_long_streams(kind, streams, rows, engine, pkg)
     ObserveCase(engine, pkg, (kind, lens, 49, 4, 2)).check(n_new=46)
 
 
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("n_q,heads,kv_heads", [(n, 16, 2) for n in (13, 20, 28, 36, 40, 44, 48, 52, 60, 64)] + [(43, 18, 3), (64, 6, 1), (50, 4, 4)])
+def test_windows_of_every_width_over_several_tiles(n_q, heads, kv_heads, kind, engine, pkg):
+    """Every number of score tiles to a key tile, for blocks that walk several key tiles, one list of rows after the other."""
+    for streams in (73, 160):
+        lens = [4 * ((i * 37) % 97) + 1 for i in range(streams)]
+        ObserveCase(engine, pkg, (kind, lens, n_q, heads, kv_heads)).check(n_new=2, decay=0.5)
+
+
 @pytest.mark.parametrize("n_new", [0, 3, 1000])
 def test_new_rows_start_from_nothing(n_new, engine, pkg):
     """n_new rows (none, some, all of them) take the weight alone, whatever their score held: NaN included."""

@@ -152,7 +152,11 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
         pdl_launch_dependents();
     }
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&tmem_slot);
-    const int rows = p.n_q * p.gqa, n_m = (rows + 127) / 128, n_b = (rows + kSub - 1) / kSub;
+    // A group of warps takes every fourth score tile or more (q8_0, first launch: three blocks of 128 rows count as four): a tile's wait
+    // tells it from the one before it in the same buffer only if the group has taken one of the kBufs tiles in between.
+    const int rows = p.n_q * p.gqa, n_b = (rows + kSub - 1) / kSub, blocks = (rows + 127) / 128;
+    const int n_m = Q8 && !kWeights && blocks == 3 ? 4 : blocks;
+    static_assert(Z::kBufs >= kGroups && (Q8 || Z::kBufs >= 2 * kMaxRows / 128), "see above");
     const int per_tile = kWeights ? n_b : 2 * n_m;  // score tiles per key tile
     auto give_up = [&]() {
         atomicOr(p.status, kStatusTimeout);
@@ -314,7 +318,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
             if (!ok && lane == 0) give_up();
         } else if (warp < kCopyWarp) {
             // ------------------------------------------------------------------ scores out, by groups of four warps.  First launch:
-            // group g has half g % 2 of a tile's keys and every other 128 query rows from g / 2 on; second: 64 query rows of every four
+            // group g has half g % 2 of a tile's keys and every other 128 query rows from g / 2 on; second: every fourth score tile.
             const int      group = warp >> 2, row = tid & 127, first_cut = w.len - p.n_q;  // first key that not every query sees
             const uint32_t t_row = tmem + ((uint32_t) (32 * (warp & 3)) << 16);
             constexpr int  kMine = kMaxRows / 256;
@@ -399,7 +403,7 @@ observe_window_kernel(const __grid_constant__ CUtensorMap map_k, const ObservePa
                 } else {
                     const int hidden = (key - first_cut) * p.gqa;  // rows before this one do not see the key
                     float     s1 = 0.0f;
-                    for (int i = group; i < n_b && ok; i += kGroups) {
+                    for (int i = (group - u) & (kGroups - 1); i < n_b && ok; i += kGroups) {
                         if (!take(u + i)) { ok = false; break; }
                         const bool cut = key0 + kKeys > first_cut;
 #pragma unroll
