@@ -185,6 +185,20 @@ def test_shared_prefix_scales_that_grow_along_the_rows(streams, engine, pkg):
     c.check()
 
 
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("streams,heads,kv_heads", [(4, 16, 2), (12, 18, 3), (20, 4, 2)])
+def test_long_prefixes_keep_their_precision(kind, streams, heads, kv_heads, engine, pkg):
+    """7000 rows of a prefix under few streams: errors of single sums must not add up along it.  A result is a sum over eight shares of
+    at most 896 keys, each a chain of 28 additions in f32 (half a step of 2^-23 each, random in sign: 6e-8 * sqrt(28)), of products
+    truncated four times at the size of 32 keys' share: 1e-6 of the result's RMS holds all of it twice over."""
+    c = SharedCase(engine, pkg, (kind, [0] * streams, [7000], [40] * streams, heads, kv_heads), junk=False)
+    out, _ = c.run()
+    engine.sync_status()
+    want, _ = c.want()
+    error = (out.double() - want).norm() / want.norm()
+    assert float(error) < 1e-6
+
+
 def test_shared_prefix_bounds_only_size_the_grid(engine, pkg):
     """Prefixes and streams longer than the bounds the host gave are attended in full; loose bounds change nothing but rounding."""
     c = SharedCase(engine, pkg, ("f16", [0, 1, 0, 1], [1500, 700], [90, 300, 0, 7], 16, 2))

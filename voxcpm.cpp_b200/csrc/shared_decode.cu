@@ -371,7 +371,11 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
             x.v_limit = dm > 0.0f ? unit * 256.0f : 0.0f;
         }
     }
-    const float to_units = Q8 ? 32.0f / x.v_unit : 1.0f;
+    // A product's sums start from zero and are added up in f32: the tensor core truncates at the size of what it accumulates, and over
+    // the 900 keys of a long prefix's share the results came out 4e-6 too small.
+    const float    to_units = Q8 ? 32.0f / x.v_unit : 1.0f;
+    const uint32_t vb = box + R::kVOff;
+    uint32_t       ph[NK][4], pl[NK][4];  // f16
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
         float pr[2][4];
@@ -379,12 +383,9 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) pr[j][e] = ex2_approx(sc[2 * k + j][e] - m_exp[e >> 1]);
-        const int      v_row = r0 + 16 * k + (((lane >> 3) & 1) << 3) + (lane & 7), v_chk = lane >> 4, pos_k = pos + 16 * k + 2 * t;
-        const uint32_t vb = box + R::kVOff;
 #pragma unroll
         for (int h = 0; h < 2; ++h) x.l[h] += (pr[0][2 * h] + pr[0][2 * h + 1]) + (pr[1][2 * h] + pr[1][2 * h + 1]);
         if constexpr (!Q8) {
-            uint32_t ph[4], pl[4];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -392,24 +393,12 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
                     float h0, l0, h1, l1;
                     split_hi_lo(pr[j][2 * h], h0, l0);
                     split_hi_lo(pr[j][2 * h + 1], h1, l1);
-                    ph[2 * j + h] = pack_half2(h0, h1);
-                    pl[2 * j + h] = pack_half2(l0, l1);
+                    ph[k][2 * j + h] = pack_half2(h0, h1);
+                    pl[k][2 * j + h] = pack_half2(l0, l1);
                 }
-#pragma unroll
-            for (int n2 = 0; n2 < 4; ++n2) {
-                uint32_t b0, b1, b2, b3;
-                ldmatrix_x4_trans(vb + v_row * 128 + (((2 * n2 + v_chk) ^ (v_row & 7)) << 4), b0, b1, b2, b3);
-                if (edge) {  // rows past the end may hold anything: zero times a NaN is none
-                    const uint32_t keep0 = keep_rows(pos_k, end), keep1 = keep_rows(pos_k + 8, end);
-                    b0 &= keep0; b1 &= keep1; b2 &= keep0; b3 &= keep1;
-                }
-                mma_16816(x.o[2 * n2], ph, b0, b1);
-                mma_16816(x.o[2 * n2 + 1], ph, b2, b3);
-                mma_16816(x.o[2 * n2], pl, b0, b1);
-                mma_16816(x.o[2 * n2 + 1], pl, b2, b3);
-            }
         } else {
-            uint2 ds[2];
+            const int v_row = r0 + 16 * k + (((lane >> 3) & 1) << 3) + (lane & 7), v_chk = lane >> 4, pos_k = pos + 16 * k + 2 * t;
+            uint2     ds[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 ds[j] = lds64(box + kQ8VScaleOff + (r0 + 16 * k + 8 * j + 2 * t) * 4);
@@ -418,7 +407,7 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
             }
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                uint32_t ph[4], pl[4];
+                uint32_t bh[4], bl[4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float s0 = to_units * (b ? half_hi(ds[j].x) : half_lo(ds[j].x)), s1 = to_units * (b ? half_hi(ds[j].y) : half_lo(ds[j].y));
@@ -427,8 +416,8 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
                         float h0, l0, h1, l1;
                         split_hi_lo(pr[j][2 * h] * s0, h0, l0);
                         split_hi_lo(pr[j][2 * h + 1] * s1, h1, l1);
-                        ph[2 * j + h] = pack_half2(h0, h1);
-                        pl[2 * j + h] = pack_half2(l0, l1);
+                        bh[2 * j + h] = pack_half2(h0, h1);
+                        bl[2 * j + h] = pack_half2(l0, l1);
                     }
                 }
                 uint32_t r[4];
@@ -437,9 +426,37 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
                 for (int n = 0; n < 4; ++n) {  // chunk n / 2 of 16 columns, even or odd ones
                     const uint32_t sel = n & 1 ? 0x4341 : 0x4240;
                     const uint32_t b0 = s8_pair_to_half2(r[2 * (n >> 1)], sel), b1 = s8_pair_to_half2(r[2 * (n >> 1) + 1], sel);
-                    mma_16816(x.o[4 * b + n], ph, b0, b1);
-                    mma_16816(x.o[4 * b + n], pl, b0, b1);
+                    float          a[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_16816(a, bl, b0, b1);
+                    mma_16816(a, bh, b0, b1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x.o[4 * b + n][e] += a[e];
                 }
+            }
+        }
+    }
+    if constexpr (!Q8) {
+#pragma unroll
+        for (int n2 = 0; n2 < 4; ++n2) {
+            float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                const int v_row = r0 + 16 * k + (((lane >> 3) & 1) << 3) + (lane & 7), v_chk = lane >> 4, pos_k = pos + 16 * k + 2 * t;
+                uint32_t  b0, b1, b2, b3;
+                ldmatrix_x4_trans(vb + v_row * 128 + (((2 * n2 + v_chk) ^ (v_row & 7)) << 4), b0, b1, b2, b3);
+                if (edge) {  // rows past the end may hold anything: zero times a NaN is none
+                    const uint32_t keep0 = keep_rows(pos_k, end), keep1 = keep_rows(pos_k + 8, end);
+                    b0 &= keep0; b1 &= keep1; b2 &= keep0; b3 &= keep1;
+                }
+                mma_16816(a0, pl[k], b0, b1);
+                mma_16816(a1, pl[k], b2, b3);
+                mma_16816(a0, ph[k], b0, b1);
+                mma_16816(a1, ph[k], b2, b3);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x.o[2 * n2][e] += a0[e];
+                x.o[2 * n2 + 1][e] += a1[e];
             }
         }
     }
