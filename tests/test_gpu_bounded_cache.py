@@ -896,6 +896,28 @@ def test_a_captured_step_follows_its_inputs(kind, streams, engine, pkg):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("prefix,rows", [(200, 700), (900, 60), (1500, 900)])
+def test_full_row_tiles_of_three_streams_at_once(prefix, rows, kind, engine, pkg):
+    """Calls whose prefix kernels (full row tiles, clusters, all of an SM's tensor memory) may meet on the same SMs."""
+    import torch
+    cases = [SharedCase(engine, pkg, (kind, [s % 2 for s in range(96)], [prefix, prefix - 9], [(rows * (s % 7 + 1)) // 7 for s in range(96)], 16, 2),
+                        seed=i) for i in range(3)]
+    ws = [torch.zeros(1 << 24, dtype=torch.uint8, device="cuda") for _ in cases]
+    want = [c.run(workspace=w)[0].clone() for c, w in zip(cases, ws)]
+    engine.sync_status()
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for c, w, st in zip(cases, ws, streams):
+            with torch.cuda.stream(st):
+                got.append(c.run(workspace=w)[0])
+        torch.cuda.synchronize()
+        engine.sync_status()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_captured_call_outlives_a_larger_workspace(pkg):
     """A graph captured with the engine's workspace is replayed after a larger call has made the engine take another one."""
     import torch

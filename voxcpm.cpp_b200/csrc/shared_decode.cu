@@ -1102,14 +1102,25 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
         if (kGroups == 2) named_bar_sync(1, 128 * kGroups);  // the first group joins both
     }
-    float4 * const part = reinterpret_cast<float4 *>(smem_gen);
-    join_and_write(p, w, part, ml, joined, rows_at, part + kRows * kPartPitch, kGroups, kRows, all_ok, tid);
-    // common exit: every role has left its loop; release TMEM
+    // Every role has left its loop and the results are in shared memory.  TMEM goes back before the cluster meets: two CTAs of this
+    // kernel fit an SM (those of two calls, or of one where the decode kernel leaves room), an allocation waits for the other's release,
+    // and two clusters that each held some SMs' TMEM while they waited for their other CTAs would wait for good.  (After a wait that
+    // ran out products may still be on their way: then at the end.)
     tc_fence_before();
     __syncthreads();
-    if (warp == kScoreWarp) {
+    const bool late = aborted();
+    if (warp == kScoreWarp && !late) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+    float4 * const part = reinterpret_cast<float4 *>(smem_gen);
+    join_and_write(p, w, part, ml, joined, rows_at, part + kRows * kPartPitch, kGroups, kRows, all_ok, tid);
+    if (late) {
+        __syncthreads();
+        if (warp == kScoreWarp) {
+            tc_fence_after();
+            tmem_dealloc(tmem, 512);
+        }
     }
 }
 
