@@ -1,0 +1,99 @@
+"""What the binding of the bounded-cache operators looks at before it hands addresses to the library.  No GPU: the library is a
+recorder, the tensors lie on the CPU, and the engine stands on the "device" that such tensors name (-1)."""
+import ctypes as C
+import sys
+
+import pytest
+import torch
+
+S, H, HK, ROWS, L = 3, 16, 2, 24, 2
+
+
+class Recorder:
+    """In the library's place: notes which entry points are called, and that all is well."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append(name) or 0
+
+
+@pytest.fixture
+def rig(pkg, monkeypatch):
+    binding, recorder = sys.modules[pkg.__name__ + ".binding"], Recorder()
+    monkeypatch.setattr(binding, "lib", lambda: recorder)
+
+    class Rig:
+        calls = recorder.calls
+        engine = object.__new__(pkg.Engine)
+        plans = []  # kept until the end: what a plan that goes asks of the library is not counted
+
+        def cache(self, kind=pkg.F16, streams=S):
+            c = object.__new__(pkg.KVCache)
+            c.engine, c.cfg, c.h, c.owned = self.engine, pkg.KVConfig(L, streams, HK, 64, ROWS, kind), C.c_void_p(64), False
+            return c
+
+        def plan(self, prefixes=2):
+            p = object.__new__(pkg.PrefixPlan)
+            p.engine, p.h, p.n_streams, p.n_prefixes = self.engine, C.c_void_p(128), S, prefixes
+            self.plans.append(p)
+            return p
+
+    r = Rig()
+    r.engine.h, r.engine.device, r.engine._ws, r.engine._outgrown = C.c_void_p(32), -1, None, []
+    yield r
+    r.engine.h = None
+    for p in r.plans:
+        p.h = None
+
+
+def decode(rig, **kw):
+    a = {"cache": rig.cache(), "layer": 0, "q": torch.zeros(S, H, 64), "kv_len": torch.ones(S, dtype=torch.int32), "kv_bound": ROWS,
+         "prefix": rig.cache(streams=2), "plan": rig.plan(), "prefix_len": torch.ones(2, dtype=torch.int32), "prefix_bound": 9,
+         "dst": torch.zeros(S, H, 64), "lse": torch.zeros(S, H), "k_new": torch.zeros(S, HK, 64), "v_new": torch.zeros(S, HK, 64),
+         "rope_table": torch.zeros(S, 32, 2), "workspace": torch.zeros(4096, dtype=torch.uint8), "stream": 0} | kw
+    return a.pop("cache").decode_shared(a.pop("layer"), a.pop("q"), a.pop("kv_len"), a.pop("kv_bound"), **a)
+
+
+def observe(rig, n_q=1, **kw):
+    one = n_q == 1
+    a = {"cache": rig.cache(), "q": torch.zeros(S, n_q, H, 64), "kv_len": torch.ones(S, dtype=torch.int32), "kv_bound": ROWS,
+         "score": torch.zeros(S, HK, ROWS), "row_pos": torch.zeros(S, HK, ROWS, dtype=torch.int32), "n_seen": torch.ones(S, dtype=torch.int32),
+         "lse": torch.zeros(S, H) if one else None, "rope_table": torch.zeros(S, 32, 2) if one else None,
+         "workspace": torch.zeros(4096, dtype=torch.uint8), "stream": 0} | kw
+    a.pop("cache").observe(0, a.pop("q"), a.pop("kv_len"), a.pop("kv_bound"), a.pop("score"), **a)
+
+
+def evict(rig, budget=8, **kw):
+    a = {"cache": rig.cache(), "kv_len": torch.ones(S, dtype=torch.int32), "kv_bound": ROWS, "score": torch.zeros(L, S, HK, ROWS),
+         "row_pos": torch.zeros(L, S, HK, ROWS, dtype=torch.int32), "n_seen": torch.ones(S, dtype=torch.int32),
+         "new_len": torch.zeros(S, dtype=torch.int32), "kept": torch.zeros(L, S, HK, budget, dtype=torch.int32), "n_sink": 0, "n_recent": 0, "stream": 0} | kw
+    a.pop("cache").evict(a.pop("kv_len"), a.pop("kv_bound"), budget, a.pop("score"), a.pop("row_pos"), a.pop("n_seen"), a.pop("new_len"), **a)
+
+
+def refused(rig, pkg, reason, call, *args, **kw):
+    before = len(rig.calls)
+    with pytest.raises(pkg.VoxError, match=reason) as err:
+        call(rig, *args, **kw)
+    assert err.value.status_name == "INVALID_ARGUMENT" and len(rig.calls) == before
+
+
+def test_a_call_that_fits_goes_to_the_library(rig):
+    decode(rig)
+    decode(rig, prefix=None, plan=None, prefix_len=None, prefix_bound=0, lse=None, k_new=None, v_new=None, rope_table=None, dst=None)
+    observe(rig)
+    observe(rig, n_q=5, row_pos=None, n_seen=None)
+    evict(rig)
+    evict(rig, n_seen=None, kept=None)
+    assert rig.calls == ["vox_attn_decode_shared"] * 2 + ["vox_kv_observe"] * 2 + ["vox_kv_evict"] * 2
+
+
+def test_closed_handles_are_refused(rig, pkg):
+    """NULL in the place of a prefix and its plan means that there is none: a closed one must not become NULL."""
+    cache, plan = rig.cache(), rig.plan()
+    cache.h = plan.h = None
+    for kw in ({"prefix": cache, "plan": plan}, {"prefix": cache}, {"plan": plan}, {"cache": cache}):
+        refused(rig, pkg, "closed", decode, **kw)
+    refused(rig, pkg, "closed", observe, cache=cache)
+    refused(rig, pkg, "closed", evict, cache=cache)

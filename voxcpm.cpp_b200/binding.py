@@ -268,7 +268,12 @@ def _addr(x):
 
 
 def _handle(x):
-    return x.h.value if x is not None and x.h else 0
+    """The handle behind a cache or a plan; NULL for none, which means something (no prefix): one that was closed is refused."""
+    if x is None:
+        return 0
+    if not x.h:
+        raise VoxError(1, f"{type(x).__name__} was closed")
+    return x.h.value
 
 
 def attn_args(q, k, v, dst, mask=None, scale=0.125, k_type=None, v_type=None) -> AttnArgs:
