@@ -387,7 +387,7 @@ void vox_prefix_plan_destroy(vox_prefix_plan * p);
  *   prefix_bound host-known upper bound of every prefix_len in use (sizes the grid and the workspace; 0: no prefix is read)
  *   lse          optional, [H, n_streams] f32: the natural log-sum-exp of every row's scores (-inf: nothing visible),
  *                which vox_kv_observe takes
- * prefix, plan and prefix_len all NULL: own rows only (vox_attn_decode with lse).  Results agree with vox_attn_decode over a
+ * prefix, plan and prefix_len all NULL, prefix_bound 0: own rows only (vox_attn_decode with lse).  Results agree with vox_attn_decode over a
  * cache that holds both parts to rounding; q8_0 weights are not rounded to f16 here (error under 1e-5 of the output's RMS).
  * A stream without a prefix row and without an own row gives zeros.  Rows past a length may hold anything, NaN included.
  * dst must not overlap q.  Two launches, the second on the SMs that the first leaves room on.

@@ -1192,7 +1192,10 @@ int check_shared(const vox_engine * e, const vox_decode_shared_args * a) {
     const vox_kv_cache * c = a->own.cache;
     VOX_REQUIRE(a->own.stream_order == nullptr, VOX_ATTN_UNSUPPORTED, "vox_attn_decode_shared takes no stream_order");
     VOX_REQUIRE((reinterpret_cast<uintptr_t>(a->lse) & 3) == 0, VOX_ATTN_INVALID_ARGUMENT, "lse must be 4-byte aligned");
-    if (a->prefix == nullptr && a->plan == nullptr) return VOX_ATTN_OK;  // own rows only
+    if (a->prefix == nullptr && a->plan == nullptr) {  // own rows only: nothing of a prefix may be given
+        VOX_REQUIRE(a->prefix_len == nullptr && a->prefix_bound == 0, VOX_ATTN_INVALID_ARGUMENT, "prefix, plan and prefix_len must be given together");
+        return VOX_ATTN_OK;
+    }
     {
         // the prefix kernel reads the queries while the decode kernel writes its results: they must not share memory
         const uintptr_t q0 = reinterpret_cast<uintptr_t>(a->own.q), d0 = reinterpret_cast<uintptr_t>(a->own.dst);
