@@ -419,7 +419,8 @@ int    vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, 
  *   n_new      the last n_new rows of every stream are new: their score starts here, and row_pos[j] becomes
  *              n_seen - kv_len + j, the token's position in its stream
  *   score, row_pos  [max_len, HK, n_streams] f32 / int32 on the device, rows contiguous, strides nb_head, nb_stream in bytes
- *              (the same for both, no row list over another); row_pos may be NULL.  Rows at kv_len and beyond are left as they are.
+ *              (the same for both); row_pos may be NULL.  No list of kv_bound rows may lie over another, of scores or of
+ *              positions, nor over kv_len, n_seen or lse.  Rows at kv_len and beyond are left as they are.
  *   n_seen     device array [n_streams]: tokens every stream has seen, the new ones included (NULL: kv_len)
  *   kv_bound   host-known upper bound of every kv_len; a longer stream raises VOX_ATTN_DEVICE_STATE and is left alone
  * The same call gives the same bits.  workspace: vox_kv_observe_workspace_bytes (0 for most calls with n_q == 1), 16-byte
@@ -458,7 +459,8 @@ int    vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * work
  *   kv_len     device array [n_streams]; kv_bound its host-known upper bound (a longer stream raises
  *              VOX_ATTN_DEVICE_STATE and is left alone, its new_len its kv_len)
  *   n_sink + n_recent <= budget;  budget >= 1;  kv_bound <= 49152 (VOX_ATTN_UNSUPPORTED beyond)
- *   score, row_pos  as vox_kv_observe leaves them, layers nb_layer bytes apart
+ *   score, row_pos  as vox_kv_observe leaves them, layers nb_layer bytes apart; no list of kv_bound rows over another, of scores or of
+ *              positions, nor over kv_len, n_seen, new_len or kept
  *   new_len    device out [n_streams]: min(kv_len, budget); must not overlap kv_len or n_seen
  *   kept       optional out [budget, HK, n_streams, n_layers] int32 contiguous: for every row below new_len the index it had
  *              (rows beyond are left as they are)

@@ -15,6 +15,7 @@
 // and fewer CTAs with more loads in flight, came out equal or slower.  Six lists of 300 rows: 5 us, latency (10 us when a bin of more than
 // 96 keys took another histogram and the others were ranked a key at a time).
 #include "kv_cache.cuh"
+#include "row_lists.h"
 
 #include <algorithm>
 
@@ -466,9 +467,20 @@ int check_evict(const vox_engine * e, const vox_kv_evict_args * a) {
                   reinterpret_cast<uintptr_t>(a->kept)) & 3) == 0 && a->nb_head % 4 == 0 && a->nb_stream % 4 == 0 && a->nb_layer % 4 == 0,
                 VOX_ATTN_INVALID_ARGUMENT, "score, row_pos, new_len and kept must be 4-byte aligned");
     const size_t row_bytes = (size_t) a->kv_bound * sizeof(float);
-    VOX_REQUIRE((c->cfg.n_kv_heads == 1 || a->nb_head >= row_bytes) && (a->n_streams == 1 || a->nb_stream >= row_bytes) &&
-                    (a->n_layers == 1 || a->nb_layer >= row_bytes),
-                VOX_ATTN_INVALID_ARGUMENT, "the scores of %d rows overlap (strides %zu, %zu, %zu bytes)", a->kv_bound, a->nb_head, a->nb_stream, a->nb_layer);
+    const RowLists lists(a->score, row_bytes, {{c->cfg.n_kv_heads, a->nb_head}, {a->n_streams, a->nb_stream}, {a->n_layers, a->nb_layer}});
+    VOX_REQUIRE(!lists.overlap(), VOX_ATTN_INVALID_ARGUMENT, "the scores of %d rows overlap (strides %zu, %zu, %zu bytes)", a->kv_bound, a->nb_head,
+                a->nb_stream, a->nb_layer);
+    VOX_REQUIRE(!lists.overlap_shifted(a->row_pos), VOX_ATTN_INVALID_ARGUMENT, "score and row_pos overlap");
+    const RowLists positions(a->row_pos, row_bytes, {{c->cfg.n_kv_heads, a->nb_head}, {a->n_streams, a->nb_stream}, {a->n_layers, a->nb_layer}});
+    const size_t lens_bytes = (size_t) a->n_streams * sizeof(int32_t);
+    const size_t kept_bytes = a->kept ? (size_t) a->n_layers * a->n_streams * c->cfg.n_kv_heads * a->budget * sizeof(int32_t) : 0;
+    for (const int32_t * x : {a->kv_len, a->n_seen, static_cast<const int32_t *>(a->new_len)}) {
+        VOX_REQUIRE(!lists.meets(x, lens_bytes) && !positions.meets(x, lens_bytes), VOX_ATTN_INVALID_ARGUMENT,
+                    "score and row_pos must not overlap kv_len, n_seen or new_len");
+        VOX_REQUIRE(!ranges_meet(x, lens_bytes, a->kept, kept_bytes), VOX_ATTN_INVALID_ARGUMENT, "kept must not overlap kv_len, n_seen or new_len");
+    }
+    VOX_REQUIRE(!lists.meets(a->kept, kept_bytes) && !positions.meets(a->kept, kept_bytes), VOX_ATTN_INVALID_ARGUMENT,
+                "kept must not overlap score or row_pos");
     VOX_REQUIRE((long long) a->n_layers * a->n_streams * c->cfg.n_kv_heads < (1LL << 31), VOX_ATTN_UNSUPPORTED, "more than 2^31 row lists in one call");
     return VOX_ATTN_OK;
 }

@@ -15,6 +15,7 @@
 // (For smaller pieces and more CTAs of fewer registers: 32 keys of a warp 42 - 53 us, three CTAs per SM 43 us, against 40.4 us before a
 // CTA took several chunks.)
 #include "kv_observe.cuh"
+#include "row_lists.h"
 
 using namespace vox;
 
@@ -452,8 +453,16 @@ int check_observe(const vox_engine * e, const vox_kv_observe_args * a) {
                     a->nb_head % 4 == 0 && a->nb_stream % 4 == 0,
                 VOX_ATTN_INVALID_ARGUMENT, "score, row_pos and lse must be 4-byte aligned");
     const size_t row_bytes = (size_t) a->kv_bound * sizeof(float);
-    VOX_REQUIRE((c->cfg.n_kv_heads == 1 || a->nb_head >= row_bytes) && (a->n_streams == 1 || a->nb_stream >= row_bytes), VOX_ATTN_INVALID_ARGUMENT,
-                "the scores of %d rows overlap (strides %zu, %zu bytes)", a->kv_bound, a->nb_head, a->nb_stream);
+    const RowLists lists(a->score, row_bytes, {{c->cfg.n_kv_heads, a->nb_head}, {a->n_streams, a->nb_stream}});
+    VOX_REQUIRE(!lists.overlap(), VOX_ATTN_INVALID_ARGUMENT, "the scores of %d rows overlap (strides %zu, %zu bytes)", a->kv_bound, a->nb_head, a->nb_stream);
+    VOX_REQUIRE(a->row_pos == nullptr || !lists.overlap_shifted(a->row_pos), VOX_ATTN_INVALID_ARGUMENT, "score and row_pos overlap");
+    const RowLists positions(a->row_pos, a->row_pos ? row_bytes : 0, {{c->cfg.n_kv_heads, a->nb_head}, {a->n_streams, a->nb_stream}});
+    for (const int32_t * in : {a->kv_len, a->n_seen})
+        VOX_REQUIRE(!lists.meets(in, a->n_streams * sizeof(int32_t)) && !positions.meets(in, a->n_streams * sizeof(int32_t)), VOX_ATTN_INVALID_ARGUMENT,
+                    "score and row_pos must not overlap kv_len or n_seen");
+    VOX_REQUIRE(!lists.meets(a->lse, (size_t) a->n_streams * a->n_heads * sizeof(float)) &&
+                    !positions.meets(a->lse, (size_t) a->n_streams * a->n_heads * sizeof(float)),
+                VOX_ATTN_INVALID_ARGUMENT, "score and row_pos must not overlap lse");
     VOX_REQUIRE((long long) a->n_streams * c->cfg.n_kv_heads <= 65535, VOX_ATTN_UNSUPPORTED, "more than 65535 (stream, kv head) pairs in one call");
     return VOX_ATTN_OK;
 }
