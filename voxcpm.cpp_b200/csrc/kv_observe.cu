@@ -45,19 +45,23 @@ template <bool Q8> struct KeyTile;
 template <> struct KeyTile<false> { uint4 x[2]; };
 template <> struct KeyTile<true>  { uint2 x[2]; uint32_t d; };
 
+// Ordinary loads: the rows are read-only to this kernel, but its CTAs may be on the SMs while the launch in front still appends some
+// (they wait for it before they read), and the non-coherent path asks for memory that nobody writes while the kernel lives.  q8_0 from L2,
+// f16 through L1: the other way round the compiler orders them worse (a window of 4 queries over 128 streams of 4096 q8_0 rows 97
+// against 86 us, a step over 256 f16 streams 32.5 against 32.2 us).
 template <bool Q8>
 __device__ __forceinline__ KeyTile<Q8> load_keys(const uint8_t * pair, int row, int t, bool live) {
     KeyTile<Q8> k;
     if constexpr (!Q8) {
         const uint4 * src = reinterpret_cast<const uint4 *>(pair + (size_t) row * 128) + t;
-        k.x[0] = live ? __ldg(src) : make_uint4(0u, 0u, 0u, 0u);
-        k.x[1] = live ? __ldg(src + 4) : make_uint4(0u, 0u, 0u, 0u);
+        k.x[0] = live ? *src : make_uint4(0u, 0u, 0u, 0u);
+        k.x[1] = live ? src[4] : make_uint4(0u, 0u, 0u, 0u);
     } else {
         const uint8_t * tile = pair + q8_tile_off(row);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-            k.x[b] = live ? __ldg(reinterpret_cast<const uint2 *>(tile + q8_byte_off(row, 32 * b + 8 * t))) : make_uint2(0u, 0u);
-        k.d = live ? __ldg(reinterpret_cast<const uint32_t *>(tile + kQ8KScaleOff + q8_scale_off(row, 0))) : 0u;
+            k.x[b] = live ? __ldcg(reinterpret_cast<const uint2 *>(tile + q8_byte_off(row, 32 * b + 8 * t))) : make_uint2(0u, 0u);
+        k.d = live ? __ldcg(reinterpret_cast<const uint32_t *>(tile + kQ8KScaleOff + q8_scale_off(row, 0))) : 0u;
     }
     return k;
 }
