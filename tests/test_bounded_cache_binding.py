@@ -22,7 +22,7 @@ class Recorder:
 @pytest.fixture
 def rig(pkg, monkeypatch):
     binding, recorder = sys.modules[pkg.__name__ + ".binding"], Recorder()
-    monkeypatch.setattr(binding, "lib", lambda: recorder)
+    monkeypatch.setattr(binding, "_LIB", recorder)
 
     class Rig:
         calls = recorder.calls
@@ -31,17 +31,17 @@ def rig(pkg, monkeypatch):
 
         def cache(self, kind=pkg.F16, streams=S):
             c = object.__new__(pkg.KVCache)
-            c.engine, c.cfg, c.h, c.owned = self.engine, pkg.KVConfig(L, streams, HK, 64, ROWS, kind), C.c_void_p(64), False
+            c.engine, c.cfg, c.h, c._at, c.owned = self.engine, pkg.KVConfig(L, streams, HK, 64, ROWS, kind), C.c_void_p(64), 64, False
             return c
 
         def plan(self, prefixes=2):
             p = object.__new__(pkg.PrefixPlan)
-            p.engine, p.h, p.n_streams, p.n_prefixes = self.engine, C.c_void_p(128), S, prefixes
+            p.engine, p.h, p._at, p.n_streams, p.n_prefixes = self.engine, C.c_void_p(128), 128, S, prefixes
             self.plans.append(p)
             return p
 
     r = Rig()
-    r.engine.h, r.engine.device, r.engine._ws, r.engine._outgrown = C.c_void_p(32), -1, None, []
+    r.engine.h, r.engine.device, r.engine._ws, r.engine._ws_at, r.engine._outgrown = C.c_void_p(32), -1, None, (0, 0), []
     yield r
     r.engine.h = None
     for p in r.plans:
@@ -92,8 +92,83 @@ def test_a_call_that_fits_goes_to_the_library(rig):
 def test_closed_handles_are_refused(rig, pkg):
     """NULL in the place of a prefix and its plan means that there is none: a closed one must not become NULL."""
     cache, plan = rig.cache(), rig.plan()
-    cache.h = plan.h = None
+    cache.close()
+    plan.close()
     for kw in ({"prefix": cache, "plan": plan}, {"prefix": cache}, {"plan": plan}, {"cache": cache}):
         refused(rig, pkg, "closed", decode, **kw)
     refused(rig, pkg, "closed", observe, cache=cache)
     refused(rig, pkg, "closed", evict, cache=cache)
+
+
+def ints(*shape):
+    return torch.ones(shape, dtype=torch.int32)
+
+
+def wide(x):
+    """The same values, every second element of a larger tensor."""
+    w = torch.zeros(*x.shape, 2, dtype=x.dtype)
+    w[..., 0] = x
+    return w[..., 0]
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("q", torch.zeros(S, H, 32)), ("q", torch.zeros(S, H, 64).half()), ("q", wide(torch.zeros(S, H, 64))),
+    ("kv_len", ints(S - 1)), ("kv_len", ints(S).long()), ("kv_len", ints(S).float()), ("kv_len", wide(ints(S))),
+    ("prefix_len", ints(1)), ("prefix_len", ints(2).long()), ("prefix_len", wide(ints(2))),
+    ("k_new", torch.zeros(S, HK, 64).half()), ("k_new", torch.zeros(S, 1, 64)), ("k_new", torch.zeros(S, HK, 65)[..., :64]),
+    ("v_new", torch.zeros(S, HK, 64).double()), ("v_new", torch.zeros(S - 1, HK, 64)), ("v_new", torch.zeros(HK, S, 64).transpose(0, 1)),
+    ("rope_table", torch.zeros(S, 32)), ("rope_table", torch.zeros(S, 32, 2).half()), ("rope_table", torch.zeros(S, 64, 2)[:, ::2]),
+    ("lse", torch.zeros(S, H - 1)), ("lse", torch.zeros(S, H).double()), ("lse", torch.zeros(H, S).T),
+    ("dst", torch.zeros(S, H, 63)), ("dst", torch.zeros(S, H, 64).half()), ("dst", torch.zeros(H, S, 64).transpose(0, 1)),
+])
+def test_decode_shared_looks_at_what_it_passes_on(name, bad, rig, pkg):
+    refused(rig, pkg, name, decode, **{name: bad})
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("q", torch.zeros(S, 1, H, 32)), ("q", torch.zeros(S, 1, H, 64).double()),
+    ("kv_len", ints(S - 1)), ("kv_len", ints(S).long()), ("kv_len", wide(ints(S))),
+    ("n_seen", ints(S).long()), ("n_seen", ints(S - 1)),
+    ("lse", torch.zeros(S - 1, H)), ("lse", torch.zeros(S, H).half()), ("lse", torch.zeros(H, S).T),
+    ("rope_table", torch.zeros(S, 32)), ("rope_table", torch.zeros(S, 32, 2).double()),
+    ("score", torch.zeros(S, 1, ROWS)), ("score", torch.zeros(S, HK, ROWS).half()), ("score", torch.zeros(S - 1, HK, ROWS)),
+    ("score", torch.zeros(S, HK, ROWS, 2)[..., 0]),
+    ("row_pos", ints(S, HK, ROWS).long()), ("row_pos", ints(S, HK, ROWS + 1)), ("row_pos", ints(S, HK, ROWS + 1)[..., :ROWS]),
+])
+def test_observe_looks_at_what_it_passes_on(name, bad, rig, pkg):
+    refused(rig, pkg, name, observe, **{name: bad})
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("kv_len", ints(S - 1)), ("kv_len", ints(S).long()), ("n_seen", ints(S).long()), ("n_seen", wide(ints(S))),
+    ("new_len", ints(S - 1)), ("new_len", ints(S).long()), ("new_len", wide(ints(S))),
+    ("score", torch.zeros(L, S, HK + 1, ROWS)), ("score", torch.zeros(L, S, HK, ROWS).double()),
+    ("row_pos", ints(L, S, HK, ROWS - 1)), ("row_pos", ints(L, S, HK, ROWS).float()), ("row_pos", ints(L, S, ROWS, HK).transpose(2, 3)),
+    ("kept", ints(L, S, HK, 7)), ("kept", ints(L, S, HK, 9)), ("kept", ints(L - 1, S, HK, 8)), ("kept", ints(L, S, HK, 8).long()),
+    ("kept", ints(L, S, HK, 9)[..., :8]),
+])
+def test_evict_looks_at_what_it_passes_on(name, bad, rig, pkg):
+    refused(rig, pkg, name, evict, **{name: bad})
+
+
+def test_scores_of_fewer_rows_than_the_bound_are_refused(rig, pkg):
+    """One stream of one kv head has no stride that the library could compare with the bound."""
+    refused(rig, pkg, "kv_bound 24 exceeds the 23 rows", observe, score=torch.zeros(S, HK, ROWS - 1), row_pos=None)
+    refused(rig, pkg, "kv_bound 24 exceeds the 23 rows", evict, score=torch.zeros(L, S, HK, ROWS - 1), row_pos=ints(L, S, HK, ROWS - 1))
+
+
+def test_larger_tensors_than_the_call_needs_are_taken(rig):
+    """Lengths of more streams than are decoded, rows of more than the bound, strided queries and rows."""
+    decode(rig, kv_len=ints(S + 4), prefix_len=ints(9), q=torch.zeros(S, H, 66)[..., :64], k_new=torch.zeros(S, HK, 66)[..., :64],
+           v_new=torch.zeros(S, HK, 66)[..., :64])
+    score, pos = torch.zeros(S, HK, ROWS + 9)[..., 2: ROWS + 3], ints(S, HK, ROWS + 9)[..., 2: ROWS + 3]
+    observe(rig, score=score, row_pos=pos, n_seen=ints(S + 1), kv_len=ints(S + 1))
+    evict(rig, score=torch.zeros(S, L, HK, ROWS + 1).transpose(0, 1), row_pos=ints(S, L, HK, ROWS + 1).transpose(0, 1), new_len=ints(S + 1))
+    assert rig.calls == ["vox_attn_decode_shared", "vox_kv_observe", "vox_kv_evict"]
+
+
+def test_tensors_of_another_device_are_refused(rig, pkg):
+    rig.engine.device = 0  # the tensors are the host's
+    refused(rig, pkg, "on device 0", decode)
+    refused(rig, pkg, "on device 0", observe)
+    refused(rig, pkg, "on device 0", evict)

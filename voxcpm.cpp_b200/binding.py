@@ -263,17 +263,33 @@ def _raw_stream(device: int) -> int:
     return _raw_stream(device)
 
 
-def _addr(x):
-    return 0 if x is None else x.data_ptr()
+def _closed(x):
+    """NULL in the place of a cache or a plan means that there is none: one that was closed is refused."""
+    raise VoxError(1, f"{type(x).__name__} was closed")
 
 
-def _handle(x):
-    """The handle behind a cache or a plan; NULL for none, which means something (no prefix): one that was closed is refused."""
-    if x is None:
-        return 0
-    if not x.h:
-        raise VoxError(1, f"{type(x).__name__} was closed")
-    return x.h.value
+def _wrong(name, x, dtype, n, device):
+    """A tensor that cannot stand in a call: its address (and strides) alone would go to the library."""
+    return VoxError(1, f"{name} must be {n} elements of {dtype}, contiguous (rows at least), on device {device}; got {tuple(x.shape)} of {x.dtype}, "
+                       f"strides {x.stride()}, on {x.device}")
+
+
+_f32 = _i32 = _empty_like = None  # torch's, once it is there
+
+
+def _types():
+    global _f32, _i32, _empty_like
+    import torch
+    _f32, _i32, _empty_like = torch.float32, torch.int32, torch.empty_like
+
+
+def _wrong_lists(score, row_pos, want, kv_bound, dev):
+    """What is the matter with the scores and positions of a call: the same shape and strides, kv_bound rows or more."""
+    if score.shape[:-1] != want or score.stride(-1) != 1 or score.dtype is not _f32 or score.get_device() != dev:
+        return _wrong("score", score, _f32, (*want, "rows"), dev)
+    if score.shape[-1] < kv_bound:
+        return VoxError(1, f"kv_bound {kv_bound} exceeds the {score.shape[-1]} rows of score")
+    return _wrong(f"row_pos (strides as score's, {score.stride()})", row_pos, _i32, tuple(score.shape), dev)
 
 
 def attn_args(q, k, v, dst, mask=None, scale=0.125, k_type=None, v_type=None) -> AttnArgs:
@@ -295,7 +311,7 @@ class Engine:
         _check(lib().vox_engine_create(device, C.byref(h)))
         self.h = h
         self.device = device
-        self._ws, self._outgrown = None, []
+        self._ws, self._ws_at, self._outgrown = None, (0, 0), []  # the tensor; its address and size
         self._children = weakref.WeakSet()  # caches and groups created from this engine: they go before it does
 
     def close(self):
@@ -340,18 +356,22 @@ class Engine:
                 nbytes = max(nbytes, self._ws.numel() + min(self._ws.numel(), 64 << 20))
                 self._outgrown.append(self._ws)
             self._ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=f"cuda:{self.device}")
+            self._ws_at = (self._ws.data_ptr(), self._ws.numel())
         return self._ws
 
     def _run(self, call, args, size, workspace, stream):
         """One call with a workspace: the caller's, or the engine's, which grows when the call says that it is too small (asking
         for the size every time costs a third of what the launch does)."""
         st = _raw_stream(self.device) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
-        ws = workspace if workspace is not None else self._ws if self._ws is not None else self.workspace(1 << 16)
-        rc = call(self.h, args, ws.data_ptr(), ws.numel(), st)
-        if rc == 3 and workspace is None:
-            ws = self.workspace(size(args))
-            rc = call(self.h, args, ws.data_ptr(), ws.numel(), st)
-        _check(rc)
+        if workspace is not None:
+            rc = call(self.h, args, workspace.data_ptr(), workspace.numel(), st)
+        else:
+            rc = call(self.h, args, *self._ws_at, st)
+            if rc == 3:
+                self.workspace(max(size(args), 1 << 16))
+                rc = call(self.h, args, *self._ws_at, st)
+        if rc:
+            _check(rc)
 
     def forward(self, q, k, v, mask=None, scale=0.125, stream=None, dst=None):
         """``ggml_flash_attn_ext`` on device tensors: q [B,H,n_q,64] f32, k/v [B,HK,n_kv,*],
@@ -460,11 +480,12 @@ class KVCache:
             engine._children.add(self)
         else:
             self.h = C.c_void_p(handle)
+        self._at = self.h.value  # the handle as a number, 0 once closed
 
     def close(self):
         if self.h and self.owned and self.engine.h:  # a cache never outlives its engine (Engine.close closes it first)
             lib().vox_kv_destroy(self.h)
-        self.h = None
+        self.h, self._at = None, 0
 
     def __del__(self):
         try:
@@ -573,17 +594,47 @@ class KVCache:
         ``prefix``: the KVCache that holds the prefixes; ``plan``: a PrefixPlan; ``prefix_len`` int32 device [prefixes];
         ``lse`` [n_streams, H] f32 receives the log-sum-exp; ``workspace``: a uint8 tensor (None: the engine's, for calls on
         one stream).  Returns [n_streams, H, 64]."""
+        if _f32 is None:
+            _types()
+        # (written out: what these questions cost in calls of a helper is a fifth of a small call)
         S, H, D = q.shape
+        q_s, n_s, dev = q.stride(), (0, 0, 1), self.engine.device
+        if D != 64 or q_s[2] != 1 or q.dtype is not _f32 or q.get_device() != dev:
+            raise _wrong("q", q, _f32, f"[{S}, {H}, 64]", dev)
+        if kv_len.numel() < S or kv_len.dtype is not _i32 or not kv_len.is_contiguous() or kv_len.get_device() != dev:
+            raise _wrong("kv_len", kv_len, _i32, S, dev)
+        k_at = v_at = rope_at = lse_at = len_at = 0
+        if k_new is not None:
+            k_at, n_s, new = k_new.data_ptr(), k_new.stride(), (S, self.cfg.n_kv_heads, 64)
+            if k_new.shape != new or n_s[2] != 1 or k_new.dtype is not _f32 or k_new.get_device() != dev:
+                raise _wrong("k_new", k_new, _f32, new, dev)
+        if v_new is not None:
+            v_at = v_new.data_ptr()
+            if k_new is not None and (v_new.shape != new or v_new.stride() != n_s or v_new.dtype is not _f32 or v_new.get_device() != dev):
+                raise _wrong(f"v_new (strides as k_new's, {n_s})", v_new, _f32, new, dev)
+        if rope_table is not None:
+            rope_at = rope_table.data_ptr()
+            if rope_table.numel() < S * 64 or rope_table.dtype is not _f32 or not rope_table.is_contiguous() or rope_table.get_device() != dev:
+                raise _wrong("rope_table", rope_table, _f32, S * 64, dev)
+        if lse is not None:
+            lse_at = lse.data_ptr()
+            if lse.numel() < S * H or lse.dtype is not _f32 or not lse.is_contiguous() or lse.get_device() != dev:
+                raise _wrong("lse", lse, _f32, S * H, dev)
+        if prefix_len is not None:
+            len_at = prefix_len.data_ptr()
+            if (prefix_len.dtype is not _i32 or not prefix_len.is_contiguous() or prefix_len.get_device() != dev or
+                    plan is not None and prefix_len.numel() < plan.n_prefixes and  # (a plan of more prefixes than there are is refused below)
+                    (prefix is None or plan.n_prefixes <= prefix.cfg.n_streams)):
+                raise _wrong("prefix_len", prefix_len, _i32, plan.n_prefixes if plan is not None else 1, dev)
         if dst is None:
-            dst = q.new_empty((S, H, D))
-        q_s = q.stride()
-        n_s = k_new.stride() if k_new is not None else (0, 0, 1)
-        assert D == 64 and q_s[2] == n_s[2] == 1 and q.element_size() == kv_len.element_size() == 4
-        assert k_new is None or v_new is None or v_new.stride() == n_s
-        a = _pack_decode_shared(_handle(self), layer, S, H, kv_len.data_ptr(), kv_bound, q.data_ptr(), q_s[1] * 4, q_s[0] * 4, dst.data_ptr(),
-                                scale, _addr(k_new), _addr(v_new), n_s[1] * 4, n_s[0] * 4, 1 if cache_stable else 0, _addr(rope_table), 0,
-                                _handle(prefix), _handle(plan), _addr(prefix_len), prefix_bound, _addr(lse))
-        L = lib()
+            dst = _empty_like(q) if q.is_contiguous() else q.new_empty((S, H, D))
+        elif dst.numel() < S * H * 64 or dst.dtype is not _f32 or not dst.is_contiguous() or dst.get_device() != dev:
+            raise _wrong("dst", dst, _f32, S * H * 64, dev)
+        a = _pack_decode_shared(self._at or _closed(self), layer, S, H, kv_len.data_ptr(), kv_bound, q.data_ptr(), q_s[1] * 4, q_s[0] * 4,
+                                dst.data_ptr(), scale, k_at, v_at, n_s[1] * 4, n_s[0] * 4, 1 if cache_stable else 0, rope_at, 0,
+                                0 if prefix is None else prefix._at or _closed(prefix), 0 if plan is None else plan._at or _closed(plan), len_at,
+                                prefix_bound, lse_at)
+        L = _LIB
         self.engine._run(L.vox_attn_decode_shared, a, L.vox_attn_decode_shared_workspace_bytes, workspace, stream)
         return dst
 
@@ -592,27 +643,64 @@ class KVCache:
         """``vox_kv_observe``: adds the attention weight that the queries q [n_streams, n_q, H, 64] (the last n_q rows') give to
         every row to ``score`` [n_streams, HK, rows] f32, and notes the positions of the ``n_new`` new rows in ``row_pos``
         (int32, the same shape and strides)."""
+        if _f32 is None:
+            _types()
         S, n_q, H, D = q.shape
-        q_s, s_s = q.stride(), score.stride()
-        assert D == 64 and q_s[3] == 1 and q.element_size() == kv_len.element_size() == score.element_size() == 4
-        assert s_s[2] == 1 and (row_pos is None or row_pos.stride() == s_s)
-        a = _pack_observe(_handle(self), layer, S, H, n_q, kv_len.data_ptr(), _addr(n_seen), kv_bound, q.data_ptr(), q_s[2] * 4, q_s[1] * 4,
-                          q_s[0] * 4, _addr(rope_table), _addr(lse), scale, decay, n_new, score.data_ptr(), _addr(row_pos), s_s[1] * 4, s_s[0] * 4)
-        L = lib()
+        q_s, dev = q.stride(), self.engine.device
+        if D != 64 or q_s[3] != 1 or q.dtype is not _f32 or q.get_device() != dev:
+            raise _wrong("q", q, _f32, f"[{S}, {n_q}, {H}, 64]", dev)
+        if kv_len.numel() < S or kv_len.dtype is not _i32 or not kv_len.is_contiguous() or kv_len.get_device() != dev:
+            raise _wrong("kv_len", kv_len, _i32, S, dev)
+        seen_at = lse_at = rope_at = pos_at = 0
+        if n_seen is not None:
+            seen_at = n_seen.data_ptr()
+            if n_seen.numel() < S or n_seen.dtype is not _i32 or not n_seen.is_contiguous() or n_seen.get_device() != dev:
+                raise _wrong("n_seen", n_seen, _i32, S, dev)
+        if lse is not None:
+            lse_at = lse.data_ptr()
+            if lse.numel() < S * H or lse.dtype is not _f32 or not lse.is_contiguous() or lse.get_device() != dev:
+                raise _wrong("lse", lse, _f32, S * H, dev)
+        if rope_table is not None:
+            rope_at = rope_table.data_ptr()
+            if rope_table.numel() < S * 64 or rope_table.dtype is not _f32 or not rope_table.is_contiguous() or rope_table.get_device() != dev:
+                raise _wrong("rope_table", rope_table, _f32, S * 64, dev)
+        HK, at, s_s = self.cfg.n_kv_heads, score.shape, score.stride()
+        if len(at) != 3 or at[2] < kv_bound or at[1] != HK or at[0] != S or s_s[2] != 1 or score.dtype is not _f32 or score.get_device() != dev:
+            raise _wrong_lists(score, row_pos, (S, HK), kv_bound, dev)
+        if row_pos is not None:
+            pos_at = row_pos.data_ptr()
+            if row_pos.shape != at or row_pos.stride() != s_s or row_pos.dtype is not _i32 or row_pos.get_device() != dev:
+                raise _wrong_lists(score, row_pos, (S, HK), kv_bound, dev)
+        a = _pack_observe(self._at or _closed(self), layer, S, H, n_q, kv_len.data_ptr(), seen_at, kv_bound, q.data_ptr(), q_s[2] * 4, q_s[1] * 4,
+                          q_s[0] * 4, rope_at, lse_at, scale, decay, n_new, score.data_ptr(), pos_at, s_s[1] * 4, s_s[0] * 4)
+        L = _LIB
         self.engine._run(L.vox_kv_observe, a, L.vox_kv_observe_workspace_bytes, workspace, stream)
 
     def evict(self, kv_len, kv_bound, budget, score, row_pos, n_seen, new_len, n_sink=4, n_recent=32, kept=None, layer0=0, stream=None):
         """``vox_kv_evict``: cuts the streams' rows to ``budget`` by ``score`` in the layers that ``score`` and ``row_pos``
         [n_layers, n_streams, HK, rows] span; ``new_len`` int32 [n_streams] receives the lengths, ``kept`` (int32
         [n_layers, n_streams, HK, budget], optional) the rows' former indices."""
-        s_s = score.stride()
-        assert s_s[3] == 1 and row_pos.stride() == s_s and (kept is None or kept.is_contiguous())
-        assert score.element_size() == row_pos.element_size() == kv_len.element_size() == new_len.element_size() == 4
-        L, S = score.shape[:2]
-        a = _pack_evict(_handle(self), layer0, L, S, kv_len.data_ptr(), _addr(n_seen), kv_bound, budget, n_sink, n_recent, score.data_ptr(),
-                        row_pos.data_ptr(), s_s[2] * 4, s_s[1] * 4, s_s[0] * 4, new_len.data_ptr(), _addr(kept))
+        if _f32 is None:
+            _types()
+        at, s_s, HK, dev = score.shape, score.stride(), self.cfg.n_kv_heads, self.engine.device
+        L, S = at[0], at[1]
+        if (len(at) != 4 or at[3] < kv_bound or at[2] != HK or s_s[3] != 1 or score.dtype is not _f32 or score.get_device() != dev or
+                row_pos.shape != at or row_pos.stride() != s_s or row_pos.dtype is not _i32 or row_pos.get_device() != dev):
+            raise _wrong_lists(score, row_pos, (L, S, HK), kv_bound, dev)
+        if kv_len.numel() < S or kv_len.dtype is not _i32 or not kv_len.is_contiguous() or kv_len.get_device() != dev:
+            raise _wrong("kv_len", kv_len, _i32, S, dev)
+        if n_seen is not None and (n_seen.numel() < S or n_seen.dtype is not _i32 or not n_seen.is_contiguous() or n_seen.get_device() != dev):
+            raise _wrong("n_seen", n_seen, _i32, S, dev)
+        if new_len.numel() < S or new_len.dtype is not _i32 or not new_len.is_contiguous() or new_len.get_device() != dev:
+            raise _wrong("new_len (which must not overlap kv_len or n_seen)", new_len, _i32, S, dev)
+        if kept is not None and (kept.shape != (L, S, HK, budget) or kept.dtype is not _i32 or not kept.is_contiguous() or kept.get_device() != dev):
+            raise _wrong("kept", kept, _i32, (L, S, HK, budget), dev)
+        a = _pack_evict(self._at or _closed(self), layer0, L, S, kv_len.data_ptr(), 0 if n_seen is None else n_seen.data_ptr(), kv_bound, budget, n_sink, n_recent, score.data_ptr(),
+                        row_pos.data_ptr(), s_s[2] * 4, s_s[1] * 4, s_s[0] * 4, new_len.data_ptr(), 0 if kept is None else kept.data_ptr())
         st = _raw_stream(self.engine.device) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
-        _check(lib().vox_kv_evict(self.engine.h, a, st))
+        rc = _LIB.vox_kv_evict(self.engine.h, a, st)
+        if rc:
+            _check(rc)
 
 
 class PrefixPlan:
@@ -622,7 +710,7 @@ class PrefixPlan:
         a = self._ints(prefix_of)
         h = C.c_void_p()
         _check(lib().vox_prefix_plan_create(engine.h, len(a), n_prefixes, n_heads, n_kv_heads, a.ctypes.data_as(C.c_void_p), C.byref(h)))
-        self.engine, self.h, self.n_streams = engine, h, len(a)
+        self.engine, self.h, self._at, self.n_streams, self.n_prefixes = engine, h, h.value, len(a), n_prefixes
         engine._children.add(self)
 
     @staticmethod
@@ -639,7 +727,7 @@ class PrefixPlan:
     def close(self):
         if self.h and self.engine.h:
             lib().vox_prefix_plan_destroy(self.h)
-        self.h = None
+        self.h, self._at = None, 0
 
     def __del__(self):
         try:
