@@ -461,7 +461,8 @@ int    vox_kv_observe(vox_engine * e, const vox_kv_observe_args * a, void * work
  *   n_sink + n_recent <= budget;  budget >= 1;  kv_bound <= 49152 (VOX_ATTN_UNSUPPORTED beyond)
  *   score, row_pos  as vox_kv_observe leaves them, layers nb_layer bytes apart; no list of kv_bound rows over another, of scores or of
  *              positions, nor over kv_len, n_seen, new_len or kept
- *   new_len    device out [n_streams]: min(kv_len, budget); must not overlap kv_len or n_seen
+ *   new_len    device out [n_streams]: min(kv_len, budget); must not overlap kv_len or n_seen.  The kv_len of a step that appends
+ *              (k_new) counts the arriving row: it is new_len + 1 then, new_len itself would store the row over the last one kept
  *   kept       optional out [budget, HK, n_streams, n_layers] int32 contiguous: for every row below new_len the index it had
  *              (rows beyond are left as they are)
  * Rows at new_len and beyond are left as they are.  The engine's device must be the current one. */

@@ -1,7 +1,8 @@
 """Calls of the bounded-cache operators that must be refused, and what the operators promise about calls in a row: beside
 test_gpu_bounded_cache.py, whose cases and definitions these use."""
+import numpy as np
 import pytest
-from test_gpu_bounded_cache import EvictCase, ObserveCase, SharedCase, ints
+from test_gpu_bounded_cache import D, EvictCase, ObserveCase, SharedCase, gen, ints, new_cache, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,81 @@ def test_row_lists_over_one_another_are_refused_by_evict(engine, pkg):
     refuses(engine, pkg, "kept must not overlap kv_len", call(new_len=kept.view(-1)[7:9]))
     refuses(engine, pkg, "kept must not overlap kv_len", call(kv_len=kept.view(-1)[78:]))
     c.check(10)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+def test_a_captured_loop_loses_no_row_that_it_keeps(kind, engine, pkg):
+    """A step as it is documented, one graph: kv_len = new_len + 1 and n_seen + 1 on the device, decode with the arriving row, weights,
+    eviction.  Replayed far past the budget, every row that is left is the one that its position was given when it arrived, the newest
+    among them, and the outputs are those of the calls made one at a time with lengths from the host."""
+    import torch
+    S, budget, rows, layers, of, P = 4, 40, 64, 2, [0, 1, -1, 0], [70, 9]
+    start = np.array([3, 39, 40, 20])
+    prefix = new_cache(engine, pkg, kind, layers, 2, 2, 72)
+    for layer in range(layers):
+        prefix.append(layer, randn(gen(layer), 2, 72, 2, D), randn(gen(9 + layer), 2, 72, 2, D))
+    plan, prefix_len, behind = pkg.PrefixPlan(engine, of, 2), ints(P), ints([P[p] if p >= 0 else 0 for p in of])
+
+    class State:
+        def __init__(self):
+            self.cache = new_cache(engine, pkg, kind, layers, S, 2, rows)
+            for layer in range(layers):
+                self.cache.append(layer, randn(gen(20 + layer), S, rows, 2, D), randn(gen(30 + layer), S, rows, 2, D))
+            self.score = torch.zeros((layers, S, 2, rows), device="cuda")
+            self.pos = torch.arange(rows, dtype=torch.int32, device="cuda").expand(layers, S, 2, -1).contiguous()
+            self.kv_len, self.new_len, self.n_seen = ints(start * 0), ints(start), ints(start)
+            self.q, self.k, self.v = (torch.zeros((layers, S, n, D), device="cuda") for n in (16, 2, 2))
+            self.lse, self.out = torch.zeros((layers, S, 16), device="cuda"), torch.zeros((layers, S, 16, D), device="cuda")
+            self.ws = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+
+        def step(self):
+            table = engine.rope_table(self.n_seen + behind, pos_offset=-1)
+            for layer in range(layers):
+                self.cache.decode_shared(layer, self.q[layer], self.kv_len, rows, prefix=prefix, plan=plan, prefix_len=prefix_len, prefix_bound=72,
+                                         k_new=self.k[layer], v_new=self.v[layer], rope_table=table, lse=self.lse[layer], dst=self.out[layer],
+                                         workspace=self.ws)
+                self.cache.observe(layer, self.q[layer][:, None], self.kv_len, rows, self.score[layer], row_pos=self.pos[layer],
+                                   n_seen=self.n_seen, lse=self.lse[layer], rope_table=table, workspace=self.ws)
+            self.cache.evict(self.kv_len, rows, budget, self.score, self.pos, self.n_seen, self.new_len, n_sink=1, n_recent=6)
+
+        def step_on_device(self):
+            torch.add(self.new_len, 1, out=self.kv_len)
+            self.n_seen += 1
+            self.step()
+
+    looped, eager = State(), State()
+    here = [{(s, h, j): looped.cache.export(layer, s, start[s])[0][h, j].tobytes() for s in range(S) for h in range(2) for j in range(start[s])}
+            for layer in range(layers)]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        looped.step_on_device()
+    n, seen = start.copy(), start.copy()
+    g = gen(50)
+    for t in range(60):
+        for x in "qkv":
+            new = randn(g, *getattr(looped, x).shape)
+            getattr(looped, x).copy_(new)
+            getattr(eager, x).copy_(new)
+        graph.replay()
+        engine.sync_status()
+        n, seen = n + 1, seen + 1
+        eager.kv_len.copy_(ints(n))
+        eager.n_seen.copy_(ints(seen))
+        eager.step()
+        engine.sync_status()
+        n = np.minimum(n, budget)
+        assert looped.new_len.tolist() == n.tolist() and looped.n_seen.tolist() == seen.tolist()
+        for name in ("out", "lse", "score", "pos"):
+            assert torch.equal(getattr(looped, name), getattr(eager, name)), (t, name)
+        pos = looped.pos.cpu().numpy()
+        for layer in range(layers):
+            for s in range(S):
+                k = looped.cache.export(layer, s, n[s])[0]
+                for h in range(2):
+                    at = pos[layer, s, h, : n[s]]
+                    assert len(set(at)) == n[s] and seen[s] - 1 in at
+                    for j, p in enumerate(at):
+                        if p == seen[s] - 1:
+                            here[layer][s, h, p] = k[h, j].tobytes()
+                        assert here[layer][s, h, p] == k[h, j].tobytes(), (t, layer, s, h, j, p)
