@@ -369,8 +369,8 @@ int    vox_attn_decode_static(vox_engine * e, const vox_decode_args * a, void * 
  *
  * A plan says which stream starts with which prefix (arranged on the host, kept on the device).
  *   prefix_of  host array [n_streams]: a stream of the prefix cache in [0, n_prefixes), or -1 for none
- * vox_prefix_plan_set changes the assignment in stream order (not during a capture: it copies from the host); calls
- * captured with the plan follow it.  A plan belongs to its engine's device and must outlive the calls that use it. */
+ * vox_prefix_plan_set changes the assignment in stream order (not during a capture: it copies from the host; the engine's
+ * device must be the current one); calls captured with the plan follow it.  A plan belongs to its engine's device and must outlive the calls that use it. */
 typedef struct vox_prefix_plan vox_prefix_plan;
 int  vox_prefix_plan_create(vox_engine * e, int n_streams, int n_prefixes, int n_heads, int n_kv_heads, const int32_t * prefix_of,
                             vox_prefix_plan ** out);

@@ -1,5 +1,7 @@
 """Calls of the bounded-cache operators that must be refused, and what the operators promise about calls in a row: beside
 test_gpu_bounded_cache.py, whose cases and definitions these use."""
+import ctypes
+
 import numpy as np
 import pytest
 from test_gpu_bounded_cache import D, EvictCase, ObserveCase, SharedCase, gen, ints, new_cache, randn
@@ -156,3 +158,23 @@ def test_a_captured_loop_loses_no_row_that_it_keeps(kind, engine, pkg):
                         if p == seen[s] - 1:
                             here[layer][s, h, p] = k[h, j].tobytes()
                         assert here[layer][s, h, p] == k[h, j].tobytes(), (t, layer, s, h, j, p)
+
+
+def test_calls_under_another_device_are_refused(engine, pkg):
+    """With another device current a stream (the default one above all) would be that device's.  One device is enough for this test: the
+    engine is told that it belongs to the next one."""
+    c, o, v = (SharedCase(engine, pkg, ("f16", [0, 0], [20], [5, 9], 16, 2)), ObserveCase(engine, pkg, ("f16", [5, 9], 1, 16, 2)),
+               EvictCase(engine, pkg, "f16", [30, 20], 1, 2, 32))
+    n2 = ints([0, 0])
+    calls = [lambda: c.run(stream=0), lambda: o.run(stream=0), lambda: c.plan.set([0, -1], stream=0),
+             lambda: v.cache.evict(v.kv_len, 30, 10, v.score, v.row_pos, v.n_seen, n2, n_sink=0, n_recent=0, stream=0)]
+    engine.sync_status()
+    device = ctypes.c_int.from_address(engine.h.value)  # the engine's first member
+    assert device.value == 0
+    try:
+        device.value = 1
+        for call in calls:
+            refuses(engine, pkg, "device 1 must be the current", call)
+    finally:
+        device.value = 0
+    c.check()

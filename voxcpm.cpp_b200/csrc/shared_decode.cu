@@ -1270,6 +1270,9 @@ void vox_prefix_plan_destroy(vox_prefix_plan * pl) {
 
 int vox_prefix_plan_set(vox_prefix_plan * pl, const int32_t * prefix_of, void * stream) {
     VOX_REQUIRE(pl && prefix_of, VOX_ATTN_INVALID_ARGUMENT, "vox_prefix_plan_set: null argument");
+    int current = -1;  // as the calls that read the plan: a stream of another device would not order the copy with them
+    VOX_CUDA_TRY(cudaGetDevice(&current));
+    VOX_REQUIRE(current == pl->e->device, VOX_ATTN_INVALID_ARGUMENT, "the engine's device %d must be the current device (current is %d)", pl->e->device, current);
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     VOX_CUDA_TRY(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture));
     VOX_REQUIRE(capture == cudaStreamCaptureStatusNone, VOX_ATTN_UNSUPPORTED, "vox_prefix_plan_set copies from the host: call it outside a capture");
