@@ -178,3 +178,64 @@ def test_calls_under_another_device_are_refused(engine, pkg):
     finally:
         device.value = 0
     c.check()
+
+
+# q8_0 values over many magnitudes.  The weights, each times its row's scale, travel as two f16 parts in units that follow the largest
+# such product of a query row so far: 2^-25 / 32 of it is the most that a part's rounding takes off a product, 8 * 2^-30 of the
+# result's RMS (one of 64 columns at least is at its block's largest), and over n rows the square root of n times that: 4e-7 for 3000.
+# Scores are sums of 64 products of at most 5 (the one that tells rows apart) and about 0.1 (the others), added up in f32: a few times
+# 2^-24 * 5.  1e-5 of the result, which the header promises, leaves a factor of ten.
+FORMS = {  # streams, own rows, prefix rows: which kernel takes the prefix
+    "small row tiles": (2, 200, 512),
+    "full row tiles beside long streams": (40, 3000, 512),
+    "full row tiles, two groups": (20, 64, 512),
+    "own rows only": (3, 1500, 0),
+    "one tile": (2, 30, 30),
+}
+
+
+def magnitudes(engine, pkg, form, k0, v_size):
+    """Rows j of n whose first K element is k0(j / n) and whose V rows are v_size(j / n) times as large; queries whose first element is 8, so
+    that a row's score is k0 and something of standard deviation 1."""
+    import torch
+    streams, own, prefix = FORMS[form]
+    c = SharedCase(engine, pkg, ("q8_0", [0 if prefix else -1] * streams, [prefix], [own, max(1, own // 3)] * (streams // 2) + [own] * (streams % 2), 16, 2),
+                   junk=False)
+    for i, (cache, n) in enumerate(((c.own, own), (c.prefix, prefix))):
+        rows = cache.cfg.max_len
+        k, v = randn(gen(3 + i), cache.cfg.n_streams, rows, 2, D), randn(gen(5 + i), cache.cfg.n_streams, rows, 2, D)
+        at = (torch.arange(rows, device="cuda", dtype=torch.float64) / max(n, 1)).float()
+        k[..., 0] = k0(at)[None, :, None]
+        cache.append(0, k, v * v_size(at)[None, :, None, None])
+    c.q[..., 0] = 8.0
+    out, lse = c.run()
+    engine.sync_status()
+    want, want_lse = c.want()
+    assert float((lse.double() - want_lse).abs().max()) < 6e-5
+    error = (out.double() - want).norm(dim=-1) / want.norm(dim=-1).clamp(min=1e-30)  # of every stream and head (nothing but zeros: none)
+    assert float(error.max()) < 1e-5, float(error.max())
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e6])
+@pytest.mark.parametrize("where", [0.0, 0.4, 0.96])
+def test_a_large_row_of_no_weight_takes_nothing_off_the_others(form, size, where, engine, pkg):
+    """A few V rows are far larger than the others and their keys far away (e^-40)."""
+    import torch
+    there = lambda at: (at >= where) & (at < where + 0.04)  # noqa: E731
+    magnitudes(engine, pkg, form, lambda at: torch.where(there(at), -40.0, 0.0), lambda at: torch.where(there(at), size, 1.0))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rise", [6.0, 40.0, 200.0])
+def test_large_rows_first_and_the_weight_behind(form, rise, engine, pkg):
+    """The weight rises along the rows while their size falls: what was largest when it was met is next to nothing at the end."""
+    import torch
+    magnitudes(engine, pkg, form, lambda at: rise * (at - 1.0), lambda at: 10.0 ** (6.0 * (0.5 - at.clamp(max=1.0))))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_of_zeros_beside_others(form, engine, pkg):
+    """V rows of nothing (scale 0) carry all the weight at first."""
+    import torch
+    magnitudes(engine, pkg, form, lambda at: torch.where(at < 0.5, 0.0, -6.0), lambda at: torch.where(at < 0.5, 0.0, 1.0))

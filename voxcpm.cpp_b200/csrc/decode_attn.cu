@@ -772,7 +772,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         // q8_0: sums of the V-scaled weights (accumulator tile of the product with ones: [0] = [1] = head g with the
         // scales of block 0, [2] = [3] = with those of block 1)
         float v_bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        float v_unit = 1.0f, v_limit = -1.0f;  // kShared q8_0: see the products below
+        float to_units = kMostInverse;  // kShared q8_0: see the products below
 
         // Tiles per pass of a consumer warp: one.  Two (both cache types were tried: two independent tiles in one pass
         // give the scheduler something to overlap the dependency chains with) measured the same or slower: f16 50.6
@@ -892,6 +892,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                 const float m_new = fmaxf(m, tmax);
                 const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
                 const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+                const float m_old = m;
                 m                 = m_new;
                 // kShared, f16: weights up to 2^10 instead of 1, so that the remainders of small ones are still normal f16
                 // numbers (their spacing below 2^-14 is 2^-24: seen from a weight of 1 that loses the last two bits)
@@ -907,9 +908,13 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                         psum_q8 += pr[u][j][0] + pr[u][j][1];
                     }
                 if (__any_sync(0xffffffffu, alpha != 1.0f)) {  // after the first tiles the running maxima rarely move
+                    if constexpr (Q8 && kShared) {
+                        to_units *= ex2_approx(fmaxf(m_use - m_old, 0.0f));
+                    } else {
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        o[n][0] *= alpha; o[n][1] *= alpha; o[n][2] *= alpha; o[n][3] *= alpha;
+                        for (int n = 0; n < 8; ++n) {
+                            o[n][0] *= alpha; o[n][1] *= alpha; o[n][2] *= alpha; o[n][3] *= alpha;
+                        }
                     }
                     v_bias[0] *= alpha; v_bias[2] *= alpha;
                 }
@@ -959,9 +964,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                             // times the scales of the block rounded to f16, rows 8-15 what the rounding left.  As many
                             // products as below (there one operand serves both blocks and half of every tile is dropped),
                             // and both halves of a tile belong to its columns.
-                            // The products are taken in units of v_unit, a power of two that follows the largest scale seen (as the
-                            // running maximum does, but it moves only when a scale outgrows it by 2^8): the f16 parts of
-                            // weights of any magnitude of V neither overflow nor lose bits below 2^-14.
+                            // The products are taken in units (see inverse_unit; to_units holds 32 of them back), which take part in
+                            // every rise of the running maximum in the accumulators' place; they are looked at again where a scale
+                            // could outgrow them by 2^8.  At first the largest weight is 1, and the smallest scale no more than the
+                            // largest product.
                             uint2 d0 = lds64(vsc + s_off), d1 = lds64(vsc + s_off + 32);
                             if (edge) {  // rows past the length may hold anything: zero times a NaN is none
                                 const int pos = p0[u] + 2 * t;
@@ -972,20 +978,32 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                             }
                             const __half2 big = __hmax2(__hmax2(__habs2(as_half2(d0.x)), __habs2(as_half2(d0.y))),
                                                         __hmax2(__habs2(as_half2(d1.x)), __habs2(as_half2(d1.y))));
-                            float dm = fmaxf(__low2float(big), __high2float(big));
-                            if (__any_sync(0xffffffffu, dm > v_limit)) {
-                                dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 1));
-                                dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 2));
-                                const float unit = dm > 0.0f ? __uint_as_float(__float_as_uint(dm) & 0x7f800000u) : kTwoM24;
-                                const float f    = v_unit / unit;
-#pragma unroll
-                                for (int n = 0; n < 8; ++n) {
-                                    o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f;
-                                }
-                                v_unit  = unit;
-                                v_limit = dm > 0.0f ? unit * 256.0f : 0.0f;
+                            const bool  first = m_old == -INFINITY;
+                            const float dm = fmaxf(__low2float(big), __high2float(big));
+                            if (__any_sync(0xffffffffu, first)) {
+                                const int pos = p0[u] + 2 * t;
+                                float     low = pos < c1 ? larger_scale(d0.x) : INFINITY;
+                                if (pos + 1 < c1) low = fminf(low, larger_scale(d0.y));
+                                if (pos + 8 < c1) low = fminf(low, larger_scale(d1.x));
+                                if (pos + 9 < c1) low = fminf(low, larger_scale(d1.y));
+                                low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 1));
+                                low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 2));
+                                if (first) to_units = 32.0f * inverse_unit(low);
                             }
-                            const float to_units = 32.0f / v_unit;
+                            if (__any_sync(0xffffffffu, dm * to_units > 8192.0f || !(to_units < 32.0f * kMostInverse))) {
+                                float most = fmaxf(fmaxf(pr[u][0][0] * larger_scale(d0.x), pr[u][0][1] * larger_scale(d0.y)),
+                                                   fmaxf(pr[u][1][0] * larger_scale(d1.x), pr[u][1][1] * larger_scale(d1.y)));
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                                if (most * to_units > 8192.0f || !(to_units < 32.0f * kMostInverse)) {
+                                    const float now = 32.0f * inverse_unit(most), f = now / to_units;
+#pragma unroll
+                                    for (int n = 0; n < 8; ++n) {
+                                        o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f;
+                                    }
+                                    to_units = now;
+                                }
+                            }
                             uint32_t    pb[2][4];
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
@@ -1060,10 +1078,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             // (the other block's scales on this block's bytes) is dropped.
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-                const float b = -128.0f * v_bias[n < 4 ? 0 : 2];
+                const float b = -128.0f * v_bias[n < 4 ? 0 : 2], from_units = 1.0f / to_units;
                 if constexpr (kShared) {
-                    o[n][0] = (o[n][0] + o[n][2]) * (v_unit / 32.0f);
-                    o[n][1] = (o[n][1] + o[n][3]) * (v_unit / 32.0f);
+                    o[n][0] = (o[n][0] + o[n][2]) * from_units;
+                    o[n][1] = (o[n][1] + o[n][3]) * from_units;
                 } else {
                     o[n][0] = fmaf(n < 4 ? o[n][0] : o[n][2], kTwo24, b);
                     o[n][1] = fmaf(n < 4 ? o[n][1] : o[n][3], kTwo24, b);

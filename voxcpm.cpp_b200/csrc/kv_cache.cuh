@@ -108,6 +108,20 @@ __device__ __forceinline__ uint32_t s8_pair_to_half2(uint32_t bytes, uint32_t se
     const __half2 r = __hsub2(as_half2(__byte_perm(bytes, 0x64646464u, selector)), __float2half2_rn(1152.0f));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
+// q8_0 P.V products take V's scales into the weights, and these travel as two f16 parts in units per query row: of the largest product of
+// weight and scale that the row has met, times the factors by which its running maximum rose since.  So no part overflows or falls below
+// f16's normal range however far the scales of a row's keys lie apart, and what a key of great scale and no weight is worth does not
+// count (units that followed the scales alone left the other keys no bits: results 3 % off beside keys 10^6 as large).
+// A row keeps the inverse, what a product is multiplied by: a rise of the maximum by 2^x multiplies it by 2^x, in the accumulators'
+// place, and no division waits for the maximum.  kMostInverse, or more: a row that has met nothing yet, or next to nothing.
+constexpr float kMostInverse = 1.2676506002282294e30f;  // 2^100
+__device__ __forceinline__ float inverse_unit(float largest) {  // the power of two that takes the largest product to [1, 2)
+    return fminf(__uint_as_float(0x7f000000u - (__float_as_uint(largest) & 0x7f800000u)), kMostInverse);
+}
+__device__ __forceinline__ float larger_scale(uint32_t d) {  // of a row's two blocks
+    const __half2 a = __habs2(as_half2(d));
+    return fmaxf(__low2float(a), __high2float(a));
+}
 #endif
 
 }  // namespace vox

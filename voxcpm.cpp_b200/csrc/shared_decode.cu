@@ -261,7 +261,7 @@ constexpr float kShift = 10.0f;  // f16 caches: weights up to 2^10, so that the 
 struct Rows {
     uint32_t qh[4][4], ql[4][4];
     float    o[8][4], m[2], l[2];
-    float    v_unit, v_limit;  // q8_0: the unit of the weights that take V's scales in, and the scale at which it moves
+    float    to_units[2];      // q8_0: 32 / the unit of the weights that take V's scales in (inverse_unit)
 };
 
 // One step of the online softmax: NK * 16 keys from row r0 of the 64-row box at `box`; `pos` is the first one's place, `end`
@@ -325,7 +325,8 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
             for (int e = 0; e < 4; ++e)
                 if (pos + 8 * j + 2 * t + (e & 1) >= end) sc[j][e] = -INFINITY;
     }
-    float alpha[2], m_exp[2];
+    float alpha[2], m_exp[2], rise[2];
+    bool  first[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         float top = -INFINITY;
@@ -334,46 +335,75 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float m_new = fmaxf(x.m[h], top);
+        first[h] = x.m[h] == -INFINITY;
+        rise[h]  = m_new == -INFINITY ? 0.0f : fmaxf(m_new - x.m[h], 0.0f);
         alpha[h] = m_new == -INFINITY ? 1.0f : ex2_approx(x.m[h] - m_new);
         m_exp[h] = (m_new == -INFINITY ? 0.0f : m_new) - (Q8 ? 0.0f : kShift);
         x.m[h]   = m_new;
     }
     if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+        if constexpr (!Q8) {
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            x.o[n][0] *= alpha[0]; x.o[n][1] *= alpha[0]; x.o[n][2] *= alpha[1]; x.o[n][3] *= alpha[1];
+            for (int n = 0; n < 8; ++n) {
+                x.o[n][0] *= alpha[0]; x.o[n][1] *= alpha[0]; x.o[n][2] *= alpha[1]; x.o[n][3] *= alpha[1];
+            }
+        } else {  // the accumulators' unit instead
+            x.to_units[0] *= ex2_approx(rise[0]);
+            x.to_units[1] *= ex2_approx(rise[1]);
         }
         x.l[0] *= alpha[0];
         x.l[1] *= alpha[1];
     }
     if constexpr (Q8) {
-        // V's scales go into the weights; rows past the end count as zeros.  The products are taken in units of v_unit, a
-        // power of two that follows the largest scale seen: f16 parts of weights for values of any size neither overflow
-        // nor lose bits below 2^-14.
+        // V's scales go into the weights; rows past the end count as zeros.  A row's unit is looked at again where a scale could
+        // outgrow it by 2^8.  At first the largest weight is 1, and the smallest scale no more than the largest product.
+        auto scale_at = [&](int j, int e) {
+            const uint2 ds = lds64(box + kQ8VScaleOff + (r0 + 8 * j + 2 * t) * 4);
+            return pos + 8 * j + 2 * t + e < end ? larger_scale(e ? ds.y : ds.x) : 0.0f;
+        };
         float dm = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 2 * NK; ++j) {
-            const uint2   ds  = lds64(box + kQ8VScaleOff + (r0 + 8 * j + 2 * t) * 4);
-            const __half2 lo = __habs2(as_half2(ds.x)), hi = __habs2(as_half2(ds.y));
-            if (pos + 8 * j + 2 * t < end) dm = fmaxf(dm, fmaxf(__low2float(lo), __high2float(lo)));
-            if (pos + 8 * j + 2 * t + 1 < end) dm = fmaxf(dm, fmaxf(__low2float(hi), __high2float(hi)));
-        }
-        if (__any_sync(0xffffffffu, dm > x.v_limit)) {
-            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 1));
-            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 2));
-            const float unit = dm > 0.0f ? __uint_as_float(__float_as_uint(dm) & 0x7f800000u) : kTwoM24;
-            const float f    = x.v_unit / unit;
+        for (int j = 0; j < 2 * NK; ++j) dm = fmaxf(dm, fmaxf(scale_at(j, 0), scale_at(j, 1)));
+        if (__any_sync(0xffffffffu, first[0] || first[1])) {
+            float low = INFINITY;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                x.o[n][0] *= f; x.o[n][1] *= f; x.o[n][2] *= f; x.o[n][3] *= f;
+            for (int j = 0; j < 2 * NK; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) low = pos + 8 * j + 2 * t + e < end ? fminf(low, scale_at(j, e)) : low;
+            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 1));
+            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 2));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x.to_units[h] = first[h] ? 32.0f * inverse_unit(low) : x.to_units[h];
+        }
+        const float top = fmaxf(x.to_units[0], x.to_units[1]);
+        if (__any_sync(0xffffffffu, dm * top > 8192.0f || !(top < 32.0f * kMostInverse))) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float most = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 2 * NK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float w;  // volatile: or the weights would be made for this rare branch in every step and kept
+                        asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(sc[j][2 * h + e] - m_exp[h]));
+                        most = fmaxf(most, w * scale_at(j, e));
+                    }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                if (most * x.to_units[h] > 8192.0f || !(x.to_units[h] < 32.0f * kMostInverse)) {
+                    const float now = 32.0f * inverse_unit(most), f = now / x.to_units[h];
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        x.o[n][2 * h] *= f;
+                        x.o[n][2 * h + 1] *= f;
+                    }
+                    x.to_units[h] = now;
+                }
             }
-            x.v_unit  = unit;
-            x.v_limit = dm > 0.0f ? unit * 256.0f : 0.0f;
         }
     }
     // A product's sums start from zero and are added up in f32: the tensor core truncates at the size of what it accumulates, and over
     // the 900 keys of a long prefix's share the results came out 4e-6 too small.
-    const float    to_units = Q8 ? 32.0f / x.v_unit : 1.0f;
     const uint32_t vb = box + R::kVOff;
     uint32_t       ph[NK][4], pl[NK][4];  // f16
 #pragma unroll
@@ -406,11 +436,15 @@ __device__ __forceinline__ void step(Rows & x, uint32_t box, int r0, int pos, in
                 if (pos_k + 8 * j + 1 >= end) ds[j].y = 0u;
             }
 #pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pr[j][e] *= x.to_units[e >> 1];
+#pragma unroll
             for (int b = 0; b < 2; ++b) {
                 uint32_t bh[4], bl[4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float s0 = to_units * (b ? half_hi(ds[j].x) : half_lo(ds[j].x)), s1 = to_units * (b ? half_hi(ds[j].y) : half_lo(ds[j].y));
+                    const float s0 = b ? half_hi(ds[j].x) : half_lo(ds[j].x), s1 = b ? half_hi(ds[j].y) : half_lo(ds[j].y);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         float h0, l0, h1, l1;
@@ -582,8 +616,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int n = 0; n < 8; ++n) x.o[n][0] = x.o[n][1] = x.o[n][2] = x.o[n][3] = 0.0f;
         x.m[0] = x.m[1] = -INFINITY;
         x.l[0] = x.l[1] = 0.0f;
-        x.v_unit = 1.0f;
-        x.v_limit = -1.0f;
+        x.to_units[0] = x.to_units[1] = kMostInverse;
         for (int it = 0; it < n_tiles; ++it) {
             const int s = it % R::kStages, key = w.key0 + it * kKeys;
             if (!mbar_wait_bounded(full0 + 8 * s, (it / R::kStages) & 1)) {
@@ -618,8 +651,8 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 for (int n = 0; n < 8; ++n) {
                     if constexpr (Q8) {  // tile n: chunk n / 2, this lane 16 (n / 2) + 4t + (n % 2) and two further
                         const int d = 16 * (n >> 1) + 4 * t + (n & 1);
-                        out[d]     = x.o[n][2 * h] * (x.v_unit / 32.0f);
-                        out[d + 2] = x.o[n][2 * h + 1] * (x.v_unit / 32.0f);
+                        out[d]     = x.o[n][2 * h] * (1.0f / x.to_units[h]);
+                        out[d + 2] = x.o[n][2 * h + 1] * (1.0f / x.to_units[h]);
                     } else {
                         *reinterpret_cast<float2 *>(out + 8 * n + 2 * t) = make_float2(x.o[n][2 * h], x.o[n][2 * h + 1]);
                     }
@@ -650,7 +683,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 //
 // q8_0: the softmax warps turn a tile's bytes into f16 numbers q (exact; a tile ahead of the scores they work on) and keep the
 // scales apart.  Either 32-value block has a score accumulator of its own (s = d0 S0 + d1 S1), and its 32 output columns have
-// weights of their own, with V's scale of the block taken in, in units of v_unit as in the other kernel.
+// weights of their own, with V's scale of the block taken in, in units (inverse_unit; a thread's row has its own).
 constexpr int kSub       = 64;                    // keys of a score tile and of a stage
 constexpr int kQTile     = kRows * 128;
 constexpr int kTcStage   = 2 * kSub * 128;        // 64 rows of K, 64 rows of V, in f16
@@ -668,6 +701,9 @@ template <bool Q8, int kGroups> struct Tc {
     static_assert(kRawBytes == kQ8TileBytes && 2 * kQTile + kStages * kTcStage >= 2 * kRows * kPartPitch * 16, "shared memory");
 };
 constexpr float kTcShift = 6.0f;                  // weights up to 2^(8 + 6): their remainders stay normal f16 numbers
+// q8_0: a row's largest product of weight and scale is made 2^4 .. 2^5.  Its unit is looked at where one could be 2^13, and follows if one is
+// 2^11.
+constexpr float kUnitFirst = 16.0f, kUnitMost = 2048.0f;
 
 // multiply this thread's row of the accumulators by f; rare, kept out of line so that its registers do not weigh on the loop
 __device__ __noinline__ void rescale_row(uint32_t t_o, int blocks, float f) {
@@ -681,6 +717,28 @@ __device__ __noinline__ void rescale_row(uint32_t t_o, int blocks, float f) {
         tmem_st32(t_o + 32 * h, o);
     }
     tc_fence_before();
+}
+
+// q8_0: the inverse unit of this thread's row for a tile whose scores lie at t_s (S0, and S1 behind it), whatever its scales (shared memory); where
+// it changes, the accumulators at t_o (0: there are none yet) follow.  Rare; it reads the scores again, so that nothing is kept for it.
+template <int kBlocks> __device__ __forceinline__ float refit_row(uint32_t t_s, uint32_t scales, float m, uint32_t t_o, float to_units) {
+    float most = 0.0f;  // the largest product of weight and V scale (keys past the end have scales of 0)
+#pragma unroll 1
+    for (int c = 0; c < kSub; c += 8) {
+        uint32_t a[8], b[8];
+        tmem_ld8_sync(t_s + c, a);
+        tmem_ld8_sync(t_s + kSub + c, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint2 k = lds64(scales + 16 * (c + i)), v = lds64(scales + 16 * (c + i) + 8);
+            const float e = ex2_approx(fmaf(__uint_as_float(b[i]), __uint_as_float(k.y), __uint_as_float(a[i]) * __uint_as_float(k.x)) - m);
+            most = fmaxf(most, e * fmaxf(fabsf(__uint_as_float(v.x)), fabsf(__uint_as_float(v.y))));
+        }
+    }
+    float now = to_units;
+    if (most * to_units > kUnitMost || !(to_units < kUnitFirst * kMostInverse)) now = kUnitFirst * inverse_unit(most);
+    if (t_o != 0 && __any_sync(0xffffffffu, now != to_units)) rescale_row(t_o, kBlocks, now / to_units);
+    return now;
 }
 
 // one row of a q8_0 tile: 64 bytes to 64 f16 at their swizzled places; zeros where the row does not exist
@@ -709,7 +767,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * kTcStages + 3 * kSBufs + 1 + 2 * kRaw];
     __shared__ float4   scales[Q8 ? kTcStages : 1][kSub];   // q8_0: of a row's K and V blocks
-    __shared__ uint32_t largest[kTcStages];                 // q8_0: the largest of a stage's V scales, as bits
+    __shared__ uint32_t largest[kTcStages], smallest[kGroups];  // q8_0: the largest of a stage's V scales, the smallest of a group's first tile, as bits
     __shared__ const uint8_t * row_q[kRows];
     __shared__ const float2 *  row_rope[kRows];
     __shared__ uint32_t tmem_slot;
@@ -737,6 +795,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             mbar_init(empty0 + 8 * s, 1);
             largest[s] = 0;
         }
+        for (int g = 0; g < kGroups; ++g) smallest[g] = 0x7f800000u;
         for (int s = 0; s < kRaw; ++s) {
             mbar_init(rfull0 + 8 * s, 1);
             mbar_init(rempty0 + 8 * s, 4);
@@ -923,7 +982,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const int      group = warp >> 2, row = tid & 127;
         // accumulators: [parity of the tile][value, remainder][64]; with two groups a group has those of one parity
         const uint32_t t_row = tmem + ((uint32_t) (32 * (warp & 3)) << 16), t_o = t_row + kTcOCol + (kGroups == 2 ? 2 * kHeadDim * group : 0);
-        float          m = -INFINITY, l = 0.0f, v_unit = 1.0f, v_limit = -1.0f;
+        float          m = -INFINITY, l = 0.0f, to_units = 1.0f;  // q8_0: see inverse_unit
         bool           ok = true;
         // q8_0: tile U's bytes to f16, K by the group's first two warps, V by the others; its scales, and the largest of V's
         auto expand = [&](int U) {
@@ -940,6 +999,10 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 const __half2  a   = __habs2(as_half2(d));
                 const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(a), __high2float(a))));
                 if (lane == 0) atomicMax(&largest[st], top);
+                if (U < kGroups) {
+                    const uint32_t low = __reduce_min_sync(0xffffffffu, here ? __float_as_uint(fmaxf(__low2float(a), __high2float(a))) : 0x7f800000u);
+                    if (lane == 0) atomicMin(&smallest[U], low);
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -949,7 +1012,11 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             return true;
         };
-        if (Q8 && group < n_sub) ok = expand(group);
+        if (Q8 && group < n_sub) {
+            // the first tile's largest weight is 1, so the smallest scale is no more than the largest product
+            ok     = expand(group) && mbar_wait_bounded(full0 + 8 * (group % kTcStages), 0);
+            to_units = kUnitFirst * inverse_unit(__uint_as_float(*reinterpret_cast<volatile uint32_t *>(&smallest[group])));
+        }
         for (int U = group; U < n_sub && (Q8 || ok); U += kGroups) {
             const int sb = U % kSBufs, left = n_keys - U * kSub;  // keys of this tile and after
             // (q8_0: a warp whose wait ran out stays until the barrier at the end of the tile, which the others wait at)
@@ -998,33 +1065,35 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 t1 = max3(t1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
             }
             const float top = fmaxf(t0, t1);
-            float unit = 1.0f;  // q8_0: by how much the unit of the weights grows (the same for all rows)
+            const bool first = U < kGroups;
+            if (first) m = top;
             if constexpr (Q8) {
-                const float dm = __uint_as_float(*reinterpret_cast<volatile uint32_t *>(&largest[U % kTcStages]));
-                if (dm > v_limit) {
-                    const float now = dm > 0.0f ? __uint_as_float(__float_as_uint(dm) & 0x7f800000u) : kTwoM24;
-                    unit    = v_unit / now;
-                    v_unit  = now;
-                    v_limit = dm > 0.0f ? now * 8.0f : 0.0f;
+                // A product is below 2^(top - m) times a scale below 2^(e0 + 1) times less than 2^(e1 + 1).  (By exponents: what `top` is waited
+                // for is a subtraction and a comparison.  With the powers themselves 256 streams under 4096 rows took 2.5 us longer.)
+                auto room = [&]() {
+                    const int e = (int) (*reinterpret_cast<volatile uint32_t *>(&largest[U % kTcStages]) >> 23) + (int) (__float_as_uint(to_units) >> 23) - 254;
+                    return to_units < kUnitFirst * kMostInverse ? (float) (11 - e) : -INFINITY;
+                };
+                if (top - m > 8.0f) {
+                    l *= ex2_approx(m - top);
+                    to_units *= ex2_approx(top - m);  // in the accumulators' place
+                    m = top;
                 }
-            }
-            if (U < kGroups) {
-                m = top;
-            } else {
+                if (__any_sync(0xffffffffu, top - m > room())) {
+                    if (!first && !retired(U - kGroups)) ok = false;  // the accumulators are at rest once P.V of the group's tile before has retired
+                    to_units = refit_row<8 / kGroups>(t_s, smem_u32(sc), m, first ? 0u : t_o, to_units);
+                }
+            } else if (!first) {
                 const bool raise = top > m + 8.0f;
-                if (__any_sync(0xffffffffu, raise || unit != 1.0f)) {
+                if (__any_sync(0xffffffffu, raise)) {
                     const float f = raise ? ex2_approx(m - top) : 1.0f;
                     if (raise) m = top;
                     l *= f;
-                    // the accumulators are at rest once P.V of the group's tile before has retired
-                    if (!retired(U - kGroups)) {
-                        ok = false;
-                        if (!Q8) break;
-                    }
-                    rescale_row(t_o, 8 / kGroups, f * unit);
+                    if (!retired(U - kGroups)) { ok = false; break; }
+                    rescale_row(t_o, 8 / kGroups, f);
                 }
             }
-            const float ref = Q8 ? m : m - kTcShift, to_units = 4.0f / v_unit;  // weights up to 2^8 * 8 * 4 = 2^13
+            const float ref = Q8 ? m : m - kTcShift;
 #pragma unroll
             for (int g = 0; g < kSub / 16; ++g) {
                 if constexpr (Q8) {
@@ -1077,7 +1146,7 @@ shared_rows_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (all_ok && n_sub > 0) {
             tc_fence_after();
             float4 * const part  = reinterpret_cast<float4 *>(smem_gen) + (group * kRows + row) * kPartPitch;
-            const float    f     = Q8 ? v_unit / 4.0f : 1.0f;
+            const float    f     = Q8 ? 1.0f / to_units : 1.0f;
             const int      parts = group >= n_sub ? 0 : kGroups == 2 || n_sub == 1 ? 2 : 4;  // accumulators with something in them
 #pragma unroll
             for (int h = 0; h < 2; ++h) {

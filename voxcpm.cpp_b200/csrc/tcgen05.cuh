@@ -59,6 +59,14 @@ __device__ __forceinline__ void tmem_ld32_sync(uint32_t taddr, uint32_t * r) {
         : "memory");
 }
 // 64 consecutive columns (two loads in flight, one wait)
+__device__ __forceinline__ void tmem_ld8_sync(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_ld64_sync(uint32_t taddr, uint32_t * r) {
     asm volatile(
         "{\n\t.reg .b32 second;\n\t"
