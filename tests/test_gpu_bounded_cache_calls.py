@@ -1,10 +1,13 @@
 """Calls of the bounded-cache operators that must be refused, and what the operators promise about calls in a row: beside
 test_gpu_bounded_cache.py, whose cases and definitions these use."""
+import contextlib
 import ctypes
 
 import numpy as np
 import pytest
-from test_gpu_bounded_cache import D, EvictCase, ObserveCase, SharedCase, gen, ints, new_cache, randn
+import test_gpu_bounded_cache as cases
+from test_bounded_cache_border import scores_with_a_bin_of
+from test_gpu_bounded_cache import OBSERVE, WEIGHT, D, EvictCase, ObserveCase, SharedCase, gen, ints, new_cache, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +242,85 @@ def test_rows_of_zeros_beside_others(form, engine, pkg):
     """V rows of nothing (scale 0) carry all the weight at first."""
     import torch
     magnitudes(engine, pkg, form, lambda at: torch.where(at < 0.5, 0.0, -6.0), lambda at: torch.where(at < 0.5, 0.0, 1.0))
+
+
+def test_no_refusal_launches_anything(engine, pkg, monkeypatch):
+    """All of test_refusals again, with a look at the launch count around every refused call."""
+    seen = []
+
+    class Counting:
+        @staticmethod
+        @contextlib.contextmanager
+        def raises(*args, **kw):
+            before = engine.launches
+            with pytest.raises(*args, **kw) as err:
+                yield err
+            assert engine.launches == before
+            seen.append(err)
+
+    monkeypatch.setattr(cases, "pytest", Counting)
+    cases.test_refusals(engine, pkg)
+    assert len(seen) >= 40
+
+
+# The weights themselves, to the relative error that their derivation allows (test_gpu_bounded_cache.py: 1.2e-4, whatever their size: a score's
+# error does not depend on it).  From scores of 0, since beside an old score of about 1 a weight of 1 / rows could be missing and
+# not be seen; 1e-30: weights below 2^-126 count as 0.
+
+def check_weights(c, n_new=1):
+    c.score.zero_()
+    want, pos = c.want(n_new, 0.75)
+    c.run(n_new, 0.75)
+    c.engine.sync_status()
+    error = (c.score.double() - want).abs() - WEIGHT * want - 1e-30
+    assert float(error.max()) <= 0, float(((c.score.double() - want).abs() / want.clamp(min=1e-30)).max())
+    # and beside old scores of the weights' size: one addition more, rounded once
+    rows = float(np.mean([max(n, 1) for n in c.n]))
+    c.score.copy_(randn(gen(1), *c.score.shape).abs() * (c.n_q * c.H / c.HK / rows))
+    old = c.score.double().clone()
+    both, _ = c.want(n_new, 0.75)
+    c.run(n_new, 0.75)
+    c.engine.sync_status()
+    live = cases.cuda(np.arange(old.shape[-1])[None] < np.array(c.n)[:, None])[:, None]
+    error = ((c.score.double() - both).abs() - WEIGHT * want - 2.0 ** -23 * both)[live.expand_as(both)]
+    assert float(error.max()) <= 0
+    assert bool((c.score.double() == old)[~live.expand_as(both)].all())
+
+
+@pytest.mark.parametrize("case", OBSERVE)
+def test_every_weight_to_its_relative_error(case, engine, pkg):
+    check_weights(ObserveCase(engine, pkg, case), n_new=OBSERVE[case][2])
+
+
+@pytest.mark.parametrize("given_lse", [True, False])
+@pytest.mark.parametrize("kind,streams,rows", [("f16", 128, 4700), ("q8_0", 64, 9300), ("f16", 12, 24576), ("q8_0", 9, 26000)])
+def test_every_weight_of_many_long_streams(kind, streams, rows, given_lse, engine, pkg):
+    lens = [min(rows, max(0, 512 * (i % 11) + (0, 1, -1, 64, 257)[i % 5])) for i in range(streams - 2)] + [rows, rows - 1]
+    check_weights(ObserveCase(engine, pkg, (kind, lens, 1, 4, 2), given_lse=given_lse))
+
+
+@pytest.mark.parametrize("kind,streams,rows", [("f16", 128, 4700), ("q8_0", 64, 9300)])
+@pytest.mark.parametrize("n_q", [3, 46, 49])
+def test_every_weight_of_a_window_over_many_long_streams(kind, streams, rows, n_q, engine, pkg):
+    lens = [min(rows, max(0, 512 * (i % 11) + (0, 1, -1, 64, 257)[i % 5])) for i in range(streams - 2)] + [rows, rows - 1]
+    check_weights(ObserveCase(engine, pkg, (kind, lens, n_q, 4, 2)), n_new=2)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("n_q,heads,kv_heads", [(13, 16, 2), (28, 16, 2), (44, 16, 2), (64, 16, 2), (43, 18, 3), (50, 4, 4)])
+def test_every_weight_of_wide_windows(n_q, heads, kv_heads, kind, engine, pkg):
+    check_weights(ObserveCase(engine, pkg, (kind, [4 * ((i * 37) % 97) + 1 for i in range(73)] + [2600], n_q, heads, kv_heads)), n_new=2)
+
+
+@pytest.mark.parametrize("count", [97, 255, 256, 257])
+def test_eviction_where_the_border_is_in_a_full_bin(count, engine, pkg):
+    """As many keys in the border's bin as are ranked against one another, one more and one less."""
+    c = EvictCase(engine, pkg, "f16", [700, 700], 1, 2, 704)
+    w = np.zeros(c.score.shape, np.float32)
+    for s in range(2):
+        for h in range(2):
+            w[0, s, h, :700] = scores_with_a_bin_of(count, 700, 4 * s + h)
+    above = int((w[0, 0, 0] >= 1.25).sum())
+    c.score.copy_(cases.cuda(w))
+    c.row_pos.copy_(c.row_pos + 100)
+    c.check(above + count // 2)
