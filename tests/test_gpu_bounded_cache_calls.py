@@ -324,3 +324,19 @@ def test_eviction_where_the_border_is_in_a_full_bin(count, engine, pkg):
     c.score.copy_(cases.cuda(w))
     c.row_pos.copy_(c.row_pos + 100)
     c.check(above + count // 2)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("streams,prefix", [(64, 8000), (256, 8000), (40, 16000)])
+def test_full_row_tiles_under_long_prefixes(kind, streams, prefix, engine, pkg):
+    """The tensor core truncates a sum once every 32 keys (sums of even and of odd tiles of 64 keys apart, 16 keys a product), by less than
+    2^-23 of it and half of that on average.  A CTA's share of the keys is the prefix over the CTAs of a cluster: as many as there are
+    SMs for, eight at most."""
+    tiles = 2 * -(-streams // 16)
+    share = prefix / min(8, 148 // tiles)
+    c = SharedCase(engine, pkg, (kind, [0] * streams, [prefix], [1 + s % 3 for s in range(streams)], 16, 2), junk=False)
+    out, lse = c.run()
+    engine.sync_status()
+    want, want_lse = c.want()
+    assert float((out.double() - want).norm() / want.norm()) < share / 32 * 2.0 ** -23 + 5e-7
+    assert float((lse.double() - want_lse).abs().max()) < 6e-5
