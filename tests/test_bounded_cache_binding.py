@@ -172,3 +172,26 @@ def test_tensors_of_another_device_are_refused(rig, pkg):
     refused(rig, pkg, "on device 0", decode)
     refused(rig, pkg, "on device 0", observe)
     refused(rig, pkg, "on device 0", evict)
+
+
+@pytest.mark.parametrize("step", [1 << 10, 1 << 20, 50 << 20, 700 << 20])
+def test_outgrown_workspaces_do_not_pile_up(step, rig, monkeypatch):
+    """Needs that grow a little with every call: the workspaces kept for captured graphs stay in proportion to the largest."""
+    class Memory:
+        def __init__(self, n, **_):
+            self.n = n
+
+        def numel(self):
+            return self.n
+
+        def data_ptr(self):
+            return 256
+    monkeypatch.setattr(torch, "empty", Memory)
+    e, largest = rig.engine, 0
+    for i in range(1, 400):
+        largest = i * step
+        ws = e.workspace(largest)
+        assert ws.numel() >= largest and e._ws_at == (256, ws.numel())
+    assert e._ws.numel() <= max(2 * largest, 256)
+    assert e._ws.numel() + sum(w.numel() for w in e._outgrown) <= 6 * largest
+    assert len(e._outgrown) < 40

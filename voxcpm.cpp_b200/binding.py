@@ -349,11 +349,13 @@ class Engine:
 
     def workspace(self, nbytes: int):
         """The engine's workspace, for calls that are given none.  It grows; smaller ones before it stay allocated, since a
-        captured call may hold their addresses.  Calls that may run at the same time need workspaces of their own."""
+        captured call may hold their addresses: by half at least, so that all of them together are less than three of the last.
+        Calls that may run at the same time need workspaces of their own."""
         import torch
         if self._ws is None or self._ws.numel() < nbytes:
             if self._ws is not None:
-                nbytes = max(nbytes, self._ws.numel() + min(self._ws.numel(), 64 << 20))
+                size = self._ws.numel()
+                nbytes = max(nbytes, size + max(size >> 1, min(size, 64 << 20)))
                 self._outgrown.append(self._ws)
             self._ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=f"cuda:{self.device}")
             self._ws_at = (self._ws.data_ptr(), self._ws.numel())
