@@ -381,7 +381,7 @@ void vox_prefix_plan_destroy(vox_prefix_plan * p);
  *   own          as for vox_attn_decode (kv_len counts own rows only; k_new / v_new, rope_table and flags mean the same;
  *                the table is built for positions that count the prefix).  stream_order must be NULL.
  *   prefix       the cache that holds the prefixes: same type and kv heads as own.cache, own.layer is taken of both; it may
- *                be own.cache itself (streams of it that the call does not decode)
+ *                be own.cache itself (with k_new: streams of it that the call does not decode, now and at every replay)
  *   prefix_len   device array [streams of the prefix cache]: rows of each prefix (more than its capacity: cut off there, and
  *                VOX_ATTN_DEVICE_STATE raised)
  *   prefix_bound host-known upper bound of every prefix_len in use (sizes the grid and the workspace; 0: no prefix is read)

@@ -35,6 +35,34 @@ def test_half_a_prefix_is_refused(engine, pkg):
     engine.sync_status()
 
 
+def test_a_stream_that_is_appended_to_is_no_prefix_of_the_call(engine, pkg):
+    """The row that arrives would be stored while the prefix is read.  Without one the streams may be each other's prefixes."""
+    import torch
+    cache = new_cache(engine, pkg, "f16", 1, 4, 2, 64)
+    cache.append(0, randn(gen(1), 4, 64, 2, D), randn(gen(2), 4, 64, 2, D))
+    q, new, n, P = randn(gen(3), 2, 16, D), randn(gen(4), 2, 2, D), [20, 33], [30, 40, 50, 60]
+
+    def call(of, **kw):
+        return lambda: cache.decode_shared(0, q, ints(n), 64, prefix=cache, plan=pkg.PrefixPlan(engine, of, 4), prefix_len=ints(P), prefix_bound=60, **kw)
+
+    for of in ([0, 2], [3, 1], [-1, 0]):
+        refuses(engine, pkg, "is a prefix and one of the 2", call(of, k_new=new, v_new=new))
+    plan = pkg.PrefixPlan(engine, [2, 3], 4)
+    plan.set([2, 1])
+    refuses(engine, pkg, "is a prefix", lambda: cache.decode_shared(0, q, ints(n), 64, prefix=cache, plan=plan, prefix_len=ints(P), prefix_bound=60,
+                                                                    k_new=new, v_new=new))
+    for of in ([1, 0], [2, 3]):
+        out = call(of)()
+        engine.sync_status()
+        for s in range(2):
+            kv = [torch.cat([a, b], 1) for a, b in zip(cases.stored(cache, pkg, 0, of[s], P[of[s]]), cases.stored(cache, pkg, 0, s, n[s]))]
+            want, _ = cases.attend(q[s].double(), *kv, 0.125)
+            cases.check_rows(out[s], None, want, None)
+    call([2, 3], k_new=new, v_new=new)()
+    call([-1, -1], k_new=new, v_new=new)()
+    engine.sync_status()
+
+
 # what else lies over one another is tried on the host's own look at it: test_row_lists.py
 
 def colliding(torch, lists, rows, dtype=None):

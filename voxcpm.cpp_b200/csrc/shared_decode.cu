@@ -46,6 +46,7 @@ struct vox_prefix_plan {
     int                  max_tiles[kArrangements] = {}, n_tiles[kArrangements] = {};
     size_t               at[kArrangements + 1] = {};  // where an arrangement starts
     bool                 full = false;  // the tiles of 128 rows are more than half full on average
+    int                  first = 0;     // the lowest prefix in use
     std::vector<int32_t> host, next;    // next: scratch of the arrangement
     int32_t *            dev = nullptr;
     int    per_tile(int k) const { return (kRows >> k) / gqa; }
@@ -1227,8 +1228,12 @@ int arrange(vox_prefix_plan * pl, const int32_t * prefix_of) {
         set_error("out of host memory");
         return VOX_ATTN_OUT_OF_MEMORY;
     }
+    pl->first = pl->n_prefixes;
     for (int s = 0; s < pl->n_streams; ++s)
-        if (prefix_of[s] >= 0) count[prefix_of[s]] += 1;
+        if (prefix_of[s] >= 0) {
+            count[prefix_of[s]] += 1;
+            pl->first = std::min(pl->first, prefix_of[s]);
+        }
     for (int k = 0; k < kArrangements; ++k) {
         const int per_tile = pl->per_tile(k);
         int32_t * tiles = pl->host.data() + pl->at[k], * members = pl->host.data() + pl->members_at(k);
@@ -1284,6 +1289,9 @@ int check_shared(const vox_engine * e, const vox_decode_shared_args * a) {
                 a->plan->n_streams, a->own.n_streams);
     VOX_REQUIRE(a->plan->n_prefixes <= pc.n_streams, VOX_ATTN_INVALID_ARGUMENT, "the plan names %d prefixes, the prefix cache holds %d",
                 a->plan->n_prefixes, pc.n_streams);
+    // the arriving rows are stored while the prefixes are read, in no order
+    VOX_REQUIRE(a->prefix != c || a->own.k_new == nullptr || a->plan->first >= a->own.n_streams, VOX_ATTN_INVALID_ARGUMENT,
+                "stream %d of the cache is a prefix and one of the %d that the call appends to", a->plan->first, a->own.n_streams);
     VOX_REQUIRE(a->plan->gqa * c->cfg.n_kv_heads == a->own.n_heads, VOX_ATTN_INVALID_ARGUMENT, "the plan was made for %d heads per kv head",
                 a->plan->gqa);
     return VOX_ATTN_OK;
