@@ -86,7 +86,10 @@ int make_tensor_map(const vox_engine * e, CUtensorMap * out, void * base, CUtens
 
 // Launch with programmatic dependent launch: the grid may be scheduled while the previous kernel of the
 // stream is still draining, and its threads block in pdl_wait() until that kernel has completed and its
-// writes are visible.  Every kernel launched this way calls pdl_wait() before its first global access.
+// writes are visible.  Every kernel launched this way calls pdl_wait() before it reads what the launch in front of it may
+// write and before its first write.  What some read earlier was complete before that launch was let start: inputs that it waited
+// for itself before it called pdl_launch_dependents() (the prefix kernels behind their decode kernel, the second launches
+// of a window), and rows that a caller has promised to be a step old (VOX_DECODE_CACHE_STABLE).
 // VOX_NO_PDL=1 in the environment turns the attribute off.
 bool pdl_enabled();
 

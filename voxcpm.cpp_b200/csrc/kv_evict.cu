@@ -11,7 +11,8 @@
 // 10 bits at a time.  Lists are few when one stream is cut: then a cluster of CTAs takes each, every CTA
 // selecting for itself (the scores are in L2) and moving a share of the rows.
 // 1440 lists of up to 2048 f16 rows cut to 512 (194 MB read and written): 46 us, 4.2 TB/s.  The rows move at HBM's rate (29 us); what
-// comes before is a chain of short phases (keys 8, border 5, places 4 us, over one round of CTAs and a part); 128, 192 and 512 threads,
+// comes before is a chain of short phases (keys 8, border 5, places 4 us, over one round of CTAs and a part); q8_0 rows 40 us (17 at HBM's
+// rate).  128, 192 and 512 threads,
 // and fewer CTAs with more loads in flight, came out equal or slower.  Six lists of 300 rows: 5 us, latency (10 us when a bin of more than
 // 96 keys took another histogram and the others were ranked a key at a time).
 #include "kv_cache.cuh"

@@ -11,7 +11,8 @@
 //   two:      longer streams: a launch that finds the (max, sum) of every CTA's keys, and one that joins them.
 // 256 streams of 4096 f16 rows, given the log-sum-exp: 32.5 us = 5.5 TB/s, 84 % of the copy bandwidth; without it 53.4 us (a CTA
 // waits for its cluster with its loads done); 64 streams 12.7 / 15.9 us.  Four streams of 300 rows: 4.7 us, the latency of a launch.
-// q8_0 rows cost the conversion of every byte: 34.3 us at 256 x 4096, 2.9 TB/s.
+// q8_0 rows: 34.0 us at 256 x 4096, 2.9 TB/s.  HBM is a third busy (f16: 63 %), issue slots 54 % (f16: 32 %): per byte there are twice
+// the instructions, the conversion of every byte among them, and with half the bytes in a lane's registers half of them in flight.
 // (For smaller pieces and more CTAs of fewer registers: 32 keys of a warp 42 - 53 us, three CTAs per SM 43 us, against 40.4 us before a
 // CTA took several chunks.)
 #include "kv_observe.cuh"
@@ -307,9 +308,11 @@ __global__ void __launch_bounds__(kThreads, 2) observe_kernel(const ObserveParam
 
 // A window of few query rows (at most kFewRows, queries times the heads of a group): as above, with the rows in groups of eight.  A
 // warp's keys stay in its registers while the groups' operands come from shared memory one after the other.  Two launches: the
-// rows' (max, sum) over every CTA's keys, and the weights.  Bound by the rows: 0.3 us a group and launch where nothing else runs, the
-// issue of products and exponentials where much does (128 streams of 4096 rows, 4 queries of 8 heads: 60 us, of which K twice
-// from HBM or L2 would be 28; q8_0, whose bytes are converted for every group, 86 us).
+// rows' (max, sum) over every CTA's keys, and the weights.  Bound by latency: a group is a chain of products, shuffles, exponentials and
+// the join of its statistics, 0.3 us of it where nothing else runs, and 16 warps an SM do not hide it: 128 streams of 4096 rows, 4
+// queries of 8 heads take 60 us, of which K twice from HBM or L2 would be 28, with no unit much busier than a third (issue 32 %, tensor
+// 29 %, special functions 20 %, DRAM 31 %).  q8_0, whose bytes are converted for every group, 86 us: issue 47 and 39 %; the kernel
+// of the weights spills 304 bytes a thread.
 template <bool Q8, bool kWeights>
 __global__ void __launch_bounds__(kThreads, 2) observe_rows_kernel(const ObserveParams p) {
     __shared__ uint4  q_op[kFewRows / 8][4][32];

@@ -679,8 +679,9 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // One softmax group (192 threads of 128 registers, 81 KB of shared memory; q8_0 107 KB): the CTA runs beside two CTAs of the decode
 // kernel, whose time is HBM's, and takes about 1.1 us for 64 keys (q8_0 2.3 us), most of it latency that nothing hides: 0.5 us of
 // it are products and exponentials.  Two groups, which take tiles in turn with a reference and accumulators of their own, hide
-// some of it (256 streams under two prompts of 2048 / 4096 rows, one row of their own: 25.2 / 34.2 -> 20.3 / 28.4 us), but leave
-// room for one decode CTA per SM only: taken where the streams' own rows are few against the prefix (see vox_attn_decode_shared).
+// some of it (256 streams under two prompts of 2048 / 4096 rows, one row of their own: 23.5 / 28.6 -> 19.8 / 27.6 us; q8_0 34.9 / 54.8
+// -> 33.3 / 43.4 us), but leave room for one decode CTA per SM only: taken where the streams' own rows are few against the prefix (see
+// vox_attn_decode_shared).
 //
 // q8_0: the softmax warps turn a tile's bytes into f16 numbers q (exact; a tile ahead of the scores they work on) and keep the
 // scales apart.  Either 32-value block has a score accumulator of its own (s = d0 S0 + d1 S1), and its 32 output columns have
@@ -1387,8 +1388,8 @@ int vox_attn_decode_shared(vox_engine * e, const vox_decode_shared_args * a, voi
     const int               cluster = shares ? cluster_size(sms, pl->n_tiles[k], HK, a->prefix_bound, tc) : 1;
     // Two softmax groups, beside one decode CTA per SM, where the streams' own 64-row tiles per SM are few against the tiles that a
     // CTA of the prefix kernel walks: then the prefix kernel is what the call waits for.  256 streams under two prompts of 4096
-    // rows, own rows 1 / 128 / 512 / 1024 / 2048: f16 28 / 25 / 38 / 47 / 68 us against 34 / 35 / 33 / 37 / 49 us with one group;
-    // q8_0, whose scores cost more, 44 / 45 / 51 / 59 / 77 against 56 / 58 / 62 / 67 / 71 us.
+    // rows, own rows 1 / 128 / 512 / 1024 / 2048: f16 28 / 25 / 36 / 47 / 68 us against 29 / 30 / 32 / 38 / 49 us with one group;
+    // q8_0, whose scores cost more, 44 / 44 / 50 / 57 / 75 against 55 / 56 / 61 / 63 / 71 us.
     const long long own_tiles = (long long) a->own.n_streams * HK * ((a->own.kv_bound + kKvTile - 1) / kKvTile) / sms;
     const bool      wide = tc && 4 * own_tiles <= (q8 ? 20LL : 5LL) * ((a->prefix_bound + kSub - 1) / kSub) / cluster;
     rc = launch_decode_shared(e, &a->own, OwnRows{a->lse, ml, !shares ? 0 : wide ? 1 : 2}, workspace, own, st);
