@@ -195,3 +195,19 @@ def test_outgrown_workspaces_do_not_pile_up(step, rig, monkeypatch):
     assert e._ws.numel() <= max(2 * largest, 256)
     assert e._ws.numel() + sum(w.numel() for w in e._outgrown) <= 6 * largest
     assert len(e._outgrown) < 40
+
+
+@pytest.mark.parametrize("bad", [[0, 1], [0, 1, 0, 1], [], [[0, 1, 0]], [0.5, 1, 0], [0, 1, float("nan")], torch.tensor([0, 1 << 32, 0]).numpy(), 0])
+def test_assignments_that_are_not_one_whole_number_per_stream_are_refused(bad, rig, pkg):
+    """The library reads as many numbers as the plan has streams."""
+    plan = rig.plan()
+    refused(rig, pkg, "prefix_of", lambda rig: plan.set(bad, stream=0))
+    plan.set([0, 1, -1], stream=0)
+    plan.set(torch.tensor([1, 1, 0]), stream=0)
+    assert rig.calls == ["vox_prefix_plan_set"] * 2
+
+
+def test_a_closed_plan_is_not_set(rig, pkg):
+    plan = rig.plan()
+    plan.close()
+    refused(rig, pkg, "closed", lambda rig: plan.set([0, 1, -1], stream=0))

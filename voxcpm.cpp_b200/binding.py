@@ -718,12 +718,20 @@ class PrefixPlan:
     @staticmethod
     def _ints(prefix_of):
         import numpy as np
-        return np.ascontiguousarray(prefix_of, np.int32)
+        given = np.asarray(prefix_of)
+        with np.errstate(invalid="ignore"):
+            a = np.ascontiguousarray(given, np.int32)
+        if given.ndim != 1 or not np.array_equal(a, given):
+            raise VoxError(1, f"prefix_of must be whole numbers of 32 bits, one per stream, got {given.dtype} of shape {given.shape}")
+        return a
 
     def set(self, prefix_of, stream=None):
         """Another assignment, in stream order."""
         a = self._ints(prefix_of)
-        assert a.shape == (self.n_streams,)
+        if len(a) != self.n_streams:
+            raise VoxError(1, f"prefix_of holds {len(a)} streams, the plan {self.n_streams}")
+        if not self.h:
+            _closed(self)
         _check(lib().vox_prefix_plan_set(self.h, a.ctypes.data_as(C.c_void_p), _stream_ptr(stream)))
 
     def close(self):
