@@ -211,3 +211,19 @@ def test_a_closed_plan_is_not_set(rig, pkg):
     plan = rig.plan()
     plan.close()
     refused(rig, pkg, "closed", lambda rig: plan.set([0, 1, -1], stream=0))
+
+
+def test_a_workspace_that_the_device_cannot_use_is_refused(rig, pkg):
+    """It is written by the kernels over its whole length."""
+    for call in (decode, observe):
+        refused(rig, pkg, "workspace", call, workspace=wide(torch.zeros(4096, dtype=torch.uint8)))
+
+    class Elsewhere:
+        dtype, device = torch.uint8, "elsewhere"
+        get_device = staticmethod(lambda: 5)
+        is_contiguous = staticmethod(lambda: True)
+        data_ptr = staticmethod(lambda: 256)
+        numel = staticmethod(lambda: 4096)
+        stride = staticmethod(lambda: (1,))
+    for call in (decode, observe):
+        refused(rig, pkg, "workspace", call, workspace=Elsewhere())

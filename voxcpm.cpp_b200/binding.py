@@ -366,6 +366,8 @@ class Engine:
         for the size every time costs a third of what the launch does)."""
         st = _raw_stream(self.device) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
         if workspace is not None:
+            if workspace.get_device() != self.device or not workspace.is_contiguous():
+                raise VoxError(1, f"workspace must be contiguous on device {self.device}, got strides {workspace.stride()} on {workspace.device}")
             rc = call(self.h, args, workspace.data_ptr(), workspace.numel(), st)
         else:
             rc = call(self.h, args, *self._ws_at, st)
