@@ -389,9 +389,9 @@ void vox_prefix_plan_destroy(vox_prefix_plan * p);
  *                which vox_kv_observe takes
  * prefix, plan and prefix_len all NULL, prefix_bound 0: own rows only (vox_attn_decode with lse).  Results agree with vox_attn_decode over a
  * cache that holds both parts to rounding; q8_0 weights keep 22 bits here, however far the scales of a head's rows lie apart, where that
- * call rounds them to f16.  Error (in the norm, relative to the result): under 1e-6, but for the tensor core's truncation of long sums
- * where many streams share a prefix: 2e-6 for each 1000 keys of it to a CTA of a cluster (64 streams under 8000 rows 2e-6, 256
- * streams 4e-6).
+ * call rounds them to f16.  Queries do too, so a score s is off by up to 2^-22 s, and a weight by as much of itself.  Error of a result
+ * (its norm, relative to the result's) where scores are below 10: under 1e-6, but for the tensor core's truncation of long sums where
+ * many streams share a prefix: 2e-6 for each 1000 keys of it to a CTA of a cluster (64 streams under 8000 rows 2e-6, 256 streams 4e-6).
  * A stream without a prefix row and without an own row gives zeros.  Rows past a length may hold anything, NaN included.
  * dst must not overlap q.  Two launches, the second on the SMs that the first leaves room on.
  * workspace: vox_attn_decode_shared_workspace_bytes, 16-byte aligned.  The engine's device must be the current one. */
