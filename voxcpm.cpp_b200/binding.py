@@ -370,7 +370,8 @@ class Engine:
                 raise VoxError(1, f"workspace must be contiguous on device {self.device}, got strides {workspace.stride()} on {workspace.device}")
             rc = call(self.h, args, workspace.data_ptr(), workspace.numel(), st)
         else:
-            rc = call(self.h, args, *self._ws_at, st)
+            at, n = self._ws_at
+            rc = call(self.h, args, at, n, st)
             if rc == 3:
                 self.workspace(max(size(args), 1 << 16))
                 rc = call(self.h, args, *self._ws_at, st)
